@@ -507,6 +507,116 @@ int rq_sgemm_nt(rq_ctx ctx, const float* a, const float* b, float* c, int64_t m,
 int rq_linear(rq_ctx ctx, const float* x, const float* w, const float* b, float* y, int64_t batch, int64_t in_f,
               int64_t out_f, void* stream);
 
+/* ---- attention over prompts, and a cache in pages ------------------------------
+ * What a decoder needs around rq_decode_attention's single step: prompts of many
+ * sequences at once with their gradient, and a cache that sequences share page by
+ * page. Common to all: device pointers unless said otherwise, 16-byte aligned
+ * (int32 arrays and lse 4-byte); row strides in elements, a multiple of 16
+ * bytes, at least a row's elements and at most 2^22, so q, k and v may be
+ * columns of one product's output; head_dim a multiple of 8 up to 256; query
+ * head h reads KV head h / (n_q/n_kv); all asynchronous on `stream`, nothing
+ * allocated and no scratch of the context used, so any number of calls and
+ * captured graphs may run at once as long as their buffers differ. Results do not
+ * depend on scheduling. */
+
+/* A packed batch of sequences. Sequence b's queries are the rows cu_q[b] ..
+ * cu_q[b+1] - 1 of q, out and dout, its keys the rows cu_k[b] .. cu_k[b+1] - 1
+ * of k and v (device int32[batch + 1], not decreasing, at most rows_q / rows_k;
+ * NULL cu_k: the queries'). Rows of no sequence are neither read nor written. */
+typedef struct {
+  int dtype; /* RQ_F32 or RQ_BF16: q, k, v, out and their gradients */
+  int64_t batch, rows_q, rows_k;
+  int64_t n_q, n_kv, head_dim;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int causal; /* 1: of a queries and b keys, query i sees the keys j <= i + b - a; 0: all */
+  double scale; /* of the scores, positive */
+} rq_prompt;
+
+/* out[i] = sum_j p_ij v_j, p_ij = exp(scale q_i . k_j - lse_i), lse_i = log sum_j
+ * exp(scale q_i . k_j) over the keys that query i sees, per head
+ * (gqa-attention's softmax, raster/dl/attention.clj:248-287, for every token of a
+ * prompt). A query that sees no key, or only scores of -inf, gets zeros and lse
+ * -inf. lse f32[n_q][rows_q], or NULL. f32: products and sums in f32; bf16: products of
+ * bf16, weights rounded to bf16 for theirs, sums, maxima and lse in f32. A NaN or
+ * an inf in v also reaches the queries before it within its tile of keys. */
+int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
+                        void* stream);
+
+/* The gradient of rq_prompt_attention: from dout and the forward's out and lse,
+ * dq, dk and dv (fully overwritten in every row of a sequence, dk and dv summed
+ * over the query heads of a KV head; none may overlap an input). p_ij is
+ * recomputed from lse. f32: in f32; bf16: products of bf16 with p and its gradient
+ * rounded to bf16, sums in f32. work: rq_prompt_attention_bwd_work bytes of
+ * device memory (f32[n_q][rows_q], the rows' dout . out), 16-byte aligned, used by this call alone
+ * until it has run. */
+int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes);
+int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, int64_t dout_stride, const void* q,
+                            int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            const void* out, int64_t out_stride, const float* lse, void* dq, int64_t dq_stride,
+                            void* dk, int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
+                            void* stream);
+
+/* One layer's cache in pages: kpages and vpages hold `pages` pages of page_size
+ * rows (a power of two, 16 to 65536) of n_kv * head_dim elements, a row of
+ * rq_decode_attention's caches each. Row r of sequence b lies in page
+ * table[b * table_stride + r / page_size] at r % page_size (device int32, read
+ * only as far as the sequence has rows). */
+typedef struct {
+  int dtype; /* RQ_F32 or RQ_BF16: the pages */
+  void* kpages;
+  void* vpages;
+  int64_t pages, page_size;
+  int64_t n_kv, head_dim;
+  const int32_t* table;
+  int64_t table_stride;
+} rq_pages;
+
+/* rq_decode_attention for one new token of each of `batch` sequences over a
+ * paged cache: RoPE of q [n_q * head_dim] and k [n_kv * head_dim] at position
+ * lens[b] (NeoX half split, angles formed in double; theta 0: q and k as they are),
+ * append of the rotated k and of v at row lens[b], rounded to the pages' type, and
+ * attention of the rotated query over rows 0 .. lens[b] as they are stored.
+ * k and v NULL: nothing is appended, and rows 0 .. lens[b] - 1 are attended.
+ * lens (device int32[batch], rows before the call) is left as it is, so that a
+ * model's layers share it. lens[b] < 0: an idle slot, its out row is zeros and its pages
+ * are not touched; so is the out row of a sequence without rows. max_len: no sequence has more
+ * rows than this, the new one included; it sizes work (rq_paged_attention_work
+ * bytes, none when 0). A sequence with more rows than max_len or its table holds, or a page
+ * number outside 0 .. pages - 1, gets NaN, and nothing is written outside the pages.
+ * Rows that two sequences share are only read, provided each appends to a page of its own.
+ * dtype is that of q, k, v and out: RQ_F32 over f32 or bf16 pages (f32 results:
+ * over bf16 pages q and the weights enter as three bf16 terms), or RQ_BF16 over
+ * bf16 pages (rotated q and the weights rounded to bf16). The cached rows are split over
+ * workgroups and their softmax states joined in order. */
+int rq_paged_attention_work(rq_ctx ctx, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
+                            size_t* bytes);
+int rq_paged_attention(rq_ctx ctx, const rq_pages* pg, int dtype, const void* q, int64_t q_stride, const void* k,
+                       int64_t k_stride, const void* v, int64_t v_stride, const int32_t* lens, int64_t batch,
+                       int64_t n_q, int64_t max_len, double theta, double scale, void* out, int64_t out_stride,
+                       void* work, size_t work_bytes, void* stream);
+
+/* A packed prompt into the pages: sequence b's rows cu[b] .. cu[b+1] - 1 (as in
+ * rq_prompt) are its positions past[b], past[b] + 1, ...: q_out and, unless NULL,
+ * k_out get the rotated q and k in their own type (either may be its input), and
+ * the pages the rotated k and v. past[b] < 0: the sequence is left out. Rows whose
+ * page is missing (as in rq_paged_attention) get NaN in q_out and k_out and are not stored.
+ * Types as for rq_paged_attention; theta 0: no rotation. */
+int rq_pages_append(rq_ctx ctx, const rq_pages* pg, int dtype, const void* q, int64_t q_stride, const void* k,
+                    int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, const int32_t* past,
+                    int64_t batch, int64_t rows, int64_t n_q, double theta, void* q_out, int64_t q_out_stride,
+                    void* k_out, int64_t k_out_stride, void* stream);
+
+/* Copies n pages inside a cache of `planes` planes (every layer's kpages and
+ * vpages), plane_bytes apart, each of `pages` pages of page_bytes: page src[i] to
+ * page dst[i] in every plane. src and dst are host arrays, read during the call
+ * (a captured graph keeps these numbers). All dst must differ, and none may be
+ * a src, else RQ_ERR_SHAPE and nothing is copied. plane_bytes and page_bytes
+ * multiples of 16. */
+int rq_pages_copy(rq_ctx ctx, void* base, int64_t planes, int64_t plane_bytes, int64_t pages, int64_t page_bytes,
+                  const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

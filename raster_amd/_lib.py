@@ -66,6 +66,15 @@ SIGNATURES = {
     "rq_sgemm_tn": ([_p, _p, _p, _p, _i64, _i64, _i64, C.c_float, C.c_float, _p], _i),
     "rq_sgemm_nt": ([_p, _p, _p, _p, _i64, _i64, _i64, C.c_float, C.c_float, _p], _i),
     "rq_linear": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _p], _i),
+    "rq_prompt_attention": ([_p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p], _i),
+    "rq_prompt_attention_bwd_work": ([_p, C.POINTER(_sz)], _i),
+    "rq_prompt_attention_bwd": ([_p, _p, *[_p, _i64] * 5, _p, *[_p, _i64] * 3, _p, _sz, _p], _i),
+    "rq_paged_attention_work": ([_p, _i64, _i64, _i64, _i64, _i64, C.POINTER(_sz)], _i),
+    "rq_paged_attention": ([_p, _p, _i, *[_p, _i64] * 3, _p, _i64, _i64, _i64, C.c_double, C.c_double, _p, _i64, _p,
+                            _sz, _p], _i),
+    "rq_pages_append": ([_p, _p, _i, *[_p, _i64] * 3, _p, _p, _i64, _i64, _i64, C.c_double, _p, _i64, _p, _i64, _p],
+                        _i),
+    "rq_pages_copy": ([_p, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _p], _i),
 }
 
 
@@ -73,6 +82,20 @@ class FusedOps(C.Structure):
     """rq_fused_ops of include/rq.h."""
 
     _fields_ = [("norm_gain", _p), ("norm_eps", C.c_float), ("residual", _p), ("swiglu", _i), ("act_i8", _i)]
+
+
+class Prompt(C.Structure):
+    """rq_prompt of include/rq.h."""
+
+    _fields_ = [("dtype", _i), ("batch", _i64), ("rows_q", _i64), ("rows_k", _i64), ("n_q", _i64), ("n_kv", _i64),
+                ("head_dim", _i64), ("cu_q", _p), ("cu_k", _p), ("causal", _i), ("scale", C.c_double)]
+
+
+class Pages(C.Structure):
+    """rq_pages of include/rq.h."""
+
+    _fields_ = [("dtype", _i), ("kpages", _p), ("vpages", _p), ("pages", _i64), ("page_size", _i64), ("n_kv", _i64),
+                ("head_dim", _i64), ("table", _p), ("table_stride", _i64)]
 
 
 class RqError(RuntimeError):

@@ -25,7 +25,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librq.so")
-HEADERS = [os.path.join(CSRC, "rq_internal.h"), os.path.join(os.path.dirname(HERE), "include", "rq.h")]
+HEADERS = [*sorted(glob.glob(os.path.join(CSRC, "*.h"))), os.path.join(os.path.dirname(HERE), "include", "rq.h")]
 ARCH = "gfx950"
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",

@@ -6,7 +6,9 @@
 // thread-local string (rq_last_error).
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <new>
 #include <string>
@@ -14,6 +16,9 @@
 #include <unordered_set>
 #include <vector>
 
+#include "attn_tile.h"
+#include "paged.h"
+#include "prompt.h"
 #include "rq_internal.h"
 
 namespace rq {
@@ -1432,6 +1437,315 @@ int rq_linear(rq_ctx h, const float* x, const float* w, const float* b, float* y
   // y = b in every row, then y = 1 x W^T + 1 y (nn.clj:166-173)
   if (hipError_t e = launch_bias_rows(b, y, batch, out_f, (hipStream_t)stream)) return hip_fail(e, "bias launch");
   return dense_call(h, 0, 1, x, w, y, batch, in_f, out_f, 1.0f, 1.0f, stream);
+}
+
+// ---- attention over prompts and the paged cache --------------------------------
+// (arguments are checked before the context, so that a caller without a GPU can check its own)
+
+}  // extern "C"
+
+namespace rq {
+
+static constexpr int64_t kMaxRows = (int64_t)1 << 30;
+
+static size_t elem_size(int dtype) { return dtype == RQ_F32 ? 4 : 2; }
+
+static int check_heads(int64_t n_q, int64_t n_kv, int64_t head_dim) {
+  if (n_q <= 0 || n_kv <= 0 || head_dim <= 0) return fail(RQ_ERR_SHAPE, "n_q, n_kv and head_dim must be positive");
+  if (n_q % n_kv != 0) return fail(RQ_ERR_SHAPE, "n_q must be a multiple of n_kv");
+  if (n_q > 65535) return fail(RQ_ERR_SHAPE, "n_q too large");
+  if (head_dim % 8 != 0 || head_dim > 256) return fail(RQ_ERR_SHAPE, "head_dim must be a multiple of 8 up to 256");
+  return RQ_OK;
+}
+
+// A row operand: pointer, alignment and stride of `width` elements a row.
+static int check_rows(const char* what, const void* p, int64_t stride, int64_t width, int dtype) {
+  if (!p) return fail(RQ_ERR_NULL, std::string(what) + " is NULL");
+  if (((uintptr_t)p & 15) != 0) return fail(RQ_ERR_SHAPE, std::string(what) + " must be 16-byte aligned");
+  if (stride < width || stride > kMaxTileStride)
+    return fail(RQ_ERR_SHAPE, std::string(what) + "'s row stride must be at least its row and at most 2^22 elements");
+  if ((size_t)stride * elem_size(dtype) % 16 != 0)
+    return fail(RQ_ERR_SHAPE, std::string(what) + "'s row stride must be a multiple of 16 bytes");
+  return RQ_OK;
+}
+
+static int check_i32(const char* what, const void* p) {
+  if (!p) return fail(RQ_ERR_NULL, std::string(what) + " is NULL");
+  if (((uintptr_t)p & 3) != 0) return fail(RQ_ERR_SHAPE, std::string(what) + " must be 4-byte aligned");
+  return RQ_OK;
+}
+
+static int check_scale(double scale) {
+  // the kernels take the maximum before the factor, and the factor must be a normal f32
+  if (!(scale >= 1e-30 && scale <= 1e30)) return fail(RQ_ERR_SHAPE, "scale must be between 1e-30 and 1e30");
+  return RQ_OK;
+}
+
+static int check_prompt(const rq_prompt* p) {
+  if (!p) return fail(RQ_ERR_NULL, "rq_prompt is NULL");
+  if (p->dtype != RQ_F32 && p->dtype != RQ_BF16) return fail(RQ_ERR_DTYPE, "dtype must be RQ_F32 or RQ_BF16");
+  if (int s = check_heads(p->n_q, p->n_kv, p->head_dim)) return s;
+  if (p->batch < 0 || p->rows_q < 0 || p->rows_k < 0) return fail(RQ_ERR_SHAPE, "negative dimension");
+  if (p->rows_q > kMaxRows || p->rows_k > kMaxRows || p->batch > kMaxRows) return fail(RQ_ERR_SHAPE, "too many rows");
+  if ((p->rows_q / 32 + p->batch) * p->n_q > INT32_MAX || (p->rows_k / 32 + p->batch) * p->n_q > INT32_MAX ||
+      p->rows_q * p->n_q > (int64_t)INT32_MAX * 8)
+    return fail(RQ_ERR_SHAPE, "rows times heads too large for one launch");
+  if (!p->cu_k && p->rows_k != p->rows_q) return fail(RQ_ERR_SHAPE, "without cu_k, rows_k must be rows_q");
+  if (int s = check_scale(p->scale)) return s;
+  return RQ_OK;
+}
+
+static PromptArgs prompt_args(const rq_prompt* p) {
+  PromptArgs a = {};
+  a.cu_q = p->cu_q;
+  a.cu_k = p->cu_k ? p->cu_k : p->cu_q;
+  a.rows_q = p->rows_q;
+  a.rows_k = p->rows_k;
+  a.batch = (int)p->batch;
+  a.n_q = (int)p->n_q;
+  a.n_kv = (int)p->n_kv;
+  a.head_dim = (int)p->head_dim;
+  a.causal = p->causal != 0;
+  a.scale = (float)p->scale;
+  a.scale2 = (float)(p->scale * 1.4426950408889634);
+  return a;
+}
+
+static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) {
+  if (!g) return fail(RQ_ERR_NULL, "rq_pages is NULL");
+  if ((dtype != RQ_F32 && dtype != RQ_BF16) || (g->dtype != RQ_F32 && g->dtype != RQ_BF16))
+    return fail(RQ_ERR_DTYPE, "types must be RQ_F32 or RQ_BF16");
+  if (dtype == RQ_BF16 && g->dtype == RQ_F32) return fail(RQ_ERR_DTYPE, "bf16 rows over f32 pages are not supported");
+  if (int s = check_heads(n_q, g->n_kv, g->head_dim)) return s;
+  if (g->page_size < 16 || g->page_size > 65536 || (g->page_size & (g->page_size - 1)) != 0)
+    return fail(RQ_ERR_SHAPE, "page_size must be a power of two from 16 to 65536");
+  if (g->pages <= 0 || g->pages > INT32_MAX) return fail(RQ_ERR_SHAPE, "bad number of pages");
+  if (g->table_stride < 0 || g->table_stride > INT32_MAX) return fail(RQ_ERR_SHAPE, "bad table_stride");
+  if (!g->kpages || !g->vpages) return fail(RQ_ERR_NULL, "kpages or vpages is NULL");
+  if ((((uintptr_t)g->kpages | (uintptr_t)g->vpages) & 15) != 0)
+    return fail(RQ_ERR_SHAPE, "kpages and vpages must be 16-byte aligned");
+  if (g->n_kv * g->head_dim > kMaxTileStride) return fail(RQ_ERR_SHAPE, "n_kv * head_dim too large");
+  if (!(theta >= 0.0 && theta <= 1e30)) return fail(RQ_ERR_SHAPE, "theta must be positive, or 0 for no rotation");
+  return check_i32("table", g->table);
+}
+
+static PagesArgs pages_args(const rq_pages* g, int64_t n_q, int64_t batch, double theta) {
+  PagesArgs a = {};
+  a.kpages = g->kpages;
+  a.vpages = g->vpages;
+  a.pages = g->pages;
+  a.table = g->table;
+  a.table_stride = g->table_stride;
+  while (((int64_t)1 << a.page_bits) < g->page_size) a.page_bits++;
+  a.n_q = (int)n_q;
+  a.n_kv = (int)g->n_kv;
+  a.head_dim = (int)g->head_dim;
+  a.batch = (int)batch;
+  a.rope = theta > 0.0;
+  a.log2_theta = a.rope ? std::log2(theta) : 0.0;
+  return a;
+}
+
+}  // namespace rq
+
+extern "C" {
+
+int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
+                        void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_prompt(p)) return s;
+  if (p->batch == 0 || p->rows_q == 0) return RQ_OK;
+  const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
+  if (int s = check_i32("cu_q", p->cu_q)) return s;
+  if (p->cu_k)
+    if (int s = check_i32("cu_k", p->cu_k)) return s;
+  if (int s = check_rows("q", q, q_stride, qw, p->dtype)) return s;
+  if (p->rows_k > 0) {
+    if (int s = check_rows("k", k, k_stride, kw, p->dtype)) return s;
+    if (int s = check_rows("v", v, v_stride, kw, p->dtype)) return s;
+  }
+  if (int s = check_rows("out", out, out_stride, qw, p->dtype)) return s;
+  if (lse)
+    if (int s = check_i32("lse", lse)) return s;
+  if (int s = check_ctx(c)) return s;
+  if (int s = set_device(c)) return s;
+  PromptArgs a = prompt_args(p);
+  a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
+  a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
+  const hipError_t e = launch_prompt_fwd(p->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "prompt attention launch");
+  return RQ_OK;
+}
+
+int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes) {
+  if (int s = check_prompt(p)) return s;
+  if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
+  *bytes = (size_t)(p->n_q * p->rows_q) * sizeof(float);
+  return RQ_OK;
+}
+
+int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int64_t dout_stride, const void* q,
+                            int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            const void* out, int64_t out_stride, const float* lse, void* dq, int64_t dq_stride,
+                            void* dk, int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
+                            void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_prompt(p)) return s;
+  if (p->batch == 0 || (p->rows_q == 0 && p->rows_k == 0)) return RQ_OK;
+  const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
+  if (int s = check_i32("cu_q", p->cu_q)) return s;
+  if (p->cu_k)
+    if (int s = check_i32("cu_k", p->cu_k)) return s;
+  if (p->rows_q > 0) {
+    if (int s = check_rows("dout", dout, dout_stride, qw, p->dtype)) return s;
+    if (int s = check_rows("q", q, q_stride, qw, p->dtype)) return s;
+    if (int s = check_rows("out", out, out_stride, qw, p->dtype)) return s;
+    if (int s = check_rows("dq", dq, dq_stride, qw, p->dtype)) return s;
+    if (int s = check_i32("lse", lse)) return s;
+    if (!work) return fail(RQ_ERR_NULL, "work is NULL");
+    if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
+    if (work_bytes < (size_t)(p->n_q * p->rows_q) * sizeof(float))
+      return fail(RQ_ERR_SHAPE, "work is smaller than rq_prompt_attention_bwd_work says");
+  }
+  if (p->rows_k > 0) {
+    if (int s = check_rows("k", k, k_stride, kw, p->dtype)) return s;
+    if (int s = check_rows("v", v, v_stride, kw, p->dtype)) return s;
+    if (int s = check_rows("dk", dk, dk_stride, kw, p->dtype)) return s;
+    if (int s = check_rows("dv", dv, dv_stride, kw, p->dtype)) return s;
+  }
+  if (int s = check_ctx(c)) return s;
+  if (int s = set_device(c)) return s;
+  PromptArgs a = prompt_args(p);
+  a.q = q, a.k = k, a.v = v, a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
+  a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
+  a.dout_stride = dout_stride, a.dq_stride = dq_stride, a.dk_stride = dk_stride, a.dv_stride = dv_stride;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.delta = static_cast<float*>(work);
+  const hipError_t e = launch_prompt_bwd(p->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "prompt attention gradient launch");
+  return RQ_OK;
+}
+
+int rq_paged_attention_work(rq_ctx h, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
+                            size_t* bytes) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_heads(n_q, n_kv, head_dim)) return s;
+  if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
+  if (int s = check_ctx(c)) return s;
+  *bytes = batch == 0 ? 0 : plan_paged_attention(batch, n_q, n_kv, head_dim, max_len, c->cu_count).work;
+  return RQ_OK;
+}
+
+int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, int64_t q_stride, const void* k,
+                       int64_t k_stride, const void* v, int64_t v_stride, const int32_t* lens, int64_t batch,
+                       int64_t n_q, int64_t max_len, double theta, double scale, void* out, int64_t out_stride,
+                       void* work, size_t work_bytes, void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_pages(pg, dtype, n_q, theta)) return s;
+  if (int s = check_scale(scale)) return s;
+  if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (batch == 0) return RQ_OK;
+  const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
+  if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
+  if (!k != !v) return fail(RQ_ERR_NULL, "k and v must both be given, or neither");
+  if (k) {
+    if (int s = check_rows("k", k, k_stride, kw, dtype)) return s;
+    if (int s = check_rows("v", v, v_stride, kw, dtype)) return s;
+  }
+  if (int s = check_i32("lens", lens)) return s;
+  if (int s = check_rows("out", out, out_stride, qw, dtype)) return s;
+  if (int s = check_ctx(c)) return s;
+  const PagedPlan plan = plan_paged_attention(batch, n_q, pg->n_kv, pg->head_dim, max_len, c->cu_count);
+  if (plan.work > 0 && !work) return fail(RQ_ERR_NULL, "work is NULL");
+  if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
+  if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
+  const int64_t htiles = (n_q / pg->n_kv + 15) / 16;
+  if (plan.nsplit > INT32_MAX / (batch * pg->n_kv * htiles) || batch * n_q > INT32_MAX)
+    return fail(RQ_ERR_SHAPE, "batch times heads times rows too large for one launch");
+  if (int s = set_device(c)) return s;
+  PagedAttnArgs a = {};
+  a.p = pages_args(pg, n_q, batch, theta);
+  a.p.q = q, a.p.k = k, a.p.v = v;
+  a.p.q_stride = q_stride, a.p.k_stride = k_stride, a.p.v_stride = v_stride;
+  a.lens = lens;
+  a.max_len = max_len;
+  a.scale2 = (float)(scale * 1.4426950408889634);
+  a.out = out;
+  a.out_stride = out_stride;
+  a.split_rows = plan.split_rows;
+  a.nsplit = plan.nsplit;
+  a.part = static_cast<float*>(work);
+  const hipError_t e = launch_paged_attention(dtype, pg->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+  return RQ_OK;
+}
+
+int rq_pages_append(rq_ctx h, const rq_pages* pg, int dtype, const void* q, int64_t q_stride, const void* k,
+                    int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, const int32_t* past,
+                    int64_t batch, int64_t rows, int64_t n_q, double theta, void* q_out, int64_t q_out_stride,
+                    void* k_out, int64_t k_out_stride, void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_pages(pg, dtype, n_q, theta)) return s;
+  if (batch < 0 || batch > kMaxRows || rows < 0 || rows > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (batch == 0 || rows == 0) return RQ_OK;
+  const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
+  if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
+  if (int s = check_rows("k", k, k_stride, kw, dtype)) return s;
+  if (int s = check_rows("v", v, v_stride, kw, dtype)) return s;
+  if (int s = check_rows("q_out", q_out, q_out_stride, qw, dtype)) return s;
+  if (k_out)
+    if (int s = check_rows("k_out", k_out, k_out_stride, kw, dtype)) return s;
+  if (int s = check_i32("cu", cu)) return s;
+  if (int s = check_i32("past", past)) return s;
+  if (int s = check_ctx(c)) return s;
+  if (int s = set_device(c)) return s;
+  PagesAppendArgs a = {};
+  a.p = pages_args(pg, n_q, batch, theta);
+  a.p.q = q, a.p.k = k, a.p.v = v;
+  a.p.q_stride = q_stride, a.p.k_stride = k_stride, a.p.v_stride = v_stride;
+  a.cu = cu;
+  a.past = past;
+  a.rows = rows;
+  a.q_out = q_out, a.k_out = k_out;
+  a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
+  const hipError_t e = launch_pages_append(dtype, pg->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "pages append launch");
+  return RQ_OK;
+}
+
+int rq_pages_copy(rq_ctx h, void* base, int64_t planes, int64_t plane_bytes, int64_t pages, int64_t page_bytes,
+                  const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (planes < 0 || n < 0 || pages <= 0 || page_bytes <= 0) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (pages > INT32_MAX || page_bytes > (int64_t)1 << 30 || plane_bytes < 0 || plane_bytes / page_bytes < pages)
+    return fail(RQ_ERR_SHAPE, "a plane must hold its pages");
+  if (page_bytes % 16 != 0 || plane_bytes % 16 != 0)
+    return fail(RQ_ERR_SHAPE, "page_bytes and plane_bytes must be multiples of 16");
+  if (planes == 0 || n == 0) return RQ_OK;
+  if (!base || !src || !dst) return fail(RQ_ERR_NULL, "NULL argument");
+  if (((uintptr_t)base & 15) != 0) return fail(RQ_ERR_SHAPE, "base must be 16-byte aligned");
+  if (n > pages) return fail(RQ_ERR_SHAPE, "more copies than pages");
+  if (planes > (int64_t)1 << 20 || pages_copy_groups(page_bytes) * planes > INT32_MAX / 256)
+    return fail(RQ_ERR_SHAPE, "planes times page_bytes too large for one launch");
+  try {
+    std::vector<int32_t> d(dst, dst + n);
+    std::sort(d.begin(), d.end());
+    if (d.front() < 0 || d.back() >= pages) return fail(RQ_ERR_SHAPE, "dst page out of range");
+    if (std::adjacent_find(d.begin(), d.end()) != d.end()) return fail(RQ_ERR_SHAPE, "a page is a dst twice");
+    for (int64_t i = 0; i < n; i++) {
+      if (src[i] < 0 || src[i] >= pages) return fail(RQ_ERR_SHAPE, "src page out of range");
+      if (std::binary_search(d.begin(), d.end(), src[i])) return fail(RQ_ERR_SHAPE, "a page is both src and dst");
+    }
+  } catch (const std::exception&) {
+    return fail(RQ_ERR_OOM, "host allocation failed");
+  }
+  if (int s = check_ctx(c)) return s;
+  if (int s = set_device(c)) return s;
+  const hipError_t e =
+      launch_pages_copy(base, planes, plane_bytes, page_bytes, src, dst, n, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page copy launch");
+  return RQ_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,32 @@
+// prompt.h — arguments of the attention over packed prompts (prompt.hip, prompt_bwd.hip).
+#pragma once
+
+#include "rq_internal.h"
+
+namespace rq {
+
+// Rows are q, k, v, out rows of the packed batch; strides in elements.
+struct PromptArgs {
+  const int32_t *cu_q, *cu_k;
+  int64_t rows_q, rows_k, slots;
+  int batch, n_q, n_kv, head_dim, causal;
+  float scale, scale2;  // scale2 = scale log2 e
+  const void *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  void* out;
+  int64_t out_stride;
+  float* lse;  // [n_q][rows_q], natural logarithm, or NULL
+  // gradient only
+  const void* dout;
+  int64_t dout_stride;
+  void *dq, *dk, *dv;
+  int64_t dq_stride, dk_stride, dv_stride;
+  float* delta;  // [n_q][rows_q]: dout . out
+};
+
+hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream);
+hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream);
+// Lets a kernel take `bytes` of dynamic LDS on the current device.
+hipError_t allow_lds(const void* kernel, int bytes);
+
+}  // namespace rq

@@ -1,0 +1,301 @@
+// prompt_bwd.hip — gradient of the attention over packed prompts (prompt.hip).
+//
+// With P the forward's weights, recomputed as exp(s - L) from its log-sum-exp L:
+//   D_i  = dO_i . O_i
+//   dV_j = sum_i p_ij dO_i
+//   dS_ij = p_ij (dO_i . V_j - D_i)
+//   dQ_i = scale sum_j dS_ij K_j      dK_j = scale sum_i dS_ij Q_i
+// the sums over i of dK and dV also over the query heads of the KV head.
+//
+// Three kernels, none with an atomic, so results do not depend on scheduling: D; dK
+// and dV (a wave owns 32 keys and walks the queries of every head of its group); dQ
+// (a wave owns 32 queries and walks the keys). The scores and dO V^T are formed
+// in both of the last two: 7 products for the 5 that a single kernel would need, which
+// would have to add dQ from many workgroups.
+#include <algorithm>
+#include <cmath>
+
+#include "attn_tile.h"
+#include "prompt.h"
+
+namespace rq {
+
+namespace {
+
+// L in base 2; +inf, which makes every weight 0, where no key had one (L = -inf)
+__device__ __forceinline__ float base2_lse(float lse) {
+  return lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+}
+
+// D of a row and head: LANES lanes a (row, head), 16 bytes each at a time.
+constexpr int kDeltaLanes = 16;
+template <typename T>
+__global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
+  constexpr int E = TileType<T>::kPiece;
+  typedef T TE __attribute__((ext_vector_type(E)));
+  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kDeltaLanes;
+  const int sub = threadIdx.x % kDeltaLanes;
+  if (id >= a.rows_q * a.n_q) return;
+  const int64_t row = id / a.n_q;
+  const int hq = (int)(id % a.n_q);
+  const T* o = static_cast<const T*>(a.out) + row * a.out_stride + hq * a.head_dim;
+  const T* d = static_cast<const T*>(a.dout) + row * a.dout_stride + hq * a.head_dim;
+  float sum = 0.0f;
+  for (int e = sub * E; e < a.head_dim; e += kDeltaLanes * E) {
+    const TE x = *reinterpret_cast<const TE*>(o + e), y = *reinterpret_cast<const TE*>(d + e);
+#pragma unroll
+    for (int j = 0; j < E; j++) sum += (float)x[j] * (float)y[j];
+  }
+#pragma unroll
+  for (int k = kDeltaLanes / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
+  if (sub == 0) a.delta[(int64_t)hq * a.rows_q + row] = sum;
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[HD / 32], float f, int h, int hd) {
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int e = 32 * d + 2 * i + 4 * h;
+      if (e >= hd) continue;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 y;
+#pragma unroll
+      for (int j = 0; j < 4; j++) y[j] = (T)(acc[d][i + j] * f);
+      *reinterpret_cast<T4*>(row + e) = y;
+    }
+}
+
+// dK and dV: NW waves of 32 keys each, query tiles of 32 rows through LDS.
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void prompt_dkv_kernel(PromptArgs a) {
+  using TL = Tile<T, HD>;
+  using Frag = typename TL::Frag;
+  constexpr int THREADS = NW * 64, BKV = NW * 32, BQ = 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kTile = TL::bytes(BQ);
+  constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
+  const int group = a.n_q / a.n_kv;
+  const int hkv = blockIdx.x % a.n_kv;
+  const int64_t slot = blockIdx.x / a.n_kv;  // a sequence's first keys, which most queries see, first
+  const TileSpan tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, BKV, slot);
+  if (tk.len == 0) return;
+  const int64_t q0 = clamp_cu(a.cu_q, tk.seq, a.rows_q), q1 = clamp_cu(a.cu_q, tk.seq + 1, a.rows_q);
+  const int lq = (int)(q1 > q0 ? q1 - q0 : 0), off = tk.len - lq;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w_key = tk.row0 + wave * 32, kj = w_key + (lane & 31);
+  const bool live = kj < tk.len;
+
+  const T* krow = live ? static_cast<const T*>(a.k) + (tk.begin + kj) * a.k_stride + hkv * a.head_dim : nullptr;
+  const T* vrow = live ? static_cast<const T*>(a.v) + (tk.begin + kj) * a.v_stride + hkv * a.head_dim : nullptr;
+  Frag kf[HD / 16], vf[HD / 16];
+#pragma unroll
+  for (int s = 0; s < HD / 16; s++) {
+    kf[s] = TL::frag_global(krow, s, h, a.head_dim);
+    vf[s] = TL::frag_global(vrow, s, h, a.head_dim);
+  }
+  f32x16 dk[HD / 32], dv[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++) dk[d] = dv[d] = f32x16{};
+
+  // the first query that sees the tile's first key, down to a whole query tile
+  const int qstart = a.causal ? max(tk.row0 - off, 0) / BQ * BQ : 0;
+  const int per_head = lq > qstart ? (lq - qstart + BQ - 1) / BQ : 0, steps = per_head * group;
+  Stage<T, HD, BQ, THREADS> qs, os;
+  float rowv = 0.0f;  // L (threads 0 .. 31) or D (32 .. 63) of the next tile's rows
+  auto load = [&](int step) {
+    const int hq = hkv * group + step / per_head, r = qstart + step % per_head * BQ;
+    qs.load(static_cast<const T*>(a.q) + (q0 + r) * a.q_stride + hq * a.head_dim, a.q_stride, lq - r, a.head_dim, tid);
+    os.load(static_cast<const T*>(a.dout) + (q0 + r) * a.dout_stride + hq * a.head_dim, a.dout_stride, lq - r,
+            a.head_dim, tid);
+    if (tid < 2 * BQ) {
+      const int64_t at = (int64_t)hq * a.rows_q + q0 + min(r + (tid & (BQ - 1)), lq - 1);
+      rowv = tid < BQ ? base2_lse(a.lse[at]) : a.delta[at];
+    }
+  };
+  auto store = [&](char* b) {
+    qs.store(b, tid);
+    os.store(b + kTile, tid);
+    if (tid < 2 * BQ) reinterpret_cast<float*>(b + 2 * kTile)[tid] = rowv;
+  };
+  if (steps > 0) {
+    load(0);
+    store(lds);
+  }
+  for (int step = 0; step < steps; step++) {
+    const char* qt = lds + (step & 1) * kBuf;
+    const char* ot = qt + kTile;
+    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
+    if (step + 1 < steps) load(step + 1);
+    __syncthreads();
+    const int r = qstart + step % per_head * BQ;
+    if (!a.causal || r + BQ - 1 + off >= w_key) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(qt, lane & 31, d, h), kf[d], s);
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(ot, lane & 31, d, h), vf[d], dp);
+      // value i: query r + 8 (i / 4) + 4 h + i % 4, the lane's key
+      float p[16], ds[16];
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(rows + 8 * g + 4 * h);
+        const f32x4 del = *reinterpret_cast<const f32x4*>(rows + BQ + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int i = 4 * g + j, qi = r + 8 * g + 4 * h + j;
+          const bool see = qi < lq && live && (!a.causal || kj <= qi + off);
+          p[i] = see ? __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse[j])) : 0.0f;
+          ds[i] = see ? p[i] * (dp[i] - del[j]) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        Frag pf, sf;  // bf16: weights and their gradients rounded to nearest for the products
+        tile_pack(p + 8 * u, pf);
+        tile_pack(ds + 8 * u, sf);
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) {
+          dv[d] = tile_mma(TL::frag_t(ot, 16 * u, d, lane), pf, dv[d]);
+          dk[d] = tile_mma(TL::frag_t(qt, 16 * u, d, lane), sf, dk[d]);
+        }
+      }
+    }
+    if (step + 1 < steps) store(lds + ((step + 1) & 1) * kBuf);
+  }
+  if (!live) return;
+  store_rows<T, HD>(static_cast<T*>(a.dk) + (tk.begin + kj) * a.dk_stride + hkv * a.head_dim, dk, a.scale, h,
+                    a.head_dim);
+  store_rows<T, HD>(static_cast<T*>(a.dv) + (tk.begin + kj) * a.dv_stride + hkv * a.head_dim, dv, 1.0f, h,
+                    a.head_dim);
+}
+
+// dQ: NW waves of 32 queries each, key tiles of 32 rows through LDS.
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void prompt_dq_kernel(PromptArgs a) {
+  using TL = Tile<T, HD>;
+  using Frag = typename TL::Frag;
+  constexpr int THREADS = NW * 64, BQ = NW * 32, BK = 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kTile = TL::bytes(BK);
+  const int group = a.n_q / a.n_kv;
+  const int hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, hq = hkv * group + rest % group;
+  const int64_t slot = a.slots - 1 - rest / group;
+  const TileSpan tq = tile_of_slot(a.cu_q, a.batch, a.rows_q, BQ, slot);
+  if (tq.len == 0) return;
+  const int64_t k0 = clamp_cu(a.cu_k, tq.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tq.seq + 1, a.rows_k);
+  const int lk = (int)(k1 > k0 ? k1 - k0 : 0), off = lk - tq.len;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w_row = tq.row0 + wave * 32, qi = w_row + (lane & 31);
+  const bool live = qi < tq.len;
+  const int q_last = min(tq.row0 + BQ, tq.len) - 1;
+  const int nk = a.causal ? min(max(q_last + off + 1, 0), lk) : lk;
+
+  const T* kbase = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
+  const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
+  Stage<T, HD, BK, THREADS> ks, vs;
+  if (nk > 0) {
+    ks.load(kbase, a.k_stride, lk, a.head_dim, tid);
+    vs.load(vbase, a.v_stride, lk, a.head_dim, tid);
+  }
+  const T* qrow = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;
+  const T* orow = live ? static_cast<const T*>(a.dout) + (tq.begin + qi) * a.dout_stride + hq * a.head_dim : nullptr;
+  Frag qf[HD / 16], of[HD / 16];
+#pragma unroll
+  for (int s = 0; s < HD / 16; s++) {
+    qf[s] = TL::frag_global(qrow, s, h, a.head_dim);
+    of[s] = TL::frag_global(orow, s, h, a.head_dim);
+  }
+  const int64_t at = (int64_t)hq * a.rows_q + tq.begin + min(qi, tq.len - 1);
+  const float lse = base2_lse(a.lse[at]), del = a.delta[at];
+  f32x16 dq[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++) dq[d] = f32x16{};
+  if (nk > 0) {
+    ks.store(lds, tid);
+    vs.store(lds + kTile, tid);
+  }
+  const int see = !live ? -1 : a.causal ? min(lk - 1, qi + off) : lk - 1;
+  for (int kb = 0, buf = 0; kb < nk; kb += BK, buf ^= 1) {
+    const char* kt = lds + buf * 2 * kTile;
+    const char* vt = kt + kTile;
+    const bool more = kb + BK < nk;
+    if (more) {
+      ks.load(kbase + (int64_t)(kb + BK) * a.k_stride, a.k_stride, lk - kb - BK, a.head_dim, tid);
+      vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
+    }
+    __syncthreads();
+    if (!a.causal || kb <= w_row + 31 + off) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, lane & 31, d, h), qf[d], s);
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, lane & 31, d, h), of[d], dp);
+      float ds[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const bool in = kb + 8 * (i >> 2) + 4 * h + (i & 3) <= see;
+        ds[i] = in ? __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse)) * (dp[i] - del) : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        Frag sf;
+        tile_pack(ds + 8 * u, sf);
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 16 * u, d, lane), sf, dq[d]);
+      }
+    }
+    if (more) {
+      char* next = lds + (buf ^ 1) * 2 * kTile;
+      ks.store(next, tid);
+      vs.store(next + kTile, tid);
+    }
+  }
+  if (live)
+    store_rows<T, HD>(static_cast<T*>(a.dq) + (tq.begin + qi) * a.dq_stride + hq * a.head_dim, dq, a.scale, h,
+                      a.head_dim);
+}
+
+template <typename T, int HD, int NW>
+hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
+  if (a.rows_q > 0) {
+    const int64_t n = a.rows_q * a.n_q * kDeltaLanes;
+    hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (a.rows_k > 0) {
+    constexpr int lds = 2 * (2 * Tile<T, HD>::bytes(32) + 2 * 32 * 4);
+    a.slots = tile_slots(a.rows_k, a.batch, NW * 32);
+    const auto kernel = prompt_dkv_kernel<T, HD, NW>;
+    if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_kv)), dim3(NW * 64), lds, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (a.rows_q > 0) {
+    constexpr int lds = 4 * Tile<T, HD>::bytes(32);
+    a.slots = tile_slots(a.rows_q, a.batch, NW * 32);
+    const auto kernel = prompt_dq_kernel<T, HD, NW>;
+    if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(NW * 64), lds, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+  if (dtype == RQ_BF16) {
+    if (a.head_dim <= 64) return run_bwd<__bf16, 64, 4>(a, stream);
+    if (a.head_dim <= 128) return run_bwd<__bf16, 128, 4>(a, stream);
+    return run_bwd<__bf16, 256, 4>(a, stream);
+  }
+  if (a.head_dim <= 64) return run_bwd<float, 64, 4>(a, stream);
+  if (a.head_dim <= 128) return run_bwd<float, 128, 4>(a, stream);
+  return run_bwd<float, 256, 4>(a, stream);
+}
+
+}  // namespace rq

@@ -1,0 +1,277 @@
+"""rq_paged_attention, rq_pages_append and rq_pages_copy against 64 bits
+(attn_ref.py states the tolerances)."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+THETA = 1e4
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+
+    if not t.cuda.is_available():
+        pytest.skip("no GPU")
+    return t
+
+
+@pytest.fixture(scope="module")
+def ctx(torch):
+    import raster_amd
+
+    c = raster_amd.Context(0)
+    yield c
+    c.close()
+
+
+def make(torch, seed, act, cache, nq, nkv, hd, need, page, rows):
+    """A cache for sequences of `need` rows in shuffled pages (NaN where nothing is
+    stored yet), and `rows` rows of q, k, v as columns of one array."""
+    ty = {"f32": torch.float32, "bf16": torch.bfloat16}
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = [-(-n // page) for n in need]
+    total = sum(pages) + 2
+    ids = torch.randperm(total, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(need), max(pages) + 1), 2 ** 30, dtype=torch.int32)
+    for b, n in enumerate(pages):
+        table[b, :n] = torch.tensor([ids.pop() for _ in range(n)], dtype=torch.int32)
+    kp, vp = (torch.full((total, page, nkv * hd), float("nan"), dtype=ty[cache], device="cuda") for _ in range(2))
+    qkv = torch.randn((rows, (nq + 2 * nkv) * hd), generator=g, device="cuda").to(ty[act])
+    return g, table.cuda(), kp, vp, qkv.split([nq * hd, nkv * hd, nkv * hd], 1)
+
+
+def fill(torch, g, kp, vp, table, lens):
+    page = kp.shape[1]
+    for b, n in enumerate(lens):
+        for i in range(0, max(n, 0), page):
+            m = min(page, n - i)
+            for p in (kp, vp):
+                p[int(table[b, i // page]), :m] = torch.randn((m, p.shape[2]), generator=g, device="cuda").to(p.dtype)
+
+
+def gather(p, table, b, n):
+    return p[table[b, :-(-n // p.shape[1])].long()].reshape(-1, p.shape[2])[:n]
+
+
+# activations, pages, heads, KV heads, head_dim, page, cached rows
+CASES = [
+    ("f32", "f32", 4, 4, 128, 16, [0]),
+    ("f32", "f32", 16, 16, 128, 16, [128, 0, 31, 32, 33]),
+    ("f32", "f32", 8, 2, 64, 32, [7, 700, 255, 256, 257]),
+    ("f32", "f32", 6, 2, 40, 16, [100, 3]),
+    ("f32", "f32", 4, 1, 256, 16, [300, 40]),
+    ("f32", "f32", 2, 2, 136, 16, [77]),
+    ("f32", "bf16", 8, 2, 128, 16, [0, 1, 15, 16, 17, 513]),
+    ("f32", "bf16", 4, 4, 64, 64, [1000]),
+    ("f32", "bf16", 8, 4, 256, 16, [130]),
+    ("f32", "bf16", 2, 1, 200, 32, [130, 4]),
+    ("f32", "bf16", 5, 1, 8, 16, [130, 4]),
+    ("bf16", "bf16", 32, 8, 128, 16, [2500, 77, 0, 1024]),
+    ("bf16", "bf16", 64, 2, 64, 128, [300, 5000]),  # 32 heads a KV head: two head tiles
+    ("bf16", "bf16", 17, 1, 128, 16, [40]),
+    ("bf16", "bf16", 3, 3, 80, 16, [90, 12]),
+    ("bf16", "bf16", 2, 1, 248, 16, [400]),
+]
+
+
+@pytest.mark.parametrize("act,cache,nq,nkv,hd,page,lens", CASES)
+@pytest.mark.parametrize("mode", ["append", "read", "no_rope"])
+def test_paged_attention(torch, ctx, act, cache, nq, nkv, hd, page, lens, mode):
+    import attn_ref as ref
+    import raster_amd
+
+    print(f"[gpu] paged {act}/{cache} {nq}/{nkv}x{hd} page={page} {lens} {mode}", flush=True)
+    add = mode != "read"
+    lens = lens + [-1]  # an idle slot
+    n = len(lens)
+    g, table, kp, vp, (q, k, v) = make(torch, hd + sum(lens), act, cache, nq, nkv, hd, [x + 1 for x in lens], page, n)
+    fill(torch, g, kp, vp, table, lens)
+    k0, v0 = kp.clone(), vp.clone()
+    theta, scale = 0.0 if mode == "no_rope" else THETA, hd ** -0.5
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = raster_amd.paged_attention(ctx, q, k if add else None, v if add else None, kp, vp, table, lt, nq, nkv, hd,
+                                     theta, scale, max_len=max(lens) + 1)
+    pos = torch.tensor(lens, device="cuda")
+    rq, rk = (ref.rope(x.double().view(n, -1, hd), pos, THETA) if theta else x.double().view(n, -1, hd)
+              for x in (q, k))
+    half, hq = ref.HALF[q.dtype], 2.0 ** -8 if act == "bf16" else 2.0 ** -22
+    for b, m in enumerate(lens):
+        if m < 0:
+            assert bool((out[b] == 0).all())
+            continue
+        if add:  # the new row: rotated in f32 (two products and their sum), rounded once
+            page_id, r = int(table[b, m // page]), m % page
+            got = kp[page_id, r].double().view(nkv, hd)
+            tol = (ref.HALF[kp.dtype] + 2.0 ** -21) * (rk[b].abs() + 1)
+            assert bool(((got - rk[b]).abs() <= tol).all())
+            assert torch.equal(vp[page_id, r], v[b].to(vp.dtype))
+            k0[page_id, r], v0[page_id, r] = kp[page_id, r], vp[page_id, r]
+        if m + add == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        keys, values = (gather(p, table, b, m + add).double().view(-1, nkv, hd) for p in (kp, vp))
+        see = torch.ones((1, m + add), dtype=torch.bool, device="cuda")
+        for h in range(nq):
+            j = h // (nq // nkv)
+            want, _, bound = ref.attend(rq[b, h:h + 1], keys[:, j], values[:, j], scale, see, half, hq)
+            got = out[b, h * hd:(h + 1) * hd].double()
+            assert bool(((got - want[0]).abs() <= bound[0]).all()), (b, h, float(((got - want[0]).abs() / bound).max()))
+    # nothing else was written
+    assert torch.equal(kp.nan_to_num(7.0), k0.nan_to_num(7.0)) and torch.equal(vp.nan_to_num(7.0), v0.nan_to_num(7.0))
+
+
+def test_any_split_gives_the_same_within_rounding(torch, ctx):
+    """max_len only sizes the split: a larger one changes sums' order, nothing else."""
+    import raster_amd
+
+    nq, nkv, hd, lens = 8, 2, 128, [700, 3000, 9]
+    print("[gpu] paged max_len", flush=True)
+    g, table, kp, vp, (q, _, _) = make(torch, 3, "f32", "f32", nq, nkv, hd, lens, 16, 3)
+    fill(torch, g, kp, vp, table, lens)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    outs = [raster_amd.paged_attention(ctx, q, None, None, kp, vp, table, lt, nq, nkv, hd, THETA, hd ** -0.5, max_len=m)
+            for m in (3000, 50000, 10 ** 6)]
+    for o in outs[1:]:
+        assert float((o - outs[0]).abs().max()) <= 1e-5 * float(outs[0].abs().max())
+    again = raster_amd.paged_attention(ctx, q, None, None, kp, vp, table, lt, nq, nkv, hd, THETA, hd ** -0.5,
+                                       max_len=3000)
+    assert torch.equal(again, outs[0])
+
+
+def test_bad_pages_and_lengths(torch, ctx):
+    """Page numbers outside the cache and sequences past max_len or their table: NaN, the
+    other sequences as ever, nothing written."""
+    import raster_amd
+
+    nq, nkv, hd, lens = 4, 2, 64, [40, 50, 60, 70]
+    print("[gpu] paged bad pages", flush=True)
+    g, table, kp, vp, (q, k, v) = make(torch, 5, "f32", "f32", nq, nkv, hd, [n + 1 for n in lens], 16, 4)
+    fill(torch, g, kp, vp, table, lens)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    args = (nq, nkv, hd, THETA, hd ** -0.5)
+    good = raster_amd.paged_attention(ctx, q, k, v, kp.clone(), vp.clone(), table, lt, *args)
+    bad = table.clone()
+    bad[0, 1] = kp.shape[0]      # read
+    bad[1, 3] = -1               # appended (row 50 is in page 3)
+    far = lt.clone()
+    far[3] = 10 ** 6             # past the table
+    k1, v1 = kp.clone(), vp.clone()
+    out = raster_amd.paged_attention(ctx, q, k, v, k1, v1, bad, far, *args)
+    for b in (0, 1, 3):
+        assert bool(torch.isnan(out[b]).all())
+    assert torch.equal(out[2], good[2])
+    wrote = [(int(table[b, lens[b] // 16]), lens[b] % 16) for b in (0, 2)]
+    for p, was in ((k1, kp), (v1, vp)):
+        same = (p.nan_to_num(7.0) == was.nan_to_num(7.0)).all(-1)
+        for at in wrote:
+            same[at] = True
+        assert bool(same.all())
+    out = raster_amd.paged_attention(ctx, q, k, v, kp.clone(), vp.clone(), table, lt, *args, max_len=61)
+    assert torch.equal(out[:3], good[:3]) and bool(torch.isnan(out[3]).all())
+
+
+@pytest.mark.parametrize("act,cache,nq,nkv,hd,page,lens,past", [
+    ("f32", "f32", 4, 2, 128, 16, [37, 0, 1, 16], [0, 5, 15, 1000]),
+    ("f32", "bf16", 3, 1, 40, 32, [33, 2], [31, 100000]),
+    ("bf16", "bf16", 32, 8, 128, 16, [300, 1, 77], [0, 128, 5]),
+    ("bf16", "bf16", 2, 2, 8, 16, [5], [3]),
+    ("bf16", "bf16", 2, 1, 256, 64, [70], [0]),
+])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append(torch, ctx, act, cache, nq, nkv, hd, page, lens, past, in_place):
+    import attn_ref as ref
+    import raster_amd
+
+    print(f"[gpu] append {act}/{cache} {nq}/{nkv}x{hd} {lens} {past}", flush=True)
+    n, tail = sum(lens), 3
+    lens2, past2 = lens + [2], past + [-1]  # a sequence left out, and rows of none behind it
+    _, table, kp, vp, (q, k, v) = make(torch, n, act, cache, nq, nkv, hd,
+                                       [a + b for a, b in zip(lens, past)] + [1], page, n + 2 + tail)
+    cu = torch.tensor([sum(lens2[:i]) for i in range(len(lens2) + 1)], dtype=torch.int32, device="cuda")
+    pt = torch.tensor(past2, dtype=torch.int32, device="cuda")
+    q0, k0, v0 = q.clone(), k.clone(), v.clone()
+    qo, ko = (q, k) if in_place else (torch.full_like(q, 7.0), torch.full_like(k, 7.0))
+    raster_amd.pages_append(ctx, q, k, v, kp, vp, table, cu, pt, nq, nkv, hd, THETA, q_out=qo, k_out=ko)
+    seen = torch.zeros(kp.shape[:2], dtype=torch.bool, device="cuda")
+    at = 0
+    for b, (m, p0) in enumerate(zip(lens, past)):
+        if m == 0:
+            continue
+        pos = torch.arange(p0, p0 + m, device="cuda")
+        wq, wk = (ref.rope(x[at:at + m].double().view(m, -1, hd), pos, THETA).view(m, -1) for x in (q0, k0))
+        for got, want in ((qo[at:at + m], wq), (ko[at:at + m], wk)):
+            tol = (ref.HALF[got.dtype] + 2.0 ** -21) * (want.abs() + 1)
+            assert bool(((got.double() - want).abs() <= tol).all())
+        pages, r = table[b].long()[pos // page], pos % page
+        stored = kp[pages, r].double()
+        assert bool(((stored - wk).abs() <= (ref.HALF[kp.dtype] + 2.0 ** -21) * (wk.abs() + 1)).all())
+        assert torch.equal(vp[pages, r], v0[at:at + m].to(vp.dtype))
+        seen[pages, r] = True
+        at += m
+    assert torch.equal(qo[n:], q0[n:] if in_place else torch.full_like(qo[n:], 7.0))
+    assert torch.equal(ko[n:], k0[n:] if in_place else torch.full_like(ko[n:], 7.0))
+    assert torch.equal(v, v0) and bool(torch.isnan(kp[~seen]).all()) and bool(torch.isnan(vp[~seen]).all())
+
+
+def test_append_without_a_page(torch, ctx):
+    import raster_amd
+
+    print("[gpu] append without a page", flush=True)
+    _, table, kp, vp, (q, k, v) = make(torch, 1, "f32", "f32", 2, 2, 64, [40], 16, 70)
+    table[0, 1] = 10 ** 6
+    cu = torch.tensor([0, 70], dtype=torch.int32, device="cuda")
+    past = torch.zeros(1, dtype=torch.int32, device="cuda")
+    qo, ko = raster_amd.pages_append(ctx, q, k, v, kp, vp, table, cu, past, 2, 2, 64, THETA)
+    lost = torch.zeros(70, dtype=torch.bool, device="cuda")
+    lost[16:32] = lost[48:] = True  # the bad page, and what the table (4 pages) does not reach or has none for
+    ok = ~lost
+    assert bool(torch.isnan(qo[lost]).all()) and bool(torch.isnan(ko[lost]).all())
+    assert bool(torch.isfinite(qo[ok]).all()) and int(torch.isfinite(kp).all(-1).sum()) == int(ok.sum())
+
+
+@pytest.mark.parametrize("planes,pages,page,width,n", [(1, 2, 16, 8, 1), (6, 40, 16, 72, 17), (4, 700, 16, 64, 300),
+                                                       (3, 10, 16, 1032, 5)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_copy(torch, ctx, planes, pages, page, width, n, t):
+    import raster_amd
+
+    print(f"[gpu] copy {planes}x{pages}x{page}x{width} {n} {t}", flush=True)
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16}[t]
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn((planes, pages, page, width), generator=g, device="cuda").to(dt)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(n)).tolist()
+    src, dst = order[:n], order[n:2 * n]
+    if n > 2:
+        src[1] = src[0]  # one page to two places
+    want = x.clone()
+    want[:, dst] = x[:, src]
+    raster_amd.pages_copy(ctx, x, src, dst)
+    assert torch.equal(x, want)
+
+
+def test_graphs(torch, ctx):
+    """Append, attention and copy captured, replayed on another stream between eager work."""
+    import raster_amd
+
+    nq, nkv, hd, lens = 8, 2, 128, [300, 2000]
+    print("[gpu] paged graphs", flush=True)
+    g, table, kp, vp, (q, k, v) = make(torch, 8, "bf16", "bf16", nq, nkv, hd, [n + 1 for n in lens], 16, 2)
+    fill(torch, g, kp, vp, table, lens)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def call():
+        return raster_amd.paged_attention(ctx, q, k, v, kp, vp, table, lt, nq, nkv, hd, THETA, hd ** -0.5, max_len=2001)
+
+    want = call().clone()
+    torch.cuda.synchronize()
+    gr, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(gr, stream=s):
+        out = call()
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(other):
+            gr.replay()
+        again = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(again, want)
