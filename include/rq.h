@@ -549,8 +549,8 @@ int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q
  * over the query heads of a KV head; none may overlap an input). p_ij is
  * recomputed from lse. f32: in f32; bf16: products of bf16 with p and its gradient
  * rounded to bf16, sums in f32. work: rq_prompt_attention_bwd_work bytes of
- * device memory (f32[n_q][rows_q], the rows' dout . out), 16-byte aligned, used by this call alone
- * until it has run. */
+ * device memory (the rows' dout . out, and partial sums where few keys leave
+ * compute units idle), 16-byte aligned, used by this call alone until it has run. */
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes);
 int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, int64_t dout_stride, const void* q,
                             int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,

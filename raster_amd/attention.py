@@ -104,15 +104,17 @@ def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_
     os = _rows(out, ctx, qw, "out", q.dtype, rows)
     _need(lse.is_cuda and lse.get_device() == ctx.device and lse.dtype == torch.float32 and lse.is_contiguous()
           and lse.numel() == n_q * rows, "lse must be the forward's f32 CUDA tensor [n_q, rows]")
+    need = C.c_size_t()
+    call("rq_prompt_attention_bwd_work", C.byref(p), C.byref(need))
     raw, scope = _on(stream, q)
     new = [((rows, qw), q.dtype)] * (dq is None) + [((rows_k, kw), q.dtype)] * ((dk is None) + (dv is None))
-    work, *made = _empty(scope, ((n_q * rows,), torch.float32), *new, device=q.device)
+    work, *made = _empty(scope, ((need.value // 4,), torch.float32), *new, device=q.device)
     dq, dk, dv = (made.pop(0) if t is None else t for t in (dq, dk, dv))
     dqs = _rows(dq, ctx, qw, "dq", q.dtype, rows)
     dks, dvs = (_rows(t, ctx, kw, n, q.dtype, rows_k) for t, n in ((dk, "dk"), (dv, "dv")))
     call("rq_prompt_attention_bwd", ctx.handle, C.byref(p), dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
          v.data_ptr(), vs, out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(),
-         dvs, work.data_ptr(), work.numel() * 4, raw)
+         dvs, work.data_ptr(), need.value, raw)
     return dq, dk, dv
 
 

@@ -1581,7 +1581,7 @@ int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_s
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes) {
   if (int s = check_prompt(p)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
-  *bytes = (size_t)(p->n_q * p->rows_q) * sizeof(float);
+  *bytes = plan_prompt_bwd(p->batch, p->rows_q, p->rows_k, p->n_q, p->n_kv, p->head_dim).work;
   return RQ_OK;
 }
 
@@ -1594,19 +1594,19 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
   if (int s = check_prompt(p)) return s;
   if (p->batch == 0 || (p->rows_q == 0 && p->rows_k == 0)) return RQ_OK;
   const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
+  const PromptBwdPlan plan = plan_prompt_bwd(p->batch, p->rows_q, p->rows_k, p->n_q, p->n_kv, p->head_dim);
   if (int s = check_i32("cu_q", p->cu_q)) return s;
   if (p->cu_k)
     if (int s = check_i32("cu_k", p->cu_k)) return s;
+  if (!work && plan.work > 0) return fail(RQ_ERR_NULL, "work is NULL");
+  if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
+  if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_prompt_attention_bwd_work says");
   if (p->rows_q > 0) {
     if (int s = check_rows("dout", dout, dout_stride, qw, p->dtype)) return s;
     if (int s = check_rows("q", q, q_stride, qw, p->dtype)) return s;
     if (int s = check_rows("out", out, out_stride, qw, p->dtype)) return s;
     if (int s = check_rows("dq", dq, dq_stride, qw, p->dtype)) return s;
     if (int s = check_i32("lse", lse)) return s;
-    if (!work) return fail(RQ_ERR_NULL, "work is NULL");
-    if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
-    if (work_bytes < (size_t)(p->n_q * p->rows_q) * sizeof(float))
-      return fail(RQ_ERR_SHAPE, "work is smaller than rq_prompt_attention_bwd_work says");
   }
   if (p->rows_k > 0) {
     if (int s = check_rows("k", k, k_stride, kw, p->dtype)) return s;
@@ -1621,6 +1621,8 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
   a.dout_stride = dout_stride, a.dq_stride = dq_stride, a.dk_stride = dk_stride, a.dv_stride = dv_stride;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = static_cast<float*>(work);
+  a.nsplit = plan.nsplit;
+  a.part = reinterpret_cast<float*>(static_cast<char*>(work) + plan.delta_bytes);
   const hipError_t e = launch_prompt_bwd(p->dtype, a, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "prompt attention gradient launch");
   return RQ_OK;

@@ -22,7 +22,16 @@ struct PromptArgs {
   void *dq, *dk, *dv;
   int64_t dq_stride, dk_stride, dv_stride;
   float* delta;  // [n_q][rows_q]: dout . out
+  float* part;   // [nsplit][dv, dk][rows_k][n_kv * head_dim] when nsplit > 1
+  int nsplit;
 };
+
+struct PromptBwdPlan {
+  int nsplit;
+  size_t delta_bytes, work;
+};
+PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,
+                              int64_t head_dim);
 
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream);
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream);

@@ -67,42 +67,56 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[HD / 32],
     }
 }
 
-// dK and dV: NW waves of 32 keys each, query tiles of 32 rows through LDS.
-template <typename T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void prompt_dkv_kernel(PromptArgs a) {
+// dK and dV of 64 keys: query tiles of 32 rows through LDS, two waves for each 32
+// keys. One holds K and dV: it forms S = Q K^T and P, and adds dO^T P to dV; the
+// other holds V and dK: it forms dO V^T meanwhile, takes P over through LDS and adds
+// Q^T dS to dK. So a wave needs the registers of one operand and one result only
+// (two to three waves a SIMD instead of one), and both do the same two products in
+// each half of a step.
+//
+// The steps, (query head of the group, query tile), of a workgroup are one of nsplit parts;
+// with more than one the parts' f32 sums go to a.part and prompt_dkv_sum_kernel adds them in
+// order.
+constexpr int kDkvKeys = 64, kDkvQueries = 32;
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void prompt_dkv_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
-  constexpr int THREADS = NW * 64, BKV = NW * 32, BQ = 32;
+  constexpr int THREADS = 256, BQ = kDkvQueries;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   constexpr int kTile = TL::bytes(BQ);
   constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
+  constexpr int kPair = 2 * 64 * (int)sizeof(Frag);  // the weights of 32 keys and queries
   const int group = a.n_q / a.n_kv;
-  const int hkv = blockIdx.x % a.n_kv;
-  const int64_t slot = blockIdx.x / a.n_kv;  // a sequence's first keys, which most queries see, first
-  const TileSpan tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, BKV, slot);
+  const int hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, split = rest % a.nsplit;
+  const int64_t slot = rest / a.nsplit;  // a sequence's first keys, which most queries see, first
+  const TileSpan tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, kDkvKeys, slot);
   if (tk.len == 0) return;
   const int64_t q0 = clamp_cu(a.cu_q, tk.seq, a.rows_q), q1 = clamp_cu(a.cu_q, tk.seq + 1, a.rows_q);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), off = tk.len - lq;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int w_key = tk.row0 + wave * 32, kj = w_key + (lane & 31);
+  const bool is_k = wave & 1;  // this wave forms dK
+  const int w_key = tk.row0 + (wave >> 1) * 32, kj = w_key + (lane & 31);
   const bool live = kj < tk.len;
+  char* pair = lds + 2 * kBuf + (wave >> 1) * kPair + lane * 16;
 
-  const T* krow = live ? static_cast<const T*>(a.k) + (tk.begin + kj) * a.k_stride + hkv * a.head_dim : nullptr;
-  const T* vrow = live ? static_cast<const T*>(a.v) + (tk.begin + kj) * a.v_stride + hkv * a.head_dim : nullptr;
-  Frag kf[HD / 16], vf[HD / 16];
+  const T* src = static_cast<const T*>(is_k ? a.v : a.k);
+  const int64_t src_stride = is_k ? a.v_stride : a.k_stride;
+  const T* row = live ? src + (tk.begin + kj) * src_stride + hkv * a.head_dim : nullptr;
+  Frag f[HD / 16];
 #pragma unroll
-  for (int s = 0; s < HD / 16; s++) {
-    kf[s] = TL::frag_global(krow, s, h, a.head_dim);
-    vf[s] = TL::frag_global(vrow, s, h, a.head_dim);
-  }
-  f32x16 dk[HD / 32], dv[HD / 32];
+  for (int s = 0; s < HD / 16; s++) f[s] = TL::frag_global(row, s, h, a.head_dim);
+  f32x16 acc[HD / 32];
 #pragma unroll
-  for (int d = 0; d < HD / 32; d++) dk[d] = dv[d] = f32x16{};
+  for (int d = 0; d < HD / 32; d++) acc[d] = f32x16{};
 
   // the first query that sees the tile's first key, down to a whole query tile
   const int qstart = a.causal ? max(tk.row0 - off, 0) / BQ * BQ : 0;
-  const int per_head = lq > qstart ? (lq - qstart + BQ - 1) / BQ : 0, steps = per_head * group;
+  const int per_head = lq > qstart ? (lq - qstart + BQ - 1) / BQ : 0;
+  const int64_t steps = (int64_t)per_head * group;
+  const int s0 = (int)(steps * split / a.nsplit), s1 = (int)(steps * (split + 1) / a.nsplit);
   Stage<T, HD, BQ, THREADS> qs, os;
   float rowv = 0.0f;  // L (threads 0 .. 31) or D (32 .. 63) of the next tile's rows
   auto load = [&](int step) {
@@ -120,56 +134,113 @@ __global__ __launch_bounds__(NW * 64) void prompt_dkv_kernel(PromptArgs a) {
     os.store(b + kTile, tid);
     if (tid < 2 * BQ) reinterpret_cast<float*>(b + 2 * kTile)[tid] = rowv;
   };
-  if (steps > 0) {
-    load(0);
+  if (s0 < s1) {
+    load(s0);
     store(lds);
   }
-  for (int step = 0; step < steps; step++) {
-    const char* qt = lds + (step & 1) * kBuf;
+  for (int step = s0, buf = 0; step < s1; step++, buf ^= 1) {
+    const char* qt = lds + buf * kBuf;
     const char* ot = qt + kTile;
-    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
-    if (step + 1 < steps) load(step + 1);
+    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile) + (is_k ? BQ : 0) + 4 * h;
+    if (step + 1 < s1) load(step + 1);
     __syncthreads();
     const int r = qstart + step % per_head * BQ;
-    if (!a.causal || r + BQ - 1 + off >= w_key) {
-      f32x16 s = f32x16{}, dp = f32x16{};
+    const bool seen = !a.causal || r + BQ - 1 + off >= w_key;
+    const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off);
+    // value i of a product: query r + 8 (i / 4) + 4 h + i % 4, the lane's key
+    auto see = [&](int i) {
+      const int qi = r + 8 * (i >> 2) + 4 * h + (i & 3);
+      return qi < lq && live && (!a.causal || kj <= qi + off);
+    };
+    float x[16];
+    Frag pf[2];  // bf16: weights and their gradients rounded to nearest for the products
+    if (seen) {
+      const char* t1 = is_k ? ot : qt;
+      f32x16 s = f32x16{};
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(qt, lane & 31, d, h), kf[d], s);
-#pragma unroll
-      for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(ot, lane & 31, d, h), vf[d], dp);
-      // value i: query r + 8 (i / 4) + 4 h + i % 4, the lane's key
-      float p[16], ds[16];
+      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(t1, lane & 31, d, h), f[d], s);
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(rows + 8 * g + 4 * h);
-        const f32x4 del = *reinterpret_cast<const f32x4*>(rows + BQ + 8 * g + 4 * h);
+        const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 8 * g);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int i = 4 * g + j, qi = r + 8 * g + 4 * h + j;
-          const bool see = qi < lq && live && (!a.causal || kj <= qi + off);
-          p[i] = see ? __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse[j])) : 0.0f;
-          ds[i] = see ? p[i] * (dp[i] - del[j]) : 0.0f;
-        }
+        for (int j = 0; j < 4; j++) x[4 * g + j] = is_k ? s[4 * g + j] - c[j] : fmaf(s[4 * g + j], a.scale2, -c[j]);
       }
+      if (!is_k) {
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        Frag pf, sf;  // bf16: weights and their gradients rounded to nearest for the products
-        tile_pack(p + 8 * u, pf);
-        tile_pack(ds + 8 * u, sf);
+        for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(x[i]);
+        if (!whole)
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) {
-          dv[d] = tile_mma(TL::frag_t(ot, 16 * u, d, lane), pf, dv[d]);
-          dk[d] = tile_mma(TL::frag_t(qt, 16 * u, d, lane), sf, dk[d]);
+          for (int i = 0; i < 16; i++) x[i] = see(i) ? x[i] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          tile_pack(x + 8 * u, pf[u]);
+#pragma unroll
+          for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
+            *reinterpret_cast<u32x4*>(pair + (u * (int)sizeof(Frag) + c * 16) * 64) =
+                reinterpret_cast<const u32x4*>(&pf[u])[c];
         }
       }
     }
-    if (step + 1 < steps) store(lds + ((step + 1) & 1) * kBuf);
+    __syncthreads();
+    if (seen) {
+      if (is_k) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+          for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
+            reinterpret_cast<u32x4*>(&pf[u])[c] =
+                *reinterpret_cast<const u32x4*>(pair + (u * (int)sizeof(Frag) + c * 16) * 64);
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[8 * u + j] *= (float)pf[u][j];
+        }
+        if (!whole)  // what is masked has weight 0, and its other factor may be anything
+#pragma unroll
+          for (int i = 0; i < 16; i++) x[i] = see(i) ? x[i] : 0.0f;
+        tile_pack(x, pf[0]);
+        tile_pack(x + 8, pf[1]);
+      }
+      const char* t2 = is_k ? qt : ot;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) acc[d] = tile_mma(TL::frag_t(t2, 16 * u, d, lane), pf[u], acc[d]);
+    }
+    if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
   }
   if (!live) return;
-  store_rows<T, HD>(static_cast<T*>(a.dk) + (tk.begin + kj) * a.dk_stride + hkv * a.head_dim, dk, a.scale, h,
-                    a.head_dim);
-  store_rows<T, HD>(static_cast<T*>(a.dv) + (tk.begin + kj) * a.dv_stride + hkv * a.head_dim, dv, 1.0f, h,
-                    a.head_dim);
+  const float factor = is_k ? a.scale : 1.0f;
+  const int64_t at = tk.begin + kj;
+  if (a.nsplit > 1) {
+    float* part = a.part + ((int64_t)(2 * split + is_k) * a.rows_k + at) * (a.n_kv * a.head_dim) + hkv * a.head_dim;
+    store_rows<float, HD>(part, acc, factor, h, a.head_dim);
+  } else {
+    store_rows<T, HD>(static_cast<T*>(is_k ? a.dk : a.dv) + at * (is_k ? a.dk_stride : a.dv_stride) + hkv * a.head_dim,
+                      acc, factor, h, a.head_dim);
+  }
+}
+
+// dK and dV from their parts: a thread 4 elements of both.
+template <typename T>
+__global__ __launch_bounds__(256) void prompt_dkv_sum_kernel(PromptArgs a) {
+  const int width = a.n_kv * a.head_dim, per_row = width / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per_row;
+  const int e = (int)(id - row * per_row) * 4;
+  if (row < clamp_cu(a.cu_k, 0, a.rows_k) || row >= clamp_cu(a.cu_k, a.batch, a.rows_k)) return;
+  const int64_t part = a.rows_k * width, at = row * width + e;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f}, k = v;
+  for (int s = 0; s < a.nsplit; s++) {
+    v += *reinterpret_cast<const f32x4*>(a.part + 2 * s * part + at);
+    k += *reinterpret_cast<const f32x4*>(a.part + (2 * s + 1) * part + at);
+  }
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 yv, yk;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    yv[j] = (T)v[j];
+    yk[j] = (T)k[j];
+  }
+  *reinterpret_cast<T4*>(static_cast<T*>(a.dv) + row * a.dv_stride + e) = yv;
+  *reinterpret_cast<T4*>(static_cast<T*>(a.dk) + row * a.dk_stride + e) = yk;
 }
 
 // dQ: NW waves of 32 queries each, key tiles of 32 rows through LDS.
@@ -267,12 +338,18 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     if (hipError_t e = hipGetLastError()) return e;
   }
   if (a.rows_k > 0) {
-    constexpr int lds = 2 * (2 * Tile<T, HD>::bytes(32) + 2 * 32 * 4);
-    a.slots = tile_slots(a.rows_k, a.batch, NW * 32);
-    const auto kernel = prompt_dkv_kernel<T, HD, NW>;
+    constexpr int lds = 2 * (2 * Tile<T, HD>::bytes(kDkvQueries) + 2 * kDkvQueries * 4) +
+                        2 * 2 * 64 * (int)sizeof(typename Tile<T, HD>::Frag);
+    a.slots = tile_slots(a.rows_k, a.batch, kDkvKeys);
+    const auto kernel = prompt_dkv_kernel<T, HD>;
     if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_kv)), dim3(NW * 64), lds, stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_kv * a.nsplit)), dim3(256), lds, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
+    if (a.nsplit > 1) {
+      const int64_t n = a.rows_k * (a.n_kv * a.head_dim / 4);
+      hipLaunchKernelGGL(prompt_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+      if (hipError_t e = hipGetLastError()) return e;
+    }
   }
   if (a.rows_q > 0) {
     constexpr int lds = 4 * Tile<T, HD>::bytes(32);
@@ -286,6 +363,20 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
 }
 
 }  // namespace
+
+// Parts of the (head, query tile) steps of the keys' gradients: enough that the grid is
+// kDkvGroups workgroups, while a part keeps 4 query tiles of the longest sequence that the rows allow.
+PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,
+                              int64_t head_dim) {
+  constexpr int64_t kDkvGroups = 768;
+  const int64_t groups = std::max<int64_t>(1, (rows_k + kDkvKeys - 1) / kDkvKeys * n_kv);
+  const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / kDkvQueries * (n_q / n_kv);
+  PromptBwdPlan p;
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
+  p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
+  p.work = p.delta_bytes + (p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0);
+  return p;
+}
 
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {

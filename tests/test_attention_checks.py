@@ -52,7 +52,7 @@ def test_prompt_attention():
 
 def bwd(p, **kw):
     a = dict(do=P, dos=256, q=P, qs=256, k=P, ks=128, v=P, vs=128, out=P, os=256, lse=P, dq=P, dqs=256, dk=P, dks=128,
-             dv=P, dvs=128, work=P, wb=160)
+             dv=P, dvs=128, work=P, wb=1 << 20)
     a.update(kw)
     return _lib.lib().rq_prompt_attention_bwd(CTX, C.byref(p), *a.values(), None)
 
@@ -64,11 +64,11 @@ def test_prompt_attention_bwd():
         assert bwd(prompt(), **{name: P + (2 if name == "lse" else 8)}) == RQ_ERR_SHAPE, name
     for name in ("dos", "qs", "ks", "vs", "os", "dqs", "dks", "dvs"):
         assert bwd(prompt(), **{name: 64}) == RQ_ERR_SHAPE, name
-    assert bwd(prompt(), wb=159) == RQ_ERR_SHAPE
     assert bwd(prompt(scale=0.0)) == RQ_ERR_SHAPE
     n = C.c_size_t()
     p = prompt()
-    assert _lib.lib().rq_prompt_attention_bwd_work(C.byref(p), C.byref(n)) == RQ_OK and n.value == 160
+    assert _lib.lib().rq_prompt_attention_bwd_work(C.byref(p), C.byref(n)) == RQ_OK and n.value >= 160
+    assert bwd(prompt(), wb=n.value - 1) == RQ_ERR_SHAPE and bwd(prompt(), wb=n.value) == RQ_ERR_HANDLE
     assert _lib.lib().rq_prompt_attention_bwd_work(C.byref(p), None) == RQ_ERR_NULL
     assert _lib.lib().rq_prompt_attention_bwd_work(None, C.byref(n)) == RQ_ERR_NULL
 
