@@ -14,9 +14,9 @@
 // stands for row 16 t + 8 (j / 4) + 4 h + j % 4 on both sides; tile_frag_t reads the
 // other side in that order. No value crosses lanes.
 //
-// In LDS a row's 16-byte pieces are permuted by the row (XOR of the low 3 bits), so
-// that 8 rows at one column, and the 4 rows x 32 bytes of a transposing read, fall
-// on different banks.
+// In LDS a row's 16-byte pieces are permuted by the row (XOR), so that 16 rows at one
+// column, and the 4 rows x 64 bytes of half a wave's transposing read, fall on
+// different ones of the 64 banks (256 bytes).
 #pragma once
 
 #include "rq_internal.h"
@@ -67,7 +67,12 @@ struct Tile {
   static constexpr int kPitch = (kPieces + 7) / 8 * 8 * 16;    // bytes from row to row
   static constexpr int bytes(int rows) { return rows * kPitch; }
 
-  static __device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+  // 16 pieces and more: the row's low 4 bits, the lowest two on top; 8 pieces (two rows
+  // side by side in the banks): bits 1 to 3
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (kPieces % 16 == 0) return ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
+    return ((row & 2) << 1) | ((row >> 1) & 2) | ((row >> 3) & 1);
+  }
   // byte offset of 16-byte piece c of a row
   static __device__ __forceinline__ int at(int row, int c) { return row * kPitch + ((c ^ swizzle(row)) << 4); }
 
@@ -90,10 +95,10 @@ struct Tile {
     const int h = lane >> 5;
     if constexpr (sizeof(T) == 2) {
       const int row = 4 * h + ((lane >> 2) & 3), d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const char* p = lds + r0 * kPitch + at(row, d >> 3) + (d & 7) * 2;
+      const char *p = lds + r0 * kPitch + at(row, d >> 3) + (d & 7) * 2, *p8 = lds + r0 * kPitch + at(row + 8, d >> 3) + (d & 7) * 2;
       typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
       const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
-      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 8 * kPitch));
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p8);
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       return __builtin_bit_cast(bf16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
     } else {

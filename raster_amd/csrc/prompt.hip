@@ -27,6 +27,8 @@ namespace {
 // v of lane ^ 32
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
+constexpr float kSlack = 8.0f;
+
 template <typename T, int HD, int NW, int BK>
 __global__ __launch_bounds__(NW * 64) void prompt_fwd_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
@@ -101,13 +103,16 @@ __global__ __launch_bounds__(NW * 64) void prompt_fwd_kernel(PromptArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[t][i]);
       mx = fmaxf(mx, other_half(mx)) * a.scale2;
-      const float mn = fmaxf(m, mx);
-      const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: every weight 0
-      const float alpha = __builtin_amdgcn_exp2f(m - ref);
-      m = mn;
-      l *= alpha;
+      // The reference m moves only when some query's maximum is past it by kSlack: below that
+      // the weights are at most 2^kSlack, which costs no digits, and nothing is rescaled.
+      if (__builtin_amdgcn_ballot_w64(mx > m + kSlack || m == -INFINITY)) {
+        const float mn = fmaxf(m, mx), alpha = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= alpha;
 #pragma unroll
-      for (int d = 0; d < HD / 32; d++) acc[d] *= alpha;
+        for (int d = 0; d < HD / 32; d++) acc[d] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;  // nothing seen yet: every weight 0
 #pragma unroll
       for (int t = 0; t < BK / 32; t++) {
         float p[16];
