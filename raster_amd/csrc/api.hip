@@ -1487,7 +1487,8 @@ static int check_prompt(const rq_prompt* p) {
   if (int s = check_heads(p->n_q, p->n_kv, p->head_dim)) return s;
   if (p->batch < 0 || p->rows_q < 0 || p->rows_k < 0) return fail(RQ_ERR_SHAPE, "negative dimension");
   if (p->rows_q > kMaxRows || p->rows_k > kMaxRows || p->batch > kMaxRows) return fail(RQ_ERR_SHAPE, "too many rows");
-  if ((p->rows_q / 32 + p->batch) * p->n_q > INT32_MAX || (p->rows_k / 32 + p->batch) * p->n_q > INT32_MAX ||
+  // (the gradient's grid holds a workgroup of 64 keys, at most 16 parts each where there are few, and of 128 queries)
+  if ((p->rows_q / 32 + p->batch) * p->n_q > INT32_MAX / 32 || (p->rows_k / 32 + p->batch) * p->n_q > INT32_MAX / 32 ||
       p->rows_q * p->n_q > (int64_t)INT32_MAX * 8)
     return fail(RQ_ERR_SHAPE, "rows times heads too large for one launch");
   if (!p->cu_k && p->rows_k != p->rows_q) return fail(RQ_ERR_SHAPE, "without cu_k, rows_k must be rows_q");

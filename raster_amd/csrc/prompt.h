@@ -8,7 +8,7 @@ namespace rq {
 // Rows are q, k, v, out rows of the packed batch; strides in elements.
 struct PromptArgs {
   const int32_t *cu_q, *cu_k;
-  int64_t rows_q, rows_k, slots;
+  int64_t rows_q, rows_k, slots, q_slots, k_slots;
   int batch, n_q, n_kv, head_dim, causal;
   float scale, scale2;  // scale2 = scale log2 e
   const void *q, *k, *v;

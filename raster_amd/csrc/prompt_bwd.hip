@@ -77,19 +77,18 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[HD / 32],
 // The steps, (query head of the group, query tile), of a workgroup are one of nsplit parts;
 // with more than one the parts' f32 sums go to a.part and prompt_dkv_sum_kernel adds them in
 // order.
-constexpr int kDkvKeys = 64, kDkvQueries = 32;
+constexpr int kDkvKeys = 64, kDkvQueries = 32, kDqQueries = 128;
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void prompt_dkv_kernel(PromptArgs a) {
+__device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
   constexpr int THREADS = 256, BQ = kDkvQueries;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
   constexpr int kTile = TL::bytes(BQ);
   constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
   constexpr int kPair = 2 * 64 * (int)sizeof(Frag);  // the weights of 32 keys and queries
   const int group = a.n_q / a.n_kv;
-  const int hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, split = rest % a.nsplit;
+  const int hkv = block % a.n_kv, rest = block / a.n_kv, split = rest % a.nsplit;
   const int64_t slot = rest / a.nsplit;  // a sequence's first keys, which most queries see, first
   const TileSpan tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, kDkvKeys, slot);
   if (tk.len == 0) return;
@@ -119,8 +118,7 @@ __global__ __launch_bounds__(256) void prompt_dkv_kernel(PromptArgs a) {
   const int s0 = (int)(steps * split / a.nsplit), s1 = (int)(steps * (split + 1) / a.nsplit);
   Stage<T, HD, BQ, THREADS> qs, os;
   float rowv = 0.0f;  // L (threads 0 .. 31) or D (32 .. 63) of the next tile's rows
-  auto load = [&](int step) {
-    const int hq = hkv * group + step / per_head, r = qstart + step % per_head * BQ;
+  auto load = [&](int hq, int r) {
     qs.load(static_cast<const T*>(a.q) + (q0 + r) * a.q_stride + hq * a.head_dim, a.q_stride, lq - r, a.head_dim, tid);
     os.load(static_cast<const T*>(a.dout) + (q0 + r) * a.dout_stride + hq * a.head_dim, a.dout_stride, lq - r,
             a.head_dim, tid);
@@ -134,17 +132,21 @@ __global__ __launch_bounds__(256) void prompt_dkv_kernel(PromptArgs a) {
     os.store(b + kTile, tid);
     if (tid < 2 * BQ) reinterpret_cast<float*>(b + 2 * kTile)[tid] = rowv;
   };
+  int hq = hkv * group, r = qstart;  // of the step
   if (s0 < s1) {
-    load(s0);
+    hq += s0 / per_head;
+    r += s0 % per_head * BQ;
+    load(hq, r);
     store(lds);
   }
   for (int step = s0, buf = 0; step < s1; step++, buf ^= 1) {
     const char* qt = lds + buf * kBuf;
     const char* ot = qt + kTile;
     const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile) + (is_k ? BQ : 0) + 4 * h;
-    if (step + 1 < s1) load(step + 1);
+    int next_hq = hq, next_r = r + BQ;
+    if (next_r >= lq) next_hq++, next_r = qstart;
+    if (step + 1 < s1) load(next_hq, next_r);
     __syncthreads();
-    const int r = qstart + step % per_head * BQ;
     const bool seen = !a.causal || r + BQ - 1 + off >= w_key;
     const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off);
     // value i of a product: query r + 8 (i / 4) + 4 h + i % 4, the lane's key
@@ -206,6 +208,7 @@ __global__ __launch_bounds__(256) void prompt_dkv_kernel(PromptArgs a) {
         for (int d = 0; d < HD / 32; d++) acc[d] = tile_mma(TL::frag_t(t2, 16 * u, d, lane), pf[u], acc[d]);
     }
     if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
+    hq = next_hq, r = next_r;
   }
   if (!live) return;
   const float factor = is_k ? a.scale : 1.0f;
@@ -243,17 +246,16 @@ __global__ __launch_bounds__(256) void prompt_dkv_sum_kernel(PromptArgs a) {
   *reinterpret_cast<T4*>(static_cast<T*>(a.dk) + row * a.dk_stride + e) = yk;
 }
 
-// dQ: NW waves of 32 queries each, key tiles of 32 rows through LDS.
-template <typename T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void prompt_dq_kernel(PromptArgs a) {
+// dQ: four waves of 32 queries each, key tiles of BK rows through LDS.
+template <typename T, int HD, int BK>
+__device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
-  constexpr int THREADS = NW * 64, BQ = NW * 32, BK = 32;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int THREADS = 256, BQ = kDqQueries;
   constexpr int kTile = TL::bytes(BK);
   const int group = a.n_q / a.n_kv;
-  const int hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, hq = hkv * group + rest % group;
-  const int64_t slot = a.slots - 1 - rest / group;
+  const int hkv = block % a.n_kv, rest = block / a.n_kv, hq = hkv * group + rest % group;
+  const int64_t slot = a.q_slots - 1 - rest / group;
   const TileSpan tq = tile_of_slot(a.cu_q, a.batch, a.rows_q, BQ, slot);
   if (tq.len == 0) return;
   const int64_t k0 = clamp_cu(a.cu_k, tq.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tq.seq + 1, a.rows_k);
@@ -300,23 +302,27 @@ __global__ __launch_bounds__(NW * 64) void prompt_dq_kernel(PromptArgs a) {
     }
     __syncthreads();
     if (!a.causal || kb <= w_row + 31 + off) {
-      f32x16 s = f32x16{}, dp = f32x16{};
+      const bool whole = kb + BK <= lk && w_row + 32 <= tq.len && (!a.causal || kb + BK - 1 <= w_row + off);
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, lane & 31, d, h), qf[d], s);
+      for (int t = 0; t < BK / 32; t++) {
+        f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, lane & 31, d, h), of[d], dp);
-      float ds[16];
+        for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, 32 * t + (lane & 31), d, h), qf[d], s);
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const bool in = kb + 8 * (i >> 2) + 4 * h + (i & 3) <= see;
-        ds[i] = in ? __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse)) * (dp[i] - del) : 0.0f;
-      }
+        for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, 32 * t + (lane & 31), d, h), of[d], dp);
+        float ds[16];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        Frag sf;
-        tile_pack(ds + 8 * u, sf);
+        for (int i = 0; i < 16; i++) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse)) * (dp[i] - del);
+        if (!whole)
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 16 * u, d, lane), sf, dq[d]);
+          for (int i = 0; i < 16; i++) ds[i] = kb + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) <= see ? ds[i] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          Frag sf;
+          tile_pack(ds + 8 * u, sf);
+#pragma unroll
+          for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 32 * t + 16 * u, d, lane), sf, dq[d]);
+        }
       }
     }
     if (more) {
@@ -330,34 +336,40 @@ __global__ __launch_bounds__(NW * 64) void prompt_dq_kernel(PromptArgs a) {
                       a.head_dim);
 }
 
-template <typename T, int HD, int NW>
+// Both in one launch, so that the short workgroups of one fill the compute units that the
+// last long ones of the other leave idle.
+template <typename T, int HD, int BK>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prompt_grad_kernel(PromptArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int dkv = (int)(a.k_slots * a.n_kv * a.nsplit);
+  if ((int)blockIdx.x < dkv)
+    dkv_body<T, HD>(a, blockIdx.x, lds);
+  else
+    dq_body<T, HD, BK>(a, blockIdx.x - dkv, lds);
+}
+
+template <typename T, int HD, int BK>
 hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
+  using TL = Tile<T, HD>;
   if (a.rows_q > 0) {
     const int64_t n = a.rows_q * a.n_q * kDeltaLanes;
     hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  if (a.rows_k > 0) {
-    constexpr int lds = 2 * (2 * Tile<T, HD>::bytes(kDkvQueries) + 2 * kDkvQueries * 4) +
-                        2 * 2 * 64 * (int)sizeof(typename Tile<T, HD>::Frag);
-    a.slots = tile_slots(a.rows_k, a.batch, kDkvKeys);
-    const auto kernel = prompt_dkv_kernel<T, HD>;
-    if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_kv * a.nsplit)), dim3(256), lds, stream, a);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (a.nsplit > 1) {
-      const int64_t n = a.rows_k * (a.n_kv * a.head_dim / 4);
-      hipLaunchKernelGGL(prompt_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
-      if (hipError_t e = hipGetLastError()) return e;
-    }
-  }
-  if (a.rows_q > 0) {
-    constexpr int lds = 4 * Tile<T, HD>::bytes(32);
-    a.slots = tile_slots(a.rows_q, a.batch, NW * 32);
-    const auto kernel = prompt_dq_kernel<T, HD, NW>;
-    if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(NW * 64), lds, stream, a);
-    if (hipError_t e = hipGetLastError()) return e;
+  constexpr int lds = std::max(2 * (2 * TL::bytes(kDkvQueries) + 2 * kDkvQueries * 4) +
+                                   2 * 2 * 64 * (int)sizeof(typename TL::Frag),
+                               4 * TL::bytes(BK));
+  a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
+  a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, kDqQueries) : 0;
+  const auto kernel = prompt_grad_kernel<T, HD, BK>;
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256), lds,
+                     stream, a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.nsplit > 1 && a.rows_k > 0) {
+    const int64_t n = a.rows_k * (a.n_kv * a.head_dim / 4);
+    hipLaunchKernelGGL(prompt_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+    return hipGetLastError();
   }
   return hipSuccess;
 }
@@ -380,13 +392,13 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
 
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {
-    if (a.head_dim <= 64) return run_bwd<__bf16, 64, 4>(a, stream);
-    if (a.head_dim <= 128) return run_bwd<__bf16, 128, 4>(a, stream);
-    return run_bwd<__bf16, 256, 4>(a, stream);
+    if (a.head_dim <= 64) return run_bwd<__bf16, 64, 64>(a, stream);
+    if (a.head_dim <= 128) return run_bwd<__bf16, 128, 32>(a, stream);
+    return run_bwd<__bf16, 256, 32>(a, stream);
   }
-  if (a.head_dim <= 64) return run_bwd<float, 64, 4>(a, stream);
-  if (a.head_dim <= 128) return run_bwd<float, 128, 4>(a, stream);
-  return run_bwd<float, 256, 4>(a, stream);
+  if (a.head_dim <= 64) return run_bwd<float, 64, 32>(a, stream);
+  if (a.head_dim <= 128) return run_bwd<float, 128, 32>(a, stream);
+  return run_bwd<float, 256, 32>(a, stream);
 }
 
 }  // namespace rq
