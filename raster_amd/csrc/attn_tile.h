@@ -123,6 +123,32 @@ struct Tile {
   }
 };
 
+// The fragments' loads are waited for here: otherwise the wait lands at their first use
+// inside a loop, where it also waits for the loads in flight of the tile after next.
+template <typename Frag, int N>
+__device__ __forceinline__ void settle(Frag (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+v"(f[i]));
+}
+
+// Order of a block of N products, each with R reads from LDS, and N2 more with R2: the reads
+// of kAhead products first, then a product and the reads of a later one in turn. Left to
+// itself the scheduler puts a read, its wait and its product one after another, and every
+// product waits out the latency.
+template <int N, int R, int N2 = 0, int R2 = 0>
+__device__ __forceinline__ void order_products() {
+  constexpr int kMfma = 0x008, kRead = 0x100, kAhead = 6;
+  __builtin_amdgcn_sched_group_barrier(kRead, kAhead * R, 0);
+#pragma unroll
+  for (int i = 0; i < N + N2; i++) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    if (i + kAhead < N)
+      __builtin_amdgcn_sched_group_barrier(kRead, R, 0);
+    else if (N2 > 0 && i + kAhead < N + N2)
+      __builtin_amdgcn_sched_group_barrier(kRead, R2, 0);
+  }
+}
+
 // A tile on its way from memory to LDS through registers: load() reads rows 0 ..
 // nrows - 1 (the rest, and elements from hd on, are zeros: a buffer load past
 // its range gives 0), store() writes them. `stride` is in elements and at most

@@ -107,6 +107,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
   Frag f[HD / 16];
 #pragma unroll
   for (int s = 0; s < HD / 16; s++) f[s] = TL::frag_global(row, s, h, a.head_dim);
+  settle(f);
   f32x16 acc[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; d++) acc[d] = f32x16{};
@@ -161,6 +162,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
       f32x16 s = f32x16{};
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(t1, lane & 31, d, h), f[d], s);
+      if constexpr (sizeof(T) == 2) order_products<HD / 16, 1>();
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 8 * g);
@@ -206,6 +208,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) acc[d] = tile_mma(TL::frag_t(t2, 16 * u, d, lane), pf[u], acc[d]);
+      if constexpr (sizeof(T) == 2) order_products<HD / 16, 2>();
     }
     if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
     hq = next_hq, r = next_r;
@@ -253,6 +256,8 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
   using Frag = typename TL::Frag;
   constexpr int THREADS = 256, BQ = kDqQueries;
   constexpr int kTile = TL::bytes(BK);
+  // f32 heads past 128: no registers are left to hold the next tile of both while this one is used
+  constexpr bool kOneStage = sizeof(T) == 4 && HD > 128;
   const int group = a.n_q / a.n_kv;
   const int hkv = block % a.n_kv, rest = block / a.n_kv, hq = hkv * group + rest % group;
   const int64_t slot = a.q_slots - 1 - rest / group;
@@ -282,6 +287,8 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
     qf[s] = TL::frag_global(qrow, s, h, a.head_dim);
     of[s] = TL::frag_global(orow, s, h, a.head_dim);
   }
+  settle(qf);
+  settle(of);
   const int64_t at = (int64_t)hq * a.rows_q + tq.begin + min(qi, tq.len - 1);
   const float lse = base2_lse(a.lse[at]), del = a.delta[at];
   f32x16 dq[HD / 32];
@@ -296,9 +303,11 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
     const char* kt = lds + buf * 2 * kTile;
     const char* vt = kt + kTile;
     const bool more = kb + BK < nk;
+    char* next = lds + (buf ^ 1) * 2 * kTile;
     if (more) {
       ks.load(kbase + (int64_t)(kb + BK) * a.k_stride, a.k_stride, lk - kb - BK, a.head_dim, tid);
-      vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
+      if constexpr (!kOneStage)
+        vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
     }
     __syncthreads();
     if (!a.causal || kb <= w_row + 31 + off) {
@@ -310,24 +319,27 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
         for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, 32 * t + (lane & 31), d, h), qf[d], s);
 #pragma unroll
         for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, 32 * t + (lane & 31), d, h), of[d], dp);
+        if constexpr (sizeof(T) == 2) order_products<HD / 8, 1>();
         float ds[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse)) * (dp[i] - del);
         if (!whole)
 #pragma unroll
           for (int i = 0; i < 16; i++) ds[i] = kb + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) <= see ? ds[i] : 0.0f;
+        Frag sf[2];
+        tile_pack(ds, sf[0]);
+        tile_pack(ds + 8, sf[1]);
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          Frag sf;
-          tile_pack(ds + 8 * u, sf);
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 32 * t + 16 * u, d, lane), sf, dq[d]);
-        }
+          for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 32 * t + 16 * u, d, lane), sf[u], dq[d]);
+        if constexpr (sizeof(T) == 2) order_products<HD / 16, 2>();
       }
     }
     if (more) {
-      char* next = lds + (buf ^ 1) * 2 * kTile;
       ks.store(next, tid);
+      if constexpr (kOneStage)
+        vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
       vs.store(next + kTile, tid);
     }
   }
