@@ -17,6 +17,7 @@ include/rq.h; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 from ._lib import Pages, Prompt, call
 from .quant import Context, _current_stream, _dtype_code, _need, _stream_ptr, _t
@@ -24,19 +25,33 @@ from .quant import Context, _current_stream, _dtype_code, _need, _stream_ptr, _t
 __all__ = ["prompt_attention", "prompt_attention_bwd", "paged_attention", "pages_append", "pages_copy"]
 
 
-def _rows(t, ctx: Context, width: int, what: str, dtype=None, rows: int | None = None):
-    """t [rows, width] on the context's device, elements of a row side by side -> its row stride."""
+def _code(t) -> int:
+    _t()  # (fills the table of types)
+    return _dtype_code(t)
+
+
+def _bad_rows(t, ctx: Context, rows, width: int, dtype, what: str):
     _need(t.is_cuda and t.get_device() == ctx.device, f"{what} must be a CUDA tensor of the context's device")
-    _need(t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or t.numel() == 0),
-          f"{what} must be [rows, {width}] with its rows' elements side by side")
-    _need(dtype is None or t.dtype == dtype, f"{what} has another type")
-    _need(rows is None or t.shape[0] == rows, f"{what} must have {rows} rows")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    _need(t.dtype == dtype, f"{what} must be {dtype}")
+    raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {width}] with its rows' elements side by side")
 
 
-def _i32(t, ctx: Context, n: int, what: str):
-    _need(t.is_cuda and t.get_device() == ctx.device and t.dtype == _t().int32 and t.is_contiguous()
-          and t.numel() == n, f"{what} must be a contiguous int32 CUDA tensor of {n} elements on the context's device")
+def _rows(t, ctx: Context, rows, width: int, dtype, what: str) -> int:
+    """The row stride of t, checked to be [rows, width] (rows None: any number) of
+    dtype on the context's device with the elements of a row side by side."""
+    shape = t.shape
+    if (t.dtype != dtype or t.get_device() != ctx.device or len(shape) != 2 or shape[1] != width
+            or (rows is not None and shape[0] != rows)):
+        _bad_rows(t, ctx, rows, width, dtype, what)
+    s0, s1 = t.stride()
+    if s1 != 1 and width != 1:
+        _bad_rows(t, ctx, rows, width, dtype, what)
+    return s0 if shape[0] > 1 else max(s0, width)  # (of a single row, torch's stride may be anything)
+
+
+def _i32(t, ctx: Context, n: int, what: str) -> int:
+    if t.dtype != _t().int32 or t.get_device() != ctx.device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 CUDA tensor of {n} elements on the context's device")
     return t.data_ptr()
 
 
@@ -52,25 +67,29 @@ def _on(stream, t):
     return _stream_ptr(stream), torch.cuda.stream(s)
 
 
-def _empty(scope, *shapes_dtypes, device):
-    torch = _t()
+def _empty(scope, shape, like, dtype=None):
     if scope is None:
-        return [torch.empty(s, dtype=d, device=device) for s, d in shapes_dtypes]
+        return _t().empty(shape, dtype=dtype or like.dtype, device=like.device)
     with scope:
-        return [torch.empty(s, dtype=d, device=device) for s, d in shapes_dtypes]
+        return _t().empty(shape, dtype=dtype or like.dtype, device=like.device)
 
 
 def _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal):
-    _dtype_code(q)
-    qw, kw = n_q * head_dim, n_kv * head_dim
-    _need(cu.dim() == 1 and cu.numel() >= 1, "cu must hold batch + 1 row numbers")
-    batch = cu.numel() - 1
-    qs = _rows(q, ctx, qw, "q")
-    ks = _rows(k, ctx, kw, "k", q.dtype)
-    vs = _rows(v, ctx, kw, "v", q.dtype, k.shape[0])
-    p = Prompt(_dtype_code(q), batch, q.shape[0], k.shape[0], n_q, n_kv, head_dim, _i32(cu, ctx, batch + 1, "cu"),
-               None if cu_k is None else _i32(cu_k, ctx, batch + 1, "cu_k"), 1 if causal else 0, float(scale))
+    code, dtype, kw = _code(q), q.dtype, n_kv * head_dim
+    n = cu.numel()
+    _need(n >= 1, "cu must hold batch + 1 row numbers")
+    qs = _rows(q, ctx, None, n_q * head_dim, dtype, "q")
+    ks = _rows(k, ctx, None, kw, dtype, "k")
+    rows, rows_k = q.shape[0], k.shape[0]
+    vs = _rows(v, ctx, rows_k, kw, dtype, "v")
+    p = Prompt(code, n - 1, rows, rows_k, n_q, n_kv, head_dim, _i32(cu, ctx, n, "cu"),
+               None if cu_k is None else _i32(cu_k, ctx, n, "cu_k"), 1 if causal else 0, scale)
     return p, qs, ks, vs
+
+
+def _check_lse(lse, ctx, n):
+    _need(lse.dtype == _t().float32 and lse.get_device() == ctx.device and lse.is_contiguous() and lse.numel() == n,
+          "lse must be a contiguous f32 CUDA tensor [n_q, rows] of the context's device")
 
 
 def prompt_attention(ctx: Context, q, k, v, cu, n_q: int, n_kv: int, head_dim: int, scale: float, causal: bool = True,
@@ -79,15 +98,15 @@ def prompt_attention(ctx: Context, q, k, v, cu, n_q: int, n_kv: int, head_dim: i
     (f32 or bf16), sequence b in rows cu[b] .. cu[b+1] - 1 (int32 [batch + 1];
     cu_k: the keys', when they differ) -> out [rows, n_q*head_dim]. lse f32
     [n_q, rows] is filled when given (prompt_attention_bwd needs it)."""
-    torch = _t()
     p, qs, ks, vs = _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal)
     raw, scope = _on(stream, q)
+    width = n_q * head_dim
     if out is None:
-        out, = _empty(scope, (q.shape, q.dtype), device=q.device)
-    os = _rows(out, ctx, n_q * head_dim, "out", q.dtype, q.shape[0])
+        out, os = _empty(scope, (q.shape[0], width), q), width
+    else:
+        os = _rows(out, ctx, q.shape[0], width, q.dtype, "out")
     if lse is not None:
-        _need(lse.is_cuda and lse.get_device() == ctx.device and lse.dtype == torch.float32 and lse.is_contiguous()
-              and lse.numel() == n_q * q.shape[0], "lse must be a contiguous f32 CUDA tensor [n_q, rows]")
+        _check_lse(lse, ctx, n_q * q.shape[0])
     call("rq_prompt_attention", ctx.handle, C.byref(p), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
          out.data_ptr(), os, None if lse is None else lse.data_ptr(), raw)
     return out
@@ -97,21 +116,19 @@ def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_
                          causal: bool = True, cu_k=None, dq=None, dk=None, dv=None, stream=None):
     """rq_prompt_attention_bwd: the gradient of prompt_attention for dout, from
     the forward's out and lse -> (dq, dk, dv), written into the given tensors if any."""
-    torch = _t()
     p, qs, ks, vs = _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal)
-    qw, kw, rows, rows_k = n_q * head_dim, n_kv * head_dim, q.shape[0], k.shape[0]
-    dos = _rows(dout, ctx, qw, "dout", q.dtype, rows)
-    os = _rows(out, ctx, qw, "out", q.dtype, rows)
-    _need(lse.is_cuda and lse.get_device() == ctx.device and lse.dtype == torch.float32 and lse.is_contiguous()
-          and lse.numel() == n_q * rows, "lse must be the forward's f32 CUDA tensor [n_q, rows]")
+    qw, kw, rows, rows_k, dtype = n_q * head_dim, n_kv * head_dim, q.shape[0], k.shape[0], q.dtype
+    dos = _rows(dout, ctx, rows, qw, dtype, "dout")
+    os = _rows(out, ctx, rows, qw, dtype, "out")
+    _check_lse(lse, ctx, n_q * rows)
     need = C.c_size_t()
     call("rq_prompt_attention_bwd_work", C.byref(p), C.byref(need))
     raw, scope = _on(stream, q)
-    new = [((rows, qw), q.dtype)] * (dq is None) + [((rows_k, kw), q.dtype)] * ((dk is None) + (dv is None))
-    work, *made = _empty(scope, ((need.value // 4,), torch.float32), *new, device=q.device)
-    dq, dk, dv = (made.pop(0) if t is None else t for t in (dq, dk, dv))
-    dqs = _rows(dq, ctx, qw, "dq", q.dtype, rows)
-    dks, dvs = (_rows(t, ctx, kw, n, q.dtype, rows_k) for t, n in ((dk, "dk"), (dv, "dv")))
+    work = _empty(scope, need.value // 4, q, _t().float32)
+    dq = _empty(scope, (rows, qw), q) if dq is None else dq
+    dk, dv = (_empty(scope, (rows_k, kw), q) if t is None else t for t in (dk, dv))
+    dqs = _rows(dq, ctx, rows, qw, dtype, "dq")
+    dks, dvs = _rows(dk, ctx, rows_k, kw, dtype, "dk"), _rows(dv, ctx, rows_k, kw, dtype, "dv")
     call("rq_prompt_attention_bwd", ctx.handle, C.byref(p), dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
          v.data_ptr(), vs, out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(),
          dvs, work.data_ptr(), need.value, raw)
@@ -119,14 +136,30 @@ def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_
 
 
 def _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch):
+    shape, width = kpages.shape, n_kv * head_dim
     for t, n in ((kpages, "kpages"), (vpages, "vpages")):
-        _need(t.is_cuda and t.get_device() == ctx.device and t.is_contiguous() and t.dim() == 3
-              and t.shape[2] == n_kv * head_dim,
-              f"{n} must be a contiguous CUDA tensor [pages, page_size, n_kv*head_dim] of the context's device")
-    _need(vpages.shape == kpages.shape and vpages.dtype == kpages.dtype, "kpages and vpages must be alike")
-    _need(table.dim() == 2 and table.shape[0] == batch, "table must be [batch, pages of a sequence]")
-    return Pages(_dtype_code(kpages), kpages.data_ptr(), vpages.data_ptr(), kpages.shape[0], kpages.shape[1], n_kv,
-                 head_dim, _i32(table, ctx, table.numel(), "table"), table.shape[1])
+        if t.get_device() != ctx.device or len(t.shape) != 3 or t.shape[2] != width or not t.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous CUDA tensor [pages, page_size, {width}] of the context's device")
+    _need(vpages.shape == shape and vpages.dtype == kpages.dtype, "kpages and vpages must be alike")
+    ts = table.shape
+    _need(len(ts) == 2 and ts[0] == batch, "table must be [batch, pages of a sequence]")
+    return Pages(_code(kpages), kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
+                 _i32(table, ctx, batch * ts[1], "table"), ts[1])
+
+
+_work_sizes: dict = {}  # rq_paged_attention_work by its arguments
+
+
+def _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len) -> int:
+    key = (ctx.device, batch, n_q, n_kv, head_dim, max_len)
+    n = _work_sizes.get(key)
+    if n is None:
+        need = C.c_size_t()
+        call("rq_paged_attention_work", ctx.handle, batch, n_q, n_kv, head_dim, max_len, C.byref(need))
+        if len(_work_sizes) >= 4096:
+            _work_sizes.clear()
+        n = _work_sizes[key] = need.value
+    return n
 
 
 def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int, n_kv: int, head_dim: int,
@@ -137,28 +170,28 @@ def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int
     pages of a sequence]): RoPE, append, attention over rows 0 .. lens[b] -> out
     [batch, n_q*head_dim]. k and v None: nothing appended, rows 0 .. lens[b] - 1. max_len:
     no sequence is longer, the new row included (default: what the table holds)."""
-    torch = _t()
-    dt = _dtype_code(q)
-    batch, kw = q.shape[0], n_kv * head_dim
-    qs = _rows(q, ctx, n_q * head_dim, "q")
+    code, dtype, qw, kw = _code(q), q.dtype, n_q * head_dim, n_kv * head_dim
+    qs = _rows(q, ctx, None, qw, dtype, "q")
+    batch = q.shape[0]
     _need((k is None) == (v is None), "k and v must both be given, or neither")
+    kd = vd = None
     ks = vs = 0
     if k is not None:
-        ks, vs = _rows(k, ctx, kw, "k", q.dtype, batch), _rows(v, ctx, kw, "v", q.dtype, batch)
+        ks, vs = _rows(k, ctx, batch, kw, dtype, "k"), _rows(v, ctx, batch, kw, dtype, "v")
+        kd, vd = k.data_ptr(), v.data_ptr()
     pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
     if max_len is None:
         max_len = table.shape[1] * kpages.shape[1]
-    need = C.c_size_t()
-    call("rq_paged_attention_work", ctx.handle, batch, n_q, n_kv, head_dim, max_len, C.byref(need))
+    need = _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len)
     raw, scope = _on(stream, q)
-    new = [(q.shape, q.dtype)] * (out is None)
-    work, *made = _empty(scope, ((need.value // 4,), torch.float32), *new, device=q.device)
+    work = _empty(scope, need // 4, q, _t().float32) if need else None
     if out is None:
-        out, = made
-    os = _rows(out, ctx, n_q * head_dim, "out", q.dtype, batch)
-    call("rq_paged_attention", ctx.handle, C.byref(pg), dt, q.data_ptr(), qs, None if k is None else k.data_ptr(), ks,
-         None if v is None else v.data_ptr(), vs, _i32(lens, ctx, batch, "lens"), batch, n_q, max_len, float(theta),
-         float(scale), out.data_ptr(), os, work.data_ptr() if need.value else None, need.value, raw)
+        out, os = _empty(scope, (batch, qw), q), qw
+    else:
+        os = _rows(out, ctx, batch, qw, dtype, "out")
+    call("rq_paged_attention", ctx.handle, C.byref(pg), code, q.data_ptr(), qs, kd, ks, vd, vs,
+         _i32(lens, ctx, batch, "lens"), batch, n_q, max_len, theta, scale, out.data_ptr(), os,
+         work.data_ptr() if need else None, need, raw)
     return out
 
 
@@ -168,20 +201,25 @@ def pages_append(ctx: Context, q, k, v, kpages, vpages, table, cu, past, n_q: in
     past[b] and on) of q [rows, n_q*head_dim] and k [rows, n_kv*head_dim] rotated,
     the rotated k and v stored in the pages -> (rotated q, rotated k), written
     into q_out / k_out when given (they may be q and k)."""
-    rows, qw, kw = q.shape[0], n_q * head_dim, n_kv * head_dim
-    dt = _dtype_code(q)
-    qs = _rows(q, ctx, qw, "q")
-    ks, vs = _rows(k, ctx, kw, "k", q.dtype, rows), _rows(v, ctx, kw, "v", q.dtype, rows)
-    _need(cu.dim() == 1 and cu.numel() >= 1, "cu must hold batch + 1 row numbers")
+    code, dtype, qw, kw = _code(q), q.dtype, n_q * head_dim, n_kv * head_dim
+    qs = _rows(q, ctx, None, qw, dtype, "q")
+    rows = q.shape[0]
+    ks, vs = _rows(k, ctx, rows, kw, dtype, "k"), _rows(v, ctx, rows, kw, dtype, "v")
     batch = cu.numel() - 1
+    _need(batch >= 0, "cu must hold batch + 1 row numbers")
     pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
     raw, scope = _on(stream, q)
-    made = _empty(scope, *[((rows, qw), q.dtype)] * (q_out is None), *[((rows, kw), q.dtype)] * (k_out is None),
-                  device=q.device)
-    q_out, k_out = (made.pop(0) if t is None else t for t in (q_out, k_out))
-    qos, kos = _rows(q_out, ctx, qw, "q_out", q.dtype, rows), _rows(k_out, ctx, kw, "k_out", q.dtype, rows)
-    call("rq_pages_append", ctx.handle, C.byref(pg), dt, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-         _i32(cu, ctx, batch + 1, "cu"), _i32(past, ctx, batch, "past"), batch, rows, n_q, float(theta),
+    qos, kos = qw, kw
+    if q_out is None:
+        q_out = _empty(scope, (rows, qw), q)
+    else:
+        qos = _rows(q_out, ctx, rows, qw, dtype, "q_out")
+    if k_out is None:
+        k_out = _empty(scope, (rows, kw), q)
+    else:
+        kos = _rows(k_out, ctx, rows, kw, dtype, "k_out")
+    call("rq_pages_append", ctx.handle, C.byref(pg), code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+         _i32(cu, ctx, batch + 1, "cu"), _i32(past, ctx, batch, "past"), batch, rows, n_q, theta,
          q_out.data_ptr(), qos, k_out.data_ptr(), kos, raw)
     return q_out, k_out
 
@@ -190,14 +228,14 @@ def pages_copy(ctx: Context, pages, src, dst, stream=None):
     """rq_pages_copy: page src[i] -> page dst[i] in every plane of pages [planes,
     pages, page_size, width] (src, dst host sequences of page numbers, all dst
     different and none of them a src) -> pages."""
-    _need(pages.is_cuda and pages.get_device() == ctx.device and pages.is_contiguous() and pages.dim() == 4,
+    shape = pages.shape
+    _need(pages.get_device() == ctx.device and pages.is_contiguous() and len(shape) == 4,
           "pages must be a contiguous CUDA tensor [planes, pages, page_size, width] of the context's device")
-    _need(len(src) == len(dst), "src and dst must be equally long")
     n = len(src)
-    arr = C.c_int32 * n
-    size = pages.element_size()
-    page = pages.shape[2] * pages.shape[3] * size
+    _need(len(dst) == n, "src and dst must be equally long")
+    page = shape[2] * shape[3] * pages.element_size()
+    ids = array("i", src), array("i", dst)  # (OverflowError past 32 bits)
     raw, _ = _on(stream, pages)
-    call("rq_pages_copy", ctx.handle, pages.data_ptr(), pages.shape[0], pages.shape[1] * page, pages.shape[1], page,
-         arr(*src), arr(*dst), n, raw)
+    call("rq_pages_copy", ctx.handle, pages.data_ptr(), shape[0], shape[1] * page, shape[1], page,
+         ids[0].buffer_info()[0], ids[1].buffer_info()[0], n, raw)
     return pages

@@ -19,9 +19,24 @@
 // different ones of the 64 banks (256 bytes).
 #pragma once
 
+#include <atomic>
+
 #include "rq_internal.h"
 
 namespace rq {
+
+// Lets a kernel take `bytes` of dynamic LDS on the current device; `allowed` has a bit for
+// each device that knows.
+inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>* allowed) {
+  if (bytes <= 65536) return hipSuccess;
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev)) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (allowed->load(std::memory_order_acquire) & bit) return hipSuccess;
+  if (hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  allowed->fetch_or(bit, std::memory_order_acq_rel);
+  return hipSuccess;
+}
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));

@@ -6,6 +6,7 @@
 // rows that start at a multiple of 16 lie in one page: a page number is looked up once
 // for them, by the whole wave.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "attn_tile.h"
@@ -24,6 +25,12 @@ __device__ __forceinline__ void rope_angle(int64_t pos, int i, int head_dim, dou
   sincospi(2.0 * t, &sd, &cd);
   *c = (float)cd;
   *s = (float)sd;
+}
+
+// ranges of a sequence of len cached rows: the last may hold one row more, which is the
+// new row's place in a cache that is full with it
+__host__ __device__ __forceinline__ int64_t ranges_of(int64_t len, int64_t rows) {
+  return len > rows + 1 ? (len - 1 + rows - 1) / rows : 1;
 }
 
 constexpr int kPagedThreads = 256, kPagedWaves = 4, kRec = 4;
@@ -47,6 +54,14 @@ __device__ __forceinline__ void split_terms(float x, __bf16 (&t)[NT]) {
 
 }  // namespace
 
+namespace {
+// LDS of 16 heads' queries as fragments: f32, or one or three bf16 terms
+template <typename A, typename C>
+constexpr int paged_query_bytes(int hd) {
+  return 16 * hd * (sizeof(C) == 4 ? 4 : sizeof(A) == 2 ? 2 : 6);
+}
+}  // namespace
+
 // One workgroup: up to 16 query heads of a KV head, one range of a sequence's
 // cached rows; its four waves take tiles of 32 rows in turn. With 16x16 MFMAs (operand: lane
 // l row l % 16, k slots of group g = l / 16; result: column l % 16, rows 4 g + i) the wave forms
@@ -65,17 +80,17 @@ template <typename A, typename C, int HD, bool PART>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;
   constexpr int NT = F32 || sizeof(A) == 2 ? 1 : 3;
+  constexpr int kQueryBytes = paged_query_bytes<A, C>(HD);
   constexpr int E = HD / 16, KS = F32 ? HD / 16 : HD / 32, PE = 16 / (int)sizeof(C);
   constexpr int VP = E > PE ? E / PE : 1;     // 16-byte pieces of a lane's V elements
   constexpr int VW = E * (int)sizeof(C) / 4 / VP;  // words of a piece: 2 or 4
   extern __shared__ __attribute__((aligned(16))) float sm[];
   const PagesArgs& p = a.p;
-  const int hd = p.head_dim, half = hd / 2, group = p.n_q / p.n_kv, htiles = (group + 15) / 16;
-  float* qr = sm;              // [16][HD]
-  float* kr = qr + 16 * HD;    // [HD]
-  float* vn = kr + HD;         // [HD]
-  float* wacc = vn + HD;       // [waves][16][HD]; before that cos and sin [2][HD / 2]
-  float* wm = wacc + kPagedWaves * 16 * HD;  // [waves][16]
+  const int hd = p.head_dim, half = hd / 2, group = p.n_q / p.n_kv, htiles = (group + 15) / 16, nh = min(group, 16);
+  float* kr = sm + kQueryBytes / 4;  // [HD]; before it the queries as fragments, [term][step][lane] 16 bytes
+  float* vn = kr + HD;               // [HD]
+  float* wacc = vn + HD;       // [waves][heads][HD]; before that cos and sin [2][HD / 2]
+  float* wm = wacc + kPagedWaves * nh * HD;  // [waves][16]
   float* wl = wm + kPagedWaves * 16;
   float* ns = wl + kPagedWaves * 16;  // [16]
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
@@ -87,6 +102,33 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
   id /= p.n_kv;
   const int b = id % p.batch, split = id / p.batch;
   const int hq0 = hkv * group + ht * 16, heads = min(group - ht * 16, 16);
+  constexpr int KT = 32, STEP = KT * kPagedWaves;
+  // the query rows and the new row, and the wave's first page numbers: asked for with the
+  // length, not after it
+  constexpr int NQ = HD / 32;  // pairs of query elements a thread
+  const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + hq0 * hd;
+  A q0[NQ], q1[NQ], n0[2], n1[2];  // n: of the new k and v
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    const int i = min(tid + n * kPagedThreads, heads * half - 1), hh = i / half, e = i - hh * half;
+    q0[n] = qrow[hh * hd + e];
+    q1[n] = qrow[hh * hd + e + half];
+  }
+  if (p.k != nullptr) {
+    const A* krow = static_cast<const A*>(p.k) + (int64_t)b * p.k_stride + hkv * hd;
+    const A* vrow = static_cast<const A*>(p.v) + (int64_t)b * p.v_stride + hkv * hd;
+    const int e = min(tid, half - 1);
+    n0[0] = krow[e], n0[1] = krow[e + half];
+    n1[0] = vrow[e], n1[1] = vrow[e + half];
+  }
+  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  const int r0 = split * a.split_rows, first = r0 + wave * KT;
+  const int last_entry = max((int)p.table_stride - 1, 0);
+  int page0 = -1, page1 = -1;
+  if (p.table_stride > 0) {
+    page0 = trow[min(first >> p.page_bits, last_entry)];
+    page1 = trow[min((first + 16) >> p.page_bits, last_entry)];
+  }
   const int len = a.lens[b];
   const bool add = p.k != nullptr;
   A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + hq0 * hd;
@@ -97,139 +139,163 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
       for (int i = tid; i < heads * hd; i += kPagedThreads) orow[i] = (A)(bad && len >= 0 ? NAN : 0.0f);
     return;
   }
-  const int nsplit = max(1, (len + a.split_rows - 1) / a.split_rows);
+  // one row past a whole number of ranges goes to the last range
+  const int nsplit = ranges_of(len, a.split_rows);
   if (split >= nsplit) return;
-  const int r0 = split * a.split_rows, r1 = min(r0 + a.split_rows, len);
-  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  const int r1 = split == nsplit - 1 ? len : r0 + a.split_rows;
   const int kvd = p.n_kv * hd;
   bool lost = false;  // a page number out of range
 
   // the page rows of 16 rows from r (a multiple of 16; past the end: of the range's first)
-  auto base_of = [&](int r) -> int64_t {
-    r = r < r1 ? r : r0;
-    const int page = trow[r >> p.page_bits];
+  auto row_base = [&](int page, int r) -> int64_t {
     const bool ok = (uint32_t)page < (uint64_t)p.pages;
     lost |= !ok;
     return ((int64_t)(ok ? page : 0) << p.page_bits) + (r & ((1 << p.page_bits) - 1));
   };
+  auto base_of = [&](int r) -> int64_t {
+    r = r < r1 ? r : r0;
+    return row_base(trow[r >> p.page_bits], r);
+  };
   const C* kb = static_cast<const C*>(p.kpages) + hkv * hd;
   const C* vb = static_cast<const C*>(p.vpages) + hkv * hd;
   typedef uint32_t VPiece __attribute__((ext_vector_type(VW)));
-  struct Rows {
-    u32x4 k[2][KS];
-    VPiece v[8][VP];
-  };
-  constexpr int VE = E / VP;  // elements of a piece; past the head's end it forms rows that nobody stores
-  auto load = [&](Rows& x, int r) {
+  u32x4 xk[2][KS];
+  VPiece xv[8][VP];
+  auto load_k = [&](int64_t (&base)[2]) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      const int64_t base = base_of(r + 16 * t);
-      const C* kp = kb + (base + col) * kvd;
+      const C* kp = kb + (base[t] + col) * kvd;
 #pragma unroll
       for (int s = 0; s < KS; s++) {
         const int d = (F32 ? 16 * s : 32 * s) + PE * g;
-        x.k[t][s] = *reinterpret_cast<const u32x4*>(kp + (PART ? min(d, hd - PE) : d));
+        xk[t][s] = *reinterpret_cast<const u32x4*>(kp + (PART ? min(d, hd - PE) : d));
       }
+    }
+  };
+  constexpr int VE = E / VP;  // elements of a piece; past the head's end it forms rows that nobody stores
+  auto load_v = [&](int64_t (&base)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int q = 0; q < VP; q++)
-          x.v[4 * t + j][q] = *reinterpret_cast<const VPiece*>(
-              vb + (base + 4 * g + j) * kvd + (PART ? min(E * col + VE * q, hd - VE) : E * col + VE * q));
+          xv[4 * t + j][q] = *reinterpret_cast<const VPiece*>(
+              vb + (base[t] + 4 * g + j) * kvd + (PART ? min(E * col + VE * q, hd - VE) : E * col + VE * q));
+  };
+  int64_t base[2] = {0, 0};
+  if (first < r1) {
+    base[0] = row_base(page0, first);
+    base[1] = first + 16 < r1 ? row_base(page1, first + 16) : base[0];
+    load_k(base);
+    load_v(base);
+  }
+
+  // the rotated queries as the products' operands (zeros for heads and elements past the
+  // end), and the new row as it is stored
+  float* cs = wacc;
+  if (p.rope && tid < half) rope_angle(len, tid, hd, p.log2_theta, cs + tid, cs + HD / 2 + tid);
+  for (int i = tid; i < kQueryBytes / 16; i += kPagedThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
+  __syncthreads();
+  // element e of head hh: lane 16 g + hh of a step holds 32 s + 8 g .. + 7 (f32: 16 s + 4 g .. + 3)
+  auto put_query = [&](int hh, int e, float x) {
+    if constexpr (F32) {
+      sm[((e >> 4) * 64 + ((e >> 2) & 3) * 16 + hh) * 4 + (e & 3)] = x;
+    } else {
+      __bf16 t[NT];
+      split_terms<NT>(x, t);
+      __bf16* at = reinterpret_cast<__bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
+#pragma unroll
+      for (int n = 0; n < NT; n++) at[n * 16 * HD] = t[n];
     }
   };
-  constexpr int KT = 32, STEP = KT * kPagedWaves;
-  Rows x[2];
-  const int first = r0 + wave * KT;
-  if (first < r1) load(x[0], first);
-
-  // the rotated queries (zeros for heads and elements past the end), and the new row as it is stored
-  float* cs = wacc;
-  if (p.rope)
-    for (int i = tid; i < half; i += kPagedThreads) rope_angle(len, i, hd, p.log2_theta, cs + i, cs + HD / 2 + i);
-  for (int i = tid; i < 16 * HD; i += kPagedThreads) qr[i] = 0.0f;
-  __syncthreads();
-  const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + hq0 * hd;
-  for (int i = tid; i < heads * half; i += kPagedThreads) {
-    const int hh = i / half, e = i - hh * half;
-    const float c = p.rope ? cs[e] : 1.0f, s = p.rope ? cs[HD / 2 + e] : 0.0f;
-    const float x0 = (float)qrow[hh * hd + e], x1 = (float)qrow[hh * hd + e + half];
-    qr[hh * HD + e] = x0 * c - x1 * s;
-    qr[hh * HD + e + half] = x1 * c + x0 * s;
+  auto get_query = [&](int hh, int e) {
+    if constexpr (F32) {
+      return sm[((e >> 4) * 64 + ((e >> 2) & 3) * 16 + hh) * 4 + (e & 3)];
+    } else {
+      const __bf16* at = reinterpret_cast<const __bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
+      float x = 0.0f;
+#pragma unroll
+      for (int n = NT - 1; n >= 0; n--) x += (float)at[n * 16 * HD];
+      return x;
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    const int i = tid + n * kPagedThreads, hh = i / half, e = i - hh * half;
+    if (i < heads * half) {
+      const float c = p.rope ? cs[e] : 1.0f, s = p.rope ? cs[HD / 2 + e] : 0.0f;
+      const float x0 = (float)q0[n], x1 = (float)q1[n];
+      put_query(hh, e, x0 * c - x1 * s);
+      put_query(hh, e + half, x1 * c + x0 * s);
+    }
   }
   const bool last = split == nsplit - 1;
-  if (add) {
+  if (add && (last || split == 0)) {
     const int page = trow[len >> p.page_bits];
     const bool ok = (uint32_t)page < (uint64_t)p.pages;
     lost |= !ok;
     const int64_t at = (((int64_t)(ok ? page : 0) << p.page_bits) + (len & ((1 << p.page_bits) - 1))) * kvd + hkv * hd;
-    const bool write = ok && split == 0 && ht == 0;
-    const A* krow = static_cast<const A*>(p.k) + (int64_t)b * p.k_stride + hkv * hd;
-    const A* vrow = static_cast<const A*>(p.v) + (int64_t)b * p.v_stride + hkv * hd;
-    for (int e = tid; e < half; e += kPagedThreads) {
-      const float c = p.rope ? cs[e] : 1.0f, s = p.rope ? cs[HD / 2 + e] : 0.0f;
-      const float x0 = (float)krow[e], x1 = (float)krow[e + half];
-      const C k0 = (C)(x0 * c - x1 * s), k1 = (C)(x1 * c + x0 * s), v0 = (C)(float)vrow[e],
-              v1 = (C)(float)vrow[e + half];
-      kr[e] = (float)k0;
-      kr[e + half] = (float)k1;
-      vn[e] = (float)v0;
-      vn[e + half] = (float)v1;
-      if (write) {
-        C *ko = static_cast<C*>(p.kpages) + at, *vo = static_cast<C*>(p.vpages) + at;
-        ko[e] = k0;
-        ko[e + half] = k1;
-        vo[e] = v0;
-        vo[e + half] = v1;
+    if (tid < half) {
+      const float c = p.rope ? cs[tid] : 1.0f, s = p.rope ? cs[HD / 2 + tid] : 0.0f;
+      const float x0 = (float)n0[0], x1 = (float)n0[1];
+      const C k0 = (C)(x0 * c - x1 * s), k1 = (C)(x1 * c + x0 * s), v0 = (C)(float)n1[0], v1 = (C)(float)n1[1];
+      kr[tid] = (float)k0;
+      kr[tid + half] = (float)k1;
+      vn[tid] = (float)v0;
+      vn[tid + half] = (float)v1;
+      if (ok && split == 0 && ht == 0) {
+        C *ko = static_cast<C*>(p.kpages) + at + tid, *vo = static_cast<C*>(p.vpages) + at + tid;
+        ko[0] = k0;
+        ko[half] = k1;
+        vo[0] = v0;
+        vo[half] = v1;
       }
     }
   }
   __syncthreads();
-
-  // query fragments: elements 32 s + 8 g .. (bf16), 16 s + 4 g .. (f32) of head `col`
-  bf16x8 qb[F32 ? 1 : KS][NT];
-  f32x4 qf[F32 ? KS : 1];
-  if constexpr (F32) {
-#pragma unroll
-    for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const f32x4*>(qr + col * HD + 16 * s + 4 * g);
-  } else {
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        __bf16 t[NT];
-        split_terms<NT>(qr[col * HD + 32 * s + 8 * g + j], t);
-#pragma unroll
-        for (int n = 0; n < NT; n++) qb[s][n][j] = t[n];
-      }
-  }
 
   f32x4 acc[E];
 #pragma unroll
   for (int t = 0; t < E; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
-  auto compute = [&](Rows& y, int r) {
+  for (int r = first; r < r1; r += STEP) {
+    const bool more = r + STEP < r1;
+    if (more) {  // (the last tile's rows are in flight or used: their addresses are no more needed)
+      base[0] = base_of(r + STEP);
+      base[1] = base_of(r + STEP + 16);
+    }
     float s[8];
+    f32x4 d[2] = {};
+    int ql = lane;  // read anew for every tile: kept in registers they would cost a wave a SIMD
+    asm volatile("" : "+v"(ql));
+    const u32x4* qp = reinterpret_cast<const u32x4*>(sm) + ql;
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-      f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int ks = 0; ks < KS; ks++) {
+      u32x4 qw[NT];
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        u32x4 kw = y.k[t][ks];
+      for (int n = 0; n < NT; n++) qw[n] = qp[(n * KS + ks) * 64];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        u32x4 kw = xk[t][ks];
         if (PART && (F32 ? 16 * ks : 32 * ks) + PE * g >= hd) kw = u32x4{0, 0, 0, 0};
         if constexpr (F32) {
-          const f32x4 kf = __builtin_bit_cast(f32x4, kw);
+          const f32x4 kf = __builtin_bit_cast(f32x4, kw), qf = __builtin_bit_cast(f32x4, qw[0]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[ks][j], d, 0, 0, 0);
+          for (int j = 0; j < 4; j++) d[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], d[t], 0, 0, 0);
         } else {
 #pragma unroll
           for (int n = 0; n < NT; n++)
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kw), qb[ks][n], d, 0, 0, 0);
+            d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kw),
+                                                           __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; i++) s[4 * t + i] = r + 16 * t + 4 * g + i < r1 ? d[i] : -INFINITY;
     }
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[4 * t + i] = r + 16 * t + 4 * g + i < r1 ? d[t][i] : -INFINITY;
+    if (more) load_k(base);
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i]);
@@ -252,14 +318,14 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
 #pragma unroll
           for (int q = 0; q < VP; q++)
 #pragma unroll
-            for (int w = 0; w < VW; w++) y.v[j][q][w] = 0;
+            for (int w = 0; w < VW; w++) xv[j][q][w] = 0;
     }
     if constexpr (F32) {
 #pragma unroll
       for (int t = 0; t < E; t++)
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(y.v[j][t / PE][t % PE]), s[j], acc[t], 0, 0, 0);
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[j][t / PE][t % PE]), s[j], acc[t], 0, 0, 0);
     } else {
       bf16x8 pb[NT];
 #pragma unroll
@@ -274,7 +340,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
         u32x4 lo, hi;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const uint32_t e0 = y.v[2 * j][w / VW][w % VW], e1 = y.v[2 * j + 1][w / VW][w % VW];
+          const uint32_t e0 = xv[2 * j][w / VW][w % VW], e1 = xv[2 * j + 1][w / VW][w % VW];
           lo[j] = low16_pair(e0, e1);
           hi[j] = high16_pair(e0, e1);
         }
@@ -286,22 +352,17 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
         }
       }
     }
-  };
-  for (int r = first; r < r1; r += 2 * STEP) {
-    if (r + STEP < r1) load(x[1], r + STEP);
-    compute(x[0], r);
-    if (r + STEP >= r1) break;
-    if (r + 2 * STEP < r1) load(x[0], r + 2 * STEP);
-    compute(x[1], r + STEP);
+    if (more) load_v(base);
   }
 
   // the waves' states, then the new row (last range)
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  if (col < nh)
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-    for (int t = 0; t < E; t++) wacc[(wave * 16 + col) * HD + E * (4 * g + i) + t] = acc[t][i];
+      for (int t = 0; t < E; t++) wacc[(wave * nh + col) * HD + E * (4 * g + i) + t] = acc[t][i];
   if (g == 0) {
     wm[wave * 16 + col] = m;
     wl[wave * 16 + col] = l;
@@ -309,7 +370,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
   if (add && last)
     for (int hh = wave; hh < heads; hh += kPagedWaves) {
       float dot = 0.0f;
-      for (int d = lane; d < hd; d += 64) dot += qr[hh * HD + d] * kr[d];
+      for (int d = lane; d < hd; d += 64) dot += get_query(hh, d) * kr[d];
 #pragma unroll
       for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
       if (lane == 0) ns[hh] = dot * a.scale2;
@@ -327,7 +388,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     for (int w = 0; w < kPagedWaves; w++) {
       const float f = __builtin_amdgcn_exp2f(wm[w * 16 + hh] - ref);
       sum += f * wl[w * 16 + hh];
-      o += f * wacc[(w * 16 + hh) * HD + d];
+      o += f * wacc[(w * nh + hh) * HD + d];
     }
     if (add && last) {
       const float e = __builtin_amdgcn_exp2f(sn - ref);
@@ -356,7 +417,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const int hq = blockIdx.x % p.n_q, b = blockIdx.x / p.n_q, hd = p.head_dim, len = a.lens[b];
   const int64_t rows = (int64_t)len + (p.k != nullptr);
   if (len < 0 || rows > a.max_len || rows > p.table_stride << p.page_bits) return;
-  const int n = (len + a.split_rows - 1) / a.split_rows;
+  const int n = ranges_of(len, a.split_rows);
   if (n <= 1) return;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float sums[256 * 4];
@@ -505,12 +566,17 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(char* base, int64_t pla
 
 PagedPlan plan_paged_attention(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
                                int cu_count) {
-  const int64_t group = n_q / n_kv, per_split = std::max<int64_t>(1, batch * n_kv * ((group + 15) / 16));
-  const int64_t want = (max_len * per_split + 4 * cu_count - 1) / (4 * cu_count);
-  const int64_t rows = std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 128), 1024);
+  // About one workgroup a CU at max_len, of 128 to 1024 rows (2048 where a CU has 16 Ki or more):
+  // fewer leave CUs idle, more pay for records and the start of a workgroup. us, rows a range
+  // (bf16 pages): 32/8 heads x 128, one sequence of 4096 rows 128: 12.5, 256: 13.1, 1024: 19.2; of
+  // 32768 256: 34.7, 1024: 30.3; 32 of 0 to 8191 256: 55.0, 1024: 47.0, 2048: 68.6; 64/8 heads, 8 of
+  // 33 to 65 Ki 1024: 363, 2048: 352; 8/4 x 256, 16 of 2000 128: 49.1, 512: 30.9.
+  const int64_t groups = std::max<int64_t>(1, batch * n_kv * ((n_q / n_kv + 15) / 16));
+  const int64_t share = (max_len * groups + cu_count - 1) / std::max(cu_count, 1);
+  const int64_t rows = std::min<int64_t>(std::max<int64_t>((share + 127) / 128 * 128, 128), share >= 16384 ? 2048 : 1024);
   PagedPlan p;
   p.split_rows = (int)rows;
-  p.nsplit = (int)std::max<int64_t>(1, (max_len + rows - 1) / rows);
+  p.nsplit = (int)ranges_of(max_len, rows);
   p.work = p.nsplit > 1 ? (size_t)(batch * n_q * p.nsplit * (kRec + head_dim)) * sizeof(float) : 0;
   return p;
 }
@@ -521,13 +587,12 @@ template <typename A, typename C, int HD, bool PART>
 hipError_t run_paged(const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
   const int64_t htiles = (p.n_q / p.n_kv + 15) / 16;
-  constexpr int lds = (16 * HD + 2 * HD + kPagedWaves * 16 * (HD + 2) + 16) * 4;
+  constexpr int kFixed = paged_query_bytes<A, C>(HD) + (2 * HD + kPagedWaves * 32 + 16) * 4;
+  constexpr int kMaxLds = kFixed + kPagedWaves * 16 * HD * 4;
+  const int lds = kFixed + kPagedWaves * std::min(p.n_q / p.n_kv, 16) * HD * 4;
   const auto kernel = paged_attention_kernel<A, C, HD, PART>;
-  if (lds > 65536) {
-    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds))
-      return e;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), kMaxLds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.nsplit * p.batch * p.n_kv * htiles)), dim3(kPagedThreads), lds, stream,
                      a);
   if (hipError_t e = hipGetLastError()) return e;

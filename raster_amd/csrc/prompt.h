@@ -35,7 +35,5 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
 
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream);
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream);
-// Lets a kernel take `bytes` of dynamic LDS on the current device.
-hipError_t allow_lds(const void* kernel, int bytes);
 
 }  // namespace rq

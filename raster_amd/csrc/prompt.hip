@@ -15,6 +15,7 @@
 // are the B operand of O^T += V^T P^T as they lie. Keys and values pass through LDS
 // in tiles of BK rows for all waves, the next tile's loads in flight meanwhile.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "attn_tile.h"
@@ -305,7 +306,8 @@ hipError_t run_fwd(PromptArgs a, hipStream_t stream) {
   constexpr int lds = 4 * Tile<T, HD>::bytes(BK);
   a.slots = tile_slots(a.rows_q, a.batch, 128);
   const auto kernel = prompt_fwd_kernel<T, HD, BK>;
-  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(256), lds, stream, a);
   return hipGetLastError();
 }
@@ -315,17 +317,13 @@ hipError_t run_fwd_pair(PromptArgs a, hipStream_t stream) {
   constexpr int lds = 5 * Tile<T, HD>::bytes(BK);
   a.slots = tile_slots(a.rows_q, a.batch, 256);
   const auto kernel = prompt_fwd_pair_kernel<T, HD, BK>;
-  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(512), lds, stream, a);
   return hipGetLastError();
 }
 
 }  // namespace
-
-hipError_t allow_lds(const void* kernel, int bytes) {
-  if (bytes <= 65536) return hipSuccess;
-  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
 
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {

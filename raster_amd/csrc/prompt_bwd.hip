@@ -13,6 +13,7 @@
 // in both of the last two: 7 products for the 5 that a single kernel would need, which
 // would have to add dQ from many workgroups.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "attn_tile.h"
@@ -374,7 +375,8 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
   a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, kDqQueries) : 0;
   const auto kernel = prompt_grad_kernel<T, HD, BK>;
-  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds)) return e;
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256), lds,
                      stream, a);
   if (hipError_t e = hipGetLastError()) return e;
