@@ -1572,6 +1572,7 @@ int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_s
   if (int s = check_ctx(c)) return s;
   if (int s = set_device(c)) return s;
   PromptArgs a = prompt_args(p);
+  a.cu_count = c->cu_count;
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
   const hipError_t e = launch_prompt_fwd(p->dtype, a, (hipStream_t)stream);

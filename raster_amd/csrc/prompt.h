@@ -9,7 +9,7 @@ namespace rq {
 struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int64_t rows_q, rows_k, slots, q_slots, k_slots;
-  int batch, n_q, n_kv, head_dim, causal;
+  int batch, n_q, n_kv, head_dim, causal, cu_count;
   float scale, scale2;  // scale2 = scale log2 e
   const void *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;

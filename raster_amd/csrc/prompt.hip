@@ -160,7 +160,7 @@ struct Work {
   bool live;
   const T *k, *v, *q;
   // false: nothing to do
-  __device__ __forceinline__ bool init(const PromptArgs& a, int wave, int lane) {
+  __device__ __forceinline__ bool init(const PromptArgs& a, int wave, int lane) {  // wave: of 32 queries each
     const int group = a.n_q / a.n_kv;
     // ids next to each other go to different XCDs: a KV head's tiles stay on as few as can be
     const int hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
@@ -301,6 +301,84 @@ __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
   x.finish(a, w.hq, w.tq.begin + w.qi, w.live);
 }
 
+// Four waves over the same 32 queries, each with its own 32 of the 128 keys that are staged at
+// a time, and their states joined at the end: for grids that would leave CUs idle with
+// 128 queries a workgroup. One tile in LDS, the next on its way in registers.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
+  using TL = Tile<T, HD>;
+  constexpr int THREADS = 256, BK = 128, kTile = TL::bytes(BK), kWaves = 4;
+  constexpr int kCol = HD + 4;  // floats from query to query of a joined state
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Work<T, 32> w;
+  if (!w.init(a, 0, lane)) return;
+  Stage<T, HD, BK, THREADS> ks, vs;
+  auto load = [&](int kb) {
+    ks.load(w.k + (int64_t)kb * a.k_stride, a.k_stride, w.lk - kb, a.head_dim, tid);
+    vs.load(w.v + (int64_t)kb * a.v_stride, a.v_stride, w.lk - kb, a.head_dim, tid);
+  };
+  if (w.nk > 0) load(0);
+  Queries<T, HD, 32> x;
+  x.init(w.q, a.head_dim, lane);
+  settle(x.q);
+  for (int kb = 0; kb < w.nk; kb += BK) {
+    ks.store(lds, tid);
+    vs.store(lds + kTile, tid);
+    if (kb + BK < w.nk) load(kb + BK);
+    __syncthreads();
+    const int mine = kb + 32 * wave;
+    if (mine < w.nk) {
+      const char* kt = lds + 32 * wave * TL::kPitch;
+      x.scores(kt);
+      x.softmax(mine, w.see, w.cut(a, mine, 32), a.scale2);
+      x.add_values(kt + kTile);
+    }
+    __syncthreads();
+  }
+  // state of wave u: [query][HD weighted values, maximum, sum of the half's keys x 2]
+  float* st = reinterpret_cast<float*>(lds);
+  float* own = st + (wave * 32 + (lane & 31)) * kCol;
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4*>(own + 32 * d + 2 * i + 4 * h) =
+          f32x4{x.acc[d][i], x.acc[d][i + 1], x.acc[d][i + 2], x.acc[d][i + 3]};
+  if (h == 0) own[HD] = x.m;
+  own[HD + 1 + h] = x.l;
+  __syncthreads();
+  // eight threads a query, 4 values each at a time
+  const int qn = tid >> 3, sub = tid & 7, qi = w.tq.row0 + qn;
+  if (qi >= w.tq.len) return;
+  float m = -INFINITY, l = 0.0f, f[kWaves];
+#pragma unroll
+  for (int u = 0; u < kWaves; u++) m = fmaxf(m, st[(u * 32 + qn) * kCol + HD]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+  for (int u = 0; u < kWaves; u++) {
+    const float* s = st + (u * 32 + qn) * kCol + HD;
+    f[u] = __builtin_amdgcn_exp2f(s[0] - ref);
+    l += f[u] * (s[1] + s[2]);
+  }
+  const int64_t row = w.tq.begin + qi;
+  if (a.lse && sub == 0)
+    a.lse[(int64_t)w.hq * a.rows_q + row] = l == 0.0f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a query that sees nothing: zeros
+  T* out = static_cast<T*>(a.out) + row * a.out_stride + w.hq * a.head_dim;
+  for (int e = 4 * sub; e < a.head_dim; e += 32) {
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kWaves; u++) y += f[u] * *reinterpret_cast<const f32x4*>(st + (u * 32 + qn) * kCol + e);
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 z;
+#pragma unroll
+    for (int j = 0; j < 4; j++) z[j] = (T)(y[j] * inv);
+    *reinterpret_cast<T4*>(out + e) = z;
+  }
+}
+
 template <typename T, int HD, int BK>
 hipError_t run_fwd(PromptArgs a, hipStream_t stream) {
   constexpr int lds = 4 * Tile<T, HD>::bytes(BK);
@@ -323,9 +401,40 @@ hipError_t run_fwd_pair(PromptArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T, int HD>
+hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
+  constexpr int lds = std::max(2 * Tile<T, HD>::bytes(128), 4 * 32 * (HD + 4) * 4);
+  a.slots = tile_slots(a.rows_q, a.batch, 32);
+  const auto kernel = prompt_fwd_split_kernel<T, HD>;
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(256), lds, stream, a);
+  return hipGetLastError();
+}
+
 }  // namespace
 
+// Whether the split kernel is the faster: the other's grid leaves CUs idle (`most` workgroups
+// for every 256 CUs, by type and head), unless there is hardly a tile of keys to split. us, split
+// / whole, causal, 16/16 heads x 128 unless said (workgroups of the whole kernel):
+//   bf16  37 tokens (16) 8.2 / 6.9   512 (80) 13.2 / 17.0   1024 (144) 26.5 / 28.2   2048 (272) 73 / 52
+//         64 after 4032 (16) 56 / 75   32/8 heads: 512 (160) 20.0 / 17.7   4 x 64 after 4032 (192) 60 / 76
+//   bf16  16/2 x 64: 1024 (144) 13.9 / 23.3   2048 (272) 28.9 / 41.8   8 x 256 (384) 13.9 / 10.6
+//   f32   512 (80) 39 / 81   1024 (144) 81 / 155   2048 (272) 268 / 302   8 x 256 (384) 75 / 48
+//   f32   16/2 x 64: 2048 (272) 98 / 166   8 x 256 (384) 31 / 31   8 x 512 (640) 76 / 81
+static bool fwd_splits(int dtype, const PromptArgs& a) {
+  if (a.head_dim > 128 || a.rows_k < 64 * (int64_t)a.batch) return false;
+  const bool few_queries = a.rows_k >= 4 * a.rows_q;
+  const int most = dtype == RQ_F32 ? (a.head_dim <= 64 ? 640 : 320) : a.head_dim <= 64 ? 320 : few_queries ? 256 : 144;
+  return tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 <= (int64_t)most * a.cu_count;
+}
+
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+  if (fwd_splits(dtype, a)) {
+    if (dtype == RQ_BF16)
+      return a.head_dim <= 64 ? run_fwd_split<__bf16, 64>(a, stream) : run_fwd_split<__bf16, 128>(a, stream);
+    return a.head_dim <= 64 ? run_fwd_split<float, 64>(a, stream) : run_fwd_split<float, 128>(a, stream);
+  }
   if (dtype == RQ_BF16) {
     if (a.head_dim <= 64) return run_fwd<__bf16, 64, 64>(a, stream);
     // The pair kernel reads keys and values half as often but cuts the queries in tiles of 256.
