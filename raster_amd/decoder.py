@@ -27,6 +27,11 @@ output element. Two ways to run the glue:
                    restatement kept as the second path of the parity tests).
 
 A whole step can be captured in one HIP graph (no call allocates).
+
+Batches of sequences run over a PagedCache (paged.py): prefill takes the packed
+prompts through a layer (pages_append, prompt_attention), step_paged one new
+token of each sequence (paged_attention), with the fused linears up to 16
+sequences and the unfused glue beyond.
 """
 from __future__ import annotations
 
@@ -36,6 +41,7 @@ from ctypes import byref
 import numpy as np
 
 from ._lib import RQ_F32, FusedOps, call
+from .attention import paged_attention, pages_append, prompt_attention
 from .quant import Context, QWeight, _current_stream, _need, _t
 
 
@@ -175,6 +181,54 @@ class DecoderLayer:
         linear(self.w_gu, x1, h, gain=self.g2.data_ptr(), swiglu=1)
         linear(self.w_d, h, out.data_ptr(), residual=x1)
         return out
+
+    def _mlp(self, x1):
+        """x1 + down(silu(gate) * up) of x1's rows, with torch glue."""
+        torch = _t()
+        gu = self.w_gu.matmul(rms_norm(torch, x1, self.g2, self.eps))
+        gate, up = (gu[:, 0::2], gu[:, 1::2]) if self.fused else (gu[:, :self.ffn], gu[:, self.ffn:])
+        return residual_add(x1, self.w_d.matmul(silu_mul(torch, gate, up).contiguous()))
+
+    def _split_qkv(self, qkv):
+        qd, kvd = self.n_q * self.hd, self.n_kv * self.hd
+        return qkv[:, :qd], qkv[:, qd:qd + kvd], qkv[:, qd + kvd:]
+
+    def prefill(self, x, cu, cache, layer: int, seqs, lens):
+        """Packed prompts through the layer: x f32 [rows, d], rows cu[b] .. cu[b+1] - 1
+        (int32 [batch + 1] on the device; ranges of lens[b] rows) the next tokens of cache sequence
+        seqs[b], for which cache.reserve has made room. Their keys and values go
+        into the cache's pages of `layer`; each token attends its sequence up to
+        itself, rows stored before included. Returns [rows, d]. After the last
+        layer, cache.advance(seqs, lens)."""
+        torch = _t()
+        view = cache.view(seqs)
+        q, k, v = self._split_qkv(self.w_qkv.matmul(rms_norm(torch, x, self.g1, self.eps)))
+        pages_append(self.ctx, q, k, v, cache.kpages(layer), cache.vpages(layer), view.table, cu, view.lens, self.n_q,
+                     self.n_kv, self.hd, self.theta, q_out=q, k_out=k)
+        cu_k = None
+        past = [cache.length(s) for s in seqs]
+        if any(past):  # rows stored before: the keys are the cache's, the new rows among them
+            k, v = (t.to(x.dtype) for t in cache.rows(layer, seqs, lens))
+            ends = np.cumsum([0] + [n0 + n for n0, n in zip(past, lens)])
+            cu_k = torch.tensor(ends, dtype=torch.int32, device=x.device)
+        at = prompt_attention(self.ctx, q, k, v, cu, self.n_q, self.n_kv, self.hd, 1.0 / math.sqrt(self.hd), cu_k=cu_k)
+        return self._mlp(residual_add(x, self.w_o.matmul(at)))
+
+    def step_paged(self, x, cache, layer: int, view):
+        """One new token of each sequence of `view` (cache.view): x f32 [batch, d] ->
+        [batch, d]. k and v are appended at the sequences' lengths (room reserved
+        before); after the last layer, cache.advance(seqs, 1)."""
+        fused = self.fused and x.shape[0] <= 16
+        xn = None if fused else rms_norm(_t(), x, self.g1, self.eps)
+        qkv = self.w_qkv.matmul_fused(x, norm_gain=self.g1, norm_eps=self.eps) if fused else self.w_qkv.matmul(xn)
+        at = paged_attention(self.ctx, *self._split_qkv(qkv), cache.kpages(layer), cache.vpages(layer), view.table,
+                             view.lens, self.n_q, self.n_kv, self.hd, self.theta, 1.0 / math.sqrt(self.hd),
+                             max_len=view.max_len)
+        if not fused:
+            return self._mlp(residual_add(x, self.w_o.matmul(at)))
+        x1 = self.w_o.matmul_fused(at, residual=x)
+        h = self.w_gu.matmul_fused(x1, norm_gain=self.g2, norm_eps=self.eps, swiglu=True)
+        return self.w_d.matmul_fused(h, residual=x1)
 
     def matmul_bytes(self) -> int:
         """Algorithmic weight bytes the step streams (codes + f32 scales)."""

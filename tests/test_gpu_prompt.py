@@ -70,6 +70,10 @@ CASES = [
     ("bf16", 2, 2, 128, [5, 64, 100], [300, 64, 40]),     # the end of a sequence; more queries than keys
     ("bf16", 2, 2, 128, [40, 0, 7], [0, 50, 3]),          # no keys, no queries
     ("bf16", 2, 2, 128, [1500], [1500]),
+    ("bf16", 64, 8, 128, [300, 129, 40], [300, 129, 40]),  # grids that fill the CUs: keys not split
+    ("bf16", 64, 8, 64, [300, 129, 90], [300, 129, 90]),
+    ("f32", 64, 8, 128, [300, 129, 90], [300, 129, 90]),
+    ("f32", 128, 8, 40, [300, 129, 90], [300, 129, 90]),
     ("f32", 4, 4, 128, [1], [1]),
     ("f32", 4, 2, 128, [33, 0, 130], [33, 0, 130]),
     ("f32", 6, 2, 64, [65, 200], [65, 200]),
@@ -93,6 +97,22 @@ def test_forward(torch, ctx, t, nq, nkv, hd, lq, lk, is_causal):
     out = raster_amd.prompt_attention(ctx, q, k, v, cu_of(torch, lq), nq, nkv, hd, scale, causal=is_causal,
                                       cu_k=None if lq == lk else cu_of(torch, lk), lse=lse)
     check_forward(torch, q, k, v, out, lse, lq, lk, nq, nkv, hd, scale, is_causal)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,lq,lk", [(8, 2, 128, [4600], [4600]), (6, 6, 72, [5000, 4000], [5000, 4700])])
+def test_long_sequences(torch, ctx, nq, nkv, hd, lq, lk):
+    """The kernel of long sequences (bf16, more than 4096 queries each on average)."""
+    import raster_amd
+
+    print(f"[gpu] prompt long {nq}/{nkv}x{hd} {lq} {lk}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(sum(lq))
+    q, k, v = (rows(torch, g, sum(n), w * hd, torch.bfloat16) for n, w in ((lq, nq), (lk, nkv), (lk, nkv)))
+    scale, lse = hd ** -0.5, torch.empty((nq, sum(lq)), device="cuda")
+    cu_k = None if lq == lk else cu_of(torch, lk)
+    for is_causal in (True, False):
+        out = raster_amd.prompt_attention(ctx, q, k, v, cu_of(torch, lq), nq, nkv, hd, scale, causal=is_causal,
+                                          cu_k=cu_k, lse=lse)
+        check_forward(torch, q, k, v, out, lse, lq, lk, nq, nkv, hd, scale, is_causal)
 
 
 @pytest.mark.parametrize("t,nq,nkv,hd,lq,lk", [c for c in CASES if max(c[4]) <= 400])
