@@ -517,7 +517,8 @@ int rq_linear(rq_ctx ctx, const float* x, const float* w, const float* b, float*
  * head h reads KV head h / (n_q/n_kv); all asynchronous on `stream`, nothing
  * allocated and no scratch of the context used, so any number of calls and
  * captured graphs may run at once as long as their buffers differ. Results do not
- * depend on scheduling. */
+ * depend on scheduling. A call whose largest launch would need 2^24 workgroups or more
+ * (a prompt's (rows / 32 + batch) * n_q, an append's rows) fails with RQ_ERR_SHAPE. */
 
 /* A packed batch of sequences. Sequence b's queries are the rows cu_q[b] ..
  * cu_q[b+1] - 1 of q, out and dout, its keys the rows cu_k[b] .. cu_k[b+1] - 1
@@ -539,7 +540,8 @@ typedef struct {
  * prompt). A query that sees no key, or only scores of -inf, gets zeros and lse
  * -inf. lse f32[n_q][rows_q], or NULL. f32: products and sums in f32; bf16: products of
  * bf16, weights rounded to bf16 for theirs, sums, maxima and lse in f32. A NaN or
- * an inf in v also reaches the queries before it within its tile of keys. */
+ * an inf in v also reaches the queries before it within its tile of keys (the masked weight
+ * is 0, and 0 times them is a NaN). */
 int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
                         void* stream);
@@ -548,7 +550,8 @@ int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q
  * dq, dk and dv (fully overwritten in every row of a sequence, dk and dv summed
  * over the query heads of a KV head; none may overlap an input). p_ij is
  * recomputed from lse. f32: in f32; bf16: products of bf16 with p and its gradient
- * rounded to bf16, sums in f32. work: rq_prompt_attention_bwd_work bytes of
+ * rounded to bf16, sums in f32. A NaN or an inf in k reaches dq, one in q or dout dk and dv,
+ * of masked rows too within its tile. work: rq_prompt_attention_bwd_work bytes of
  * device memory (the rows' dout . out, and partial sums where few keys leave
  * compute units idle), 16-byte aligned, used by this call alone until it has run. */
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes);
@@ -561,8 +564,8 @@ int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, in
 /* One layer's cache in pages: kpages and vpages hold `pages` pages of page_size
  * rows (a power of two, 16 to 65536) of n_kv * head_dim elements, a row of
  * rq_decode_attention's caches each. Row r of sequence b lies in page
- * table[b * table_stride + r / page_size] at r % page_size (device int32, read
- * only as far as the sequence has rows). */
+ * table[b * table_stride + r / page_size] at r % page_size (device int32;
+ * entries past a sequence's rows may hold anything). */
 typedef struct {
   int dtype; /* RQ_F32 or RQ_BF16: the pages */
   void* kpages;
@@ -599,7 +602,8 @@ int rq_paged_attention(rq_ctx ctx, const rq_pages* pg, int dtype, const void* q,
 
 /* A packed prompt into the pages: sequence b's rows cu[b] .. cu[b+1] - 1 (as in
  * rq_prompt) are its positions past[b], past[b] + 1, ...: q_out and, unless NULL,
- * k_out get the rotated q and k in their own type (either may be its input), and
+ * k_out get the rotated q and k in their own type (either may be its input, else they overlap
+ * nothing), and
  * the pages the rotated k and v. past[b] < 0: the sequence is left out. Rows whose
  * page is missing (as in rq_paged_attention) get NaN in q_out and k_out and are not stored.
  * Types as for rq_paged_attention; theta 0: no rotation. */

@@ -1487,9 +1487,7 @@ static int check_prompt(const rq_prompt* p) {
   if (int s = check_heads(p->n_q, p->n_kv, p->head_dim)) return s;
   if (p->batch < 0 || p->rows_q < 0 || p->rows_k < 0) return fail(RQ_ERR_SHAPE, "negative dimension");
   if (p->rows_q > kMaxRows || p->rows_k > kMaxRows || p->batch > kMaxRows) return fail(RQ_ERR_SHAPE, "too many rows");
-  // (the gradient's grid holds a workgroup of 64 keys, at most 16 parts each where there are few, and of 128 queries)
-  if ((p->rows_q / 32 + p->batch) * p->n_q > INT32_MAX / 32 || (p->rows_k / 32 + p->batch) * p->n_q > INT32_MAX / 32 ||
-      p->rows_q * p->n_q > (int64_t)INT32_MAX * 8)
+  if (tile_slots(p->rows_q, p->batch, 32) * p->n_q > kMaxGroups)
     return fail(RQ_ERR_SHAPE, "rows times heads too large for one launch");
   if (!p->cu_k && p->rows_k != p->rows_q) return fail(RQ_ERR_SHAPE, "without cu_k, rows_k must be rows_q");
   if (int s = check_scale(p->scale)) return s;
@@ -1597,6 +1595,7 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
   if (p->batch == 0 || (p->rows_q == 0 && p->rows_k == 0)) return RQ_OK;
   const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
   const PromptBwdPlan plan = plan_prompt_bwd(p->batch, p->rows_q, p->rows_k, p->n_q, p->n_kv, p->head_dim);
+  if (plan.groups > kMaxGroups) return fail(RQ_ERR_SHAPE, "rows times heads too large for one launch");
   if (int s = check_i32("cu_q", p->cu_q)) return s;
   if (p->cu_k)
     if (int s = check_i32("cu_k", p->cu_k)) return s;
@@ -1665,7 +1664,7 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
   if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
   const int64_t htiles = (n_q / pg->n_kv + 15) / 16;
-  if (plan.nsplit > INT32_MAX / (batch * pg->n_kv * htiles) || batch * n_q > INT32_MAX)
+  if (plan.nsplit > kMaxGroups / (batch * pg->n_kv * htiles) || batch * n_q > kMaxGroups)
     return fail(RQ_ERR_SHAPE, "batch times heads times rows too large for one launch");
   if (int s = set_device(c)) return s;
   PagedAttnArgs a = {};
@@ -1691,7 +1690,8 @@ int rq_pages_append(rq_ctx h, const rq_pages* pg, int dtype, const void* q, int6
                     void* k_out, int64_t k_out_stride, void* stream) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
   if (int s = check_pages(pg, dtype, n_q, theta)) return s;
-  if (batch < 0 || batch > kMaxRows || rows < 0 || rows > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (batch < 0 || batch > kMaxRows || rows < 0) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (rows > kMaxGroups) return fail(RQ_ERR_SHAPE, "too many rows for one launch");
   if (batch == 0 || rows == 0) return RQ_OK;
   const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
   if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
@@ -1730,7 +1730,7 @@ int rq_pages_copy(rq_ctx h, void* base, int64_t planes, int64_t plane_bytes, int
   if (!base || !src || !dst) return fail(RQ_ERR_NULL, "NULL argument");
   if (((uintptr_t)base & 15) != 0) return fail(RQ_ERR_SHAPE, "base must be 16-byte aligned");
   if (n > pages) return fail(RQ_ERR_SHAPE, "more copies than pages");
-  if (planes > (int64_t)1 << 20 || pages_copy_groups(page_bytes) * planes > INT32_MAX / 256)
+  if (planes > (int64_t)1 << 20 || pages_copy_groups(page_bytes) * planes > kMaxGroups)
     return fail(RQ_ERR_SHAPE, "planes times page_bytes too large for one launch");
   try {
     std::vector<int32_t> d(dst, dst + n);

@@ -200,6 +200,9 @@ struct Stage {
   }
 };
 
+// Workgroups of 256 threads in one launch: HIP takes fewer than 2^32 threads.
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
+
 // The sequence and its tile that slot `slot` of a packed batch stands for. With
 // tiles of `rows` rows, sequence b takes the slots floor(cu[b] / rows) + b up to
 // floor(cu[b + 1] / rows) + b, at least as many as it has tiles: the grid is known
@@ -216,17 +219,24 @@ __device__ __forceinline__ int64_t clamp_cu(const int32_t* cu, int64_t b, int64_
   return x < 0 ? 0 : x > total ? total : x;
 }
 
-__device__ __forceinline__ TileSpan tile_of_slot(const int32_t* cu, int batch, int64_t total, int rows, int64_t slot) {
-  // the last sequence whose first slot is not past `slot` (lane-parallel)
+// How many of the first n items, in order, `holds` is true for (true for a first part of them,
+// false after it), by the whole wave: 64 items spread over what is left at a time.
+template <typename F>
+__device__ __forceinline__ int count_first(int n, F holds) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int b0 = 0; b0 < batch; b0 += 64) {
-    const int b = b0 + lane;
-    const bool le = b < batch && clamp_cu(cu, b, total) / rows + b <= slot;
-    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(le));
-    n += c;
-    if (c < 64) break;
+  int lo = 0;
+  for (;;) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < n && holds(lo + at)));
+    if (step <= 1 || c == 0) return lo + c;
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
   }
+}
+
+__device__ __forceinline__ TileSpan tile_of_slot(const int32_t* cu, int batch, int64_t total, int rows, int64_t slot) {
+  // the last sequence whose first slot is not past `slot`
+  const int n = count_first(batch, [&](int b) { return clamp_cu(cu, b, total) / rows + b <= slot; });
   TileSpan t{0, 0, 0, 0};
   if (n == 0) return t;
   t.seq = n - 1;

@@ -465,13 +465,7 @@ __global__ __launch_bounds__(256) void pages_append_kernel(PagesAppendArgs a) {
   const int tid = threadIdx.x, hd = p.head_dim, half = hd / 2;
   const int64_t row = blockIdx.x;
   // the last sequence that starts at or before the row
-  int n = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const int b = b0 + (tid & 63);
-    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(b < p.batch && a.cu[b] <= row));
-    n += c;
-    if (c < 64) break;
-  }
+  const int n = count_first(p.batch, [&](int b) { return a.cu[b] <= row; });
   if (n == 0 || row >= a.cu[n]) return;  // a row of no sequence: left as it is
   const int b = n - 1, past = a.past[b];
   if (past < 0) return;
@@ -639,9 +633,10 @@ int64_t pages_copy_groups(int64_t page_bytes) { return (page_bytes + kCopyBytes 
 hipError_t launch_pages_copy(void* base, int64_t planes, int64_t plane_bytes, int64_t page_bytes, const int32_t* src,
                              const int32_t* dst, int64_t n, hipStream_t stream) {
   const int64_t parts = pages_copy_groups(page_bytes);
-  for (int64_t i = 0; i < n; i += kCopyPairs) {
+  const int64_t most = std::min<int64_t>(kCopyPairs, kMaxGroups / (parts * planes));
+  for (int64_t i = 0; i < n; i += most) {
     CopyPairs pairs;
-    const int m = (int)std::min<int64_t>(kCopyPairs, n - i);
+    const int m = (int)std::min<int64_t>(most, n - i);
     std::copy(src + i, src + i + m, pairs.src);
     std::copy(dst + i, dst + i + m, pairs.dst);
     hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)(parts * m * planes)), dim3(256), 0, stream,

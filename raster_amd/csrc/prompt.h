@@ -28,6 +28,7 @@ struct PromptArgs {
 
 struct PromptBwdPlan {
   int nsplit;
+  int64_t groups;  // of the largest launch
   size_t delta_bytes, work;
 };
 PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,

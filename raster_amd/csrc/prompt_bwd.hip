@@ -399,6 +399,8 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
   const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / kDkvQueries * (n_q / n_kv);
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
+  p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, kDqQueries) * n_q,
+                      (rows_q * n_q * kDeltaLanes + 255) / 256);
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
   p.work = p.delta_bytes + (p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0);
   return p;

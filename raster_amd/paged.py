@@ -48,9 +48,9 @@ class PagedCache:
         self._pages: dict[int, list[int]] = {}
         self._len: dict[int, int] = {}
         self._slots = list(range(max_seqs))
-        self._host_table = np.zeros((max_seqs, seq_pages or pages), np.int32)
+        self._host_table = np.full((max_seqs, seq_pages or pages), -1, np.int32)  # (-1: no page, refused by the operators)
         self._host_lens = np.full(max_seqs, -1, np.int32)
-        self._table = torch.zeros(self._host_table.shape, dtype=torch.int32, device=dev)
+        self._table = torch.full(self._host_table.shape, -1, dtype=torch.int32, device=dev)
         self._lens = torch.full((max_seqs,), -1, dtype=torch.int32, device=dev)
         self._dirty = False
 
@@ -175,7 +175,7 @@ class PagedCache:
         for p in self._pages.pop(self._known(seq)):
             self._drop(p)
         del self._len[seq]
-        self._host_lens[seq] = -1
+        self._host_lens[seq], self._host_table[seq] = -1, -1
         heapq.heappush(self._slots, seq)
         self._dirty = True
 

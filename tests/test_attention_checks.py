@@ -153,3 +153,22 @@ def test_pages_copy():
         assert copy([0], [2], **kw) == RQ_ERR_SHAPE, kw
     assert copy([0], [2], base=None) == RQ_ERR_NULL
     assert copy([], []) == RQ_OK and copy([0], [2], planes=0) == RQ_OK
+
+
+def test_launches_of_2_32_threads_are_refused():
+    """HIP takes fewer than 2^32 threads a launch: RQ_ERR_SHAPE before it is asked."""
+    def said(status):
+        return status == RQ_ERR_SHAPE and "one launch" in _lib.lib().rq_last_error().decode()
+
+    assert said(fwd(prompt(rows_q=2 ** 28, rows_k=2 ** 28)))  # 4 heads x (2^23 + 2) tiles of 32
+    assert fwd(prompt(rows_q=2 ** 26, rows_k=2 ** 26)) == RQ_ERR_HANDLE
+    assert fwd(prompt(rows_k=2 ** 30, cu_k=P)) == RQ_ERR_HANDLE  # keys take no workgroup
+    assert said(fwd(prompt(batch=2 ** 24)))
+    assert said(bwd(prompt(rows_q=2 ** 26, rows_k=2 ** 26), wb=2 ** 40))  # 16 threads a row and head
+    assert bwd(prompt(rows_q=2 ** 25, rows_k=2 ** 25), wb=2 ** 40) == RQ_ERR_HANDLE
+    # 12 parts of the keys' gradient: slots count for each of them
+    assert said(bwd(prompt(batch=2 ** 20, rows_q=2 ** 25, rows_k=64, n_q=8, n_kv=1, cu_k=P), qs=512, dos=512, os=512,
+                    dqs=512, wb=2 ** 40))
+    assert said(append(pages(), rows=2 ** 24)) and append(pages(), rows=2 ** 24 - 1) == RQ_ERR_HANDLE
+    big = dict(plane_bytes=2 ** 33, pages=8, page_bytes=2 ** 30)
+    assert said(copy([0], [2], planes=256, **big)) and copy([0], [2], planes=255, **big) == RQ_ERR_HANDLE

@@ -275,3 +275,54 @@ def test_graphs(torch, ctx):
         again = call()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("batch", [65, 300, 5000])
+def test_append_of_many_sequences(torch, ctx, batch):
+    import raster_amd
+
+    print(f"[gpu] append {batch} sequences", flush=True)
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 3, (batch,), generator=gen)
+    lens[batch // 3] = 40
+    n = int(lens.sum())
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)])
+    past = torch.randint(0, 17, (batch,), generator=gen)
+    table = torch.randperm(4 * batch, generator=gen).int().view(batch, 4)
+    kp, vp = (torch.zeros((4 * batch, 16, 64), device="cuda") for _ in range(2))
+    q, k, v = (torch.randn((n, 64), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda")
+               for i in range(3))
+    qo, ko = raster_amd.pages_append(ctx, q, k, v, kp, vp, table.cuda(), cu.int().cuda(), past.int().cuda(), 1, 1, 64,
+                                     0.0)
+    owner = torch.repeat_interleave(torch.arange(batch), lens)
+    pos = past[owner] + torch.arange(n) - cu[owner]
+    at = (table[owner, pos // 16].long() * 16 + pos % 16).cuda()
+    assert torch.equal(qo, q) and torch.equal(ko, k)
+    for p, x in ((kp, k), (vp, v)):
+        want = torch.zeros_like(p).view(-1, 64)
+        want[at] = x
+        assert torch.equal(p.view(-1, 64), want)
+
+
+def test_offsets_past_32_bits(torch, ctx):
+    """A cache of 2 x 2 planes of 4.3 GiB, its last pages used."""
+    import raster_amd
+
+    print("[gpu] paged offsets past 2^32", flush=True)
+    nq, nkv, hd, total, used = 8, 8, 128, 140000, 64
+    data = torch.empty((2, total, 16, nkv * hd), dtype=torch.bfloat16, device="cuda")
+    small = torch.randn((2, used, 16, nkv * hd), generator=torch.Generator(device="cuda").manual_seed(2),
+                        device="cuda").to(torch.bfloat16)
+    data[:, total - used:] = small
+    table = torch.randperm(used, generator=torch.Generator().manual_seed(3)).int().view(2, -1).cuda()
+    lens = torch.tensor([300, 511], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn((2, nq * hd), generator=torch.Generator(device="cuda").manual_seed(4 + i),
+                           device="cuda").to(torch.bfloat16) for i in range(3))
+    outs = []
+    for pages, first in ((small, 0), (data, total - used)):
+        outs.append(raster_amd.paged_attention(ctx, q, k, v, pages[0], pages[1], table + first, lens, nq, nkv, hd, THETA,
+                                               hd ** -0.5))
+        cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+        raster_amd.pages_append(ctx, q, k, v, pages[0], pages[1], table + first, cu, lens - 100, nq, nkv, hd, THETA)
+        raster_amd.pages_copy(ctx, pages, [first + 3, first + 40], [first + 5, first + 63])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(data[:, total - used:], small)

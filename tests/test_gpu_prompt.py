@@ -314,3 +314,63 @@ def test_graph_replays_and_streams(torch, ctx):
     a = call(sets[1], stream=st)
     st.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(a, eager[1]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch", [64, 65, 300, 5000])
+def test_many_sequences(torch, ctx, dtype, batch):
+    """More sequences than a wave has lanes, most of a few rows or none: one dense product
+    with a mask of equal sequences is the reference."""
+    import attn_ref as ref
+    import raster_amd
+
+    print(f"[gpu] prompt {dtype} {batch} sequences", flush=True)
+    nq, nkv, hd, scale = 2, 1, 64, 0.125
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    lens = torch.randint(0, 4, (batch,), generator=torch.Generator().manual_seed(batch))
+    lens[torch.randperm(batch)[batch // 4:]] = 0
+    lens[batch // 2] = 200
+    lens[-1] = 33
+    n = int(lens.sum())
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).int().cuda()
+    owner = torch.repeat_interleave(torch.arange(batch), lens).cuda()
+    see = (owner[:, None] == owner[None]) & ref.causal(n, n)
+    q, k, v, do = (rows(torch, g, n, w * hd, ty) for w in (nq, nkv, nkv, nq))
+    lse = torch.empty((nq, n), device="cuda")
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse)
+    dq, dk, dv = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale)
+    half = ref.HALF[ty]
+    sums = [0.0] * 4
+    for h in range(nq):
+        args = heads(q, h, hd), heads(k, 0, hd), heads(v, 0, hd)
+        want, wlse, bound = ref.attend(*args, scale, see, half)
+        assert bool(((heads(out, h, hd) - want).abs() <= bound).all())
+        assert bool(((lse[h].double() - wlse).abs() <= 1e-5 * (1 + wlse.abs())).all())
+        (wq, wk, wv), (bq, bk, bv) = ref.attend_grad(*args, heads(do, h, hd), scale, see, half)
+        assert bool(((heads(dq, h, hd) - wq).abs() <= bq).all())
+        sums = [a + b for a, b in zip(sums, (wk, wv, bk, bv))]
+    for got, want, bound in ((dk, sums[0], sums[2]), (dv, sums[1], sums[3])):
+        assert bool(((got.double() - want).abs() <= bound + half * want.abs()).all())
+
+
+def test_rows_more_than_4_gib_apart(torch, ctx):
+    """The widest stride, 2^22 elements, and offsets past 32 bits."""
+    import raster_amd
+
+    print("[gpu] prompt, 2^22 elements a row", flush=True)
+    n, nq, nkv, hd, scale = 620, 2, 1, 64, 0.125
+    wide = torch.empty((n, 2 ** 22), dtype=torch.bfloat16, device="cuda")  # 5 GiB, a few columns of it used
+    g = torch.Generator(device="cuda").manual_seed(5)
+    width = (nq + 2 * nkv) * hd
+    wide[:, :width] = torch.randn((n, width), generator=g, device="cuda").to(torch.bfloat16)
+    q, k, v = wide[:, :nq * hd], wide[:, nq * hd:(nq + 1) * hd], wide[:, (nq + 1) * hd:width]
+    near = [t.contiguous() for t in (q, k, v)]
+    cu = cu_of(torch, [100, 520])
+    lse = torch.empty((nq, n), device="cuda")
+    want = raster_amd.prompt_attention(ctx, *near, cu, nq, nkv, hd, scale, lse=lse)
+    assert torch.equal(raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale), want)
+    do = torch.randn((n, nq * hd), generator=g, device="cuda").to(torch.bfloat16)
+    grads = raster_amd.prompt_attention_bwd(ctx, do, *near, want, lse, cu, nq, nkv, hd, scale)
+    far = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, want, lse, cu, nq, nkv, hd, scale)
+    assert all(torch.equal(a, b) for a, b in zip(grads, far))

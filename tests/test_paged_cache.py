@@ -20,7 +20,7 @@ class Cache(paged.PagedCache):
         self.data = np.zeros((pages, page_size), np.int64)
         self._refs, self._free = [0] * pages, list(range(pages))
         self._pages, self._len, self._slots = {}, {}, list(range(max_seqs))
-        self._host_table = np.zeros((max_seqs, seq_pages), np.int32)
+        self._host_table = np.full((max_seqs, seq_pages), -1, np.int32)
         self._host_lens = np.full(max_seqs, -1, np.int32)
         self._dirty = False
 
@@ -44,8 +44,9 @@ def check(c):
     assert sorted(c._free) == [p for p, n in enumerate(c._refs) if n == 0]
     for s, pages in c._pages.items():
         assert len(set(pages)) == len(pages) and len(pages) * c.page_size >= c._len[s]
-        assert list(c._host_table[s, :len(pages)]) == pages and c._host_lens[s] == c._len[s]
-    assert all(c._host_lens[s] == -1 for s in c._slots)
+        assert list(c._host_table[s, :len(pages)]) == pages and np.all(c._host_table[s, len(pages):] == -1)
+        assert c._host_lens[s] == c._len[s]
+    assert all(c._host_lens[s] == -1 and np.all(c._host_table[s] == -1) for s in c._slots)
 
 
 def write(c, s, values):
