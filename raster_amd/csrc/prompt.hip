@@ -301,19 +301,20 @@ __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
   x.finish(a, w.hq, w.tq.begin + w.qi, w.live);
 }
 
-// Four waves over the same 32 queries, each with its own 32 of the 128 keys that are staged at
-// a time, and their states joined at the end: for grids that would leave CUs idle with
-// 128 queries a workgroup. One tile in LDS, the next on its way in registers.
-template <typename T, int HD>
+// Fewer queries a workgroup, for grids that would leave CUs idle with 128: QG groups of 32,
+// and 4 / QG waves over the same queries, each with its own 32 of the keys that are staged at
+// a time, their states joined at the end. One tile in LDS, the next on its way in registers.
+template <typename T, int HD, int QG>
 __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
-  constexpr int THREADS = 256, BK = 128, kTile = TL::bytes(BK), kWaves = 4;
+  constexpr int THREADS = 256, KG = 4 / QG, BK = 32 * KG, kTile = TL::bytes(BK);
   constexpr int kCol = HD + 4;  // floats from query to query of a joined state
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Work<T, 32> w;
-  if (!w.init(a, 0, lane)) return;
+  const int kg = wave % KG;
+  Work<T, 32 * QG> w;
+  if (!w.init(a, wave / KG, lane)) return;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int kb) {
     ks.load(w.k + (int64_t)kb * a.k_stride, a.k_stride, w.lk - kb, a.head_dim, tid);
@@ -328,9 +329,9 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
     vs.store(lds + kTile, tid);
     if (kb + BK < w.nk) load(kb + BK);
     __syncthreads();
-    const int mine = kb + 32 * wave;
-    if (mine < w.nk) {
-      const char* kt = lds + 32 * wave * TL::kPitch;
+    const int mine = kb + 32 * kg;
+    if (mine < w.nk && w.any(a, mine)) {
+      const char* kt = lds + 32 * kg * TL::kPitch;
       x.scores(kt);
       x.softmax(mine, w.see, w.cut(a, mine, 32), a.scale2);
       x.add_values(kt + kTile);
@@ -349,16 +350,18 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   if (h == 0) own[HD] = x.m;
   own[HD + 1 + h] = x.l;
   __syncthreads();
-  // eight threads a query, 4 values each at a time
-  const int qn = tid >> 3, sub = tid & 7, qi = w.tq.row0 + qn;
+  // 8 / QG threads a query, 4 values each at a time; the query's states are 32 apart
+  constexpr int kSub = 8 / QG;
+  const int qn = tid / kSub, sub = tid % kSub, qi = w.tq.row0 + qn;
   if (qi >= w.tq.len) return;
-  float m = -INFINITY, l = 0.0f, f[kWaves];
+  st += ((qn >> 5) * KG * 32 + (qn & 31)) * kCol;
+  float m = -INFINITY, l = 0.0f, f[KG];
 #pragma unroll
-  for (int u = 0; u < kWaves; u++) m = fmaxf(m, st[(u * 32 + qn) * kCol + HD]);
+  for (int u = 0; u < KG; u++) m = fmaxf(m, st[u * 32 * kCol + HD]);
   const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-  for (int u = 0; u < kWaves; u++) {
-    const float* s = st + (u * 32 + qn) * kCol + HD;
+  for (int u = 0; u < KG; u++) {
+    const float* s = st + u * 32 * kCol + HD;
     f[u] = __builtin_amdgcn_exp2f(s[0] - ref);
     l += f[u] * (s[1] + s[2]);
   }
@@ -367,10 +370,10 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
     a.lse[(int64_t)w.hq * a.rows_q + row] = l == 0.0f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a query that sees nothing: zeros
   T* out = static_cast<T*>(a.out) + row * a.out_stride + w.hq * a.head_dim;
-  for (int e = 4 * sub; e < a.head_dim; e += 32) {
+  for (int e = 4 * sub; e < a.head_dim; e += 4 * kSub) {
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int u = 0; u < kWaves; u++) y += f[u] * *reinterpret_cast<const f32x4*>(st + (u * 32 + qn) * kCol + e);
+    for (int u = 0; u < KG; u++) y += f[u] * *reinterpret_cast<const f32x4*>(st + u * 32 * kCol + e);
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 z;
 #pragma unroll
@@ -401,11 +404,11 @@ hipError_t run_fwd_pair(PromptArgs a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int QG>
 hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
-  constexpr int lds = std::max(2 * Tile<T, HD>::bytes(128), 4 * 32 * (HD + 4) * 4);
-  a.slots = tile_slots(a.rows_q, a.batch, 32);
-  const auto kernel = prompt_fwd_split_kernel<T, HD>;
+  constexpr int lds = std::max(2 * Tile<T, HD>::bytes(128 / QG), 4 * 32 * (HD + 4) * 4);
+  a.slots = tile_slots(a.rows_q, a.batch, 32 * QG);
+  const auto kernel = prompt_fwd_split_kernel<T, HD, QG>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(256), lds, stream, a);
@@ -414,27 +417,40 @@ hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
 
 }  // namespace
 
-// Whether the split kernel is the faster: the other's grid leaves CUs idle (`most` workgroups
-// for every 256 CUs, by type and head), unless there is hardly a tile of keys to split. us, split
-// / whole, causal, 16/16 heads x 128 unless said (workgroups of the whole kernel):
-//   bf16  37 tokens (16) 8.2 / 6.9   512 (80) 13.2 / 17.0   1024 (144) 26.5 / 28.2   2048 (272) 73 / 52
-//         64 after 4032 (16) 56 / 75   32/8 heads: 512 (160) 20.0 / 17.7   4 x 64 after 4032 (192) 60 / 76
-//   bf16  16/2 x 64: 1024 (144) 13.9 / 23.3   2048 (272) 28.9 / 41.8   8 x 256 (384) 13.9 / 10.6
-//   f32   512 (80) 39 / 81   1024 (144) 81 / 155   2048 (272) 268 / 302   8 x 256 (384) 75 / 48
-//   f32   16/2 x 64: 2048 (272) 98 / 166   8 x 256 (384) 31 / 31   8 x 512 (640) 76 / 81
-static bool fwd_splits(int dtype, const PromptArgs& a) {
-  if (a.head_dim > 128 || a.rows_k < 64 * (int64_t)a.batch) return false;
-  const bool few_queries = a.rows_k >= 4 * a.rows_q;
-  const int most = dtype == RQ_F32 ? (a.head_dim <= 64 ? 640 : 320) : a.head_dim <= 64 ? 320 : few_queries ? 256 : 144;
-  return tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 <= (int64_t)most * a.cu_count;
+// The split kernel's groups of 32 queries a workgroup, or 0 for the kernel of 128 queries: that reads
+// keys and values least often, the others fill the CUs with fewer queries. By the 128-query
+// kernel's workgroups for every 256 CUs; us, 128 / 64 / 32 queries, causal, 16/16 heads x 128 unless said:
+//   bf16  256 tokens (32/8 heads, 96) 11.7 / 11.0 / 10.1   512 (32/8, 160) 17.4 / 15.4 / 19.8   613, 1, 1024,
+//         250, 89 (320) 28.9 / 25.2 / 46.5   8 x 256 (384) 14.5 / 13.9 / 29.7   2048 (32/8, 544) 55 / 64 / 138
+//         4 x 64 after 4032 (32/8, 192) 80 / 71 / 60
+//   bf16  16/2 x 64: 1024 (144) 22.7 / 17.5 / 13.7   2048 (272) 41 / 29 / 29   4096 (528) 78 / 60 / 74
+//         8 x 512 (640) 16.6 / 17.5 / 24.6
+//   f32   37 tokens (16) 15.0 / 12.4 / 14.7   512 (80) 81 / 49 / 38   512 (32/8, 160) 82 / 50 / 51   613, 1, 1024,
+//         250, 89 (320) 156 / 111 / 138   8 x 256 (384) 48 / 56 / 75   2048 (32/8, 544) 327 / 363 / 532
+//   f32   16/2 x 64: 1024 (144) 86 / 48 / 37   2048 (272) 164 / 113 / 101   8 x 256 (384) 31 / 24 / 31
+//         8 x 512 (640) 80 / 69 / 77
+static int fwd_split_groups(int dtype, const PromptArgs& a) {
+  if (a.head_dim > 128) return 0;
+  const bool f32 = dtype == RQ_F32, narrow = a.head_dim <= 64;
+  if (a.rows_k < 64 * (int64_t)a.batch) return f32 ? 2 : 0;  // hardly a tile of keys to split
+  const bool few_queries = a.rows_k >= 4 * a.rows_q;  // every tile sees most keys
+  const int one = narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
+  const int two = narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
+  const int64_t groups = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256;
+  return groups <= (int64_t)one * a.cu_count ? 1 : groups <= (int64_t)two * a.cu_count ? 2 : 0;
+}
+
+template <int QG>
+static hipError_t launch_fwd_split(int dtype, const PromptArgs& a, hipStream_t stream) {
+  if (dtype == RQ_BF16)
+    return a.head_dim <= 64 ? run_fwd_split<__bf16, 64, QG>(a, stream) : run_fwd_split<__bf16, 128, QG>(a, stream);
+  return a.head_dim <= 64 ? run_fwd_split<float, 64, QG>(a, stream) : run_fwd_split<float, 128, QG>(a, stream);
 }
 
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
-  if (fwd_splits(dtype, a)) {
-    if (dtype == RQ_BF16)
-      return a.head_dim <= 64 ? run_fwd_split<__bf16, 64>(a, stream) : run_fwd_split<__bf16, 128>(a, stream);
-    return a.head_dim <= 64 ? run_fwd_split<float, 64>(a, stream) : run_fwd_split<float, 128>(a, stream);
-  }
+  const int qg = fwd_split_groups(dtype, a);
+  if (qg == 1) return launch_fwd_split<1>(dtype, a, stream);
+  if (qg == 2) return launch_fwd_split<2>(dtype, a, stream);
   if (dtype == RQ_BF16) {
     if (a.head_dim <= 64) return run_fwd<__bf16, 64, 64>(a, stream);
     // The pair kernel reads keys and values half as often but cuts the queries in tiles of 256.

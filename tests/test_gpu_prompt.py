@@ -72,6 +72,10 @@ CASES = [
     ("bf16", 2, 2, 128, [1500], [1500]),
     ("bf16", 64, 8, 128, [300, 129, 40], [300, 129, 40]),  # grids that fill the CUs: keys not split
     ("bf16", 64, 8, 64, [300, 129, 90], [300, 129, 90]),
+    ("bf16", 64, 8, 128, [300, 129, 90, 5], [300, 129, 90, 5]),
+    ("bf16", 128, 8, 64, [300, 129, 90], [300, 129, 90]),
+    ("bf16", 128, 8, 72, [300, 0, 90], [310, 129, 90]),
+    ("f32", 64, 8, 104, [300, 0, 90], [310, 129, 90]),
     ("f32", 64, 8, 128, [300, 129, 90], [300, 129, 90]),
     ("f32", 128, 8, 40, [300, 129, 90], [300, 129, 90]),
     ("f32", 4, 4, 128, [1], [1]),
