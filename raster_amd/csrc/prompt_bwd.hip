@@ -68,26 +68,40 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[HD / 32],
     }
 }
 
-// dK and dV of 64 keys: query tiles of 32 rows through LDS, two waves for each 32
+// dK and dV of 64 keys: query tiles of 32 or 64 rows through LDS, two waves for each 32
 // keys. One holds K and dV: it forms S = Q K^T and P, and adds dO^T P to dV; the
 // other holds V and dK: it forms dO V^T meanwhile, takes P over through LDS and adds
 // Q^T dS to dK. So a wave needs the registers of one operand and one result only
 // (two to three waves a SIMD instead of one), and both do the same two products in
 // each half of a step.
 //
-// The steps, (query head of the group, query tile), of a workgroup are one of nsplit parts;
+// The steps of a workgroup go from the sequence's last queries down, every query head of the group at each
+// tile: workgroups that began together read the same tiles at the same time, from their L2.
+// us, dK/dV alone, bf16, 32/8 heads x 128, 8192 queries: 1333 (heads outside, queries upwards: 1386).
+// The steps are one of nsplit parts;
 // with more than one the parts' f32 sums go to a.part and prompt_dkv_sum_kernel adds them in
 // order.
-constexpr int kDkvKeys = 64, kDkvQueries = 32, kDqQueries = 128;
+constexpr int kDkvKeys = 64, kDqQueries = 128;
+// 64 queries a step halve the barriers (the whole gradient of 2048, 777, 1500, 331, 1999 and 64 tokens:
+// 461 us, with 32 480); f32 and heads past 128 have no registers for them.
+template <typename T, int HD>
+constexpr int dkv_queries() {
+  return sizeof(T) == 2 && HD <= 128 ? 64 : 32;
+}
+template <typename T, int HD>
+constexpr int dkv_lds() {  // twice Q, dO, L and D of a step, and two pairs' weights
+  return 2 * (2 * Tile<T, HD>::bytes(dkv_queries<T, HD>()) + 2 * dkv_queries<T, HD>() * 4) +
+         2 * 2 * 64 * (int)sizeof(typename Tile<T, HD>::Frag) * dkv_queries<T, HD>() / 32;
+}
 
 template <typename T, int HD>
 __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
-  constexpr int THREADS = 256, BQ = kDkvQueries;
+  constexpr int THREADS = 256, BQ = dkv_queries<T, HD>(), NT = BQ / 32;
   constexpr int kTile = TL::bytes(BQ);
   constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
-  constexpr int kPair = 2 * 64 * (int)sizeof(Frag);  // the weights of 32 keys and queries
+  constexpr int kPair = 2 * NT * 64 * (int)sizeof(Frag);  // the weights of 32 keys and the queries
   const int group = a.n_q / a.n_kv;
   const int hkv = block % a.n_kv, rest = block / a.n_kv, split = rest % a.nsplit;
   const int64_t slot = rest / a.nsplit;  // a sequence's first keys, which most queries see, first
@@ -119,7 +133,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
   const int64_t steps = (int64_t)per_head * group;
   const int s0 = (int)(steps * split / a.nsplit), s1 = (int)(steps * (split + 1) / a.nsplit);
   Stage<T, HD, BQ, THREADS> qs, os;
-  float rowv = 0.0f;  // L (threads 0 .. 31) or D (32 .. 63) of the next tile's rows
+  float rowv = 0.0f;  // L (the first BQ threads) or D (as many more) of the next tile's rows
   auto load = [&](int hq, int r) {
     qs.load(static_cast<const T*>(a.q) + (q0 + r) * a.q_stride + hq * a.head_dim, a.q_stride, lq - r, a.head_dim, tid);
     os.load(static_cast<const T*>(a.dout) + (q0 + r) * a.dout_stride + hq * a.head_dim, a.dout_stride, lq - r,
@@ -136,8 +150,8 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
   };
   int hq = hkv * group, r = qstart;  // of the step
   if (s0 < s1) {
-    hq += s0 / per_head;
-    r += s0 % per_head * BQ;
+    hq += s0 % group;
+    r += (per_head - 1 - s0 / group) * BQ;
     load(hq, r);
     store(lds);
   }
@@ -145,44 +159,50 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
     const char* qt = lds + buf * kBuf;
     const char* ot = qt + kTile;
     const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile) + (is_k ? BQ : 0) + 4 * h;
-    int next_hq = hq, next_r = r + BQ;
-    if (next_r >= lq) next_hq++, next_r = qstart;
+    int next_hq = hq + 1, next_r = r;
+    if (next_hq == (hkv + 1) * group) next_hq = hkv * group, next_r -= BQ;
     if (step + 1 < s1) load(next_hq, next_r);
     __syncthreads();
     const bool seen = !a.causal || r + BQ - 1 + off >= w_key;
     const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off);
-    // value i of a product: query r + 8 (i / 4) + 4 h + i % 4, the lane's key
-    auto see = [&](int i) {
-      const int qi = r + 8 * (i >> 2) + 4 * h + (i & 3);
+    // value i of product t: query r + 32 t + 8 (i / 4) + 4 h + i % 4, the lane's key
+    auto see = [&](int t, int i) {
+      const int qi = r + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
       return qi < lq && live && (!a.causal || kj <= qi + off);
     };
-    float x[16];
-    Frag pf[2];  // bf16: weights and their gradients rounded to nearest for the products
+    float x[NT][16];
+    Frag pf[NT][2];  // bf16: weights and their gradients rounded to nearest for the products
     if (seen) {
       const char* t1 = is_k ? ot : qt;
-      f32x16 s = f32x16{};
+      f32x16 s[NT] = {};
 #pragma unroll
-      for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(t1, lane & 31, d, h), f[d], s);
-      if constexpr (sizeof(T) == 2) order_products<HD / 16, 1>();
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 8 * g);
+        for (int d = 0; d < HD / 16; d++) s[t] = tile_mma(TL::frag(t1, 32 * t + (lane & 31), d, h), f[d], s[t]);
+      if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 1>();
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[4 * g + j] = is_k ? s[4 * g + j] - c[j] : fmaf(s[4 * g + j], a.scale2, -c[j]);
-      }
-      if (!is_k) {
+      for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(x[i]);
-        if (!whole)
+        for (int g = 0; g < 4; g++) {
+          const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 32 * t + 8 * g);
 #pragma unroll
-          for (int i = 0; i < 16; i++) x[i] = see(i) ? x[i] : 0.0f;
+          for (int j = 0; j < 4; j++)
+            x[t][4 * g + j] = is_k ? s[t][4 * g + j] - c[j] : fmaf(s[t][4 * g + j], a.scale2, -c[j]);
+        }
+        if (!is_k) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          tile_pack(x + 8 * u, pf[u]);
+          for (int i = 0; i < 16; i++) x[t][i] = __builtin_amdgcn_exp2f(x[t][i]);
+          if (!whole)
 #pragma unroll
-          for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
-            *reinterpret_cast<u32x4*>(pair + (u * (int)sizeof(Frag) + c * 16) * 64) =
-                reinterpret_cast<const u32x4*>(&pf[u])[c];
+            for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            tile_pack(x[t] + 8 * u, pf[t][u]);
+#pragma unroll
+            for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
+              *reinterpret_cast<u32x4*>(pair + ((2 * t + u) * (int)sizeof(Frag) + c * 16) * 64) =
+                  reinterpret_cast<const u32x4*>(&pf[t][u])[c];
+          }
         }
       }
     }
@@ -190,26 +210,32 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
     if (seen) {
       if (is_k) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int t = 0; t < NT; t++) {
 #pragma unroll
-          for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
-            reinterpret_cast<u32x4*>(&pf[u])[c] =
-                *reinterpret_cast<const u32x4*>(pair + (u * (int)sizeof(Frag) + c * 16) * 64);
+          for (int u = 0; u < 2; u++) {
 #pragma unroll
-          for (int j = 0; j < 8; j++) x[8 * u + j] *= (float)pf[u][j];
+            for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
+              reinterpret_cast<u32x4*>(&pf[t][u])[c] =
+                  *reinterpret_cast<const u32x4*>(pair + ((2 * t + u) * (int)sizeof(Frag) + c * 16) * 64);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[t][8 * u + j] *= (float)pf[t][u][j];
+          }
+          if (!whole)  // what is masked has weight 0, and its other factor may be anything
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
+          tile_pack(x[t], pf[t][0]);
+          tile_pack(x[t] + 8, pf[t][1]);
         }
-        if (!whole)  // what is masked has weight 0, and its other factor may be anything
-#pragma unroll
-          for (int i = 0; i < 16; i++) x[i] = see(i) ? x[i] : 0.0f;
-        tile_pack(x, pf[0]);
-        tile_pack(x + 8, pf[1]);
       }
       const char* t2 = is_k ? qt : ot;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) acc[d] = tile_mma(TL::frag_t(t2, 16 * u, d, lane), pf[u], acc[d]);
-      if constexpr (sizeof(T) == 2) order_products<HD / 16, 2>();
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int d = 0; d < HD / 32; d++)
+            acc[d] = tile_mma(TL::frag_t(t2, 32 * t + 16 * u, d, lane), pf[t][u], acc[d]);
+      if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 2>();
     }
     if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
     hq = next_hq, r = next_r;
@@ -369,9 +395,7 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  constexpr int lds = std::max(2 * (2 * TL::bytes(kDkvQueries) + 2 * kDkvQueries * 4) +
-                                   2 * 2 * 64 * (int)sizeof(typename TL::Frag),
-                               4 * TL::bytes(BK));
+  constexpr int lds = std::max(dkv_lds<T, HD>(), 4 * TL::bytes(BK));
   a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
   a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, kDqQueries) : 0;
   const auto kernel = prompt_grad_kernel<T, HD, BK>;
@@ -396,7 +420,7 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
                               int64_t head_dim) {
   constexpr int64_t kDkvGroups = 768;
   const int64_t groups = std::max<int64_t>(1, (rows_k + kDkvKeys - 1) / kDkvKeys * n_kv);
-  const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / kDkvQueries * (n_q / n_kv);
+  const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / 32 * (n_q / n_kv);
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
   p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, kDqQueries) * n_q,
