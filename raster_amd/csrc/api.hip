@@ -1622,6 +1622,7 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
   a.dout_stride = dout_stride, a.dq_stride = dq_stride, a.dk_stride = dk_stride, a.dv_stride = dv_stride;
   a.dq = dq, a.dk = dk, a.dv = dv, a.delta = static_cast<float*>(work);
+  a.cu_count = c->cu_count;
   a.nsplit = plan.nsplit;
   a.part = reinterpret_cast<float*>(static_cast<char*>(work) + plan.delta_bytes);
   const hipError_t e = launch_prompt_bwd(p->dtype, a, (hipStream_t)stream);

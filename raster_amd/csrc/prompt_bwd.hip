@@ -276,6 +276,37 @@ __global__ __launch_bounds__(256) void prompt_dkv_sum_kernel(PromptArgs a) {
   *reinterpret_cast<T4*>(static_cast<T*>(a.dk) + row * a.dk_stride + e) = yk;
 }
 
+// dQ of a wave's 32 queries += their share of the 32 keys from row `r` of the staged tiles on,
+// keys `key` and on of the sequence.
+template <typename T, int HD>
+__device__ __forceinline__ void dq_tile(const char* kt, const char* vt, int r, int key, bool whole, int see, float lse,
+                                        float del, float scale2, int lane,
+                                        const typename Tile<T, HD>::Frag (&qf)[HD / 16],
+                                        const typename Tile<T, HD>::Frag (&of)[HD / 16], f32x16 (&dq)[HD / 32]) {
+  using TL = Tile<T, HD>;
+  const int h = lane >> 5;
+  f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+  for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, r + (lane & 31), d, h), qf[d], s);
+#pragma unroll
+  for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, r + (lane & 31), d, h), of[d], dp);
+  if constexpr (sizeof(T) == 2) order_products<HD / 8, 1>();
+  float ds[16];
+#pragma unroll
+  for (int i = 0; i < 16; i++) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale2, -lse)) * (dp[i] - del);
+  if (!whole)
+#pragma unroll
+    for (int i = 0; i < 16; i++) ds[i] = key + 8 * (i >> 2) + 4 * h + (i & 3) <= see ? ds[i] : 0.0f;
+  typename TL::Frag sf[2];
+  tile_pack(ds, sf[0]);
+  tile_pack(ds + 8, sf[1]);
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, r + 16 * u, d, lane), sf[u], dq[d]);
+  if constexpr (sizeof(T) == 2) order_products<HD / 16, 2>();
+}
+
 // dQ: four waves of 32 queries each, key tiles of BK rows through LDS.
 template <typename T, int HD, int BK>
 __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* lds) {
@@ -340,28 +371,8 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
     if (!a.causal || kb <= w_row + 31 + off) {
       const bool whole = kb + BK <= lk && w_row + 32 <= tq.len && (!a.causal || kb + BK - 1 <= w_row + off);
 #pragma unroll
-      for (int t = 0; t < BK / 32; t++) {
-        f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-        for (int d = 0; d < HD / 16; d++) s = tile_mma(TL::frag(kt, 32 * t + (lane & 31), d, h), qf[d], s);
-#pragma unroll
-        for (int d = 0; d < HD / 16; d++) dp = tile_mma(TL::frag(vt, 32 * t + (lane & 31), d, h), of[d], dp);
-        if constexpr (sizeof(T) == 2) order_products<HD / 8, 1>();
-        float ds[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -lse)) * (dp[i] - del);
-        if (!whole)
-#pragma unroll
-          for (int i = 0; i < 16; i++) ds[i] = kb + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) <= see ? ds[i] : 0.0f;
-        Frag sf[2];
-        tile_pack(ds, sf[0]);
-        tile_pack(ds + 8, sf[1]);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int d = 0; d < HD / 32; d++) dq[d] = tile_mma(TL::frag_t(kt, 32 * t + 16 * u, d, lane), sf[u], dq[d]);
-        if constexpr (sizeof(T) == 2) order_products<HD / 16, 2>();
-      }
+      for (int t = 0; t < BK / 32; t++)
+        dq_tile<T, HD>(kt, vt, 32 * t, kb + 32 * t, whole, see, lse, del, a.scale2, lane, qf, of, dq);
     }
     if (more) {
       ks.store(next, tid);
@@ -375,19 +386,98 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
                       a.head_dim);
 }
 
+// dQ of 32 QG queries, 4 / QG waves over the same ones, each with its own 32 of the keys that are
+// staged at a time, and their sums added at the end: for grids that would leave CUs idle.
+template <typename T, int HD, int QG>
+__device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, char* lds) {
+  using TL = Tile<T, HD>;
+  using Frag = typename TL::Frag;
+  constexpr int THREADS = 256, KG = 4 / QG, BQ = 32 * QG, BK = 32 * KG, kTile = TL::bytes(BK);
+  constexpr int kCol = HD + 4;  // floats from query to query of the sums
+  const int group = a.n_q / a.n_kv;
+  const int hkv = block % a.n_kv, rest = block / a.n_kv, hq = hkv * group + rest % group;
+  const TileSpan tq = tile_of_slot(a.cu_q, a.batch, a.rows_q, BQ, a.q_slots - 1 - rest / group);
+  if (tq.len == 0) return;
+  const int64_t k0 = clamp_cu(a.cu_k, tq.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tq.seq + 1, a.rows_k);
+  const int lk = (int)(k1 > k0 ? k1 - k0 : 0), off = lk - tq.len;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % KG;
+  const int w_row = tq.row0 + wave / KG * 32, qi = w_row + (lane & 31);
+  const bool live = qi < tq.len;
+  const int q_last = min(tq.row0 + BQ, tq.len) - 1;
+  const int nk = a.causal ? min(max(q_last + off + 1, 0), lk) : lk;
+  const T* kbase = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
+  const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
+  Stage<T, HD, BK, THREADS> ks, vs;
+  auto load = [&](int kb) {
+    ks.load(kbase + (int64_t)kb * a.k_stride, a.k_stride, lk - kb, a.head_dim, tid);
+    vs.load(vbase + (int64_t)kb * a.v_stride, a.v_stride, lk - kb, a.head_dim, tid);
+  };
+  if (nk > 0) load(0);
+  const T* qrow = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;
+  const T* orow = live ? static_cast<const T*>(a.dout) + (tq.begin + qi) * a.dout_stride + hq * a.head_dim : nullptr;
+  Frag qf[HD / 16], of[HD / 16];
+#pragma unroll
+  for (int s = 0; s < HD / 16; s++) {
+    qf[s] = TL::frag_global(qrow, s, h, a.head_dim);
+    of[s] = TL::frag_global(orow, s, h, a.head_dim);
+  }
+  settle(qf);
+  settle(of);
+  const int64_t at = (int64_t)hq * a.rows_q + tq.begin + min(qi, tq.len - 1);
+  const float lse = base2_lse(a.lse[at]), del = a.delta[at];
+  f32x16 dq[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++) dq[d] = f32x16{};
+  const int see = !live ? -1 : a.causal ? min(lk - 1, qi + off) : lk - 1;
+  for (int kb = 0; kb < nk; kb += BK) {
+    ks.store(lds, tid);
+    vs.store(lds + kTile, tid);
+    if (kb + BK < nk) load(kb + BK);
+    __syncthreads();
+    const int mine = kb + 32 * kg;
+    if (mine < nk && (!a.causal || mine <= w_row + 31 + off)) {
+      const bool whole = mine + 32 <= lk && w_row + 32 <= tq.len && (!a.causal || mine + 31 <= w_row + off);
+      dq_tile<T, HD>(lds, lds + kTile, 32 * kg, mine, whole, see, lse, del, a.scale2, lane, qf, of, dq);
+    }
+    __syncthreads();
+  }
+  float* st = reinterpret_cast<float*>(lds);
+  store_rows<float, HD>(st + (wave * 32 + (lane & 31)) * kCol, dq, a.scale, h, HD);
+  __syncthreads();
+  // 8 / QG threads a query, 4 values each at a time; the query's sums are 32 apart
+  constexpr int kSub = 8 / QG;
+  const int qn = tid / kSub, row = tq.row0 + qn;
+  if (row >= tq.len) return;
+  st += ((qn >> 5) * KG * 32 + (qn & 31)) * kCol;
+  T* out = static_cast<T*>(a.dq) + (tq.begin + row) * a.dq_stride + hq * a.head_dim;
+  for (int e = 4 * (tid % kSub); e < a.head_dim; e += 4 * kSub) {
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < KG; u++) y += *reinterpret_cast<const f32x4*>(st + u * 32 * kCol + e);
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 z;
+#pragma unroll
+    for (int j = 0; j < 4; j++) z[j] = (T)y[j];
+    *reinterpret_cast<T4*>(out + e) = z;
+  }
+}
+
 // Both in one launch, so that the short workgroups of one fill the compute units that the
 // last long ones of the other leave idle.
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, int QG>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prompt_grad_kernel(PromptArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int dkv = (int)(a.k_slots * a.n_kv * a.nsplit);
   if ((int)blockIdx.x < dkv)
     dkv_body<T, HD>(a, blockIdx.x, lds);
-  else
+  else if constexpr (QG == 4)
     dq_body<T, HD, BK>(a, blockIdx.x - dkv, lds);
+  else
+    dq_split_body<T, HD, QG>(a, blockIdx.x - dkv, lds);
 }
 
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, int QG>
 hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   using TL = Tile<T, HD>;
   if (a.rows_q > 0) {
@@ -395,10 +485,11 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  constexpr int lds = std::max(dkv_lds<T, HD>(), 4 * TL::bytes(BK));
+  constexpr int dq_lds = QG == 4 ? 4 * TL::bytes(BK) : std::max(2 * TL::bytes(128 / QG), 4 * 32 * (HD + 4) * 4);
+  constexpr int lds = std::max(dkv_lds<T, HD>(), dq_lds);
   a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
-  a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, kDqQueries) : 0;
-  const auto kernel = prompt_grad_kernel<T, HD, BK>;
+  a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, 32 * QG) : 0;
+  const auto kernel = prompt_grad_kernel<T, HD, BK, QG>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256), lds,
@@ -423,22 +514,32 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
   const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / 32 * (n_q / n_kv);
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
-  p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, kDqQueries) * n_q,
+  p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
                       (rows_q * n_q * kDeltaLanes + 255) / 256);
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
   p.work = p.delta_bytes + (p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0);
   return p;
 }
 
+// dQ of 64 queries a workgroup (two waves over the same 32) or of 128. f32 products are long enough
+// that the finer grid is all that counts; in bf16 128 queries read keys and values half as often,
+// which is the better from about two workgroups a CU on. us of the whole gradient, 128 / 64 queries,
+// causal, 16/16 heads x 128 unless said (workgroups of 128 queries):
+//   bf16  512 tokens (80) 47 / 42   2048 (272) 102 / 87   2048 (32/8 heads, 544) 188 / 183   8 x 512 (640) 78 / 79
+//         8 x 512 (32/8, 1280) 123 / 127   16/2 x 64: 2048 (272) 75 / 67
+//   f32   512 (80) 156 / 111   2048 (272) 760 / 601   2048 (32/8, 544) 1207 / 1186   8 x 512 (32/8, 1280) 738 / 727
+//         16/2 x 64: 129, 300, 64, 511 (176) 88 / 65   2048 (272) 480 / 341   8 x 512 (640) 215 / 194
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {
-    if (a.head_dim <= 64) return run_bwd<__bf16, 64, 64>(a, stream);
-    if (a.head_dim <= 128) return run_bwd<__bf16, 128, 32>(a, stream);
-    return run_bwd<__bf16, 256, 32>(a, stream);
+    if (a.head_dim > 128) return run_bwd<__bf16, 256, 32, 4>(a, stream);
+    const bool wide = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 > (int64_t)576 * a.cu_count;
+    if (a.head_dim <= 64)
+      return wide ? run_bwd<__bf16, 64, 64, 4>(a, stream) : run_bwd<__bf16, 64, 64, 2>(a, stream);
+    return wide ? run_bwd<__bf16, 128, 32, 4>(a, stream) : run_bwd<__bf16, 128, 32, 2>(a, stream);
   }
-  if (a.head_dim <= 64) return run_bwd<float, 64, 32>(a, stream);
-  if (a.head_dim <= 128) return run_bwd<float, 128, 32>(a, stream);
-  return run_bwd<float, 256, 32>(a, stream);
+  if (a.head_dim <= 64) return run_bwd<float, 64, 32, 2>(a, stream);
+  if (a.head_dim <= 128) return run_bwd<float, 128, 32, 2>(a, stream);
+  return run_bwd<float, 256, 32, 4>(a, stream);
 }
 
 }  // namespace rq

@@ -73,6 +73,7 @@ CASES = [
     ("bf16", 64, 8, 128, [300, 129, 40], [300, 129, 40]),  # grids that fill the CUs: keys not split
     ("bf16", 64, 8, 64, [300, 129, 90], [300, 129, 90]),
     ("bf16", 64, 8, 128, [300, 129, 90, 5], [300, 129, 90, 5]),
+    ("bf16", 96, 8, 128, [300, 129, 90, 5], [300, 129, 90, 5]),
     ("bf16", 128, 8, 64, [300, 129, 90], [300, 129, 90]),
     ("bf16", 128, 8, 72, [300, 0, 90], [310, 129, 90]),
     ("f32", 64, 8, 104, [300, 0, 90], [310, 129, 90]),
