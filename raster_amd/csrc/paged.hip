@@ -55,10 +55,10 @@ __device__ __forceinline__ void split_terms(float x, __bf16 (&t)[NT]) {
 }  // namespace
 
 namespace {
-// LDS of 16 heads' queries as fragments: f32, or one or three bf16 terms
+// LDS of 16 heads' queries as fragments: f32, or two or three bf16 terms
 template <typename A, typename C>
 constexpr int paged_query_bytes(int hd) {
-  return 16 * hd * (sizeof(C) == 4 ? 4 : sizeof(A) == 2 ? 2 : 6);
+  return 16 * hd * (sizeof(C) == 4 || sizeof(A) == 2 ? 4 : 6);
 }
 }  // namespace
 
@@ -74,12 +74,14 @@ constexpr int paged_query_bytes(int hd) {
 // pair; f32, one row a slot: nothing). Row i of result tile t is element E i + t.
 // Nothing of the cache passes through LDS.
 //
-// The queries and, over a bf16 cache, the weights P go in as NT bf16 terms: 3 for
-// f32 activations (to 2^-24), 1 for bf16 ones (rounded). An f32 cache is multiplied in f32.
+// Over a bf16 cache the rotated queries go in as NQ and the weights P as NP bf16 terms: 3 of each
+// for f32 activations (to 2^-24); for bf16 ones 2 of the queries (2^-17; 1 costs XXX us of XXX and the result's
+// error rises from 0.0024 to 0.0029 of its norm) and 1 of the weights (rounded). An f32 cache is
+// multiplied in f32.
 template <typename A, typename C, int HD, bool PART>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;
-  constexpr int NT = F32 || sizeof(A) == 2 ? 1 : 3;
+  constexpr int NQ = F32 ? 1 : sizeof(A) == 2 ? 2 : 3, NP = F32 || sizeof(A) == 2 ? 1 : 3;
   constexpr int kQueryBytes = paged_query_bytes<A, C>(HD);
   constexpr int E = HD / 16, KS = F32 ? HD / 16 : HD / 32, PE = 16 / (int)sizeof(C);
   constexpr int VP = E > PE ? E / PE : 1;     // 16-byte pieces of a lane's V elements
@@ -105,11 +107,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
   constexpr int KT = 32, STEP = KT * kPagedWaves;
   // the query rows and the new row, and the wave's first page numbers: asked for with the
   // length, not after it
-  constexpr int NQ = HD / 32;  // pairs of query elements a thread
+  constexpr int NE = HD / 32;  // pairs of query elements a thread
   const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + hq0 * hd;
-  A q0[NQ], q1[NQ], n0[2], n1[2];  // n: of the new k and v
+  A q0[NE], q1[NE], n0[2], n1[2];  // n: of the new k and v
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
+  for (int n = 0; n < NE; n++) {
     const int i = min(tid + n * kPagedThreads, heads * half - 1), hh = i / half, e = i - hh * half;
     q0[n] = qrow[hh * hd + e];
     q1[n] = qrow[hh * hd + e + half];
@@ -202,11 +204,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     if constexpr (F32) {
       sm[((e >> 4) * 64 + ((e >> 2) & 3) * 16 + hh) * 4 + (e & 3)] = x;
     } else {
-      __bf16 t[NT];
-      split_terms<NT>(x, t);
+      __bf16 t[NQ];
+      split_terms<NQ>(x, t);
       __bf16* at = reinterpret_cast<__bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
 #pragma unroll
-      for (int n = 0; n < NT; n++) at[n * 16 * HD] = t[n];
+      for (int n = 0; n < NQ; n++) at[n * 16 * HD] = t[n];
     }
   };
   auto get_query = [&](int hh, int e) {
@@ -216,12 +218,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
       const __bf16* at = reinterpret_cast<const __bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
       float x = 0.0f;
 #pragma unroll
-      for (int n = NT - 1; n >= 0; n--) x += (float)at[n * 16 * HD];
+      for (int n = NQ - 1; n >= 0; n--) x += (float)at[n * 16 * HD];
       return x;
     }
   };
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
+  for (int n = 0; n < NE; n++) {
     const int i = tid + n * kPagedThreads, hh = i / half, e = i - hh * half;
     if (i < heads * half) {
       const float c = p.rope ? cs[e] : 1.0f, s = p.rope ? cs[HD / 2 + e] : 0.0f;
@@ -272,9 +274,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     const u32x4* qp = reinterpret_cast<const u32x4*>(sm) + ql;
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
-      u32x4 qw[NT];
+      u32x4 qw[NQ];
 #pragma unroll
-      for (int n = 0; n < NT; n++) qw[n] = qp[(n * KS + ks) * 64];
+      for (int n = 0; n < NQ; n++) qw[n] = qp[(n * KS + ks) * 64];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         u32x4 kw = xk[t][ks];
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
           for (int j = 0; j < 4; j++) d[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], d[t], 0, 0, 0);
         } else {
 #pragma unroll
-          for (int n = 0; n < NT; n++)
+          for (int n = 0; n < NQ; n++)
             d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kw),
                                                            __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
         }
@@ -327,13 +329,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
         for (int j = 0; j < 8; j++)
           acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[j][t / PE][t % PE]), s[j], acc[t], 0, 0, 0);
     } else {
-      bf16x8 pb[NT];
+      bf16x8 pb[NP];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        __bf16 t[NT];
-        split_terms<NT>(s[j], t);
+        __bf16 t[NP];
+        split_terms<NP>(s[j], t);
 #pragma unroll
-        for (int n = 0; n < NT; n++) pb[n][j] = t[n];
+        for (int n = 0; n < NP; n++) pb[n][j] = t[n];
       }
 #pragma unroll
       for (int w = 0; w < E / 2; w++) {  // elements 2 w and 2 w + 1 of the lane
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
           hi[j] = high16_pair(e0, e1);
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NP; n++) {
           acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), pb[n], acc[2 * w], 0, 0, 0);
           acc[2 * w + 1] =
               __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi), pb[n], acc[2 * w + 1], 0, 0, 0);

@@ -68,6 +68,52 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[HD / 32],
     }
 }
 
+// Weights on their way from one wave to another, 16 a lane: f32 as they are; in the bf16 kernel their
+// upper 24 bits (cut off at 2^-16 of the value), for which there is just room in LDS. Rounded to bf16 here
+// and again as gradients, dK would be off by 0.0030 of its norm instead of 0.0025.
+template <typename T>
+struct Handover {
+  static constexpr int N = sizeof(T) == 4 ? 4 : 3;  // 16-byte pieces a lane
+  static __device__ __forceinline__ void put(char* at, const float* x) {
+    u32x4 w[N];
+    uint32_t* o = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t a = __float_as_uint(x[4 * i]), b = __float_as_uint(x[4 * i + 1]),
+                     c = __float_as_uint(x[4 * i + 2]), d = __float_as_uint(x[4 * i + 3]);
+      if constexpr (N == 4) {
+        o[4 * i] = a, o[4 * i + 1] = b, o[4 * i + 2] = c, o[4 * i + 3] = d;
+      } else {
+        o[3 * i] = __builtin_amdgcn_perm(b, a, 0x05030201);
+        o[3 * i + 1] = __builtin_amdgcn_perm(c, b, 0x06050302);
+        o[3 * i + 2] = __builtin_amdgcn_perm(d, c, 0x07060503);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) *reinterpret_cast<u32x4*>(at + k * 64 * 16) = w[k];
+  }
+  static __device__ __forceinline__ void take(const char* at, float* x) {
+    u32x4 w[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) w[k] = *reinterpret_cast<const u32x4*>(at + k * 64 * 16);
+    const uint32_t* o = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t y[4];
+      if constexpr (N == 4) {
+        y[0] = o[4 * i], y[1] = o[4 * i + 1], y[2] = o[4 * i + 2], y[3] = o[4 * i + 3];
+      } else {
+        y[0] = o[3 * i] << 8;
+        y[1] = __builtin_amdgcn_perm(o[3 * i + 1], o[3 * i], 0x0504030C);
+        y[2] = __builtin_amdgcn_perm(o[3 * i + 2], o[3 * i + 1], 0x0403020C);
+        y[3] = o[3 * i + 2] & 0xFFFFFF00u;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[4 * i + j] = __uint_as_float(y[j]);
+    }
+  }
+};
+
 // dK and dV of 64 keys: query tiles of 32 or 64 rows through LDS, two waves for each 32
 // keys. One holds K and dV: it forms S = Q K^T and P, and adds dO^T P to dV; the
 // other holds V and dK: it forms dO V^T meanwhile, takes P over through LDS and adds
@@ -91,7 +137,7 @@ constexpr int dkv_queries() {
 template <typename T, int HD>
 constexpr int dkv_lds() {  // twice Q, dO, L and D of a step, and two pairs' weights
   return 2 * (2 * Tile<T, HD>::bytes(dkv_queries<T, HD>()) + 2 * dkv_queries<T, HD>() * 4) +
-         2 * 2 * 64 * (int)sizeof(typename Tile<T, HD>::Frag) * dkv_queries<T, HD>() / 32;
+         2 * Handover<T>::N * 16 * 64 * dkv_queries<T, HD>() / 32;
 }
 
 template <typename T, int HD>
@@ -101,7 +147,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
   constexpr int THREADS = 256, BQ = dkv_queries<T, HD>(), NT = BQ / 32;
   constexpr int kTile = TL::bytes(BQ);
   constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
-  constexpr int kPair = 2 * NT * 64 * (int)sizeof(Frag);  // the weights of 32 keys and the queries
+  constexpr int kShare = Handover<T>::N * 16 * 64, kPair = NT * kShare;  // weights of 32 keys and 32 or all queries
   const int group = a.n_q / a.n_kv;
   const int hkv = block % a.n_kv, rest = block / a.n_kv, split = rest % a.nsplit;
   const int64_t slot = rest / a.nsplit;  // a sequence's first keys, which most queries see, first
@@ -196,13 +242,8 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
 #pragma unroll
             for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            tile_pack(x[t] + 8 * u, pf[t][u]);
-#pragma unroll
-            for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
-              *reinterpret_cast<u32x4*>(pair + ((2 * t + u) * (int)sizeof(Frag) + c * 16) * 64) =
-                  reinterpret_cast<const u32x4*>(&pf[t][u])[c];
-          }
+          for (int u = 0; u < 2; u++) tile_pack(x[t] + 8 * u, pf[t][u]);
+          Handover<T>::put(pair + t * kShare, x[t]);
         }
       }
     }
@@ -211,15 +252,10 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
       if (is_k) {
 #pragma unroll
         for (int t = 0; t < NT; t++) {
+          float p[16];
+          Handover<T>::take(pair + t * kShare, p);
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-#pragma unroll
-            for (int c = 0; c < (int)sizeof(Frag) / 16; c++)
-              reinterpret_cast<u32x4*>(&pf[t][u])[c] =
-                  *reinterpret_cast<const u32x4*>(pair + ((2 * t + u) * (int)sizeof(Frag) + c * 16) * 64);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[t][8 * u + j] *= (float)pf[t][u][j];
-          }
+          for (int i = 0; i < 16; i++) x[t][i] *= p[i];
           if (!whole)  // what is masked has weight 0, and its other factor may be anything
 #pragma unroll
             for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
