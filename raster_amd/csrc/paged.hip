@@ -75,9 +75,9 @@ constexpr int paged_query_bytes(int hd) {
 // Nothing of the cache passes through LDS.
 //
 // Over a bf16 cache the rotated queries go in as NQ and the weights P as NP bf16 terms: 3 of each
-// for f32 activations (to 2^-24); for bf16 ones 2 of the queries (2^-17; 1 costs XXX us of XXX and the result's
-// error rises from 0.0024 to 0.0029 of its norm) and 1 of the weights (rounded). An f32 cache is
-// multiplied in f32.
+// for f32 activations (to 2^-24); for bf16 ones 2 of the queries (to 2^-17; with 1, in the same time, the
+// error of 60 Ki rows' result is 0.0028 of its norm instead of 0.0022) and 1 of the weights (rounded).
+// An f32 cache is multiplied in f32.
 template <typename A, typename C, int HD, bool PART>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;

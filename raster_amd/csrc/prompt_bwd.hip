@@ -7,11 +7,13 @@
 //   dQ_i = scale sum_j dS_ij K_j      dK_j = scale sum_i dS_ij Q_i
 // the sums over i of dK and dV also over the query heads of the KV head.
 //
-// Three kernels, none with an atomic, so results do not depend on scheduling: D; dK
+// Three parts, none with an atomic, so results do not depend on scheduling: D; dK
 // and dV (a wave owns 32 keys and walks the queries of every head of its group); dQ
 // (a wave owns 32 queries and walks the keys). The scores and dO V^T are formed
 // in both of the last two: 7 products for the 5 that a single kernel would need, which
 // would have to add dQ from many workgroups.
+//
+// Rounded to bf16 in the bf16 kernels: P for dV, dS for dK and dQ (operands of their products), and the results.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -50,6 +52,67 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
 #pragma unroll
   for (int k = kDeltaLanes / 2; k >= 1; k >>= 1) sum += __shfl_xor(sum, k, 64);
   if (sub == 0) a.delta[(int64_t)hq * a.rows_q + row] = sum;
+}
+
+// D of the queries that see at most kExactKeys keys, anew. In bf16 O has been rounded, and what D is off by
+// reaches dQ and dK through every weight of its row: little where many keys share the weight, but for
+// the first queries of a sequence as much as all other roundings together (error of dQ of 37, 5 and 12
+// tokens, in roundings of the result: 1.60; of 777, 1500, 331 and 64: 1.50). Here D is formed from the
+// weights, sum_j p_ij dO_i . V_j (1.42 and 1.43; with 256 keys 1.43).
+// One workgroup a sequence and head (without a causal mask several, for its many queries): a wave
+// 32 queries and 32 keys. 5.5 us beside the other kernel's 19 at 6719 tokens in six sequences, 32/8 heads x 128
+// (from registers, each lane its row, 15: 64 cache lines a load).
+constexpr int kExactKeys = 64, kExactTiles = 8;
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void prompt_delta_exact_kernel(PromptArgs a) {
+  using TL = Tile<T, HD>;
+  constexpr int kTile = TL::bytes(64);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float part[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, i = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qb = 32 * (wave & 1), kb = 32 * (wave >> 1);
+  const int hq = blockIdx.x % a.n_q, hkv = hq / (a.n_q / a.n_kv), rest = blockIdx.x / a.n_q;
+  const int b = rest % a.batch, tile = rest / a.batch;
+  const int64_t q0 = clamp_cu(a.cu_q, b, a.rows_q), q1 = clamp_cu(a.cu_q, b + 1, a.rows_q);
+  const int64_t k0 = clamp_cu(a.cu_k, b, a.rows_k), k1 = clamp_cu(a.cu_k, b + 1, a.rows_k);
+  const int lq = (int)(q1 > q0 ? q1 - q0 : 0), lk = (int)(k1 > k0 ? k1 - k0 : 0), off = lk - lq;
+  // (queries before -off see no key: out is 0 there, and so is D already)
+  const int begin = a.causal ? max(-off, 0) : 0, end = a.causal ? min(lq, kExactKeys - off) : lk <= kExactKeys ? lq : 0;
+  for (int row0 = begin + 64 * tile; row0 < end; row0 += 64 * kExactTiles) {
+    const int64_t first = q0 + row0;
+    {
+      Stage<T, HD, 64, 256> x, y;
+      x.load(static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim, a.k_stride, lk, a.head_dim, tid);
+      y.load(static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim, a.v_stride, lk, a.head_dim, tid);
+      x.store(lds, tid);
+      y.store(lds + kTile, tid);
+      x.load(static_cast<const T*>(a.q) + first * a.q_stride + hq * a.head_dim, a.q_stride, end - row0, a.head_dim, tid);
+      y.load(static_cast<const T*>(a.dout) + first * a.dout_stride + hq * a.head_dim, a.dout_stride, end - row0,
+             a.head_dim, tid);
+      x.store(lds + 2 * kTile, tid);
+      y.store(lds + 3 * kTile, tid);
+    }
+    const int r = qb + i, see = a.causal ? min(lk - 1, row0 + r + off) : lk - 1;
+    const float lse = base2_lse(a.lse[(int64_t)hq * a.rows_q + first + min(r, end - row0 - 1)]);
+    __syncthreads();
+    f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int d = 0; d < HD / 16; d++) {
+      s = tile_mma(TL::frag(lds, kb + i, d, h), TL::frag(lds + 2 * kTile, r, d, h), s);
+      dp = tile_mma(TL::frag(lds + kTile, kb + i, d, h), TL::frag(lds + 3 * kTile, r, d, h), dp);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (kb + 8 * (j >> 2) + 4 * h + (j & 3) <= see)
+        sum += __builtin_amdgcn_exp2f(fmaf(s[j], a.scale2, -lse)) * dp[j];
+    sum += __shfl_xor(sum, 32, 64);
+    if (h == 0) part[wave][i] = sum;
+    __syncthreads();
+    if (tid < 64 && row0 + tid < end)
+      a.delta[(int64_t)hq * a.rows_q + first + tid] = part[tid >> 5][tid & 31] + part[2 + (tid >> 5)][tid & 31];
+    __syncthreads();
+  }
 }
 
 template <typename T, int HD>
@@ -520,6 +583,15 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     const int64_t n = a.rows_q * a.n_q * kDeltaLanes;
     hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
+    if (sizeof(T) == 2) {
+      constexpr int lds = 4 * Tile<__bf16, HD>::bytes(64);
+      const auto kernel = prompt_delta_exact_kernel<__bf16, HD>;
+      static std::atomic<uint64_t> allowed{0};
+      if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
+      const int64_t groups = (int64_t)a.batch * a.n_q * (a.causal ? 1 : kExactTiles);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, stream, a);
+      if (hipError_t e = hipGetLastError()) return e;
+    }
   }
   constexpr int dq_lds = QG == 4 ? 4 * TL::bytes(BK) : std::max(2 * TL::bytes(128 / QG), 4 * 32 * (HD + 4) * 4);
   constexpr int lds = std::max(dkv_lds<T, HD>(), dq_lds);
@@ -551,7 +623,7 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
   p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
-                      (rows_q * n_q * kDeltaLanes + 255) / 256);
+                      std::max((rows_q * n_q * kDeltaLanes + 255) / 256, batch * n_q * kExactTiles));
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
   p.work = p.delta_bytes + (p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0);
   return p;

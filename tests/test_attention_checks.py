@@ -165,6 +165,7 @@ def test_launches_of_2_32_threads_are_refused():
     assert fwd(prompt(rows_k=2 ** 30, cu_k=P)) == RQ_ERR_HANDLE  # keys take no workgroup
     assert said(fwd(prompt(batch=2 ** 24)))
     assert said(bwd(prompt(rows_q=2 ** 26, rows_k=2 ** 26), wb=2 ** 40))  # 16 threads a row and head
+    assert said(bwd(prompt(rows_q=2 ** 25, rows_k=2 ** 30, cu_k=P), wb=2 ** 40))  # 2^24 tiles of 64 keys x 2 heads
     assert bwd(prompt(rows_q=2 ** 25, rows_k=2 ** 25), wb=2 ** 40) == RQ_ERR_HANDLE
     # 12 parts of the keys' gradient: slots count for each of them
     assert said(bwd(prompt(batch=2 ** 20, rows_q=2 ** 25, rows_k=64, n_q=8, n_kv=1, cu_k=P), qs=512, dos=512, os=512,
