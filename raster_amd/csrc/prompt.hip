@@ -14,6 +14,13 @@
 // query's scores lie in two lanes, its maximum needs one exchange, and the weights
 // are the B operand of O^T += V^T P^T as they lie. Keys and values pass through LDS
 // in tiles of BK rows for all waves, the next tile's loads in flight meanwhile.
+//
+// Bound by the matrix instructions: 4 head_dim operations for every (query, key) pair that sees the other
+// against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 542 us, 1.01 PFLOP/s (a
+// library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 133 us, 0.69; 37
+// tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16 heads x 128,
+// 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the masked
+// halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -425,23 +432,27 @@ hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
 //         4 x 64 after 4032 (32/8, 192) 80 / 71 / 60
 //   bf16  16/2 x 64: 1024 (144) 22.7 / 17.5 / 13.7   2048 (272) 41 / 29 / 29   4096 (528) 78 / 60 / 74
 //         8 x 512 (640) 16.6 / 17.5 / 24.6
-//   f32   37 tokens (16) 15.0 / 12.4 / 14.7   512 (80) 81 / 49 / 38   512 (32/8, 160) 82 / 50 / 51   613, 1, 1024,
+//   bf16  x 256, 128 / 64 queries: 512 (80) 34.8 / 26.5   2048 (272) 115 / 91   64/8 heads, 512 (320) 37.6 / 37.7
+//         8 x 256 (384) 25.9 / 34.4   4 x 64 after 4032 (64/8, 384) 201 / 147
+//   f32   (x 256: 64 queries do not fit the registers)   37 tokens (16) 15.0 / 12.4 / 14.7   512 (80) 81 / 49 / 38   512 (32/8, 160) 82 / 50 / 51   613, 1, 1024,
 //         250, 89 (320) 156 / 111 / 138   8 x 256 (384) 48 / 56 / 75   2048 (32/8, 544) 327 / 363 / 532
 //   f32   16/2 x 64: 1024 (144) 86 / 48 / 37   2048 (272) 164 / 113 / 101   8 x 256 (384) 31 / 24 / 31
 //         8 x 512 (640) 80 / 69 / 77
 static int fwd_split_groups(int dtype, const PromptArgs& a) {
-  if (a.head_dim > 128) return 0;
-  const bool f32 = dtype == RQ_F32, narrow = a.head_dim <= 64;
+  const bool f32 = dtype == RQ_F32, narrow = a.head_dim <= 64, broad = a.head_dim > 128;
+  if (f32 && broad) return 0;
   if (a.rows_k < 64 * (int64_t)a.batch) return f32 ? 2 : 0;  // hardly a tile of keys to split
   const bool few_queries = a.rows_k >= 4 * a.rows_q;  // every tile sees most keys
-  const int one = narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
-  const int two = narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
+  const int one = broad ? 0 : narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
+  const int two = broad && !few_queries ? 320 : narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
   const int64_t groups = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256;
   return groups <= (int64_t)one * a.cu_count ? 1 : groups <= (int64_t)two * a.cu_count ? 2 : 0;
 }
 
 template <int QG>
 static hipError_t launch_fwd_split(int dtype, const PromptArgs& a, hipStream_t stream) {
+  if constexpr (QG == 2)
+    if (a.head_dim > 128) return run_fwd_split<__bf16, 256, QG>(a, stream);
   if (dtype == RQ_BF16)
     return a.head_dim <= 64 ? run_fwd_split<__bf16, 64, QG>(a, stream) : run_fwd_split<__bf16, 128, QG>(a, stream);
   return a.head_dim <= 64 ? run_fwd_split<float, 64, QG>(a, stream) : run_fwd_split<float, 128, QG>(a, stream);

@@ -13,6 +13,11 @@
 // in both of the last two: 7 products for the 5 that a single kernel would need, which
 // would have to add dQ from many workgroups.
 //
+// Bound by the matrix instructions and the chain product - exponential - product of a step, with two waves a
+// SIMD: 2048, 777, 1500, 331, 1999 and 64 tokens, bf16, 32/8 heads x 128: 19 + 5.5 us for D, 438 for the rest
+// (dQ alone 195, dK and dV alone 350), 0.73 PFLOP/s of the 7 products, matrix pipe busy 0.34. f32, 129, 300, 64
+// and 511 tokens, 16/2 heads x 64: 4.8 + 53 + 6.8 us (the parts' sum).
+//
 // Rounded to bf16 in the bf16 kernels: P for dV, dS for dK and dQ (operands of their products), and the results.
 #include <algorithm>
 #include <atomic>
@@ -631,16 +636,19 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
 
 // dQ of 64 queries a workgroup (two waves over the same 32) or of 128. f32 products are long enough
 // that the finer grid is all that counts; in bf16 128 queries read keys and values half as often,
-// which is the better from about two workgroups a CU on. us of the whole gradient, 128 / 64 queries,
+// which is the better from about two workgroups a CU on (one and a quarter past 128 elements). us of the whole gradient, 128 / 64 queries,
 // causal, 16/16 heads x 128 unless said (workgroups of 128 queries):
 //   bf16  512 tokens (80) 47 / 42   2048 (272) 102 / 87   2048 (32/8 heads, 544) 188 / 183   8 x 512 (640) 78 / 79
 //         8 x 512 (32/8, 1280) 123 / 127   16/2 x 64: 2048 (272) 75 / 67
+//   bf16  x 256: 512 (80) 90 / 78   2048 (272) 276 / 245   64/8 heads, 512 (320) 136 / 132   8 x 256 (384) 86 / 90
 //   f32   512 (80) 156 / 111   2048 (272) 760 / 601   2048 (32/8, 544) 1207 / 1186   8 x 512 (32/8, 1280) 738 / 727
 //         16/2 x 64: 129, 300, 64, 511 (176) 88 / 65   2048 (272) 480 / 341   8 x 512 (640) 215 / 194
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {
-    if (a.head_dim > 128) return run_bwd<__bf16, 256, 32, 4>(a, stream);
-    const bool wide = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 > (int64_t)576 * a.cu_count;
+    const int64_t most = a.head_dim > 128 ? 320 : 576;
+    const bool wide = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 > most * a.cu_count;
+    if (a.head_dim > 128)
+      return wide ? run_bwd<__bf16, 256, 32, 4>(a, stream) : run_bwd<__bf16, 256, 32, 2>(a, stream);
     if (a.head_dim <= 64)
       return wide ? run_bwd<__bf16, 64, 64, 4>(a, stream) : run_bwd<__bf16, 64, 64, 2>(a, stream);
     return wide ? run_bwd<__bf16, 128, 32, 4>(a, stream) : run_bwd<__bf16, 128, 32, 2>(a, stream);

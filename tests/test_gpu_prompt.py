@@ -75,6 +75,9 @@ CASES = [
     ("bf16", 64, 8, 128, [300, 129, 90, 5], [300, 129, 90, 5]),
     ("bf16", 96, 8, 128, [300, 129, 90, 5], [300, 129, 90, 5]),
     ("bf16", 128, 8, 64, [300, 129, 90], [300, 129, 90]),
+    ("bf16", 16, 4, 256, [200, 70], [200, 70]),
+    ("bf16", 4, 4, 144, [5, 40], [300, 331]),
+    ("bf16", 64, 8, 200, [300, 129, 90], [300, 129, 90]),
     ("bf16", 128, 8, 72, [300, 0, 90], [310, 129, 90]),
     ("f32", 64, 8, 104, [300, 0, 90], [310, 129, 90]),
     ("f32", 64, 8, 128, [300, 129, 90], [300, 129, 90]),
