@@ -514,7 +514,7 @@ int rq_linear(rq_ctx ctx, const float* x, const float* w, const float* b, float*
  * (int32 arrays and lse 4-byte); row strides in elements, a multiple of 16
  * bytes, at least a row's elements and at most 2^22, so q, k and v may be
  * columns of one product's output; head_dim a multiple of 8 up to 256; query
- * head h reads KV head h / (n_q/n_kv); all asynchronous on `stream`, nothing
+ * head h reads KV head h / (n_q/n_kv); outputs overlap no input unless said; all asynchronous on `stream`, nothing
  * allocated and no scratch of the context used, so any number of calls and
  * captured graphs may run at once as long as their buffers differ. Results do not
  * depend on scheduling. A call whose largest launch would need 2^24 workgroups or more

@@ -68,10 +68,10 @@ def _on(stream, t):
 
 
 def _empty(scope, shape, like, dtype=None):
-    if scope is None:
-        return _t().empty(shape, dtype=dtype or like.dtype, device=like.device)
-    with scope:
-        return _t().empty(shape, dtype=dtype or like.dtype, device=like.device)
+    if scope is not None:
+        with scope:
+            return like.new_empty(shape, dtype=dtype)
+    return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
 
 
 def _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal):

@@ -1525,8 +1525,10 @@ static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) 
     return fail(RQ_ERR_SHAPE, "kpages and vpages must be 16-byte aligned");
   if (g->n_kv * g->head_dim > kMaxTileStride) return fail(RQ_ERR_SHAPE, "n_kv * head_dim too large");
   if (!(theta >= 0.0 && theta <= 1e30)) return fail(RQ_ERR_SHAPE, "theta must be positive, or 0 for no rotation");
-  return check_i32("table", g->table);
+  return RQ_OK;
 }
+
+static int check_table(const rq_pages* g) { return g->table_stride > 0 ? check_i32("table", g->table) : RQ_OK; }
 
 static PagesArgs pages_args(const rq_pages* g, int64_t n_q, int64_t batch, double theta) {
   PagesArgs a = {};
@@ -1651,6 +1653,7 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
   if (batch == 0) return RQ_OK;
   const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
+  if (int s = check_table(pg)) return s;
   if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
   if (!k != !v) return fail(RQ_ERR_NULL, "k and v must both be given, or neither");
   if (k) {
@@ -1694,6 +1697,7 @@ int rq_pages_append(rq_ctx h, const rq_pages* pg, int dtype, const void* q, int6
   if (batch < 0 || batch > kMaxRows || rows < 0) return fail(RQ_ERR_SHAPE, "bad dimension");
   if (rows > kMaxGroups) return fail(RQ_ERR_SHAPE, "too many rows for one launch");
   if (batch == 0 || rows == 0) return RQ_OK;
+  if (int s = check_table(pg)) return s;
   const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
   if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
   if (int s = check_rows("k", k, k_stride, kw, dtype)) return s;

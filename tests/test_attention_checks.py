@@ -110,7 +110,8 @@ def test_paged_entries(call):
     for kw in (dict(q=None), dict(qs=64), dict(q=P + 2), dict(batch=-1), dict(theta=-1.0), dict(theta=float("nan")),
                dict(n_q=5)):
         assert call(pages(), **kw) in (RQ_ERR_SHAPE, RQ_ERR_NULL), kw
-    assert call(pages(), batch=0) == RQ_OK
+    assert call(pages(), batch=0) == RQ_OK and call(pages(table=None), batch=0) == RQ_OK
+    assert call(pages(table=None, table_stride=0)) == RQ_ERR_HANDLE  # no row has a page
 
 
 def test_paged_attention_only():
