@@ -136,15 +136,17 @@ def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_
 
 
 def _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch):
-    shape, width = kpages.shape, n_kv * head_dim
-    for t, n in ((kpages, "kpages"), (vpages, "vpages")):
-        if t.get_device() != ctx.device or len(t.shape) != 3 or t.shape[2] != width or not t.is_contiguous():
-            raise ValueError(f"{n} must be a contiguous CUDA tensor [pages, page_size, {width}] of the context's device")
-    _need(vpages.shape == shape and vpages.dtype == kpages.dtype, "kpages and vpages must be alike")
-    ts = table.shape
-    _need(len(ts) == 2 and ts[0] == batch, "table must be [batch, pages of a sequence]")
+    shape, dev, ts = kpages.shape, ctx.device, table.shape
+    if (len(shape) != 3 or shape[2] != n_kv * head_dim or kpages.get_device() != dev or not kpages.is_contiguous()
+            or vpages.shape != shape or vpages.dtype != kpages.dtype or vpages.get_device() != dev
+            or not vpages.is_contiguous()):
+        raise ValueError(f"kpages and vpages must be contiguous CUDA tensors [pages, page_size, {n_kv * head_dim}] of one "
+                         "type on the context's device")
+    if len(ts) != 2 or ts[0] != batch:
+        raise ValueError("table must be [batch, pages of a sequence]")
+    n = ts[1]
     return Pages(_code(kpages), kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
-                 _i32(table, ctx, batch * ts[1], "table"), ts[1])
+                 _i32(table, ctx, batch * n, "table"), n)
 
 
 _work_sizes: dict = {}  # rq_paged_attention_work by its arguments
