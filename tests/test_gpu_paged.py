@@ -251,7 +251,7 @@ def test_copy(torch, ctx, planes, pages, page, width, n, t):
 
 
 def test_graphs(torch, ctx):
-    """Append, attention and copy captured, replayed on another stream between eager work."""
+    """Attention with its append captured, replayed on another stream between eager work."""
     import raster_amd
 
     nq, nkv, hd, lens = 8, 2, 128, [300, 2000]
@@ -326,3 +326,78 @@ def test_offsets_past_32_bits(torch, ctx):
         raster_amd.pages_append(ctx, q, k, v, pages[0], pages[1], table + first, cu, lens - 100, nq, nkv, hd, THETA)
         raster_amd.pages_copy(ctx, pages, [first + 3, first + 40], [first + 5, first + 63])
     assert torch.equal(outs[0], outs[1]) and torch.equal(data[:, total - used:], small)
+
+
+def test_append_and_copy_captured(torch, ctx):
+    """The copy's page numbers belong to the graph; its host lists may change after the call."""
+    import raster_amd
+
+    print("[gpu] append and copy captured", flush=True)
+    pages = torch.zeros((4, 12, 16, 128), device="cuda")
+    q, k, v = (torch.zeros((20, 128), device="cuda") for _ in range(3))
+    table = torch.tensor([[3, 1]], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    past = torch.zeros(1, dtype=torch.int32, device="cuda")
+    src, dst = [3, 1], [7, 11]
+    gr, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(gr, stream=s):
+        qo, ko = raster_amd.pages_append(ctx, q, k, v, pages[0], pages[1], table, cu, past, 1, 1, 128, THETA)
+        raster_amd.pages_copy(ctx, pages, src, dst)
+    src[:], dst[:] = [0, 0], [2, 4]
+    for i in range(3):
+        for j, t in enumerate((q, k, v)):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator(device="cuda").manual_seed(10 * i + j), device="cuda"))
+        pages.zero_()
+        past.fill_(i)
+        gr.replay()
+        torch.cuda.synchronize()
+        want = torch.zeros_like(pages)
+        wq, wk = raster_amd.pages_append(ctx, q, k, v, want[0], want[1], table, cu, past, 1, 1, 128, THETA)
+        want[:, [7, 11]] = want[:, [3, 1]]
+        assert torch.equal(pages, want) and torch.equal(qo, wq) and torch.equal(ko, wk)
+
+
+def test_threads(torch, ctx):
+    """Four host threads, each on a stream of its own, on one context."""
+    import threading
+
+    import raster_amd
+
+    nq, nkv, hd = 8, 2, 128
+    print("[gpu] paged and prompt calls of four threads", flush=True)
+    work = []
+    for i, lens in enumerate(([300, 2000], [17], [900, 1, 64], [4000])):
+        g, table, kp, vp, (q, k, v) = make(torch, i, "bf16", "bf16", nq, nkv, hd, [n + 1 for n in lens], 16, len(lens))
+        fill(torch, g, kp, vp, table, lens)
+        lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        rows = torch.randn((200 + i, (nq + 2 * nkv) * hd), generator=g, device="cuda").to(torch.bfloat16)
+        pq, pk, pv = rows.split([nq * hd, nkv * hd, nkv * hd], 1)
+        cu = torch.tensor([0, 100, 200 + i], dtype=torch.int32, device="cuda")
+        lse = torch.empty((nq, 200 + i), device="cuda")
+
+        def call(a=(q, k, v, kp, vp, table, lt), n=max(lens) + 1, b=(pq, pk, pv), cu=cu, lse=lse):
+            x = raster_amd.paged_attention(ctx, *a, nq, nkv, hd, THETA, hd ** -0.5, max_len=n)
+            y = raster_amd.prompt_attention(ctx, *b, cu, nq, nkv, hd, hd ** -0.5, lse=lse)
+            return [x, y, *raster_amd.prompt_attention_bwd(ctx, y, *b, y, lse, cu, nq, nkv, hd, hd ** -0.5)]
+
+        work.append((call, [t.clone() for t in call()]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(call, want):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = call()
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(1)
+            s.synchronize()
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
