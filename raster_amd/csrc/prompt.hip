@@ -17,7 +17,7 @@
 //
 // Bound by the matrix instructions: 4 head_dim operations for every (query, key) pair that sees the other
 // against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 542 us, 1.01 PFLOP/s (a
-// library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 133 us, 0.69; 37
+// library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 131 us, 0.70; 37
 // tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16 heads x 128,
 // 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the masked
 // halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.
@@ -228,9 +228,14 @@ __global__ __launch_bounds__(256) void prompt_fwd_kernel(PromptArgs a) {
     }
     __syncthreads();
     if (w.any(a, kb)) {
+      // products first, the other wave's softmax in their gaps: 131 us of the six sequences above, else 140
+      __builtin_amdgcn_s_setprio(1);
       x.scores(kt);
+      __builtin_amdgcn_s_setprio(0);
       x.softmax(kb, w.see, w.cut(a, kb, BK), a.scale2);
+      __builtin_amdgcn_s_setprio(1);
       x.add_values(kt + kTile);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (more) {
       char* next = lds + (buf ^ 1) * 2 * kTile;
