@@ -540,7 +540,7 @@ typedef struct {
  * prompt). A query that sees no key, or only scores of -inf, gets zeros and lse
  * -inf. lse f32[n_q][rows_q], or NULL. f32: products and sums in f32; bf16: products of
  * bf16, weights rounded to bf16 for theirs, sums, maxima and lse in f32. A NaN or
- * an inf in v also reaches the queries before it within its tile of keys (the masked weight
+ * an inf in v also reaches the queries before it within its tile of 64 keys or fewer (the masked weight
  * is 0, and 0 times them is a NaN). */
 int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,

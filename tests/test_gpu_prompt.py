@@ -382,3 +382,25 @@ def test_rows_more_than_4_gib_apart(torch, ctx):
     grads = raster_amd.prompt_attention_bwd(ctx, do, *near, want, lse, cu, nq, nkv, hd, scale)
     far = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, want, lse, cu, nq, nkv, hd, scale)
     assert all(torch.equal(a, b) for a, b in zip(grads, far))
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,n", [("bf16", 2, 1, 128, 300), ("bf16", 64, 8, 128, 700), ("bf16", 2, 1, 128, 4500),
+                                           ("f32", 2, 2, 64, 300), ("f32", 4, 1, 256, 300)])
+def test_nan_in_masked_keys_and_values(torch, ctx, t, nq, nkv, hd, n):
+    """A NaN in k reaches no query that does not see it; one in v none before its tile (64 keys at most)."""
+    import raster_amd
+
+    print(f"[gpu] masked NaN {t} {nq}/{nkv}x{hd} {n}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[t]
+    q, k, v = (rows(torch, g, n, w * hd, ty) for w in (nq, nkv, nkv))
+    cu, scale, at = cu_of(torch, [n]), hd ** -0.5, 200
+    want = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale)
+    for x, first in ((k, at), (v, at // 64 * 64)):
+        keep = x[at].clone()
+        for bad in (float("nan"), float("inf")):
+            x[at] = bad
+            out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale)
+            assert torch.equal(out[:first], want[:first])
+            assert not bool(torch.isfinite(out[at:]).all(1).any())
+        x[at] = keep
