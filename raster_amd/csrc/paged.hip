@@ -569,16 +569,18 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(char* base, int64_t pla
 
 PagedPlan plan_paged_attention(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
                                int cu_count) {
-  // About one workgroup a CU at max_len, of 128 to 1024 rows (2048 where a CU has 16 Ki or more):
+  // About one workgroup a CU at max_len, of 128 to 512 rows, up to 1024 where a CU has more of them (2048: 16 Ki):
   // fewer leave CUs idle, more pay for records and the start of a workgroup. us, rows a range
   // (bf16 pages): 32/8 heads x 128, one sequence of 4096 rows 128: 12.5, 256: 13.1, 1024: 19.2; of
   // 32768 256: 34.7, 1024: 30.3; 32 of 0 to 8191 256: 55.0, 1024: 47.0, 2048: 68.6; 64/8 heads, 8 of
   // 33 to 65 Ki 1024: 363, 2048: 352; 8/4 x 256, 16 of 2000 128: 49.1, 512: 30.9.
-  // With a group a CU and no more than 2048 rows one range, and no join: 32 of 1200 38.7 -> 32.9, 64 of 2000
-  // 107 -> 99, 32 of 1 to 1200 26.2 -> 23.9, 64 of 1 to 2000 64.3 -> 65.4.
+  // Caches cold, 512 / 1024: 8 of 4000 (1000 rows a CU) 28.5 / 29.8, of 1 to 4000 25.5 / 27.6; 16/16 heads, 8 of 4000
+  // (2000 a CU) 57.0 / 55.4, 4 of 16000 100.6 / 99.9.
+  // With a group a CU and no more than 2048 rows before the new one, one range and no join: 32 of 1200
+  // 38.7 -> 32.9, 64 of 2000 107 -> 99, 32 of 1 to 1200 26.2 -> 23.9, 64 of 1 to 2000 64.3 -> 65.4.
   const int64_t groups = std::max<int64_t>(1, batch * n_kv * ((n_q / n_kv + 15) / 16));
   const int64_t share = (max_len * groups + cu_count - 1) / std::max(cu_count, 1);
-  const int64_t most = share >= 16384 || (max_len <= 2048 && groups >= cu_count) ? 2048 : 1024;
+  const int64_t most = share >= 16384 || (max_len <= 2049 && groups >= cu_count) ? 2048 : share > 1024 ? 1024 : 512;
   const int64_t rows = std::min<int64_t>(std::max<int64_t>((share + 127) / 128 * 128, 128), most);
   PagedPlan p;
   p.split_rows = (int)rows;

@@ -401,3 +401,25 @@ def test_threads(torch, ctx):
         t.join()
     torch.cuda.synchronize()
     assert not wrong
+
+
+@pytest.mark.parametrize("nq,nkv,lens", [(64, 64, [2048, 2047, 5, 0]), (64, 64, [2049, 300, 2048, 1]), (8, 8, [600, 513, 512, 40]),
+                                         (8, 8, [9000, 1025, 1024, 2000])])
+def test_range_sizes(torch, ctx, nq, nkv, lens):
+    """Lengths at the ends of ranges of 512, 1024 and 2048 rows, by what plan_paged_attention chooses for the shape."""
+    import attn_ref as ref
+    import raster_amd
+
+    print(f"[gpu] paged ranges {nq}/{nkv} {lens}", flush=True)
+    hd = 64
+    g, table, kp, vp, (q, k, v) = make(torch, 3, "f32", "f32", nq, nkv, hd, [n + 1 for n in lens], 16, len(lens))
+    fill(torch, g, kp, vp, table, lens)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = raster_amd.paged_attention(ctx, q, k, v, kp, vp, table, lt, nq, nkv, hd, 0.0, hd ** -0.5, max_len=max(lens) + 1)
+    for b, n in enumerate(lens):
+        kk, vv = gather(kp, table, b, n + 1).double(), gather(vp, table, b, n + 1).double()
+        see = torch.ones((1, n + 1), dtype=torch.bool, device="cuda")
+        for h in range(0, nq, 7):
+            at = slice(h * hd, (h + 1) * hd)
+            want, _, bound = ref.attend(q[b:b + 1, at].double(), kk[:, at], vv[:, at], hd ** -0.5, see, ref.U)
+            assert bool(((out[b:b + 1, at].double() - want).abs() <= bound).all()), (b, h)
