@@ -201,6 +201,8 @@ class DecoderLayer:
         itself, rows stored before included. Returns [rows, d]. After the last
         layer, cache.advance(seqs, lens)."""
         torch = _t()
+        _need(len(seqs) == len(lens) == cu.numel() - 1 and sum(lens) == x.shape[0],
+              "cu, seqs and lens must be of one batch, and x of its rows")
         view = cache.view(seqs)
         q, k, v = self._split_qkv(self.w_qkv.matmul(rms_norm(torch, x, self.g1, self.eps)))
         pages_append(self.ctx, q, k, v, cache.kpages(layer), cache.vpages(layer), view.table, cu, view.lens, self.n_q,

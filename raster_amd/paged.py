@@ -66,13 +66,14 @@ class PagedCache:
         sequence idle, and following the cache's later changes from the next view() or sync()
         on (a captured graph's view). max_len defaults to the rows that the sequences
         have pages for; of all slots, to the rows that the table can hold."""
+        seqs = None if seqs is None else self._different(seqs)
         self.sync()
         if seqs is None:
             rows = self._host_table.shape[1] * self.page_size
             table, lens = self._table, self._lens
         else:
             rows = max((len(self._pages[self._known(s)]) for s in seqs), default=0) * self.page_size
-            at = _t().tensor(list(seqs), dtype=_t().long, device=self._table.device)
+            at = _t().tensor(seqs, dtype=_t().long, device=self._table.device)
             table, lens = self._table[at], self._lens[at]
         return PagedView(table, lens, rows if max_len is None else max_len)
 
@@ -89,6 +90,11 @@ class PagedCache:
         if seq not in self._pages:
             raise ValueError(f"sequence {seq} is not in the cache")
         return seq
+
+    def _different(self, seqs) -> list:
+        seqs = list(seqs)
+        _need(len(set(seqs)) == len(seqs), "a sequence may stand in a batch once")
+        return seqs
 
     def length(self, seq: int) -> int:
         return self._len[self._known(seq)]
@@ -121,9 +127,9 @@ class PagedCache:
         """Room for `rows` more rows (a number, or one a sequence) of each sequence: pages
         of its own from the row it goes on at. All or nothing: RuntimeError when there
         are not enough pages, ValueError when a sequence would outgrow the table."""
-        seqs = list(seqs)
+        seqs = self._different(seqs)
         rows = [rows] * len(seqs) if isinstance(rows, int) else list(rows)
-        _need(len(rows) == len(seqs) and len(set(seqs)) == len(seqs), "one number of rows for each, different sequence")
+        _need(len(rows) == len(seqs), "one number of rows for each sequence")
         want, refs = 0, {}
         plan = []
         for s, n in zip(seqs, rows):
@@ -159,7 +165,7 @@ class PagedCache:
 
     def advance(self, seqs, rows) -> None:
         """The rows that the operators have appended now count."""
-        seqs = list(seqs)
+        seqs = self._different(seqs)
         rows = [rows] * len(seqs) if isinstance(rows, int) else list(rows)
         _need(len(rows) == len(seqs), "one number of rows for each sequence")
         for s, n in zip(seqs, rows):

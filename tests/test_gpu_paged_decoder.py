@@ -206,3 +206,22 @@ def test_captured_step_follows_the_cache(torch, ctx, orc, weights, fused):
         _ = torch.ones(16, device="cuda").sum().item()
     r.check_rows()
     r.close()
+
+
+def test_prefill_refuses_another_batch_and_rows_without_pages(torch, ctx, orc, weights):
+    r = Run(torch, ctx, orc, weights, False, 3)
+    a, b = r.add(), r.add()
+    x, cu = torch.zeros((9, CFG["d"]), device="cuda"), torch.tensor([0, 4, 9], dtype=torch.int32, device="cuda")
+    for seqs, lens in (([a], [4, 5]), ([a, b], [9]), ([a, b], [4, 4]), ([a, b, a], [4, 4, 1])):
+        with pytest.raises(ValueError):
+            r.layers[0].prefill(x, cu, r.cache, 0, seqs, lens)
+    with pytest.raises(ValueError):
+        r.layers[0].prefill(x, cu, r.cache, 0, [a, 7], [4, 5])
+    # nothing reserved: NaN, and nothing is written
+    out = r.layers[0].prefill(x, cu, r.cache, 0, [a, b], [4, 5])
+    assert bool(torch.isnan(out).all()) and not bool(r.cache.data.any())
+    out = r.layers[0].step_paged(x[:2].contiguous(), r.cache, 0, r.cache.view([a, b]))
+    assert bool(torch.isnan(out).all()) and not bool(r.cache.data.any())
+    with pytest.raises(ValueError):
+        r.cache.advance([a, b], [4, 5])
+    r.close()

@@ -111,6 +111,10 @@ def test_refusals_change_nothing(copies):
     with pytest.raises(ValueError):
         c.advance([a], 1)  # nothing reserved
     with pytest.raises(ValueError):
+        c.advance([a, a], 0)
+    with pytest.raises(ValueError):
+        c.view([a, a])
+    with pytest.raises(ValueError):
         c.free(7)
     with pytest.raises(ValueError):
         c.fork(7)
