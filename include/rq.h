@@ -546,6 +546,11 @@ int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q
                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
                         void* stream);
 
+/* Which kernel rq_prompt_attention takes for a call of this shape, by the queries of one head in a workgroup: 32 or
+ * 64 (waves share queries and divide the keys), 128, or 256 (bf16, long sequences); 0 when there is nothing to do. For
+ * tests and traces; cu_q and cu_k are not looked at. */
+int rq_prompt_attention_tile(rq_ctx ctx, const rq_prompt* p, int* queries);
+
 /* The gradient of rq_prompt_attention: from dout and the forward's out and lse,
  * dq, dk and dv (fully overwritten in every row of a sequence, dk and dv summed
  * over the query heads of a KV head; none may overlap an input). p_ij is

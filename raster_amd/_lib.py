@@ -67,6 +67,7 @@ SIGNATURES = {
     "rq_sgemm_nt": ([_p, _p, _p, _p, _i64, _i64, _i64, C.c_float, C.c_float, _p], _i),
     "rq_linear": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _p], _i),
     "rq_prompt_attention": ([_p, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p], _i),
+    "rq_prompt_attention_tile": ([_p, _p, C.POINTER(_i)], _i),
     "rq_prompt_attention_bwd_work": ([_p, C.POINTER(_sz)], _i),
     "rq_prompt_attention_bwd": ([_p, _p, *[_p, _i64] * 5, _p, *[_p, _i64] * 3, _p, _sz, _p], _i),
     "rq_paged_attention_work": ([_p, _i64, _i64, _i64, _i64, _i64, C.POINTER(_sz)], _i),

@@ -1580,6 +1580,17 @@ int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_s
   return RQ_OK;
 }
 
+int rq_prompt_attention_tile(rq_ctx h, const rq_prompt* p, int* queries) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_prompt(p)) return s;
+  if (!queries) return fail(RQ_ERR_NULL, "queries is NULL");
+  if (int s = check_ctx(c)) return s;
+  PromptArgs a = prompt_args(p);
+  a.cu_count = c->cu_count;
+  *queries = p->batch == 0 || p->rows_q == 0 ? 0 : prompt_fwd_tile(p->dtype, a);
+  return RQ_OK;
+}
+
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes) {
   if (int s = check_prompt(p)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");

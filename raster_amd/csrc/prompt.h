@@ -34,6 +34,8 @@ struct PromptBwdPlan {
 PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,
                               int64_t head_dim);
 
+// queries of a workgroup of the kernel that launch_prompt_fwd takes: 32, 64 (both the split kernel), 128 or 256 (pair)
+int prompt_fwd_tile(int dtype, const PromptArgs& a);
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream);
 hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream);
 

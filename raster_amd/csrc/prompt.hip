@@ -463,18 +463,24 @@ static hipError_t launch_fwd_split(int dtype, const PromptArgs& a, hipStream_t s
   return a.head_dim <= 64 ? run_fwd_split<float, 64, QG>(a, stream) : run_fwd_split<float, 128, QG>(a, stream);
 }
 
+int prompt_fwd_tile(int dtype, const PromptArgs& a) {
+  if (const int qg = fwd_split_groups(dtype, a)) return 32 * qg;
+  // The pair kernel reads keys and values half as often but cuts the queries in tiles of 256.
+  // us, this / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 54.6 / 46.2, 4 x 1024
+  // 73.6 / 61.3, 8 x 2048 346 / 344, 4096 147 / 157, 8192 519 / 544, 16384 1980 / 2117; 16/16 heads:
+  // 4096 108 / 96, 4 x 4096 293 / 301, 8192 267 / 298.
+  const bool pair = dtype == RQ_BF16 && a.head_dim > 64 && a.head_dim <= 128 && a.rows_q / a.batch > 4096;
+  return pair ? 256 : 128;
+}
+
 hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
-  const int qg = fwd_split_groups(dtype, a);
-  if (qg == 1) return launch_fwd_split<1>(dtype, a, stream);
-  if (qg == 2) return launch_fwd_split<2>(dtype, a, stream);
+  const int tile = prompt_fwd_tile(dtype, a);
+  if (tile == 32) return launch_fwd_split<1>(dtype, a, stream);
+  if (tile == 64) return launch_fwd_split<2>(dtype, a, stream);
+  if (tile == 256) return run_fwd_pair<__bf16, 128, 64>(a, stream);
   if (dtype == RQ_BF16) {
     if (a.head_dim <= 64) return run_fwd<__bf16, 64, 64>(a, stream);
-    // The pair kernel reads keys and values half as often but cuts the queries in tiles of 256.
-    // us, this / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 54.6 / 46.2, 4 x 1024
-    // 73.6 / 61.3, 8 x 2048 346 / 344, 4096 147 / 157, 8192 519 / 544, 16384 1980 / 2117; 16/16 heads:
-    // 4096 108 / 96, 4 x 4096 293 / 301, 8192 267 / 298.
-    if (a.head_dim <= 128)
-      return a.rows_q / a.batch > 4096 ? run_fwd_pair<__bf16, 128, 64>(a, stream) : run_fwd<__bf16, 128, 64>(a, stream);
+    if (a.head_dim <= 128) return run_fwd<__bf16, 128, 64>(a, stream);
     return run_fwd<__bf16, 256, 32>(a, stream);
   }
   if (a.head_dim <= 64) return run_fwd<float, 64, 32>(a, stream);

@@ -1,0 +1,94 @@
+"""Which kernel a prompt runs on, and the kernel of long sequences against every head in 64 bits.
+
+rq_prompt_attention_tile names the kernel, so that each shape below is known to reach the one that it is
+for; tolerances are attn_ref.py's, as in test_gpu_prompt.py."""
+import ctypes as C
+
+import pytest
+
+from raster_amd import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+
+    if not t.cuda.is_available():
+        pytest.skip("no GPU")
+    return t
+
+
+@pytest.fixture(scope="module")
+def ctx(torch):
+    import raster_amd
+
+    c = raster_amd.Context(0)
+    yield c
+    c.close()
+
+
+def tile(ctx, t, nq, nkv, hd, lq, lk):
+    """Queries of a workgroup of the kernel for this batch."""
+    p = _lib.Prompt({"f32": _lib.RQ_F32, "bf16": _lib.RQ_BF16}[t], len(lq), sum(lq), sum(lk), nq, nkv, hd, 0x10000,
+                    0x10000, 1, 0.125)
+    n = C.c_int(-1)
+    _lib.call("rq_prompt_attention_tile", ctx.handle, C.byref(p), C.byref(n))
+    return n.value
+
+
+MORE = [
+    ("f32", 64, 8, 64, [300, 129, 90], [300, 129, 90]),
+    ("f32", 64, 8, 56, [300, 0, 90], [310, 129, 77]),
+    ("f32", 48, 4, 128, [64, 7, 33], [900, 300, 64]),  # few queries after many keys
+]
+
+
+def test_every_kernel_has_a_case(ctx):
+    """The tiles that the cases here and in test_gpu_prompt.py reach, by type and padded head size."""
+    from test_gpu_prompt import CASES
+
+    seen = {(t, 64 if hd <= 64 else 128 if hd <= 128 else 256, tile(ctx, t, nq, nkv, hd, lq, lk))
+            for t, nq, nkv, hd, lq, lk in CASES + MORE + [("bf16", *c) for c in LONG]}
+    want = {(t, w, n) for t in ("f32", "bf16") for w in (64, 128) for n in (32, 64, 128)}
+    want |= {("bf16", 256, 64), ("bf16", 256, 128), ("f32", 256, 128), ("bf16", 128, 256)}
+    assert want <= seen, want - seen
+
+
+def test_tile_of_an_empty_batch(ctx):
+    assert tile(ctx, "bf16", 4, 2, 128, [], []) == 0 and tile(ctx, "bf16", 4, 2, 128, [0], [9]) == 0
+
+
+LONG = [
+    (16, 4, 128, [4600], [4600]),
+    (12, 3, 72, [5000, 4000], [5000, 4700]),      # the end of a longer sequence
+    (16, 16, 128, [8300, 1, 4100], [8300, 1, 4100]),  # a single token beside long ones
+    (16, 2, 104, [9000, 0], [8200, 77]),          # more queries than keys: the first see none; no queries
+    (16, 4, 128, [4200], [17000]),
+    (12, 12, 128, [4999], [0]),                   # no keys
+]
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,lq,lk", MORE)
+@pytest.mark.parametrize("is_causal", [True, False], ids=["causal", "full"])
+def test_forward(torch, ctx, t, nq, nkv, hd, lq, lk, is_causal):
+    import test_gpu_prompt
+
+    test_gpu_prompt.test_forward(torch, ctx, t, nq, nkv, hd, lq, lk, is_causal)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,lq,lk", LONG)
+@pytest.mark.parametrize("is_causal", [True, False], ids=["causal", "full"])
+def test_pair_kernel(torch, ctx, nq, nkv, hd, lq, lk, is_causal):
+    import raster_amd
+    from test_gpu_prompt import check_forward, cu_of, rows
+
+    print(f"[gpu] pair kernel {nq}/{nkv}x{hd} {lq} {lk} causal={is_causal}", flush=True)
+    assert tile(ctx, "bf16", nq, nkv, hd, lq, lk) == 256
+    g = torch.Generator(device="cuda").manual_seed(sum(lq) + sum(lk))
+    q, k, v = (rows(torch, g, sum(n), w * hd, torch.bfloat16, pad=8) for n, w in ((lq, nq), (lk, nkv), (lk, nkv)))
+    scale, lse = hd ** -0.5, torch.empty((nq, sum(lq)), device="cuda")
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu_of(torch, lq), nq, nkv, hd, scale, causal=is_causal,
+                                      cu_k=None if lq == lk else cu_of(torch, lk), lse=lse)
+    check_forward(torch, q, k, v, out, lse, lq, lk, nq, nkv, hd, scale, is_causal)
