@@ -540,8 +540,8 @@ typedef struct {
  * prompt). A query that sees no key, or only scores of -inf, gets zeros and lse
  * -inf. lse f32[n_q][rows_q], or NULL. f32: products and sums in f32; bf16: products of
  * bf16, weights rounded to bf16 for theirs, sums, maxima and lse in f32. A NaN or
- * an inf in v also reaches the queries before it within its tile of 64 keys or fewer (the masked weight
- * is 0, and 0 times them is a NaN). */
+ * an inf in v also reaches queries that do not see its key but see one less than 95 before it: queries go by 32
+ * and keys by 64 at most, the masked weight is 0, and 0 times them is a NaN. */
 int rq_prompt_attention(rq_ctx ctx, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
                         void* stream);
@@ -556,7 +556,7 @@ int rq_prompt_attention_tile(rq_ctx ctx, const rq_prompt* p, int* queries);
  * over the query heads of a KV head; none may overlap an input). p_ij is
  * recomputed from lse. f32: in f32; bf16: products of bf16 with p and its gradient
  * rounded to bf16, sums in f32. A NaN or an inf in k reaches dq, one in q or dout dk and dv,
- * of masked rows too within its tile. work: rq_prompt_attention_bwd_work bytes of
+ * of masked rows too, less than 95 past the mask's edge. work: rq_prompt_attention_bwd_work bytes of
  * device memory (the rows' dout . out, and partial sums where few keys leave
  * compute units idle), 16-byte aligned, used by this call alone until it has run. */
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes);

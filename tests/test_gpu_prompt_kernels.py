@@ -92,3 +92,35 @@ def test_pair_kernel(torch, ctx, nq, nkv, hd, lq, lk, is_causal):
     out = raster_amd.prompt_attention(ctx, q, k, v, cu_of(torch, lq), nq, nkv, hd, scale, causal=is_causal,
                                       cu_k=None if lq == lk else cu_of(torch, lk), lse=lse)
     check_forward(torch, q, k, v, out, lse, lq, lk, nq, nkv, hd, scale, is_causal)
+
+
+# queries, keys; a query sees the keys up to its own number + keys - queries
+MASKED = [("bf16", 16, 4, 128, 4600, 4600, 256), ("bf16", 16, 4, 128, 4600, 4613, 256), ("bf16", 12, 3, 72, 4999, 4000, 256),
+          ("bf16", 64, 8, 128, 700, 709, 64), ("bf16", 4, 2, 128, 300, 333, 32), ("bf16", 128, 8, 128, 700, 700, 128),
+          ("f32", 64, 8, 104, 700, 719, 128), ("f32", 4, 1, 256, 300, 307, 128)]
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,lq,lk,kernel", MASKED)
+def test_reach_of_a_masked_nan(torch, ctx, t, nq, nkv, hd, lq, lk, kernel):
+    """A NaN or inf in k reaches no query that does not see its key; one in v only queries that see a key
+    less than 95 before it, on each kernel and with queries anywhere in their tiles of keys."""
+    import raster_amd
+    from test_gpu_prompt import cu_of, rows
+
+    print(f"[gpu] masked NaN {t} {nq}/{nkv}x{hd} {lq} {lk}", flush=True)
+    assert tile(ctx, t, nq, nkv, hd, [lq], [lk]) == kernel
+    g = torch.Generator(device="cuda").manual_seed(lq + lk)
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[t]
+    q, k, v = (rows(torch, g, n, w * hd, ty) for n, w in ((lq, nq), (lk, nkv), (lk, nkv)))
+    cu, cu_k, scale = cu_of(torch, [lq]), cu_of(torch, [lk]), hd ** -0.5
+    want = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, cu_k=cu_k)
+    for at in (lk // 3, lk // 3 + 41, lk - 1):
+        sees = max(at - (lk - lq), 0)  # the first query that sees key `at`
+        for x, first in ((k, sees), (v, max(sees - 94, 0))):
+            keep = x[at].clone()
+            for bad in (float("nan"), float("inf")):
+                x[at] = bad
+                out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, cu_k=cu_k)
+                assert torch.equal(out[:first], want[:first]), (at, bad)
+                assert not bool(torch.isfinite(out[sees:]).all(1).any())
+            x[at] = keep
