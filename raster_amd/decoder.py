@@ -203,6 +203,7 @@ class DecoderLayer:
         torch = _t()
         _need(len(seqs) == len(lens) == cu.numel() - 1 and sum(lens) == x.shape[0],
               "cu, seqs and lens must be of one batch, and x of its rows")
+        cache.need_own(seqs, lens)
         view = cache.view(seqs)
         q, k, v = self._split_qkv(self.w_qkv.matmul(rms_norm(torch, x, self.g1, self.eps)))
         pages_append(self.ctx, q, k, v, cache.kpages(layer), cache.vpages(layer), view.table, cu, view.lens, self.n_q,
@@ -220,6 +221,8 @@ class DecoderLayer:
         """One new token of each sequence of `view` (cache.view): x f32 [batch, d] ->
         [batch, d]. k and v are appended at the sequences' lengths (room reserved
         before); after the last layer, cache.advance(seqs, 1)."""
+        if layer == 0 and view.seqs is not None:  # (a view of all slots may be captured; advance looks again)
+            cache.need_own(view.seqs)
         fused = self.fused and x.shape[0] <= 16
         xn = None if fused else rms_norm(_t(), x, self.g1, self.eps)
         qkv = self.w_qkv.matmul_fused(x, norm_gain=self.g1, norm_eps=self.eps) if fused else self.w_qkv.matmul(xn)

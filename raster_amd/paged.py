@@ -5,8 +5,10 @@ The pages of all layers lie in one tensor [2 * layers, pages, page_size,
 n_kv * head_dim] (a layer's keys, then its values), so one pages_copy moves a
 page in every layer. A page number means the same place in every plane. Which
 sequence holds which pages is kept on the host: pages have reference counts, so
-a fork shares them, and the last, part-filled page is copied when one of its
-holders goes on writing (copy-on-write). The sequences' page table and lengths are uploaded
+a fork shares those with rows in them, and the last, part-filled page is copied when one of
+its holders reserves room to go on writing (copy-on-write), or at the fork when the sequence
+has reserved room in it already. So rows are reserved, then appended, and a reservation
+holds until its rows are used up, forks or not. The sequences' page table and lengths are uploaded
 when they have changed, on the current stream; a graph captured over the device
 arrays goes on reading them, so its replays follow later changes. One cache is used
 by one thread and on one stream at a time.
@@ -30,6 +32,13 @@ class PagedView(NamedTuple):
     table: object   # int32 [batch, pages of a sequence]
     lens: object    # int32 [batch], rows stored
     max_len: int    # no sequence has more rows (paged_attention's max_len)
+    seqs: tuple | None = None  # the sequences; None: all slots
+
+
+class _Pages(list):
+    """A sequence's pages."""
+
+    room = 0  # rows that it has reserved, those stored included
 
 
 class PagedCache:
@@ -75,7 +84,7 @@ class PagedCache:
             rows = max((len(self._pages[self._known(s)]) for s in seqs), default=0) * self.page_size
             at = _t().tensor(seqs, dtype=_t().long, device=self._table.device)
             table, lens = self._table[at], self._lens[at]
-        return PagedView(table, lens, rows if max_len is None else max_len)
+        return PagedView(table, lens, rows if max_len is None else max_len, None if seqs is None else tuple(seqs))
 
     def sync(self) -> None:
         """Uploads the page table and the lengths if they have changed."""
@@ -107,19 +116,29 @@ class PagedCache:
         if not self._slots:
             raise RuntimeError("the cache has no free slot for a sequence")
         seq = heapq.heappop(self._slots)
-        self._pages[seq], self._len[seq] = [], 0
+        self._pages[seq], self._len[seq] = _Pages(), 0
         self._host_lens[seq] = 0
         self._dirty = True
         return seq
 
     def fork(self, seq: int) -> int:
-        """A new sequence with the rows of `seq`, on the same pages."""
+        """A new sequence with the rows of `seq`, on the same pages. Room that `seq` has reserved
+        stays its own: the new sequence reserves for itself, and gets a copy of a part-filled
+        page in which `seq` has room (RuntimeError when no page is free for it)."""
         pages, n = self._pages[self._known(seq)], self._len[seq]
+        own = n % self.page_size > 0 and pages.room > n
+        if own and not self._free:
+            raise RuntimeError("the cache is full: a page is wanted for the fork")
         new = self.add()
-        for p in pages:
+        held = _Pages(pages[:-(-n // self.page_size)])
+        for p in held[:-1] if own else held:
             self._refs[p] += 1
-        self._pages[new], self._len[new] = list(pages), n
-        self._host_table[new] = self._host_table[seq]
+        if own:
+            held[-1] = self._take()
+            pages_copy(self.ctx, self.data, [pages[len(held) - 1]], [held[-1]])
+        held.room = n
+        self._pages[new], self._len[new] = held, n
+        self._host_table[new, :len(held)] = held
         self._host_lens[new] = n
         return new
 
@@ -152,16 +171,27 @@ class PagedCache:
         for s, shared, more in plan:
             for i in shared:
                 old, new = self._pages[s][i], self._take()
-                if i * self.page_size < self._len[s]:  # (a page with rows in it)
-                    src.append(old)
-                    dst.append(new)
+                src.append(old)
+                dst.append(new)
                 self._refs[old] -= 1
                 self._pages[s][i] = new
-            self._pages[s] += [self._take() for _ in range(more)]
+            self._pages[s].extend(self._take() for _ in range(more))
             self._host_table[s, :len(self._pages[s])] = self._pages[s]
             self._dirty |= bool(shared or more)
+        for s, n in zip(seqs, rows):
+            self._pages[s].room = max(self._pages[s].room, self._len[s] + n)
         if src:
             pages_copy(self.ctx, self.data, src, dst)
+
+    def need_own(self, seqs, rows=1) -> None:
+        """ValueError when the next rows (a number, or one a sequence) of one of `seqs` would go to a page
+        that another sequence holds too: a fork after which neither has reserved. Rows without a page are not
+        looked at (the operators give NaN for them)."""
+        rows = [rows] * len(seqs) if isinstance(rows, int) else rows
+        for s, n in zip(seqs, rows):
+            pages, at = self._pages[self._known(s)], self._len[s]
+            for p in pages[at // self.page_size:-(-(at + n) // self.page_size)] if n > 0 else ():
+                _need(self._refs[p] == 1, f"sequence {s} shares the page of its next rows: reserve them first")
 
     def advance(self, seqs, rows) -> None:
         """The rows that the operators have appended now count."""
@@ -171,6 +201,7 @@ class PagedCache:
         for s, n in zip(seqs, rows):
             _need(0 <= n <= len(self._pages[self._known(s)]) * self.page_size - self._len[s],
                   f"sequence {s} has no pages for {n} more rows")
+        self.need_own(seqs, rows)
         for s, n in zip(seqs, rows):
             self._len[s] += n
             self._host_lens[s] = self._len[s]

@@ -225,3 +225,29 @@ def test_prefill_refuses_another_batch_and_rows_without_pages(torch, ctx, orc, w
     with pytest.raises(ValueError):
         r.cache.advance([a, b], [4, 5])
     r.close()
+
+
+def test_fork_after_rows_reserved_ahead(torch, ctx, orc, weights):
+    """Room reserved, then a fork, then steps of both without another reservation: each writes to pages of
+    its own. Without the room, a step after a fork is refused."""
+    r = Run(torch, ctx, orc, weights, True, 3)
+    a = r.add()
+    r.prefill([a], [18])
+    r.cache.reserve([a], 5)
+    b = r.fork(a)
+    for _ in range(3):
+        x = r.x(2)
+        h = r.step(torch.from_numpy(x).cuda(), r.cache.view([a, b]))
+        r.cache.advance([a, b], 1)
+        close(h.cpu(), np.stack([r.hist[s].token(t) for s, t in zip([a, b], x)]))
+    r.check_rows()
+    c = r.fork(b)
+    x = torch.zeros((2, CFG["d"]), device="cuda")
+    for seqs in ([a, b], [a, c]):
+        with pytest.raises(ValueError):
+            r.step(x, r.cache.view(seqs))
+    with pytest.raises(ValueError):
+        r.layers[0].prefill(x, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), r.cache, 0, [c], [2])
+    r.check_rows()  # nothing was written
+    r.decode([a, b, c])
+    r.close()

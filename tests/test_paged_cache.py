@@ -172,3 +172,102 @@ def test_random_histories(copies):
                 pass  # full: nothing may have changed
             check(c)
             assert {s: read(c, s) for s in want} == want
+
+
+def test_a_fork_leaves_rows_reserved_ahead_to_their_sequence(copies):
+    """Rows reserved before a fork stay the sequence's own; the fork shares only pages with rows, and none
+    that somebody may go on writing to."""
+    c = Cache(10)
+    a = c.add()
+    c.reserve([a], 40)
+    write(c, a, range(20))
+    b = c.fork(a)
+    assert c._pages[b][:1] == c._pages[a][:1] and len(c._pages[b]) == 2 and len(copies) == 1
+    write(c, a, range(100, 120))  # as reserved, over the page's end
+    write(c, b, range(200, 212))  # its own copy of the part-filled page
+    assert read(c, a) == [*range(20), *range(100, 120)] and read(c, b) == [*range(20), *range(200, 212)]
+    check(c)
+    with pytest.raises(ValueError):
+        c.advance([b], 1)  # the next page was a's reservation, not b's
+    c.free(a)
+    c.free(b)
+    assert c.free_pages() == 10
+
+
+def test_rows_do_not_count_on_a_page_that_another_holds(copies):
+    c = Cache(10)
+    a = c.add()
+    c.reserve([a], 20)
+    write(c, a, range(20))
+    b = c.fork(a)
+    for seqs in ([a], [b], [a, b]):
+        with pytest.raises(ValueError):
+            c.advance(seqs, 1)
+        with pytest.raises(ValueError):
+            c.need_own(seqs, 1)
+    assert c.length(a) == c.length(b) == 20
+    c.need_own([a, b], 0)
+    c.reserve([b], 1)  # b's copy: the page is a's alone again
+    c.need_own([a, b], 1)
+    write(c, a, [100])
+    write(c, b, [200])
+    check(c)
+
+
+def test_a_fork_that_wants_a_page_of_a_full_cache_changes_nothing(copies):
+    c = Cache(2)
+    a = c.add()
+    c.reserve([a], 32)
+    write(c, a, range(5))
+    with pytest.raises(RuntimeError):
+        c.fork(a)
+    check(c)
+    assert len(c._pages) == 1 and not copies
+    write(c, a, range(5, 16))
+    b = c.fork(a)  # no part-filled page
+    assert read(c, b) == list(range(16)) and not copies
+    check(c)
+
+
+def test_random_histories_with_rows_reserved_ahead(copies):
+    """Rows written later than they are reserved, with forks, ends and compaction between: no page with two
+    holders is ever written (write() looks), whoever reserved."""
+    rng = random.Random(4)
+    for _ in range(60):
+        c = Cache(rng.randint(6, 30), max_seqs=rng.randint(2, 6), seq_pages=rng.randint(2, 5))
+        want, room, k = {}, {}, 0
+        for _ in range(150):
+            op = rng.choice(["add", "reserve", "reserve", "write", "write", "write", "fork", "free", "compact"])
+            live = list(want)
+            try:
+                if op == "add":
+                    s = c.add()
+                    want[s], room[s] = [], 0
+                elif op == "reserve" and live:
+                    some = rng.sample(live, rng.randint(1, len(live)))
+                    rows = [rng.randint(0, 30) for _ in some]
+                    c.reserve(some, rows)
+                    for s, n in zip(some, rows):
+                        room[s] = max(room[s], len(want[s]) + n)
+                elif op == "write" and live:
+                    s = rng.choice(live)
+                    n = rng.randint(0, room[s] - len(want[s]))
+                    write(c, s, range(k, k + n))
+                    want[s] = want[s] + list(range(k, k + n))
+                    k += n
+                elif op == "fork" and live:
+                    s = rng.choice(live)
+                    n = c.fork(s)
+                    want[n], room[n] = list(want[s]), len(want[s])
+                elif op == "free" and live:
+                    s = rng.choice(live)
+                    c.free(s)
+                    del want[s], room[s]
+                elif op == "compact":
+                    c.compact()
+            except RuntimeError:
+                pass  # full
+            except ValueError:
+                assert op == "reserve"  # would outgrow the table
+            check(c)
+            assert {s: read(c, s) for s in want} == want
