@@ -198,7 +198,8 @@ class DecoderLayer:
         (int32 [batch + 1] on the device; ranges of lens[b] rows) the next tokens of cache sequence
         seqs[b], for which cache.reserve has made room. Their keys and values go
         into the cache's pages of `layer`; each token attends its sequence up to
-        itself, rows stored before included. Returns [rows, d]. After the last
+        itself, rows stored before included, keys and values as the pages hold them (a
+        bf16 cache rounds them), however a prompt is cut. Returns [rows, d]. After the last
         layer, cache.advance(seqs, lens)."""
         torch = _t()
         _need(len(seqs) == len(lens) == cu.numel() - 1 and sum(lens) == x.shape[0],
@@ -214,6 +215,8 @@ class DecoderLayer:
             k, v = (t.to(x.dtype) for t in cache.rows(layer, seqs, lens))
             ends = np.cumsum([0] + [n0 + n for n0, n in zip(past, lens)])
             cu_k = torch.tensor(ends, dtype=torch.int32, device=x.device)
+        else:  # as they are stored, like those of a prompt that goes on and of step_paged
+            k, v = (t.to(cache.data.dtype).to(x.dtype) for t in (k, v))
         at = prompt_attention(self.ctx, q, k, v, cu, self.n_q, self.n_kv, self.hd, 1.0 / math.sqrt(self.hd), cu_k=cu_k)
         return self._mlp(residual_add(x, self.w_o.matmul(at)))
 

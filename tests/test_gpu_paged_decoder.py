@@ -251,3 +251,50 @@ def test_fork_after_rows_reserved_ahead(torch, ctx, orc, weights):
     r.check_rows()  # nothing was written
     r.decode([a, b, c])
     r.close()
+
+
+@pytest.mark.parametrize("cache_type", ["bf16", "f32"])
+def test_prefill_does_not_depend_on_the_rest_of_the_batch(torch, ctx, weights, cache_type):
+    """A fresh prompt beside another fresh one and beside one that goes on: the same rows in the same products,
+    so the same bits, in the outputs and in the pages; over bf16 pages too, where keys are attended as stored."""
+    import ctypes as C
+
+    import raster_amd
+    from raster_amd import _lib
+    from raster_amd.decoder import DecoderLayer
+
+    layers = [DecoderLayer(ctx, L["weights"], L["gain1"], L["gain2"], CFG["d"], CFG["n_q"], CFG["n_kv"],
+                           CFG["head_dim"], CFG["ffn"], CFG["eps"], CFG["theta"], fused=False) for L in weights]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    n, past = 70, 16
+    x, first = (torch.randn((rows, CFG["d"]), generator=g, device="cuda") for rows in (2 * n, past))
+    cu = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+    tiles = []
+    for rows_k in (2 * n, 2 * n + past):  # (one kernel for both: another would add in another order)
+        p, t = _lib.Prompt(_lib.RQ_F32, 2, 2 * n, rows_k, CFG["n_q"], CFG["n_kv"], CFG["head_dim"], 16, 16, 1, 0.125), C.c_int()
+        _lib.call("rq_prompt_attention_tile", ctx.handle, C.byref(p), C.byref(t))
+        tiles.append(t.value)
+    assert tiles[0] == tiles[1]
+    got = []
+    for goes_on in (False, True):
+        print(f"[gpu] prefill over {cache_type} pages, goes on: {goes_on}", flush=True)
+        cache = raster_amd.PagedCache(ctx, len(layers), 40, CFG["n_kv"], CFG["head_dim"], max_seqs=3, seq_pages=8,
+                                      dtype={"bf16": torch.bfloat16, "f32": torch.float32}[cache_type])
+        a, b = cache.add(), cache.add()
+        if goes_on:
+            cache.reserve([b], past)
+            h = first
+            for i, layer in enumerate(layers):
+                h = layer.prefill(h, torch.tensor([0, past], dtype=torch.int32, device="cuda"), cache, i, [b], [past])
+            cache.advance([b], past)
+        cache.reserve([a, b], n)
+        h = x
+        for i, layer in enumerate(layers):
+            h = layer.prefill(h, cu, cache, i, [a, b], [n, n])
+            got.append(h[:n].clone())
+        cache.advance([a, b], n)
+        got += [t for i in range(len(layers)) for t in cache.rows(i, [a])]
+    half = len(got) // 2
+    assert all(torch.equal(s, t) for s, t in zip(got[:half], got[half:]))
+    for layer in layers:
+        layer.destroy()
