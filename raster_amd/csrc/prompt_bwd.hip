@@ -45,6 +45,7 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
   const int sub = threadIdx.x % kDeltaLanes;
   if (id >= a.rows_q * a.n_q) return;
   const int64_t row = id / a.n_q;
+  if (row < clamp_cu(a.cu_q, 0, a.rows_q) || row >= clamp_cu(a.cu_q, a.batch, a.rows_q)) return;  // of no sequence
   const int hq = (int)(id % a.n_q);
   const T* o = static_cast<const T*>(a.out) + row * a.out_stride + hq * a.head_dim;
   const T* d = static_cast<const T*>(a.dout) + row * a.dout_stride + hq * a.head_dim;

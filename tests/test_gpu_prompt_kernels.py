@@ -124,3 +124,32 @@ def test_reach_of_a_masked_nan(torch, ctx, t, nq, nkv, hd, lq, lk, kernel):
                 assert torch.equal(out[:first], want[:first]), (at, bad)
                 assert not bool(torch.isfinite(out[sees:]).all(1).any())
             x[at] = keep
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_gradient_leaves_rows_of_no_sequence_alone(torch, ctx, t):
+    """dout . out, which the workspace keeps first ([n_q][rows_q]), is formed for the rows of sequences only:
+    the others, before, behind or of a padded batch, are not read."""
+    from test_gpu_prompt import cu_of, rows
+
+    nq, nkv, hd, lens, first, n = 4, 2, 64, [70, 0, 45], 5, 160
+    print(f"[gpu] gradient, rows of no sequence {t}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[t]
+    q, k, v, out, do = (rows(torch, g, n, w * hd, ty) for w in (nq, nkv, nkv, nq, nq))
+    lse, cu = torch.zeros((nq, n), device="cuda"), cu_of(torch, lens, first)
+    p = _lib.Prompt({"f32": _lib.RQ_F32, "bf16": _lib.RQ_BF16}[t], len(lens), n, n, nq, nkv, hd, cu.data_ptr(), None, 1,
+                    0.125)
+    need = C.c_size_t()
+    _lib.call("rq_prompt_attention_bwd_work", C.byref(p), C.byref(need))
+    work = torch.full((need.value // 4,), 7.0, device="cuda")
+    grads = [torch.full_like(x, 7.0) for x in (q, k, v)]
+    args = [a for x in (do, q, k, v, out) for a in (x.data_ptr(), x.stride(0))]
+    _lib.call("rq_prompt_attention_bwd", ctx.handle, C.byref(p), *args, lse.data_ptr(),
+              *[a for x in grads for a in (x.data_ptr(), x.stride(0))], work.data_ptr(), need.value,
+              torch.cuda.current_stream().cuda_stream)
+    none = torch.ones(n, dtype=torch.bool, device="cuda")
+    none[first:first + sum(lens)] = False
+    delta = work[:nq * n].view(nq, n)
+    assert bool((delta[:, none] == 7).all()) and not bool((delta[:, ~none] == 7).any())
+    assert all(bool((x[none] == 7).all()) for x in grads)
