@@ -1528,6 +1528,16 @@ static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) 
   return RQ_OK;
 }
 
+// Sequences, heads and rows of a paged attention call. What passes keeps max_len times the groups, and the
+// bytes of their records, within 64 bits.
+static int check_paged_size(int64_t batch, int64_t n_q, int64_t n_kv, int64_t max_len) {
+  if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  const int64_t htiles = (n_q / n_kv + 15) / 16;
+  if (batch * n_q > kMaxGroups || batch * n_kv * htiles > kMaxGroups)
+    return fail(RQ_ERR_SHAPE, "batch times heads too large for one launch");
+  return RQ_OK;
+}
+
 static int check_table(const rq_pages* g) { return g->table_stride > 0 ? check_i32("table", g->table) : RQ_OK; }
 
 static PagesArgs pages_args(const rq_pages* g, int64_t n_q, int64_t batch, double theta) {
@@ -1647,7 +1657,7 @@ int rq_paged_attention_work(rq_ctx h, int64_t batch, int64_t n_q, int64_t n_kv, 
                             size_t* bytes) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
   if (int s = check_heads(n_q, n_kv, head_dim)) return s;
-  if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (int s = check_paged_size(batch, n_q, n_kv, max_len)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
   if (int s = check_ctx(c)) return s;
   *bytes = batch == 0 ? 0 : plan_paged_attention(batch, n_q, n_kv, head_dim, max_len, c->cu_count).work;
@@ -1661,7 +1671,7 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   Ctx* c = reinterpret_cast<Ctx*>(h);
   if (int s = check_pages(pg, dtype, n_q, theta)) return s;
   if (int s = check_scale(scale)) return s;
-  if (batch < 0 || batch > kMaxRows || max_len < 0 || max_len > kMaxRows) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (int s = check_paged_size(batch, n_q, pg->n_kv, max_len)) return s;
   if (batch == 0) return RQ_OK;
   const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
   if (int s = check_table(pg)) return s;
@@ -1679,7 +1689,7 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
   if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
   const int64_t htiles = (n_q / pg->n_kv + 15) / 16;
-  if (plan.nsplit > kMaxGroups / (batch * pg->n_kv * htiles) || batch * n_q > kMaxGroups)
+  if (plan.nsplit > kMaxGroups / (batch * pg->n_kv * htiles))
     return fail(RQ_ERR_SHAPE, "batch times heads times rows too large for one launch");
   if (int s = set_device(c)) return s;
   PagedAttnArgs a = {};

@@ -174,3 +174,19 @@ def test_launches_of_2_32_threads_are_refused():
     assert said(append(pages(), rows=2 ** 24)) and append(pages(), rows=2 ** 24 - 1) == RQ_ERR_HANDLE
     big = dict(plane_bytes=2 ** 33, pages=8, page_bytes=2 ** 30)
     assert said(copy([0], [2], planes=256, **big)) and copy([0], [2], planes=255, **big) == RQ_ERR_HANDLE
+
+
+def test_paged_sizes_whose_products_overflow():
+    """Batch times heads past one launch is refused before anything is planned with it: max_len times the groups
+    would not fit 64 bits, and the bytes asked for would be anything."""
+    n, L = C.c_size_t(), _lib.lib()
+
+    def work(batch, n_q, n_kv, max_len):
+        return L.rq_paged_attention_work(CTX, batch, n_q, n_kv, 64, max_len, C.byref(n))
+
+    for a in ((2 ** 30, 65535, 65535, 2 ** 30), (2 ** 30, 16, 1, 2 ** 30), (2 ** 24, 1, 1, 16), (2 ** 20, 32, 1, 16)):
+        assert work(*a) == RQ_ERR_SHAPE and "one launch" in L.rq_last_error().decode(), a
+    assert work(2 ** 24 - 1, 1, 1, 2 ** 30) == RQ_ERR_HANDLE
+    wide = dict(q=P, qs=65528 * 64, os=65528 * 64, n_q=65528)
+    assert paged(pages(n_kv=1), batch=2 ** 30, max_len=2 ** 30, **wide) == RQ_ERR_SHAPE
+    assert paged(pages(n_kv=1), batch=255, ks=64, vs=64, **wide) == RQ_ERR_HANDLE
