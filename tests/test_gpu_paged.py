@@ -423,3 +423,14 @@ def test_range_sizes(torch, ctx, nq, nkv, lens):
             at = slice(h * hd, (h + 1) * hd)
             want, _, bound = ref.attend(q[b:b + 1, at].double(), kk[:, at], vv[:, at], hd ** -0.5, see, ref.U)
             assert bool(((out[b:b + 1, at].double() - want).abs() <= bound).all()), (b, h)
+
+
+@pytest.mark.parametrize("act,cache,nq,nkv,hd,page,lens", [
+    ("f32", "f32", 40, 2, 128, 16, [40, 900, 0]),   # 20 heads a KV head: two head tiles
+    ("f32", "f32", 33, 1, 64, 32, [300, 17]),       # three
+    ("f32", "bf16", 34, 2, 256, 16, [130, 600]),
+    ("f32", "bf16", 17, 1, 80, 64, [1, 2000]),
+])
+@pytest.mark.parametrize("mode", ["append", "read", "no_rope"])
+def test_many_heads_a_kv_head_in_f32(torch, ctx, act, cache, nq, nkv, hd, page, lens, mode):
+    test_paged_attention(torch, ctx, act, cache, nq, nkv, hd, page, lens, mode)

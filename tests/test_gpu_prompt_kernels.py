@@ -153,3 +153,102 @@ def test_gradient_leaves_rows_of_no_sequence_alone(torch, ctx, t):
     delta = work[:nq * n].view(nq, n)
     assert bool((delta[:, none] == 7).all()) and not bool((delta[:, ~none] == 7).any())
     assert all(bool((x[none] == 7).all()) for x in grads)
+
+
+# longer than test_gpu_prompt.py's gradients; both forms of dQ (workgroups of 128 and 64 queries) in bf16, split and whole
+# steps of dK and dV
+GRADIENTS = [
+    ("bf16", 8, 2, 128, [2049, 700], [2049, 700]),
+    ("bf16", 32, 8, 128, [2200, 1], [2200, 1]),
+    ("bf16", 16, 2, 64, [4097], [4097]),
+    ("bf16", 6, 2, 80, [1300], [2311]),           # the end of a longer sequence
+    ("bf16", 4, 4, 256, [1025, 513], [1025, 600]),
+    ("bf16", 4, 1, 128, [1500], [401]),           # more queries than keys
+    ("f32", 16, 2, 64, [2049, 700], [2049, 700]),
+    ("f32", 8, 8, 128, [1500], [1500]),
+    ("f32", 2, 1, 256, [1025], [1100]),
+]
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,lq,lk", GRADIENTS)
+@pytest.mark.parametrize("is_causal", [True, False], ids=["causal", "full"])
+def test_long_gradient(torch, ctx, t, nq, nkv, hd, lq, lk, is_causal):
+    import test_gpu_prompt
+
+    test_gpu_prompt.test_gradient(torch, ctx, t, nq, nkv, hd, lq, lk, is_causal)
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,lq,lk", [("bf16", 4, 2, 128, 500, 513), ("bf16", 32, 8, 64, 4500, 4500),
+                                               ("f32", 4, 2, 64, 500, 461), ("f32", 2, 1, 256, 300, 307)])
+def test_reach_of_a_masked_nan_in_the_gradient(torch, ctx, t, nq, nkv, hd, lq, lk):
+    """A NaN in k or v reaches dq of no query whose last key is 95 or more before it; one in q or dout no dk or dv
+    of a key 95 or more past the last that its query sees."""
+    import raster_amd
+    from test_gpu_prompt import cu_of, rows
+
+    print(f"[gpu] masked NaN, gradient {t} {nq}/{nkv}x{hd} {lq} {lk}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(lq + lk)
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[t]
+    q, k, v, do = (rows(torch, g, n, w * hd, ty) for n, w in ((lq, nq), (lk, nkv), (lk, nkv), (lq, nq)))
+    cu, cu_k, scale, off = cu_of(torch, [lq]), cu_of(torch, [lk]), hd ** -0.5, lk - lq
+    lse = torch.empty((nq, lq), device="cuda")
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, cu_k=cu_k, lse=lse)
+
+    def grads():
+        return raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, cu_k=cu_k)
+
+    want = grads()
+    for at in (200, lq - 1):
+        for x in (k, v):
+            keep = x[at + off].clone()
+            x[at + off] = float("nan")
+            dq = grads()[0]
+            assert torch.equal(dq[:max(at - 94, 0)], want[0][:max(at - 94, 0)])
+            assert bool(torch.isnan(dq[at:]).any(1).all())
+            x[at + off] = keep
+        for x in (q, do):
+            keep = x[at].clone()
+            x[at] = float("nan")
+            for got, clean in zip(grads()[1:], want[1:]):
+                assert torch.equal(got[at + off + 95:], clean[at + off + 95:])
+                assert bool(torch.isnan(got[:at + off + 1]).any(1).all())
+            x[at] = keep
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("batch", [64, 300, 5000])
+def test_many_sequences_of_a_seeded_packing(torch, ctx, dtype, batch):
+    """More sequences than a wave has lanes, empty ones and single tokens among them, the packing from the seed
+    too: every row against one dense product with a mask of equal sequences."""
+    import attn_ref as ref
+    import raster_amd
+    from test_gpu_prompt import heads, rows
+
+    print(f"[gpu] prompt {dtype} {batch} sequences", flush=True)
+    nq, nkv, hd, scale = 2, 1, 64, 0.125
+    ty = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g, gc = torch.Generator(device="cuda").manual_seed(batch), torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 4, (batch,), generator=gc)
+    lens[torch.randperm(batch, generator=gc)[batch // 4:]] = 0
+    lens[batch // 2] = 200
+    lens[-1] = 33
+    n = int(lens.sum())
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).int().cuda()
+    owner = torch.repeat_interleave(torch.arange(batch), lens).cuda()
+    see = (owner[:, None] == owner[None]) & ref.causal(n, n)
+    q, k, v, do = (rows(torch, g, n, w * hd, ty) for w in (nq, nkv, nkv, nq))
+    lse = torch.empty((nq, n), device="cuda")
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse)
+    dq, dk, dv = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale)
+    half = ref.HALF[ty]
+    sums = [0.0] * 4
+    for h in range(nq):
+        args = heads(q, h, hd), heads(k, 0, hd), heads(v, 0, hd)
+        want, wlse, bound = ref.attend(*args, scale, see, half)
+        assert bool(((heads(out, h, hd) - want).abs() <= bound).all())
+        assert bool(((lse[h].double() - wlse).abs() <= 1e-5 * (1 + wlse.abs())).all())
+        (wq, wk, wv), (bq, bk, bv) = ref.attend_grad(*args, heads(do, h, hd), scale, see, half)
+        assert bool(((heads(dq, h, hd) - wq).abs() <= bq).all())
+        sums = [a + b for a, b in zip(sums, (wk, wv, bk, bv))]
+    for got, want, bound in ((dk, sums[0], sums[2]), (dv, sums[1], sums[3])):
+        assert bool(((got.double() - want).abs() <= bound + half * want.abs()).all())
