@@ -596,7 +596,7 @@ typedef struct {
  * Rows that two sequences share are only read, provided each appends to a page of its own.
  * dtype is that of q, k, v and out: RQ_F32 over f32 or bf16 pages (f32 results:
  * over bf16 pages q and the weights enter as three bf16 terms), or RQ_BF16 over
- * bf16 pages (rotated q as two bf16 terms, the weights rounded to bf16). The cached rows are split over
+ * bf16 pages (rotated q and the weights as two bf16 terms). The cached rows are split over
  * workgroups and their softmax states joined in order. */
 int rq_paged_attention_work(rq_ctx ctx, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
                             size_t* bytes);

@@ -79,14 +79,15 @@ constexpr int paged_query_bytes(int hd) {
 // busy 0.79); 32 of 0 to 8191 rows, 32/8 heads, f32 over bf16: 45 + 5 us for 233 MB, 5.1 TB/s. One sequence of
 // 128 rows (f32, 16 heads): 9.7 us, the chain length - page number - row - scores - values of one workgroup a head.
 //
-// Over a bf16 cache the rotated queries go in as NQ and the weights P as NP bf16 terms: 3 of each
-// for f32 activations (to 2^-24); for bf16 ones 2 of the queries (to 2^-17; with 1, in the same time, the
-// error of 60 Ki rows' result is 0.0028 of its norm instead of 0.0022) and 1 of the weights (rounded).
+// Over a bf16 cache the rotated queries and the weights P go in as NT bf16 terms: 3 for f32 activations (to
+// 2^-24), 2 for bf16 ones (to 2^-17): the result's own rounding is what is left. Error of 8 sequences of 33 to 65 Ki rows,
+// of its norm: 0.0017; with one term of the weights 0.0022, of the queries too 0.0028, all in the same time (372, 370 us
+// of cold caches; 8 of 4000 rows, 32/8 heads, 34.3, 34.1; one of 128, 16 heads, 7.0, 6.9).
 // An f32 cache is multiplied in f32.
 template <typename A, typename C, int HD, bool PART>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;
-  constexpr int NQ = F32 ? 1 : sizeof(A) == 2 ? 2 : 3, NP = F32 || sizeof(A) == 2 ? 1 : 3;
+  constexpr int NT = F32 ? 1 : sizeof(A) == 2 ? 2 : 3;
   constexpr int kQueryBytes = paged_query_bytes<A, C>(HD);
   constexpr int E = HD / 16, KS = F32 ? HD / 16 : HD / 32, PE = 16 / (int)sizeof(C);
   constexpr int VP = E > PE ? E / PE : 1;     // 16-byte pieces of a lane's V elements
@@ -209,11 +210,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     if constexpr (F32) {
       sm[((e >> 4) * 64 + ((e >> 2) & 3) * 16 + hh) * 4 + (e & 3)] = x;
     } else {
-      __bf16 t[NQ];
-      split_terms<NQ>(x, t);
+      __bf16 t[NT];
+      split_terms<NT>(x, t);
       __bf16* at = reinterpret_cast<__bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
 #pragma unroll
-      for (int n = 0; n < NQ; n++) at[n * 16 * HD] = t[n];
+      for (int n = 0; n < NT; n++) at[n * 16 * HD] = t[n];
     }
   };
   auto get_query = [&](int hh, int e) {
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
       const __bf16* at = reinterpret_cast<const __bf16*>(sm) + ((e >> 5) * 64 + ((e >> 3) & 3) * 16 + hh) * 8 + (e & 7);
       float x = 0.0f;
 #pragma unroll
-      for (int n = NQ - 1; n >= 0; n--) x += (float)at[n * 16 * HD];
+      for (int n = NT - 1; n >= 0; n--) x += (float)at[n * 16 * HD];
       return x;
     }
   };
@@ -279,9 +280,9 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     const u32x4* qp = reinterpret_cast<const u32x4*>(sm) + ql;
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
-      u32x4 qw[NQ];
+      u32x4 qw[NT];
 #pragma unroll
-      for (int n = 0; n < NQ; n++) qw[n] = qp[(n * KS + ks) * 64];
+      for (int n = 0; n < NT; n++) qw[n] = qp[(n * KS + ks) * 64];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         u32x4 kw = xk[t][ks];
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
           for (int j = 0; j < 4; j++) d[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], d[t], 0, 0, 0);
         } else {
 #pragma unroll
-          for (int n = 0; n < NQ; n++)
+          for (int n = 0; n < NT; n++)
             d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kw),
                                                            __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
         }
@@ -334,13 +335,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
         for (int j = 0; j < 8; j++)
           acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(xv[j][t / PE][t % PE]), s[j], acc[t], 0, 0, 0);
     } else {
-      bf16x8 pb[NP];
+      bf16x8 pb[NT];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        __bf16 t[NP];
-        split_terms<NP>(s[j], t);
+        __bf16 t[NT];
+        split_terms<NT>(s[j], t);
 #pragma unroll
-        for (int n = 0; n < NP; n++) pb[n][j] = t[n];
+        for (int n = 0; n < NT; n++) pb[n][j] = t[n];
       }
 #pragma unroll
       for (int w = 0; w < E / 2; w++) {  // elements 2 w and 2 w + 1 of the lane
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
           hi[j] = high16_pair(e0, e1);
         }
 #pragma unroll
-        for (int n = 0; n < NP; n++) {
+        for (int n = 0; n < NT; n++) {
           acc[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), pb[n], acc[2 * w], 0, 0, 0);
           acc[2 * w + 1] =
               __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi), pb[n], acc[2 * w + 1], 0, 0, 0);

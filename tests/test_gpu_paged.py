@@ -434,3 +434,29 @@ def test_range_sizes(torch, ctx, nq, nkv, lens):
 @pytest.mark.parametrize("mode", ["append", "read", "no_rope"])
 def test_many_heads_a_kv_head_in_f32(torch, ctx, act, cache, nq, nkv, hd, page, lens, mode):
     test_paged_attention(torch, ctx, act, cache, nq, nkv, hd, page, lens, mode)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,lens", [(32, 8, 128, [4000, 333, 64]), (16, 2, 64, [900, 5000]), (4, 1, 256, [700]),
+                                            (6, 2, 80, [1500])])
+def test_bf16_over_bf16_pages_rounds_its_result_only(torch, ctx, nq, nkv, hd, lens):
+    """Queries and weights enter in two bf16 terms, off by 2^-16 at most: but for that and f32 sums, a result
+    is off by its own rounding, half a step. (With weights rounded to bf16 the first case is past it.)"""
+    import attn_ref as ref
+    import raster_amd
+
+    print(f"[gpu] paged bf16 precision {nq}/{nkv}x{hd} {lens}", flush=True)
+    n = len(lens)
+    g, table, kp, vp, (q, _, _) = make(torch, hd, "bf16", "bf16", nq, nkv, hd, lens, 16, n)
+    fill(torch, g, kp, vp, table, lens)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = raster_amd.paged_attention(ctx, q, None, None, kp, vp, table, lt, nq, nkv, hd, 0.0, hd ** -0.5,
+                                     max_len=max(lens))
+    for b, m in enumerate(lens):
+        keys, values = (gather(p, table, b, m).double().view(-1, nkv, hd) for p in (kp, vp))
+        see = torch.ones((1, m), dtype=torch.bool, device="cuda")
+        for h in range(nq):
+            j = h // (nq // nkv)
+            want, _, bound = ref.attend(q[b:b + 1, h * hd:(h + 1) * hd].double(), keys[:, j], values[:, j], hd ** -0.5,
+                                        see, 2.0 ** -16, 2.0 ** -16)
+            err = (out[b:b + 1, h * hd:(h + 1) * hd].double() - want).abs()
+            assert bool((err <= bound + ref.HALF[torch.bfloat16] * want.abs()).all()), (b, h, float((err / want.abs()).max()))
