@@ -448,11 +448,33 @@ hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
 //         250, 89 (320) 156 / 111 / 138   8 x 256 (384) 48 / 56 / 75   2048 (32/8, 544) 327 / 363 / 532
 //   f32   16/2 x 64: 1024 (144) 86 / 48 / 37   2048 (272) 164 / 113 / 101   8 x 256 (384) 31 / 24 / 31
 //         8 x 512 (640) 80 / 69 / 77
+// f32 with few queries after many keys: every workgroup walks about all keys, so a tile's time is its rounds of
+// workgroups (two a CU to 64 elements, one past them) times that of a round, by the tiles of a sequence of
+// average length. us, 128 / 64 / 32 queries:
+//   x 128   4 x 64 after 4032 (32/8 heads) 569 / 334 / 242   (64/8) 570 / 334 / 479   8 x 16 after 984 (32/8) 146 / 88 / 70
+//           8 x 64 after 1984 (32/8) 289 / 173 / 247   8 x 128 after 896 (16/16) 153 / 91 / 132   2 x 300 after 2700
+//           (32/8) 429 / 466 / 512
+//   x 64    4 x 64 after 4032 (64/8) 523 / 290 / 164   8 x 64 after 1984 (64/8) 267 / 151 / 166   16 x 64 after 960 (64/8)
+//           269 / 155 / 176   16 x 20 after 1004 (64/8) 158 / 150 / 89   2 x 300 after 2700 (32/8) 231 / 208 / 177
+static int f32_few_queries_groups(const PromptArgs& a, bool narrow) {
+  const int64_t len = (a.rows_q + a.batch - 1) / a.batch, places = (int64_t)a.cu_count * (narrow ? 2 : 1);
+  const int64_t round[2][3] = {{242, 334, 569}, {41, 75, 134}};  // of 32, 64 and 128 queries
+  int64_t best = 0;
+  int tile = 0;
+  for (int i = 0; i < 3; i++) {
+    const int64_t groups = a.batch * ((len + (32 << i) - 1) / (32 << i)) * a.n_q;
+    const int64_t time = (groups + places - 1) / places * round[narrow][i];
+    if (i == 0 || time < best) best = time, tile = i;
+  }
+  return tile == 2 ? 0 : tile + 1;
+}
+
 static int fwd_split_groups(int dtype, const PromptArgs& a) {
   const bool f32 = dtype == RQ_F32, narrow = a.head_dim <= 64, broad = a.head_dim > 128;
   if (f32 && broad) return 0;
   if (a.rows_k < 64 * (int64_t)a.batch) return f32 ? 2 : 0;  // hardly a tile of keys to split
   const bool few_queries = a.rows_k >= 4 * a.rows_q;  // every tile sees most keys
+  if (f32 && few_queries) return f32_few_queries_groups(a, narrow);
   const int one = broad ? 0 : narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
   const int two = broad && !few_queries ? 320 : narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
   const int64_t groups = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256;
@@ -471,9 +493,9 @@ static hipError_t launch_fwd_split(int dtype, const PromptArgs& a, hipStream_t s
 int prompt_fwd_tile(int dtype, const PromptArgs& a) {
   if (const int qg = fwd_split_groups(dtype, a)) return 32 * qg;
   // The pair kernel reads keys and values half as often but cuts the queries in tiles of 256.
-  // us, this (before it left out unseen tiles) / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 54.6 / 46.2, 4 x 1024
-  // 73.6 / 61.3, 8 x 2048 346 / 344, 4096 147 / 157, 8192 519 / 544, 16384 1980 / 2117; 16/16 heads:
-  // 4096 108 / 96, 4 x 4096 293 / 301, 8192 267 / 298.
+  // us, this / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 52 / 43, 4 x 1024 68 / 58, 4 x 3000
+  // 314 / 312, 4 x 4096 548 / 548, 4096 139 / 142, 8192 502 / 520, 16384 1919 / 2021; 16/16 heads: 4096
+  // 106 / 103, 4 x 4096 279 / 281, 8192 256 / 267.
   const bool pair = dtype == RQ_BF16 && a.head_dim > 64 && a.head_dim <= 128 && a.rows_q / a.batch > 4096;
   return pair ? 256 : 128;
 }

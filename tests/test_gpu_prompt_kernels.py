@@ -42,6 +42,10 @@ MORE = [
     ("f32", 64, 8, 64, [300, 129, 90], [300, 129, 90]),
     ("f32", 64, 8, 56, [300, 0, 90], [310, 129, 77]),
     ("f32", 48, 4, 128, [64, 7, 33], [900, 300, 64]),  # few queries after many keys
+    ("f32", 32, 8, 128, [16, 1, 31], [700, 90, 131]),
+    ("f32", 32, 8, 128, [290, 300], [1900, 1300]),
+    ("f32", 64, 8, 64, [64] * 8, [300] * 8),
+    ("f32", 64, 8, 56, [20] * 8, [90] * 8),
 ]
 
 
@@ -54,6 +58,23 @@ def test_every_kernel_has_a_case(ctx):
     want = {(t, w, n) for t in ("f32", "bf16") for w in (64, 128) for n in (32, 64, 128)}
     want |= {("bf16", 256, 64), ("bf16", 256, 128), ("f32", 256, 128), ("bf16", 128, 256)}
     assert want <= seen, want - seen
+
+
+@pytest.mark.parametrize("nq,nkv,hd,batch,new,keys,want", [
+    (32, 8, 128, 4, 64, 4096, 32), (64, 8, 128, 4, 64, 4096, 64), (32, 8, 128, 8, 64, 2048, 64), (32, 8, 128, 8, 16, 1000, 32),
+    (16, 16, 128, 8, 128, 1024, 64), (32, 8, 128, 2, 300, 3000, 128), (64, 8, 64, 4, 64, 4096, 32), (64, 8, 64, 8, 64, 2048, 64),
+    (64, 8, 64, 16, 64, 1024, 64), (64, 8, 64, 16, 20, 1024, 32)])
+def test_f32_tile_of_few_queries(ctx, nq, nkv, hd, batch, new, keys, want):
+    """The fastest of the three by the times beside the rule, for queries that go on after many keys."""
+    if _cus() != 256:
+        pytest.skip("the times are of 256 CUs")
+    assert tile(ctx, "f32", nq, nkv, hd, [new] * batch, [keys] * batch) == want
+
+
+def _cus():
+    import torch
+
+    return torch.cuda.get_device_properties(0).multi_processor_count
 
 
 def test_tile_of_an_empty_batch(ctx):
