@@ -591,7 +591,8 @@ typedef struct {
  * model's layers share it. lens[b] < 0: an idle slot, its out row is zeros and its pages
  * are not touched; so is the out row of a sequence without rows. max_len: no sequence has more
  * rows than this, the new one included; it sizes work (rq_paged_attention_work
- * bytes, none when 0). A sequence with more rows than max_len or its table holds, or a page
+ * bytes, none when 0) and the ranges that the rows are split into, so one far past the real
+ * lengths costs time. A sequence with more rows than max_len or its table holds, or a page
  * number outside 0 .. pages - 1, gets NaN, and nothing is written outside the pages.
  * Rows that two sequences share are only read, provided each appends to a page of its own.
  * dtype is that of q, k, v and out: RQ_F32 over f32 or bf16 pages (f32 results:

@@ -75,7 +75,7 @@ constexpr int paged_query_bytes(int hd) {
 // Nothing of the cache passes through LDS.
 //
 // Bound by the cache rows' way from memory: 8 sequences of 33 to 65 Ki rows, 64/8 heads x 128, bf16, pages of
-// 64: 335 + 6 us (join) for 1.77 GB, 5.2 TB/s (a plain read 6.2; the workgroups' last round leaves CUs idle:
+// 64: 346 + 6 us (join) for 1.77 GB, 5.1 TB/s (a plain read 6.2; the workgroups' last round leaves CUs idle:
 // busy 0.79); 32 of 0 to 8191 rows, 32/8 heads, f32 over bf16: 45 + 5 us for 233 MB, 5.1 TB/s. One sequence of
 // 128 rows (f32, 16 heads): 9.7 us, the chain length - page number - row - scores - values of one workgroup a head.
 //

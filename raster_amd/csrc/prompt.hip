@@ -16,8 +16,8 @@
 // in tiles of BK rows for all waves, the next tile's loads in flight meanwhile.
 //
 // Bound by the matrix instructions: 4 head_dim operations for every (query, key) pair that sees the other
-// against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 542 us, 1.01 PFLOP/s (a
-// library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 125 to 131 us, 0.70; 37
+// against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 502 to 511 us, 1.08 PFLOP/s, 558 us on a
+// card warm from other work (a library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 124 us, 0.74; 37
 // tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16 heads x 128,
 // 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the masked
 // halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.

@@ -14,7 +14,7 @@
 // would have to add dQ from many workgroups.
 //
 // Bound by the matrix instructions and the chain product - exponential - product of a step, with two waves a
-// SIMD: 2048, 777, 1500, 331, 1999 and 64 tokens, bf16, 32/8 heads x 128: 19 + 5.5 us for D, 438 for the rest
+// SIMD: 2048, 777, 1500, 331, 1999 and 64 tokens, bf16, 32/8 heads x 128: 19 + 5.5 us for D, 433 for the rest
 // (dQ alone 195, dK and dV alone 350), 0.73 PFLOP/s of the 7 products, matrix pipe busy 0.34. f32, 129, 300, 64
 // and 511 tokens, 16/2 heads x 64: 4.8 + 53 + 6.8 us (the parts' sum).
 //

@@ -74,7 +74,9 @@ class PagedCache:
         """The device arrays of `seqs`, as of now; None: of all slots, those without a
         sequence idle, and following the cache's later changes from the next view() or sync()
         on (a captured graph's view). max_len defaults to the rows that the sequences
-        have pages for; of all slots, to the rows that the table can hold."""
+        have pages for; of all slots, to the rows that the table can hold: a step is planned
+        for it, so give the largest length that is served, or seq_pages, when that is far less
+        (32 sequences of 1000 rows: 32 us planned for 1001 rows, 40 for 65536, 287 for 1 Mi)."""
         seqs = None if seqs is None else self._different(seqs)
         self.sync()
         if seqs is None:
