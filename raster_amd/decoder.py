@@ -224,8 +224,8 @@ class DecoderLayer:
         """One new token of each sequence of `view` (cache.view): x f32 [batch, d] ->
         [batch, d]. k and v are appended at the sequences' lengths (room reserved
         before); after the last layer, cache.advance(seqs, 1)."""
-        if layer == 0 and view.seqs is not None:  # (a view of all slots may be captured; advance looks again)
-            cache.need_own(view.seqs)
+        if layer == 0:  # (a view of all slots has no seqs and may be captured; advance looks again)
+            cache.need_own(getattr(view, "seqs", ()))
         fused = self.fused and x.shape[0] <= 16
         xn = None if fused else rms_norm(_t(), x, self.g1, self.eps)
         qkv = self.w_qkv.matmul_fused(x, norm_gain=self.g1, norm_eps=self.eps) if fused else self.w_qkv.matmul(xn)

@@ -32,7 +32,12 @@ class PagedView(NamedTuple):
     table: object   # int32 [batch, pages of a sequence]
     lens: object    # int32 [batch], rows stored
     max_len: int    # no sequence has more rows (paged_attention's max_len)
-    seqs: tuple | None = None  # the sequences; None: all slots
+
+
+class _SeqsView(PagedView):
+    """A view of chosen sequences, which step_paged looks up again."""
+
+    seqs: tuple = ()
 
 
 class _Pages(list):
@@ -86,7 +91,10 @@ class PagedCache:
             rows = max((len(self._pages[self._known(s)]) for s in seqs), default=0) * self.page_size
             at = _t().tensor(seqs, dtype=_t().long, device=self._table.device)
             table, lens = self._table[at], self._lens[at]
-        return PagedView(table, lens, rows if max_len is None else max_len, None if seqs is None else tuple(seqs))
+        view = (PagedView if seqs is None else _SeqsView)(table, lens, rows if max_len is None else max_len)
+        if seqs is not None:
+            view.seqs = tuple(seqs)
+        return view
 
     def sync(self) -> None:
         """Uploads the page table and the lengths if they have changed."""

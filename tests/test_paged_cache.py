@@ -271,3 +271,12 @@ def test_random_histories_with_rows_reserved_ahead(copies):
                 assert op == "reserve"  # would outgrow the table
             check(c)
             assert {s: read(c, s) for s in want} == want
+
+
+def test_a_view_unpacks_into_three():
+    table, lens, max_len = paged.PagedView(1, 2, 3)
+    assert (table, lens, max_len) == (1, 2, 3)
+    view = paged._SeqsView(1, 2, 3)
+    view.seqs = (4, 5)
+    table, lens, max_len = view
+    assert view == paged.PagedView(1, 2, 3) and view.seqs == (4, 5) and isinstance(view, paged.PagedView)
