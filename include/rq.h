@@ -566,6 +566,23 @@ int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, in
                             void* dk, int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
                             void* stream);
 
+/* rq_prompt_attention and its gradient with a sliding window and sinks: the query at position i = its row +
+ * keys - queries of its sequence sees the keys j <= i with i - j < window, or with j < sinks (the first tokens, which
+ * stay visible). window 0: all keys up to i, as without; else causal must be 1. A query sees itself at least, so only one
+ * before the first key (more queries than keys) sees nothing. Otherwise as above; the reach of a NaN or an inf in
+ * keys or values that a query does not see is the same on both sides of the window. */
+int rq_prompt_attention_window(rq_ctx ctx, const rq_prompt* p, int64_t window, int64_t sinks, const void* q,
+                               int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                               void* out, int64_t out_stride, float* lse, void* stream);
+int rq_prompt_attention_window_tile(rq_ctx ctx, const rq_prompt* p, int64_t window, int64_t sinks, int* queries);
+int rq_prompt_attention_window_bwd_work(const rq_prompt* p, int64_t window, int64_t sinks, size_t* bytes);
+int rq_prompt_attention_window_bwd(rq_ctx ctx, const rq_prompt* p, int64_t window, int64_t sinks, const void* dout,
+                                   int64_t dout_stride, const void* q, int64_t q_stride, const void* k,
+                                   int64_t k_stride, const void* v, int64_t v_stride, const void* out,
+                                   int64_t out_stride, const float* lse, void* dq, int64_t dq_stride, void* dk,
+                                   int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
+                                   void* stream);
+
 /* One layer's cache in pages: kpages and vpages hold `pages` pages of page_size
  * rows (a power of two, 16 to 65536) of n_kv * head_dim elements, a row of
  * rq_decode_attention's caches each. Row r of sequence b lies in page

@@ -70,6 +70,10 @@ SIGNATURES = {
     "rq_prompt_attention_tile": ([_p, _p, C.POINTER(_i)], _i),
     "rq_prompt_attention_bwd_work": ([_p, C.POINTER(_sz)], _i),
     "rq_prompt_attention_bwd": ([_p, _p, *[_p, _i64] * 5, _p, *[_p, _i64] * 3, _p, _sz, _p], _i),
+    "rq_prompt_attention_window": ([_p, _p, _i64, _i64, *[_p, _i64] * 4, _p, _p], _i),
+    "rq_prompt_attention_window_tile": ([_p, _p, _i64, _i64, C.POINTER(_i)], _i),
+    "rq_prompt_attention_window_bwd_work": ([_p, _i64, _i64, C.POINTER(_sz)], _i),
+    "rq_prompt_attention_window_bwd": ([_p, _p, _i64, _i64, *[_p, _i64] * 5, _p, *[_p, _i64] * 3, _p, _sz, _p], _i),
     "rq_paged_attention_work": ([_p, _i64, _i64, _i64, _i64, _i64, C.POINTER(_sz)], _i),
     "rq_paged_attention": ([_p, _p, _i, *[_p, _i64] * 3, _p, _i64, _i64, _i64, C.c_double, C.c_double, _p, _i64, _p,
                             _sz, _p], _i),

@@ -87,17 +87,29 @@ def _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal):
     return p, qs, ks, vs
 
 
+def _window(window, sinks) -> tuple:
+    """(window, sinks) as the C entries take them."""
+    window = 0 if window is None else window
+    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    return min(window, _FAR), min(sinks, _FAR)
+
+
+_FAR = 1 << 40  # past every row
+
+
 def _check_lse(lse, ctx, n):
     _need(lse.dtype == _t().float32 and lse.get_device() == ctx.device and lse.is_contiguous() and lse.numel() == n,
           "lse must be a contiguous f32 CUDA tensor [n_q, rows] of the context's device")
 
 
 def prompt_attention(ctx: Context, q, k, v, cu, n_q: int, n_kv: int, head_dim: int, scale: float, causal: bool = True,
-                     cu_k=None, out=None, lse=None, stream=None):
+                     cu_k=None, out=None, lse=None, stream=None, window: int | None = None, sinks: int = 0):
     """rq_prompt_attention: q [rows, n_q*head_dim], k and v [rows_k, n_kv*head_dim]
     (f32 or bf16), sequence b in rows cu[b] .. cu[b+1] - 1 (int32 [batch + 1];
     cu_k: the keys', when they differ) -> out [rows, n_q*head_dim]. lse f32
-    [n_q, rows] is filled when given (prompt_attention_bwd needs it)."""
+    [n_q, rows] is filled when given (prompt_attention_bwd needs it). window
+    (rq_prompt_attention_window, causal only): a query sees the last `window` keys up to
+    itself and the sequence's first `sinks`; None or 0: all."""
     p, qs, ks, vs = _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal)
     raw, scope = _on(stream, q)
     width = n_q * head_dim
@@ -107,29 +119,31 @@ def prompt_attention(ctx: Context, q, k, v, cu, n_q: int, n_kv: int, head_dim: i
         os = _rows(out, ctx, q.shape[0], width, q.dtype, "out")
     if lse is not None:
         _check_lse(lse, ctx, n_q * q.shape[0])
-    call("rq_prompt_attention", ctx.handle, C.byref(p), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-         out.data_ptr(), os, None if lse is None else lse.data_ptr(), raw)
+    call("rq_prompt_attention_window", ctx.handle, C.byref(p), *_window(window, sinks), q.data_ptr(), qs, k.data_ptr(),
+         ks, v.data_ptr(), vs, out.data_ptr(), os, None if lse is None else lse.data_ptr(), raw)
     return out
 
 
 def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_kv: int, head_dim: int, scale: float,
-                         causal: bool = True, cu_k=None, dq=None, dk=None, dv=None, stream=None):
-    """rq_prompt_attention_bwd: the gradient of prompt_attention for dout, from
-    the forward's out and lse -> (dq, dk, dv), written into the given tensors if any."""
+                         causal: bool = True, cu_k=None, dq=None, dk=None, dv=None, stream=None,
+                         window: int | None = None, sinks: int = 0):
+    """rq_prompt_attention_bwd (with a window rq_prompt_attention_window_bwd): the gradient of
+    prompt_attention for dout, from the forward's out and lse -> (dq, dk, dv), written into the given
+    tensors if any. window and sinks: the forward's."""
     p, qs, ks, vs = _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal)
     qw, kw, rows, rows_k, dtype = n_q * head_dim, n_kv * head_dim, q.shape[0], k.shape[0], q.dtype
     dos = _rows(dout, ctx, rows, qw, dtype, "dout")
     os = _rows(out, ctx, rows, qw, dtype, "out")
     _check_lse(lse, ctx, n_q * rows)
-    need = C.c_size_t()
-    call("rq_prompt_attention_bwd_work", C.byref(p), C.byref(need))
+    need, seen = C.c_size_t(), _window(window, sinks)
+    call("rq_prompt_attention_window_bwd_work", C.byref(p), *seen, C.byref(need))
     raw, scope = _on(stream, q)
     work = _empty(scope, need.value // 4, q, _t().float32)
     dq = _empty(scope, (rows, qw), q) if dq is None else dq
     dk, dv = (_empty(scope, (rows_k, kw), q) if t is None else t for t in (dk, dv))
     dqs = _rows(dq, ctx, rows, qw, dtype, "dq")
     dks, dvs = _rows(dk, ctx, rows_k, kw, dtype, "dk"), _rows(dv, ctx, rows_k, kw, dtype, "dv")
-    call("rq_prompt_attention_bwd", ctx.handle, C.byref(p), dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
+    call("rq_prompt_attention_window_bwd", ctx.handle, C.byref(p), *seen, dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
          v.data_ptr(), vs, out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(),
          dvs, work.data_ptr(), need.value, raw)
     return dq, dk, dv

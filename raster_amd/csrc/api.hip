@@ -1494,8 +1494,25 @@ static int check_prompt(const rq_prompt* p) {
   return RQ_OK;
 }
 
-static PromptArgs prompt_args(const rq_prompt* p) {
+static int check_window(int64_t window, int64_t sinks) {
+  if (window < 0 || sinks < 0) return fail(RQ_ERR_SHAPE, "window and sinks must not be negative");
+  return RQ_OK;
+}
+
+static int check_prompt_window(const rq_prompt* p, int64_t window, int64_t sinks) {
+  if (int s = check_prompt(p)) return s;
+  if (int s = check_window(window, sinks)) return s;
+  if (window > 0 && !p->causal) return fail(RQ_ERR_SHAPE, "a window needs causal");
+  return RQ_OK;
+}
+
+static PromptArgs prompt_args(const rq_prompt* p, int64_t window, int64_t sinks) {
   PromptArgs a = {};
+  // with window + sinks keys or fewer every query sees all up to itself
+  if (window > 0 && window < p->rows_k && sinks < p->rows_k - window) {
+    a.window = (int)window;
+    a.sinks = (int)sinks;
+  }
   a.cu_q = p->cu_q;
   a.cu_k = p->cu_k ? p->cu_k : p->cu_q;
   a.rows_q = p->rows_q;
@@ -1564,8 +1581,14 @@ extern "C" {
 int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, void* out, int64_t out_stride, float* lse,
                         void* stream) {
+  return rq_prompt_attention_window(h, p, 0, 0, q, q_stride, k, k_stride, v, v_stride, out, out_stride, lse, stream);
+}
+
+int rq_prompt_attention_window(rq_ctx h, const rq_prompt* p, int64_t window, int64_t sinks, const void* q,
+                               int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                               void* out, int64_t out_stride, float* lse, void* stream) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
-  if (int s = check_prompt(p)) return s;
+  if (int s = check_prompt_window(p, window, sinks)) return s;
   if (p->batch == 0 || p->rows_q == 0) return RQ_OK;
   const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
   if (int s = check_i32("cu_q", p->cu_q)) return s;
@@ -1581,7 +1604,7 @@ int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_s
     if (int s = check_i32("lse", lse)) return s;
   if (int s = check_ctx(c)) return s;
   if (int s = set_device(c)) return s;
-  PromptArgs a = prompt_args(p);
+  PromptArgs a = prompt_args(p, window, sinks);
   a.cu_count = c->cu_count;
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
@@ -1591,20 +1614,28 @@ int rq_prompt_attention(rq_ctx h, const rq_prompt* p, const void* q, int64_t q_s
 }
 
 int rq_prompt_attention_tile(rq_ctx h, const rq_prompt* p, int* queries) {
+  return rq_prompt_attention_window_tile(h, p, 0, 0, queries);
+}
+
+int rq_prompt_attention_window_tile(rq_ctx h, const rq_prompt* p, int64_t window, int64_t sinks, int* queries) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
-  if (int s = check_prompt(p)) return s;
+  if (int s = check_prompt_window(p, window, sinks)) return s;
   if (!queries) return fail(RQ_ERR_NULL, "queries is NULL");
   if (int s = check_ctx(c)) return s;
-  PromptArgs a = prompt_args(p);
+  PromptArgs a = prompt_args(p, window, sinks);
   a.cu_count = c->cu_count;
   *queries = p->batch == 0 || p->rows_q == 0 ? 0 : prompt_fwd_tile(p->dtype, a);
   return RQ_OK;
 }
 
 int rq_prompt_attention_bwd_work(const rq_prompt* p, size_t* bytes) {
-  if (int s = check_prompt(p)) return s;
+  return rq_prompt_attention_window_bwd_work(p, 0, 0, bytes);
+}
+
+int rq_prompt_attention_window_bwd_work(const rq_prompt* p, int64_t window, int64_t sinks, size_t* bytes) {
+  if (int s = check_prompt_window(p, window, sinks)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
-  *bytes = plan_prompt_bwd(p->batch, p->rows_q, p->rows_k, p->n_q, p->n_kv, p->head_dim).work;
+  *bytes = plan_prompt_bwd(prompt_args(p, window, sinks)).work;
   return RQ_OK;
 }
 
@@ -1613,11 +1644,23 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
                             const void* out, int64_t out_stride, const float* lse, void* dq, int64_t dq_stride,
                             void* dk, int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
                             void* stream) {
+  return rq_prompt_attention_window_bwd(h, p, 0, 0, dout, dout_stride, q, q_stride, k, k_stride, v, v_stride, out,
+                                        out_stride, lse, dq, dq_stride, dk, dk_stride, dv, dv_stride, work, work_bytes,
+                                        stream);
+}
+
+int rq_prompt_attention_window_bwd(rq_ctx h, const rq_prompt* p, int64_t window, int64_t sinks, const void* dout,
+                                   int64_t dout_stride, const void* q, int64_t q_stride, const void* k,
+                                   int64_t k_stride, const void* v, int64_t v_stride, const void* out,
+                                   int64_t out_stride, const float* lse, void* dq, int64_t dq_stride, void* dk,
+                                   int64_t dk_stride, void* dv, int64_t dv_stride, void* work, size_t work_bytes,
+                                   void* stream) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
-  if (int s = check_prompt(p)) return s;
+  if (int s = check_prompt_window(p, window, sinks)) return s;
   if (p->batch == 0 || (p->rows_q == 0 && p->rows_k == 0)) return RQ_OK;
   const int64_t qw = p->n_q * p->head_dim, kw = p->n_kv * p->head_dim;
-  const PromptBwdPlan plan = plan_prompt_bwd(p->batch, p->rows_q, p->rows_k, p->n_q, p->n_kv, p->head_dim);
+  PromptArgs a = prompt_args(p, window, sinks);
+  const PromptBwdPlan plan = plan_prompt_bwd(a);
   if (plan.groups > kMaxGroups) return fail(RQ_ERR_SHAPE, "rows times heads too large for one launch");
   if (int s = check_i32("cu_q", p->cu_q)) return s;
   if (p->cu_k)
@@ -1640,7 +1683,6 @@ int rq_prompt_attention_bwd(rq_ctx h, const rq_prompt* p, const void* dout, int6
   }
   if (int s = check_ctx(c)) return s;
   if (int s = set_device(c)) return s;
-  PromptArgs a = prompt_args(p);
   a.q = q, a.k = k, a.v = v, a.out = const_cast<void*>(out), a.lse = const_cast<float*>(lse), a.dout = dout;
   a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
   a.dout_stride = dout_stride, a.dq_stride = dq_stride, a.dk_stride = dk_stride, a.dv_stride = dv_stride;

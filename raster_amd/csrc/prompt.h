@@ -10,6 +10,7 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int64_t rows_q, rows_k, slots, q_slots, k_slots;
   int batch, n_q, n_kv, head_dim, causal, cu_count;
+  int window, sinks;  // keys that a query sees up to itself and, before those, of the first ones; 0, 0: all
   float scale, scale2;  // scale2 = scale log2 e
   const void *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;
@@ -26,13 +27,61 @@ struct PromptArgs {
   int nsplit;
 };
 
+// With a window (WIN) the query at position i of its sequence sees the keys j <= i with i - j < window or
+// j < sinks. Whole tiles of keys that no query of a workgroup sees, between the sinks and the first query's
+// window, are walked past; what is left is masked where a tile is cut.
+template <bool WIN>
+struct Seen {  // by one query
+  int last;
+  __device__ __forceinline__ void init(const PromptArgs& a, int qi, int off, int lk) {
+    last = a.causal ? min(lk - 1, qi + off) : lk - 1;
+  }
+  __device__ __forceinline__ bool sees(int key) const { return key <= last; }
+};
+template <>
+struct Seen<true> {
+  int last, first, sinks;
+  __device__ __forceinline__ void init(const PromptArgs& a, int qi, int off, int lk) {
+    last = min(lk - 1, qi + off);
+    first = qi + off - a.window + 1;
+    sinks = a.sinks;
+  }
+  __device__ __forceinline__ bool sees(int key) const { return key <= last && (key >= first || key < sinks); }
+};
+
+template <bool WIN>
+struct Walk {  // the keys of a workgroup's steps
+  __device__ __forceinline__ int leave_out(const PromptArgs&, int, int) { return 0; }
+  __device__ __forceinline__ int key(int at) const { return at; }
+};
+template <>
+struct Walk<true> {
+  int sink_end, skip;
+  // pos: position of the first query, bk: keys of a step. Returns how many keys are left out.
+  __device__ __forceinline__ int leave_out(const PromptArgs& a, int pos, int bk) {
+    sink_end = (a.sinks + bk - 1) / bk * bk;
+    skip = max(max(pos - a.window + 1, 0) / bk * bk - sink_end, 0);
+    return skip;
+  }
+  __device__ __forceinline__ int key(int at) const { return at < sink_end ? at : at + skip; }
+};
+
+// whether the query at `pos` sees by its window or the sinks any, or all, of the n keys from `key` on
+template <bool WIN>
+__device__ __forceinline__ bool window_any(const PromptArgs& a, int pos, int key, int n) {
+  return !WIN || key + n - 1 > pos - a.window || key < a.sinks;
+}
+template <bool WIN>
+__device__ __forceinline__ bool window_all(const PromptArgs& a, int pos, int key, int n) {
+  return !WIN || key > pos - a.window || key + n <= a.sinks;
+}
+
 struct PromptBwdPlan {
   int nsplit;
   int64_t groups;  // of the largest launch
   size_t delta_bytes, work;
 };
-PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,
-                              int64_t head_dim);
+PromptBwdPlan plan_prompt_bwd(const PromptArgs& a);  // of its sizes
 
 // queries of a workgroup of the kernel that launch_prompt_fwd takes: 32, 64 (both the split kernel), 128 or 256 (pair)
 int prompt_fwd_tile(int dtype, const PromptArgs& a);

@@ -74,14 +74,15 @@ struct Queries {
     if constexpr (sizeof(T) == 2) order_products<HD / 16 * (BK / 32), 1>();
   }
 
-  // The weights of the tile's keys from kb on; those after `see` are masked when `cut`.
-  __device__ __forceinline__ void softmax(int kb, int see, bool cut, float scale2) {
+  // The weights of the tile's keys from kb on; those that `v` does not see are masked when `cut`.
+  template <bool WIN>
+  __device__ __forceinline__ void softmax(int kb, const Seen<WIN>& v, bool cut, float scale2) {
     if (cut)
 #pragma unroll
       for (int t = 0; t < BK / 32; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++)
-          if (kb + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > see) s[t][i] = -INFINITY;
+          if (!v.sees(kb + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3))) s[t][i] = -INFINITY;
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < BK / 32; t++)
@@ -159,11 +160,13 @@ struct Queries {
   }
 };
 
-// What a workgroup and a wave of it work on.
-template <typename T, int BQ>
-struct Work {
+// What a workgroup and a wave of it work on. BK: keys of its steps. nk: keys that it walks over, which are the
+// sequence's first ones or, with a window, w.key() of them.
+template <typename T, int BQ, int BK, bool WIN>
+struct Work : Walk<WIN> {
   TileSpan tq;
-  int hq, lk, off, nk, q_first, qi, see;
+  int hq, lk, off, nk, q_first, qi;
+  Seen<WIN> see;
   bool live;
   const T *k, *v, *q;
   // false: nothing to do
@@ -181,37 +184,39 @@ struct Work {
     q_first = tq.row0 + wave * 32;
     qi = q_first + (lane & 31);  // the lane's query
     live = qi < tq.len;
-    see = a.causal ? min(lk - 1, qi + off) : lk - 1;  // its last key
+    see.init(a, qi, off, lk);
     const int q_last = min(tq.row0 + BQ, tq.len) - 1;
     nk = a.causal ? min(max(q_last + off + 1, 0), lk) : lk;  // keys that the tile sees
+    nk -= this->leave_out(a, tq.row0 + off, BK);
     k = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
     v = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
     q = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;
     return true;
   }
-  // whether the wave sees any of the keys from kb on, and whether it sees less than all of BK
-  __device__ __forceinline__ bool any(const PromptArgs& a, int kb) const {
-    return q_first < tq.len && (!a.causal || kb <= q_first + 31 + off);
+  // whether the wave sees any of the bk keys from kb on, and whether it sees less than all of them
+  __device__ __forceinline__ bool any(const PromptArgs& a, int kb, int bk) const {
+    return q_first < tq.len && (!a.causal || kb <= q_first + 31 + off) && window_any<WIN>(a, q_first + off, kb, bk);
   }
   __device__ __forceinline__ bool cut(const PromptArgs& a, int kb, int bk) const {
-    return kb + bk > lk || (a.causal && kb + bk - 1 > q_first + off);
+    return kb + bk > lk || (a.causal && kb + bk - 1 > q_first + off) || !window_all<WIN>(a, q_first + 31 + off, kb, bk);
   }
 };
 
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, bool WIN>
 __global__ __launch_bounds__(256) void prompt_fwd_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
   constexpr int THREADS = 256, kTile = TL::bytes(BK);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Work<T, 128> w;
+  Work<T, 128, BK, WIN> w;
   if (!w.init(a, wave, lane)) return;
   Stage<T, HD, BK, THREADS> ks, vs;
-  if (w.nk > 0) {
-    ks.load(w.k, a.k_stride, w.lk, a.head_dim, tid);
-    vs.load(w.v, a.v_stride, w.lk, a.head_dim, tid);
-  }
+  auto load = [&](int key) {
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
+  };
+  if (w.nk > 0) load(w.key(0));
   Queries<T, HD, BK> x;
   x.init(w.q, a.head_dim, lane);
   settle(x.q);
@@ -222,17 +227,15 @@ __global__ __launch_bounds__(256) void prompt_fwd_kernel(PromptArgs a) {
   for (int kb = 0, buf = 0; kb < w.nk; kb += BK, buf ^= 1) {
     const char* kt = lds + buf * 2 * kTile;
     const bool more = kb + BK < w.nk;
-    if (more) {
-      ks.load(w.k + (int64_t)(kb + BK) * a.k_stride, a.k_stride, w.lk - kb - BK, a.head_dim, tid);
-      vs.load(w.v + (int64_t)(kb + BK) * a.v_stride, a.v_stride, w.lk - kb - BK, a.head_dim, tid);
-    }
+    if (more) load(w.key(kb + BK));
     __syncthreads();
-    if (w.any(a, kb)) {
+    const int key = w.key(kb);
+    if (w.any(a, key, BK)) {
       // products first, the other wave's softmax in their gaps: 131 us of the six sequences above, else 140
       __builtin_amdgcn_s_setprio(1);
       x.scores(kt);
       __builtin_amdgcn_s_setprio(0);
-      x.softmax(kb, w.see, w.cut(a, kb, BK), a.scale2);
+      x.softmax(key, w.see, w.cut(a, key, BK), a.scale2);
       __builtin_amdgcn_s_setprio(1);
       x.add_values(kt + kTile);
       __builtin_amdgcn_s_setprio(0);
@@ -256,20 +259,21 @@ __global__ __launch_bounds__(256) void prompt_fwd_kernel(PromptArgs a) {
 // shadow it also stores its share of tile i + 1 and asks for that of tile i + 2, and its softmax
 // in the next slot. Tile t is complete before slot 2 t; its keys are read in slots 2 t and
 // 2 t + 1, its values two later: rings of 2 and 3 tiles.
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, bool WIN>
 __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
   constexpr int THREADS = 512, kTile = TL::bytes(BK);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = wave >> 2;
-  Work<T, 256> w;
+  Work<T, 256, BK, WIN> w;
   if (!w.init(a, wave, lane)) return;
   const int n = (w.nk + BK - 1) / BK;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int t) {
-    ks.load(w.k + (int64_t)t * BK * a.k_stride, a.k_stride, w.lk - t * BK, a.head_dim, tid);
-    vs.load(w.v + (int64_t)t * BK * a.v_stride, a.v_stride, w.lk - t * BK, a.head_dim, tid);
+    const int key = w.key(t * BK);
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
   };
   auto k_tile = [&](int t) { return lds + (t & 1) * kTile; };
   auto v_tile = [&](int t) { return lds + (2 + t % 3) * kTile; };
@@ -299,16 +303,20 @@ __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
   for (int i = 0; i < n; i++) {
     // A tile that none of the wave's queries see is left out: a NaN in its values must not reach them, and
     // the wave's matrix pipe is the other group's (4200 tokens, 32/8 heads 165 -> 160 us, 8192 517 -> 511).
-    const bool any = w.any(a, i * BK);
+    const int key = w.key(i * BK);
+    const bool any = w.any(a, key, BK);
     if (any) {
-      x.softmax(i * BK, w.see, w.cut(a, i * BK, BK), a.scale2);
+      x.softmax(key, w.see, w.cut(a, key, BK), a.scale2);
       settle(x.p);  // (else the exponentials sink past the barrier, to the products)
     }
     slot_end();
     __builtin_amdgcn_s_setprio(1);
     if (i + 2 < n) store(i + 2);
     if (i + 3 < n) load(i + 3);
-    if (any) x.add_values_and_scores(vc, kn);  // (after the last tile the scores are of an old one, not used)
+    if (any)
+      x.add_values_and_scores(vc, kn);  // (after the last tile the scores are of an old one, not used)
+    else if (WIN && i + 1 < n && w.any(a, w.key((i + 1) * BK), BK))  // a window begins with the next tile
+      x.scores(kn);
     __builtin_amdgcn_s_setprio(0);
     slot_end();
     kn = kn == lds ? lds + kTile : lds;
@@ -321,7 +329,7 @@ __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
 // Fewer queries a workgroup, for grids that would leave CUs idle with 128: QG groups of 32,
 // and 4 / QG waves over the same queries, each with its own 32 of the keys that are staged at
 // a time, their states joined at the end. One tile in LDS, the next on its way in registers.
-template <typename T, int HD, int QG>
+template <typename T, int HD, int QG, bool WIN>
 __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   using TL = Tile<T, HD>;
   constexpr int THREADS = 256, KG = 4 / QG, BK = 32 * KG, kTile = TL::bytes(BK);
@@ -330,24 +338,24 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave % KG;
-  Work<T, 32 * QG> w;
+  Work<T, 32 * QG, BK, WIN> w;
   if (!w.init(a, wave / KG, lane)) return;
   Stage<T, HD, BK, THREADS> ks, vs;
-  auto load = [&](int kb) {
-    ks.load(w.k + (int64_t)kb * a.k_stride, a.k_stride, w.lk - kb, a.head_dim, tid);
-    vs.load(w.v + (int64_t)kb * a.v_stride, a.v_stride, w.lk - kb, a.head_dim, tid);
+  auto load = [&](int key) {
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
   };
-  if (w.nk > 0) load(0);
+  if (w.nk > 0) load(w.key(0));
   Queries<T, HD, 32> x;
   x.init(w.q, a.head_dim, lane);
   settle(x.q);
   for (int kb = 0; kb < w.nk; kb += BK) {
     ks.store(lds, tid);
     vs.store(lds + kTile, tid);
-    if (kb + BK < w.nk) load(kb + BK);
+    if (kb + BK < w.nk) load(w.key(kb + BK));
     __syncthreads();
-    const int mine = kb + 32 * kg;
-    if (mine < w.nk && w.any(a, mine)) {
+    const int mine = w.key(kb) + 32 * kg;
+    if (kb + 32 * kg < w.nk && w.any(a, mine, 32)) {
       const char* kt = lds + 32 * kg * TL::kPitch;
       x.scores(kt);
       x.softmax(mine, w.see, w.cut(a, mine, 32), a.scale2);
@@ -399,33 +407,33 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   }
 }
 
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, bool WIN>
 hipError_t run_fwd(PromptArgs a, hipStream_t stream) {
   constexpr int lds = 4 * Tile<T, HD>::bytes(BK);
   a.slots = tile_slots(a.rows_q, a.batch, 128);
-  const auto kernel = prompt_fwd_kernel<T, HD, BK>;
+  const auto kernel = prompt_fwd_kernel<T, HD, BK, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(256), lds, stream, a);
   return hipGetLastError();
 }
 
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, bool WIN>
 hipError_t run_fwd_pair(PromptArgs a, hipStream_t stream) {
   constexpr int lds = 5 * Tile<T, HD>::bytes(BK);
   a.slots = tile_slots(a.rows_q, a.batch, 256);
-  const auto kernel = prompt_fwd_pair_kernel<T, HD, BK>;
+  const auto kernel = prompt_fwd_pair_kernel<T, HD, BK, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(512), lds, stream, a);
   return hipGetLastError();
 }
 
-template <typename T, int HD, int QG>
+template <typename T, int HD, int QG, bool WIN>
 hipError_t run_fwd_split(PromptArgs a, hipStream_t stream) {
   constexpr int lds = std::max(2 * Tile<T, HD>::bytes(128 / QG), 4 * 32 * (HD + 4) * 4);
   a.slots = tile_slots(a.rows_q, a.batch, 32 * QG);
-  const auto kernel = prompt_fwd_split_kernel<T, HD, QG>;
+  const auto kernel = prompt_fwd_split_kernel<T, HD, QG, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.slots * a.n_q)), dim3(256), lds, stream, a);
@@ -481,13 +489,13 @@ static int fwd_split_groups(int dtype, const PromptArgs& a) {
   return groups <= (int64_t)one * a.cu_count ? 1 : groups <= (int64_t)two * a.cu_count ? 2 : 0;
 }
 
-template <int QG>
+template <int QG, bool WIN>
 static hipError_t launch_fwd_split(int dtype, const PromptArgs& a, hipStream_t stream) {
   if constexpr (QG == 2)
-    if (a.head_dim > 128) return run_fwd_split<__bf16, 256, QG>(a, stream);
+    if (a.head_dim > 128) return run_fwd_split<__bf16, 256, QG, WIN>(a, stream);
   if (dtype == RQ_BF16)
-    return a.head_dim <= 64 ? run_fwd_split<__bf16, 64, QG>(a, stream) : run_fwd_split<__bf16, 128, QG>(a, stream);
-  return a.head_dim <= 64 ? run_fwd_split<float, 64, QG>(a, stream) : run_fwd_split<float, 128, QG>(a, stream);
+    return a.head_dim <= 64 ? run_fwd_split<__bf16, 64, QG, WIN>(a, stream) : run_fwd_split<__bf16, 128, QG, WIN>(a, stream);
+  return a.head_dim <= 64 ? run_fwd_split<float, 64, QG, WIN>(a, stream) : run_fwd_split<float, 128, QG, WIN>(a, stream);
 }
 
 int prompt_fwd_tile(int dtype, const PromptArgs& a) {
@@ -500,19 +508,24 @@ int prompt_fwd_tile(int dtype, const PromptArgs& a) {
   return pair ? 256 : 128;
 }
 
-hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+template <bool WIN>
+static hipError_t launch_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   const int tile = prompt_fwd_tile(dtype, a);
-  if (tile == 32) return launch_fwd_split<1>(dtype, a, stream);
-  if (tile == 64) return launch_fwd_split<2>(dtype, a, stream);
-  if (tile == 256) return run_fwd_pair<__bf16, 128, 64>(a, stream);
+  if (tile == 32) return launch_fwd_split<1, WIN>(dtype, a, stream);
+  if (tile == 64) return launch_fwd_split<2, WIN>(dtype, a, stream);
+  if (tile == 256) return run_fwd_pair<__bf16, 128, 64, WIN>(a, stream);
   if (dtype == RQ_BF16) {
-    if (a.head_dim <= 64) return run_fwd<__bf16, 64, 64>(a, stream);
-    if (a.head_dim <= 128) return run_fwd<__bf16, 128, 64>(a, stream);
-    return run_fwd<__bf16, 256, 32>(a, stream);
+    if (a.head_dim <= 64) return run_fwd<__bf16, 64, 64, WIN>(a, stream);
+    if (a.head_dim <= 128) return run_fwd<__bf16, 128, 64, WIN>(a, stream);
+    return run_fwd<__bf16, 256, 32, WIN>(a, stream);
   }
-  if (a.head_dim <= 64) return run_fwd<float, 64, 32>(a, stream);
-  if (a.head_dim <= 128) return run_fwd<float, 128, 32>(a, stream);
-  return run_fwd<float, 256, 32>(a, stream);
+  if (a.head_dim <= 64) return run_fwd<float, 64, 32, WIN>(a, stream);
+  if (a.head_dim <= 128) return run_fwd<float, 128, 32, WIN>(a, stream);
+  return run_fwd<float, 256, 32, WIN>(a, stream);
+}
+
+hipError_t launch_prompt_fwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+  return a.window > 0 ? launch_fwd<true>(dtype, a, stream) : launch_fwd<false>(dtype, a, stream);
 }
 
 }  // namespace rq

@@ -99,6 +99,7 @@ __global__ __launch_bounds__(256) void prompt_delta_exact_kernel(PromptArgs a) {
       y.store(lds + 3 * kTile, tid);
     }
     const int r = qb + i, see = a.causal ? min(lk - 1, row0 + r + off) : lk - 1;
+    const int from = a.window > 0 ? row0 + r + off - a.window + 1 : 0;
     const float lse = base2_lse(a.lse[(int64_t)hq * a.rows_q + first + min(r, end - row0 - 1)]);
     __syncthreads();
     f32x16 s = f32x16{}, dp = f32x16{};
@@ -109,9 +110,11 @@ __global__ __launch_bounds__(256) void prompt_delta_exact_kernel(PromptArgs a) {
     }
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 16; j++)
-      if (kb + 8 * (j >> 2) + 4 * h + (j & 3) <= see)
+    for (int j = 0; j < 16; j++) {
+      const int key = kb + 8 * (j >> 2) + 4 * h + (j & 3);
+      if (key <= see && (key >= from || key < a.sinks))
         sum += __builtin_amdgcn_exp2f(fmaf(s[j], a.scale2, -lse)) * dp[j];
+    }
     sum += __shfl_xor(sum, 32, 64);
     if (h == 0) part[wave][i] = sum;
     __syncthreads();
@@ -209,7 +212,7 @@ constexpr int dkv_lds() {  // twice Q, dO, L and D of a step, and two pairs' wei
          2 * Handover<T>::N * 16 * 64 * dkv_queries<T, HD>() / 32;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool WIN>
 __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
@@ -244,7 +247,9 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
 
   // the first query that sees the tile's first key, down to a whole query tile
   const int qstart = a.causal ? max(tk.row0 - off, 0) / BQ * BQ : 0;
-  const int per_head = lq > qstart ? (lq - qstart + BQ - 1) / BQ : 0;
+  // behind the last one that does
+  const int qend = WIN && tk.row0 >= a.sinks ? min(lq, tk.row0 + kDkvKeys - 1 - off + a.window) : lq;
+  const int per_head = qend > qstart ? (qend - qstart + BQ - 1) / BQ : 0;
   const int64_t steps = (int64_t)per_head * group;
   const int s0 = (int)(steps * split / a.nsplit), s1 = (int)(steps * (split + 1) / a.nsplit);
   Stage<T, HD, BQ, THREADS> qs, os;
@@ -278,12 +283,13 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, char* l
     if (next_hq == (hkv + 1) * group) next_hq = hkv * group, next_r -= BQ;
     if (step + 1 < s1) load(next_hq, next_r);
     __syncthreads();
-    const bool seen = !a.causal || r + BQ - 1 + off >= w_key;
-    const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off);
+    const bool seen = (!a.causal || r + BQ - 1 + off >= w_key) && window_any<WIN>(a, r + off, w_key, 32);
+    const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off) &&
+                       window_all<WIN>(a, r + BQ - 1 + off, w_key, 32);
     // value i of product t: query r + 32 t + 8 (i / 4) + 4 h + i % 4, the lane's key
     auto see = [&](int t, int i) {
       const int qi = r + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-      return qi < lq && live && (!a.causal || kj <= qi + off);
+      return qi < lq && live && (!a.causal || kj <= qi + off) && window_any<WIN>(a, qi + off, kj, 1);
     };
     float x[NT][16];
     Frag pf[NT][2];  // bf16: weights and their gradients rounded to nearest for the products
@@ -383,9 +389,9 @@ __global__ __launch_bounds__(256) void prompt_dkv_sum_kernel(PromptArgs a) {
 
 // dQ of a wave's 32 queries += their share of the 32 keys from row `r` of the staged tiles on,
 // keys `key` and on of the sequence.
-template <typename T, int HD>
-__device__ __forceinline__ void dq_tile(const char* kt, const char* vt, int r, int key, bool whole, int see, float lse,
-                                        float del, float scale2, int lane,
+template <typename T, int HD, bool WIN>
+__device__ __forceinline__ void dq_tile(const char* kt, const char* vt, int r, int key, bool whole,
+                                        const Seen<WIN>& see, float lse, float del, float scale2, int lane,
                                         const typename Tile<T, HD>::Frag (&qf)[HD / 16],
                                         const typename Tile<T, HD>::Frag (&of)[HD / 16], f32x16 (&dq)[HD / 32]) {
   using TL = Tile<T, HD>;
@@ -401,7 +407,7 @@ __device__ __forceinline__ void dq_tile(const char* kt, const char* vt, int r, i
   for (int i = 0; i < 16; i++) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], scale2, -lse)) * (dp[i] - del);
   if (!whole)
 #pragma unroll
-    for (int i = 0; i < 16; i++) ds[i] = key + 8 * (i >> 2) + 4 * h + (i & 3) <= see ? ds[i] : 0.0f;
+    for (int i = 0; i < 16; i++) ds[i] = see.sees(key + 8 * (i >> 2) + 4 * h + (i & 3)) ? ds[i] : 0.0f;
   typename TL::Frag sf[2];
   tile_pack(ds, sf[0]);
   tile_pack(ds + 8, sf[1]);
@@ -413,7 +419,7 @@ __device__ __forceinline__ void dq_tile(const char* kt, const char* vt, int r, i
 }
 
 // dQ: four waves of 32 queries each, key tiles of BK rows through LDS.
-template <typename T, int HD, int BK>
+template <typename T, int HD, int BK, bool WIN>
 __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
@@ -433,14 +439,21 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
   const int w_row = tq.row0 + wave * 32, qi = w_row + (lane & 31);
   const bool live = qi < tq.len;
   const int q_last = min(tq.row0 + BQ, tq.len) - 1;
-  const int nk = a.causal ? min(max(q_last + off + 1, 0), lk) : lk;
+  Walk<WIN> walk;
+  const int nk = (a.causal ? min(max(q_last + off + 1, 0), lk) : lk) - walk.leave_out(a, tq.row0 + off, BK);
 
   const T* kbase = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
   const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
   Stage<T, HD, BK, THREADS> ks, vs;
+  auto load_k = [&](int key) {
+    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, lk - key, a.head_dim, tid);
+  };
+  auto load_v = [&](int key) {
+    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, lk - key, a.head_dim, tid);
+  };
   if (nk > 0) {
-    ks.load(kbase, a.k_stride, lk, a.head_dim, tid);
-    vs.load(vbase, a.v_stride, lk, a.head_dim, tid);
+    load_k(walk.key(0));
+    load_v(walk.key(0));
   }
   const T* qrow = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;
   const T* orow = live ? static_cast<const T*>(a.dout) + (tq.begin + qi) * a.dout_stride + hq * a.head_dim : nullptr;
@@ -461,28 +474,30 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
     ks.store(lds, tid);
     vs.store(lds + kTile, tid);
   }
-  const int see = !live ? -1 : a.causal ? min(lk - 1, qi + off) : lk - 1;
+  Seen<WIN> see;
+  see.init(a, qi, off, lk);
+  if (!live) see.last = -1;
   for (int kb = 0, buf = 0; kb < nk; kb += BK, buf ^= 1) {
     const char* kt = lds + buf * 2 * kTile;
     const char* vt = kt + kTile;
     const bool more = kb + BK < nk;
     char* next = lds + (buf ^ 1) * 2 * kTile;
     if (more) {
-      ks.load(kbase + (int64_t)(kb + BK) * a.k_stride, a.k_stride, lk - kb - BK, a.head_dim, tid);
-      if constexpr (!kOneStage)
-        vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
+      load_k(walk.key(kb + BK));
+      if constexpr (!kOneStage) load_v(walk.key(kb + BK));
     }
     __syncthreads();
-    if (!a.causal || kb <= w_row + 31 + off) {
-      const bool whole = kb + BK <= lk && w_row + 32 <= tq.len && (!a.causal || kb + BK - 1 <= w_row + off);
+    const int key = walk.key(kb);
+    if ((!a.causal || key <= w_row + 31 + off) && window_any<WIN>(a, w_row + off, key, BK)) {
+      const bool whole = key + BK <= lk && w_row + 32 <= tq.len && (!a.causal || key + BK - 1 <= w_row + off) &&
+                         window_all<WIN>(a, w_row + 31 + off, key, BK);
 #pragma unroll
       for (int t = 0; t < BK / 32; t++)
-        dq_tile<T, HD>(kt, vt, 32 * t, kb + 32 * t, whole, see, lse, del, a.scale2, lane, qf, of, dq);
+        dq_tile<T, HD, WIN>(kt, vt, 32 * t, key + 32 * t, whole, see, lse, del, a.scale2, lane, qf, of, dq);
     }
     if (more) {
       ks.store(next, tid);
-      if constexpr (kOneStage)
-        vs.load(vbase + (int64_t)(kb + BK) * a.v_stride, a.v_stride, lk - kb - BK, a.head_dim, tid);
+      if constexpr (kOneStage) load_v(walk.key(kb + BK));
       vs.store(next + kTile, tid);
     }
   }
@@ -493,7 +508,7 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
 
 // dQ of 32 QG queries, 4 / QG waves over the same ones, each with its own 32 of the keys that are
 // staged at a time, and their sums added at the end: for grids that would leave CUs idle.
-template <typename T, int HD, int QG>
+template <typename T, int HD, int QG, bool WIN>
 __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
@@ -510,15 +525,16 @@ __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, ch
   const int w_row = tq.row0 + wave / KG * 32, qi = w_row + (lane & 31);
   const bool live = qi < tq.len;
   const int q_last = min(tq.row0 + BQ, tq.len) - 1;
-  const int nk = a.causal ? min(max(q_last + off + 1, 0), lk) : lk;
+  Walk<WIN> walk;
+  const int nk = (a.causal ? min(max(q_last + off + 1, 0), lk) : lk) - walk.leave_out(a, tq.row0 + off, BK);
   const T* kbase = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
   const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
   Stage<T, HD, BK, THREADS> ks, vs;
-  auto load = [&](int kb) {
-    ks.load(kbase + (int64_t)kb * a.k_stride, a.k_stride, lk - kb, a.head_dim, tid);
-    vs.load(vbase + (int64_t)kb * a.v_stride, a.v_stride, lk - kb, a.head_dim, tid);
+  auto load = [&](int key) {
+    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, lk - key, a.head_dim, tid);
+    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, lk - key, a.head_dim, tid);
   };
-  if (nk > 0) load(0);
+  if (nk > 0) load(walk.key(0));
   const T* qrow = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;
   const T* orow = live ? static_cast<const T*>(a.dout) + (tq.begin + qi) * a.dout_stride + hq * a.head_dim : nullptr;
   Frag qf[HD / 16], of[HD / 16];
@@ -534,16 +550,19 @@ __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, ch
   f32x16 dq[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; d++) dq[d] = f32x16{};
-  const int see = !live ? -1 : a.causal ? min(lk - 1, qi + off) : lk - 1;
+  Seen<WIN> see;
+  see.init(a, qi, off, lk);
+  if (!live) see.last = -1;
   for (int kb = 0; kb < nk; kb += BK) {
     ks.store(lds, tid);
     vs.store(lds + kTile, tid);
-    if (kb + BK < nk) load(kb + BK);
+    if (kb + BK < nk) load(walk.key(kb + BK));
     __syncthreads();
-    const int mine = kb + 32 * kg;
-    if (mine < nk && (!a.causal || mine <= w_row + 31 + off)) {
-      const bool whole = mine + 32 <= lk && w_row + 32 <= tq.len && (!a.causal || mine + 31 <= w_row + off);
-      dq_tile<T, HD>(lds, lds + kTile, 32 * kg, mine, whole, see, lse, del, a.scale2, lane, qf, of, dq);
+    const int mine = walk.key(kb) + 32 * kg;
+    if (kb + 32 * kg < nk && (!a.causal || mine <= w_row + 31 + off) && window_any<WIN>(a, w_row + off, mine, 32)) {
+      const bool whole = mine + 32 <= lk && w_row + 32 <= tq.len && (!a.causal || mine + 31 <= w_row + off) &&
+                         window_all<WIN>(a, w_row + 31 + off, mine, 32);
+      dq_tile<T, HD, WIN>(lds, lds + kTile, 32 * kg, mine, whole, see, lse, del, a.scale2, lane, qf, of, dq);
     }
     __syncthreads();
   }
@@ -570,19 +589,19 @@ __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, ch
 
 // Both in one launch, so that the short workgroups of one fill the compute units that the
 // last long ones of the other leave idle.
-template <typename T, int HD, int BK, int QG>
+template <typename T, int HD, int BK, int QG, bool WIN>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prompt_grad_kernel(PromptArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int dkv = (int)(a.k_slots * a.n_kv * a.nsplit);
   if ((int)blockIdx.x < dkv)
-    dkv_body<T, HD>(a, blockIdx.x, lds);
+    dkv_body<T, HD, WIN>(a, blockIdx.x, lds);
   else if constexpr (QG == 4)
-    dq_body<T, HD, BK>(a, blockIdx.x - dkv, lds);
+    dq_body<T, HD, BK, WIN>(a, blockIdx.x - dkv, lds);
   else
-    dq_split_body<T, HD, QG>(a, blockIdx.x - dkv, lds);
+    dq_split_body<T, HD, QG, WIN>(a, blockIdx.x - dkv, lds);
 }
 
-template <typename T, int HD, int BK, int QG>
+template <typename T, int HD, int BK, int QG, bool WIN>
 hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   using TL = Tile<T, HD>;
   if (a.rows_q > 0) {
@@ -603,7 +622,7 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   constexpr int lds = std::max(dkv_lds<T, HD>(), dq_lds);
   a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
   a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, 32 * QG) : 0;
-  const auto kernel = prompt_grad_kernel<T, HD, BK, QG>;
+  const auto kernel = prompt_grad_kernel<T, HD, BK, QG, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256), lds,
@@ -621,11 +640,14 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
 
 // Parts of the (head, query tile) steps of the keys' gradients: enough that the grid is
 // kDkvGroups workgroups, while a part keeps 4 query tiles of the longest sequence that the rows allow.
-PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int64_t n_q, int64_t n_kv,
-                              int64_t head_dim) {
+// (With a window a key's queries are those of the window.)
+PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   constexpr int64_t kDkvGroups = 768;
+  const int64_t batch = a.batch, rows_q = a.rows_q, rows_k = a.rows_k, n_q = a.n_q, n_kv = a.n_kv, head_dim = a.head_dim;
   const int64_t groups = std::max<int64_t>(1, (rows_k + kDkvKeys - 1) / kDkvKeys * n_kv);
-  const int64_t steps = rows_q / std::max<int64_t>(batch, 1) / 32 * (n_q / n_kv);
+  int64_t longest = rows_q / std::max<int64_t>(batch, 1);
+  if (a.window > 0) longest = std::min<int64_t>(longest, a.window + kDkvKeys);
+  const int64_t steps = longest / 32 * (n_q / n_kv);
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
   p.groups = std::max(tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
@@ -644,19 +666,24 @@ PromptBwdPlan plan_prompt_bwd(int64_t batch, int64_t rows_q, int64_t rows_k, int
 //   bf16  x 256: 512 (80) 90 / 78   2048 (272) 276 / 245   64/8 heads, 512 (320) 136 / 132   8 x 256 (384) 86 / 90
 //   f32   512 (80) 156 / 111   2048 (272) 760 / 601   2048 (32/8, 544) 1207 / 1186   8 x 512 (32/8, 1280) 738 / 727
 //         16/2 x 64: 129, 300, 64, 511 (176) 88 / 65   2048 (272) 480 / 341   8 x 512 (640) 215 / 194
-hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+template <bool WIN>
+static hipError_t launch_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
   if (dtype == RQ_BF16) {
     const int64_t most = a.head_dim > 128 ? 320 : 576;
     const bool wide = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256 > most * a.cu_count;
     if (a.head_dim > 128)
-      return wide ? run_bwd<__bf16, 256, 32, 4>(a, stream) : run_bwd<__bf16, 256, 32, 2>(a, stream);
+      return wide ? run_bwd<__bf16, 256, 32, 4, WIN>(a, stream) : run_bwd<__bf16, 256, 32, 2, WIN>(a, stream);
     if (a.head_dim <= 64)
-      return wide ? run_bwd<__bf16, 64, 64, 4>(a, stream) : run_bwd<__bf16, 64, 64, 2>(a, stream);
-    return wide ? run_bwd<__bf16, 128, 32, 4>(a, stream) : run_bwd<__bf16, 128, 32, 2>(a, stream);
+      return wide ? run_bwd<__bf16, 64, 64, 4, WIN>(a, stream) : run_bwd<__bf16, 64, 64, 2, WIN>(a, stream);
+    return wide ? run_bwd<__bf16, 128, 32, 4, WIN>(a, stream) : run_bwd<__bf16, 128, 32, 2, WIN>(a, stream);
   }
-  if (a.head_dim <= 64) return run_bwd<float, 64, 32, 2>(a, stream);
-  if (a.head_dim <= 128) return run_bwd<float, 128, 32, 2>(a, stream);
-  return run_bwd<float, 256, 32, 4>(a, stream);
+  if (a.head_dim <= 64) return run_bwd<float, 64, 32, 2, WIN>(a, stream);
+  if (a.head_dim <= 128) return run_bwd<float, 128, 32, 2, WIN>(a, stream);
+  return run_bwd<float, 256, 32, 4, WIN>(a, stream);
+}
+
+hipError_t launch_prompt_bwd(int dtype, const PromptArgs& a, hipStream_t stream) {
+  return a.window > 0 ? launch_bwd<true>(dtype, a, stream) : launch_bwd<false>(dtype, a, stream);
 }
 
 }  // namespace rq
