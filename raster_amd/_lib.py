@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "librq.so")
 
 RQ_OK, RQ_ERR_SHAPE, RQ_ERR_DTYPE, RQ_ERR_NULL, RQ_ERR_OOM, RQ_ERR_HIP, RQ_ERR_HANDLE, RQ_ERR_DEVICE = range(8)
-RQ_F32, RQ_BF16, RQ_F16 = 0, 1, 2
+RQ_F32, RQ_BF16, RQ_F16, RQ_I8 = 0, 1, 2, 3
 RQ_Q8_0, RQ_Q4_0, RQ_Q4_K, RQ_Q6_K = 0, 1, 2, 3
 
 # every exported symbol of include/rq.h with (argtypes, restype)
@@ -77,6 +77,12 @@ SIGNATURES = {
     "rq_paged_attention_work": ([_p, _i64, _i64, _i64, _i64, _i64, C.POINTER(_sz)], _i),
     "rq_paged_attention": ([_p, _p, _i, *[_p, _i64] * 3, _p, _i64, _i64, _i64, C.c_double, C.c_double, _p, _i64, _p,
                             _sz, _p], _i),
+    "rq_paged_attention_window_work": ([_p, _i, *[_i64] * 7, C.POINTER(_sz)], _i),
+    "rq_paged_attention_window": ([_p, _p, _p, _p, _i64, _i64, _i64, _i, *[_p, _i64] * 3, _p, _i64, _i64, _i64,
+                                   C.c_double, C.c_double, _p, _i64, _p, _sz, _p], _i),
+    "rq_pages_append_q8": ([_p, _p, _p, _p, _i64, _i, *[_p, _i64] * 3, _p, _p, _i64, _i64, _i64, C.c_double, _p, _i64,
+                            _p, _i64, _p], _i),
+    "rq_pages_rows": ([_p, _p, _p, _p, _i64, _i, _p, _i64, _i64, _p, _i64, _p, _i64, _p], _i),
     "rq_pages_append": ([_p, _p, _i, *[_p, _i64] * 3, _p, _p, _i64, _i64, _i64, C.c_double, _p, _i64, _p, _i64, _p],
                         _i),
     "rq_pages_copy": ([_p, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _p], _i),

@@ -7,7 +7,12 @@ The batched companions of quant.decode_attention (raster/dl/attention.clj:197-28
   prompt_attention_bwd  its gradient (explicit, like matmul_dx)
   paged_attention       one new token of every sequence: RoPE, append, attention over pages
   pages_append          RoPE of packed prompts' q and k; k and v into the pages
+  pages_rows            stored rows of sequences as values, packed
   pages_copy            pages copied in every plane of a cache
+
+The attentions take a sliding window with sinks. Pages are f32, bf16 or int8; int8 pages
+come with their scales, kscales and vscales f32 [pages, page_size / 16, n_kv] (pages may be strided),
+one for each 16 rows and KV head; include/rq.h says what an append makes of them.
 
 Arrays are torch CUDA tensors of the context's device (memory and streams only);
 rows may be strided (columns of one product's output), their elements may not. Without
@@ -19,10 +24,10 @@ from __future__ import annotations
 import ctypes as C
 from array import array
 
-from ._lib import Pages, Prompt, call
+from ._lib import RQ_I8, Pages, Prompt, call
 from .quant import Context, _current_stream, _dtype_code, _need, _stream_ptr, _t
 
-__all__ = ["prompt_attention", "prompt_attention_bwd", "paged_attention", "pages_append", "pages_copy"]
+__all__ = ["prompt_attention", "prompt_attention_bwd", "paged_attention", "pages_append", "pages_rows", "pages_copy"]
 
 
 def _code(t) -> int:
@@ -159,19 +164,36 @@ def _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch):
     if len(ts) != 2 or ts[0] != batch:
         raise ValueError("table must be [batch, pages of a sequence]")
     n = ts[1]
-    return Pages(_code(kpages), kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
+    return Pages(RQ_I8 if kpages.dtype == _t().int8 else _code(kpages), kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
                  _i32(table, ctx, batch * n, "table"), n)
 
 
-_work_sizes: dict = {}  # rq_paged_attention_work by its arguments
+def _scales(ctx, pg, kscales, vscales) -> tuple:
+    """(kscales, vscales, scale_stride) of int8 pages; of others none may be given."""
+    if pg.dtype != RQ_I8:
+        _need(kscales is None and vscales is None, "kscales and vscales are for int8 pages")
+        return None, None, 0
+    shape, out = (pg.pages, pg.page_size // 16, pg.n_kv), []
+    for t in (kscales, vscales):
+        if (t is None or t.dtype != _t().float32 or t.get_device() != ctx.device or t.shape != shape
+                or not t[0].is_contiguous()):
+            raise ValueError(f"int8 pages need kscales and vscales, f32 CUDA tensors {list(shape)} of the context's "
+                             "device, a page's scales side by side")
+        out.append(t.stride(0) if shape[0] > 1 else max(t.stride(0), shape[1] * shape[2]))
+    _need(out[0] == out[1], "kscales and vscales must have one stride from page to page")
+    return kscales.data_ptr(), vscales.data_ptr(), out[0]
 
 
-def _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len) -> int:
-    key = (ctx.device, batch, n_q, n_kv, head_dim, max_len)
+_work_sizes: dict = {}  # rq_paged_attention_window_work by its arguments
+
+
+def _paged_work(ctx, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks) -> int:
+    key = (ctx.device, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks)
     n = _work_sizes.get(key)
     if n is None:
         need = C.c_size_t()
-        call("rq_paged_attention_work", ctx.handle, batch, n_q, n_kv, head_dim, max_len, C.byref(need))
+        call("rq_paged_attention_window_work", ctx.handle, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks,
+             C.byref(need))
         if len(_work_sizes) >= 4096:
             _work_sizes.clear()
         n = _work_sizes[key] = need.value
@@ -179,13 +201,15 @@ def _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len) -> int:
 
 
 def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int, n_kv: int, head_dim: int,
-                    theta: float, scale: float, max_len: int | None = None, out=None, stream=None):
-    """rq_paged_attention: one new token of each sequence b (rows of q [batch,
+                    theta: float, scale: float, max_len: int | None = None, out=None, stream=None,
+                    window: int | None = None, sinks: int = 0, kscales=None, vscales=None):
+    """rq_paged_attention (with a window or int8 pages rq_paged_attention_window): one new token of each sequence b (rows of q [batch,
     n_q*head_dim], k and v [batch, n_kv*head_dim]) at position lens[b] of its
     pages (kpages, vpages [pages, page_size, n_kv*head_dim], table int32 [batch,
     pages of a sequence]): RoPE, append, attention over rows 0 .. lens[b] -> out
     [batch, n_q*head_dim]. k and v None: nothing appended, rows 0 .. lens[b] - 1. max_len:
-    no sequence is longer, the new row included (default: what the table holds)."""
+    no sequence is longer, the new row included (default: what the table holds). window: the
+    last `window` rows and the first `sinks` are attended; None or 0: all."""
     code, dtype, qw, kw = _code(q), q.dtype, n_q * head_dim, n_kv * head_dim
     qs = _rows(q, ctx, None, qw, dtype, "q")
     batch = q.shape[0]
@@ -198,22 +222,23 @@ def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int
     pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
     if max_len is None:
         max_len = table.shape[1] * kpages.shape[1]
-    need = _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len)
+    sc, seen = _scales(ctx, pg, kscales, vscales), _window(window, sinks)
+    need = _paged_work(ctx, pg.dtype, batch, n_q, n_kv, head_dim, max_len, *seen)
     raw, scope = _on(stream, q)
     work = _empty(scope, need // 4, q, _t().float32) if need else None
     if out is None:
         out, os = _empty(scope, (batch, qw), q), qw
     else:
         os = _rows(out, ctx, batch, qw, dtype, "out")
-    call("rq_paged_attention", ctx.handle, C.byref(pg), code, q.data_ptr(), qs, kd, ks, vd, vs,
+    call("rq_paged_attention_window", ctx.handle, C.byref(pg), *sc, *seen, code, q.data_ptr(), qs, kd, ks, vd, vs,
          _i32(lens, ctx, batch, "lens"), batch, n_q, max_len, theta, scale, out.data_ptr(), os,
          work.data_ptr() if need else None, need, raw)
     return out
 
 
 def pages_append(ctx: Context, q, k, v, kpages, vpages, table, cu, past, n_q: int, n_kv: int, head_dim: int,
-                 theta: float, q_out=None, k_out=None, stream=None):
-    """rq_pages_append: packed rows (sequence b: cu[b] .. cu[b+1] - 1, at positions
+                 theta: float, q_out=None, k_out=None, stream=None, kscales=None, vscales=None):
+    """rq_pages_append (int8 pages: rq_pages_append_q8): packed rows (sequence b: cu[b] .. cu[b+1] - 1, at positions
     past[b] and on) of q [rows, n_q*head_dim] and k [rows, n_kv*head_dim] rotated,
     the rotated k and v stored in the pages -> (rotated q, rotated k), written
     into q_out / k_out when given (they may be q and k)."""
@@ -234,10 +259,30 @@ def pages_append(ctx: Context, q, k, v, kpages, vpages, table, cu, past, n_q: in
         k_out = _empty(scope, (rows, kw), q)
     else:
         kos = _rows(k_out, ctx, rows, kw, dtype, "k_out")
-    call("rq_pages_append", ctx.handle, C.byref(pg), code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+    sc = _scales(ctx, pg, kscales, vscales)
+    name, sc = ("rq_pages_append_q8", sc) if pg.dtype == RQ_I8 else ("rq_pages_append", ())
+    call(name, ctx.handle, C.byref(pg), *sc, code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
          _i32(cu, ctx, batch + 1, "cu"), _i32(past, ctx, batch, "past"), batch, rows, n_q, theta,
          q_out.data_ptr(), qos, k_out.data_ptr(), kos, raw)
     return q_out, k_out
+
+
+def pages_rows(ctx: Context, kpages, vpages, table, cu, rows: int, n_kv: int, head_dim: int, dtype=None, k_out=None,
+               v_out=None, stream=None, kscales=None, vscales=None):
+    """rq_pages_rows: rows 0, 1, ... of each sequence b as values of `dtype` (f32 or bf16;
+    default f32) to the packed rows cu[b] .. cu[b+1] - 1 (`rows` in all) of k_out and v_out
+    [rows, n_kv*head_dim] -> (k_out, v_out). Rows of no sequence are not written."""
+    kw, batch = n_kv * head_dim, cu.numel() - 1
+    _need(batch >= 0 and rows >= 0, "cu must hold batch + 1 row numbers, and rows must not be negative")
+    pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
+    sc = _scales(ctx, pg, kscales, vscales)
+    raw, scope = _on(stream, kpages)
+    dtype = (_t().float32 if k_out is None else k_out.dtype) if dtype is None else dtype
+    k_out, v_out = (_empty(scope, (rows, kw), kpages, dtype) if t is None else t for t in (k_out, v_out))
+    ks, vs = _rows(k_out, ctx, rows, kw, dtype, "k_out"), _rows(v_out, ctx, rows, kw, dtype, "v_out")
+    call("rq_pages_rows", ctx.handle, C.byref(pg), *sc, _code(k_out), _i32(cu, ctx, batch + 1, "cu"), batch, rows,
+         k_out.data_ptr(), ks, v_out.data_ptr(), vs, raw)
+    return k_out, v_out
 
 
 def pages_copy(ctx: Context, pages, src, dst, stream=None):

@@ -1527,11 +1527,7 @@ static PromptArgs prompt_args(const rq_prompt* p, int64_t window, int64_t sinks)
   return a;
 }
 
-static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) {
-  if (!g) return fail(RQ_ERR_NULL, "rq_pages is NULL");
-  if ((dtype != RQ_F32 && dtype != RQ_BF16) || (g->dtype != RQ_F32 && g->dtype != RQ_BF16))
-    return fail(RQ_ERR_DTYPE, "types must be RQ_F32 or RQ_BF16");
-  if (dtype == RQ_BF16 && g->dtype == RQ_F32) return fail(RQ_ERR_DTYPE, "bf16 rows over f32 pages are not supported");
+static int check_page_layout(const rq_pages* g, int64_t n_q, double theta) {
   if (int s = check_heads(n_q, g->n_kv, g->head_dim)) return s;
   if (g->page_size < 16 || g->page_size > 65536 || (g->page_size & (g->page_size - 1)) != 0)
     return fail(RQ_ERR_SHAPE, "page_size must be a power of two from 16 to 65536");
@@ -1543,6 +1539,49 @@ static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) 
   if (g->n_kv * g->head_dim > kMaxTileStride) return fail(RQ_ERR_SHAPE, "n_kv * head_dim too large");
   if (!(theta >= 0.0 && theta <= 1e30)) return fail(RQ_ERR_SHAPE, "theta must be positive, or 0 for no rotation");
   return RQ_OK;
+}
+
+static int check_pages(const rq_pages* g, int dtype, int64_t n_q, double theta) {
+  if (!g) return fail(RQ_ERR_NULL, "rq_pages is NULL");
+  if ((dtype != RQ_F32 && dtype != RQ_BF16) || (g->dtype != RQ_F32 && g->dtype != RQ_BF16))
+    return fail(RQ_ERR_DTYPE, "types must be RQ_F32 or RQ_BF16");
+  if (dtype == RQ_BF16 && g->dtype == RQ_F32) return fail(RQ_ERR_DTYPE, "bf16 rows over f32 pages are not supported");
+  return check_page_layout(g, n_q, theta);
+}
+
+// Scales of int8 pages; of others none
+static int check_scales(const rq_pages* g, const float* kscales, const float* vscales, int64_t stride) {
+  if (g->dtype != RQ_I8) return kscales || vscales ? fail(RQ_ERR_DTYPE, "scales are for int8 pages") : RQ_OK;
+  if (int s = check_i32("kscales", kscales)) return s;
+  if (int s = check_i32("vscales", vscales)) return s;
+  if (stride < g->page_size / 16 * g->n_kv || stride > (int64_t)1 << 40)
+    return fail(RQ_ERR_SHAPE, "scale_stride must be at least page_size / 16 * n_kv");
+  return RQ_OK;
+}
+
+static int check_any_pages(const rq_pages* g, const float* kscales, const float* vscales, int64_t stride, int dtype,
+                           int64_t n_q, double theta) {
+  if (!g) return fail(RQ_ERR_NULL, "rq_pages is NULL");
+  if (g->dtype != RQ_I8) {
+    if (int s = check_pages(g, dtype, n_q, theta)) return s;
+  } else {
+    if (dtype != RQ_F32 && dtype != RQ_BF16) return fail(RQ_ERR_DTYPE, "types must be RQ_F32 or RQ_BF16");
+    if (int s = check_page_layout(g, n_q, theta)) return s;
+  }
+  return check_scales(g, kscales, vscales, stride);
+}
+
+// A window that leaves rows out of max_len, or none
+struct CacheWindow {
+  int window = 0, sinks = 0;
+  CacheWindow(int64_t max_len, int64_t w, int64_t z) {
+    if (w > 0 && w < max_len && z < max_len - w) window = (int)w, sinks = (int)z;
+  }
+};
+
+static PagedPlan paged_plan(int cache_dtype, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim,
+                            int64_t max_len, const CacheWindow& w, int cu_count) {
+  return plan_paged_attention(batch, n_q, n_kv, head_dim, walked_rows(max_len, w.window, w.sinks), cu_count);
 }
 
 // Sequences, heads and rows of a paged attention call. What passes keeps max_len times the groups, and the
@@ -1572,6 +1611,46 @@ static PagesArgs pages_args(const rq_pages* g, int64_t n_q, int64_t batch, doubl
   a.rope = theta > 0.0;
   a.log2_theta = a.rope ? std::log2(theta) : 0.0;
   return a;
+}
+
+static int pages_append(rq_ctx h, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride, int dtype,
+                       const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                       int64_t v_stride, const int32_t* cu, const int32_t* past, int64_t batch, int64_t rows,
+                       int64_t n_q, double theta, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                       void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_any_pages(pg, kscales, vscales, scale_stride, dtype, n_q, theta)) return s;
+  if (batch < 0 || batch > kMaxRows || rows < 0) return fail(RQ_ERR_SHAPE, "bad dimension");
+  if (rows > kMaxGroups) return fail(RQ_ERR_SHAPE, "too many rows for one launch");
+  if (batch == 0 || rows == 0) return RQ_OK;
+  if (int s = check_table(pg)) return s;
+  const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
+  if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
+  if (int s = check_rows("k", k, k_stride, kw, dtype)) return s;
+  if (int s = check_rows("v", v, v_stride, kw, dtype)) return s;
+  if (int s = check_rows("q_out", q_out, q_out_stride, qw, dtype)) return s;
+  if (k_out)
+    if (int s = check_rows("k_out", k_out, k_out_stride, kw, dtype)) return s;
+  if (int s = check_i32("cu", cu)) return s;
+  if (int s = check_i32("past", past)) return s;
+  if (int s = check_ctx(c)) return s;
+  if (int s = set_device(c)) return s;
+  PagesAppendArgs a = {};
+  a.p = pages_args(pg, n_q, batch, theta);
+  a.p.q = q, a.p.k = k, a.p.v = v;
+  a.p.q_stride = q_stride, a.p.k_stride = k_stride, a.p.v_stride = v_stride;
+  a.cu = cu;
+  a.past = past;
+  a.rows = rows;
+  a.q_out = q_out, a.k_out = k_out;
+  a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
+  a.kscales = kscales, a.vscales = vscales, a.scale_stride = scale_stride;
+  if (pg->dtype == RQ_I8 && append_q8_slots(a) > kMaxGroups)
+    return fail(RQ_ERR_SHAPE, "too many rows and sequences for one launch");
+  const hipError_t e = pg->dtype == RQ_I8 ? launch_pages_append_q8(dtype, a, (hipStream_t)stream)
+                                          : launch_pages_append(dtype, pg->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "pages append launch");
+  return RQ_OK;
 }
 
 }  // namespace rq
@@ -1697,12 +1776,23 @@ int rq_prompt_attention_window_bwd(rq_ctx h, const rq_prompt* p, int64_t window,
 
 int rq_paged_attention_work(rq_ctx h, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
                             size_t* bytes) {
+  return rq_paged_attention_window_work(h, RQ_F32, batch, n_q, n_kv, head_dim, max_len, 0, 0, bytes);
+}
+
+int rq_paged_attention_window_work(rq_ctx h, int cache_dtype, int64_t batch, int64_t n_q, int64_t n_kv,
+                                   int64_t head_dim, int64_t max_len, int64_t window, int64_t sinks, size_t* bytes) {
   Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (cache_dtype != RQ_F32 && cache_dtype != RQ_BF16 && cache_dtype != RQ_I8)
+    return fail(RQ_ERR_DTYPE, "pages must be RQ_F32, RQ_BF16 or RQ_I8");
   if (int s = check_heads(n_q, n_kv, head_dim)) return s;
+  if (int s = check_window(window, sinks)) return s;
   if (int s = check_paged_size(batch, n_q, n_kv, max_len)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
   if (int s = check_ctx(c)) return s;
-  *bytes = batch == 0 ? 0 : plan_paged_attention(batch, n_q, n_kv, head_dim, max_len, c->cu_count).work;
+  *bytes = batch == 0 ? 0
+                      : paged_plan(cache_dtype, batch, n_q, n_kv, head_dim, max_len,
+                                   CacheWindow(max_len, window, sinks), c->cu_count)
+                            .work;
   return RQ_OK;
 }
 
@@ -1710,8 +1800,19 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
                        int64_t k_stride, const void* v, int64_t v_stride, const int32_t* lens, int64_t batch,
                        int64_t n_q, int64_t max_len, double theta, double scale, void* out, int64_t out_stride,
                        void* work, size_t work_bytes, void* stream) {
-  Ctx* c = reinterpret_cast<Ctx*>(h);
   if (int s = check_pages(pg, dtype, n_q, theta)) return s;
+  return rq_paged_attention_window(h, pg, nullptr, nullptr, 0, 0, 0, dtype, q, q_stride, k, k_stride, v, v_stride, lens,
+                                   batch, n_q, max_len, theta, scale, out, out_stride, work, work_bytes, stream);
+}
+
+int rq_paged_attention_window(rq_ctx h, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride,
+                              int64_t window, int64_t sinks, int dtype, const void* q, int64_t q_stride, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride, const int32_t* lens, int64_t batch,
+                              int64_t n_q, int64_t max_len, double theta, double scale, void* out, int64_t out_stride,
+                              void* work, size_t work_bytes, void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (int s = check_any_pages(pg, kscales, vscales, scale_stride, dtype, n_q, theta)) return s;
+  if (int s = check_window(window, sinks)) return s;
   if (int s = check_scale(scale)) return s;
   if (int s = check_paged_size(batch, n_q, pg->n_kv, max_len)) return s;
   if (batch == 0) return RQ_OK;
@@ -1726,7 +1827,8 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   if (int s = check_i32("lens", lens)) return s;
   if (int s = check_rows("out", out, out_stride, qw, dtype)) return s;
   if (int s = check_ctx(c)) return s;
-  const PagedPlan plan = plan_paged_attention(batch, n_q, pg->n_kv, pg->head_dim, max_len, c->cu_count);
+  const CacheWindow seen(max_len, window, sinks);
+  const PagedPlan plan = paged_plan(pg->dtype, batch, n_q, pg->n_kv, pg->head_dim, max_len, seen, c->cu_count);
   if (plan.work > 0 && !work) return fail(RQ_ERR_NULL, "work is NULL");
   if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
   if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
@@ -1740,13 +1842,18 @@ int rq_paged_attention(rq_ctx h, const rq_pages* pg, int dtype, const void* q, i
   a.p.q_stride = q_stride, a.p.k_stride = k_stride, a.p.v_stride = v_stride;
   a.lens = lens;
   a.max_len = max_len;
+  a.window = seen.window;
+  a.sinks = seen.sinks;
+  a.i8 = pg->dtype == RQ_I8;
+  a.kscales = kscales, a.vscales = vscales, a.scale_stride = scale_stride;
   a.scale2 = (float)(scale * 1.4426950408889634);
   a.out = out;
   a.out_stride = out_stride;
   a.split_rows = plan.split_rows;
   a.nsplit = plan.nsplit;
   a.part = static_cast<float*>(work);
-  const hipError_t e = launch_paged_attention(dtype, pg->dtype, a, (hipStream_t)stream);
+  const hipError_t e = a.i8 ? launch_paged_attention_q8(dtype, a, (hipStream_t)stream)
+                            : launch_paged_attention(dtype, pg->dtype, a, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return RQ_OK;
 }
@@ -1755,34 +1862,50 @@ int rq_pages_append(rq_ctx h, const rq_pages* pg, int dtype, const void* q, int6
                     int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, const int32_t* past,
                     int64_t batch, int64_t rows, int64_t n_q, double theta, void* q_out, int64_t q_out_stride,
                     void* k_out, int64_t k_out_stride, void* stream) {
-  Ctx* c = reinterpret_cast<Ctx*>(h);
   if (int s = check_pages(pg, dtype, n_q, theta)) return s;
+  return pages_append(h, pg, nullptr, nullptr, 0, dtype, q, q_stride, k, k_stride, v, v_stride, cu, past,
+                      batch, rows, n_q, theta, q_out, q_out_stride, k_out, k_out_stride, stream);
+}
+
+int rq_pages_append_q8(rq_ctx h, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride, int dtype,
+                       const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                       int64_t v_stride, const int32_t* cu, const int32_t* past, int64_t batch, int64_t rows,
+                       int64_t n_q, double theta, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                       void* stream) {
+  if (!pg) return fail(RQ_ERR_NULL, "rq_pages is NULL");
+  if (pg->dtype != RQ_I8) return fail(RQ_ERR_DTYPE, "pages must be RQ_I8");
+  return pages_append(h, pg, kscales, vscales, scale_stride, dtype, q, q_stride, k, k_stride, v, v_stride, cu, past,
+                      batch, rows, n_q, theta, q_out, q_out_stride, k_out, k_out_stride, stream);
+}
+
+int rq_pages_rows(rq_ctx h, const rq_pages* pg, const float* kscales, const float* vscales, int64_t scale_stride,
+                  int dtype, const int32_t* cu, int64_t batch, int64_t rows, void* k_out, int64_t k_out_stride,
+                  void* v_out, int64_t v_out_stride, void* stream) {
+  Ctx* c = reinterpret_cast<Ctx*>(h);
+  if (!pg) return fail(RQ_ERR_NULL, "rq_pages is NULL");
+  if ((dtype != RQ_F32 && dtype != RQ_BF16) || (pg->dtype != RQ_F32 && pg->dtype != RQ_BF16 && pg->dtype != RQ_I8))
+    return fail(RQ_ERR_DTYPE, "rows must be RQ_F32 or RQ_BF16, pages these or RQ_I8");
+  if (int s = check_page_layout(pg, pg->n_kv, 0.0)) return s;
+  if (int s = check_scales(pg, kscales, vscales, scale_stride)) return s;
   if (batch < 0 || batch > kMaxRows || rows < 0) return fail(RQ_ERR_SHAPE, "bad dimension");
   if (rows > kMaxGroups) return fail(RQ_ERR_SHAPE, "too many rows for one launch");
   if (batch == 0 || rows == 0) return RQ_OK;
   if (int s = check_table(pg)) return s;
-  const int64_t qw = n_q * pg->head_dim, kw = pg->n_kv * pg->head_dim;
-  if (int s = check_rows("q", q, q_stride, qw, dtype)) return s;
-  if (int s = check_rows("k", k, k_stride, kw, dtype)) return s;
-  if (int s = check_rows("v", v, v_stride, kw, dtype)) return s;
-  if (int s = check_rows("q_out", q_out, q_out_stride, qw, dtype)) return s;
-  if (k_out)
-    if (int s = check_rows("k_out", k_out, k_out_stride, kw, dtype)) return s;
+  const int64_t kw = pg->n_kv * pg->head_dim;
+  if (int s = check_rows("k_out", k_out, k_out_stride, kw, dtype)) return s;
+  if (int s = check_rows("v_out", v_out, v_out_stride, kw, dtype)) return s;
   if (int s = check_i32("cu", cu)) return s;
-  if (int s = check_i32("past", past)) return s;
   if (int s = check_ctx(c)) return s;
   if (int s = set_device(c)) return s;
-  PagesAppendArgs a = {};
-  a.p = pages_args(pg, n_q, batch, theta);
-  a.p.q = q, a.p.k = k, a.p.v = v;
-  a.p.q_stride = q_stride, a.p.k_stride = k_stride, a.p.v_stride = v_stride;
+  PagesRowsArgs a = {};
+  a.p = pages_args(pg, pg->n_kv, batch, 0.0);
   a.cu = cu;
-  a.past = past;
   a.rows = rows;
-  a.q_out = q_out, a.k_out = k_out;
-  a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
-  const hipError_t e = launch_pages_append(dtype, pg->dtype, a, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_fail(e, "pages append launch");
+  a.kscales = kscales, a.vscales = vscales, a.scale_stride = scale_stride;
+  a.k_out = k_out, a.v_out = v_out;
+  a.k_out_stride = k_out_stride, a.v_out_stride = v_out_stride;
+  const hipError_t e = launch_pages_rows(dtype, pg->dtype, a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "page rows launch");
   return RQ_OK;
 }
 

@@ -10,51 +10,14 @@
 #include <cmath>
 
 #include "attn_tile.h"
-#include "paged.h"
+#include "paged_tile.h"
 
 namespace rq {
 
 namespace {
 
-// cos and sin of pos * theta^(-2 i / head_dim). The angle is formed in double in turns
-// and its whole turns taken off there, so far positions keep their digits.
-__device__ __forceinline__ void rope_angle(int64_t pos, int i, int head_dim, double log2_theta, float* c, float* s) {
-  double t = (double)pos * exp2(-2.0 * (double)i / (double)head_dim * log2_theta) * 0.15915494309189535;
-  t -= rint(t);
-  double sd, cd;
-  sincospi(2.0 * t, &sd, &cd);
-  *c = (float)cd;
-  *s = (float)sd;
-}
+constexpr int kPagedThreads = 256, kPagedWaves = 4;
 
-// ranges of a sequence of len cached rows: the last may hold one row more, which is the
-// new row's place in a cache that is full with it
-__host__ __device__ __forceinline__ int64_t ranges_of(int64_t len, int64_t rows) {
-  return len > rows + 1 ? (len - 1 + rows - 1) / rows : 1;
-}
-
-constexpr int kPagedThreads = 256, kPagedWaves = 4, kRec = 4;
-
-__device__ __forceinline__ uint32_t low16_pair(uint32_t a, uint32_t b) {  // a.lo | b.lo << 16
-  return __builtin_amdgcn_perm(b, a, 0x05040100);
-}
-__device__ __forceinline__ uint32_t high16_pair(uint32_t a, uint32_t b) {  // a.hi | b.hi << 16
-  return __builtin_amdgcn_perm(b, a, 0x07060302);
-}
-
-// The bf16 terms of x: x = t0 + t1 + t2 within 2^-24 |x|
-template <int NT>
-__device__ __forceinline__ void split_terms(float x, __bf16 (&t)[NT]) {
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    t[n] = (__bf16)x;
-    x -= (float)t[n];
-  }
-}
-
-}  // namespace
-
-namespace {
 // LDS of 16 heads' queries as fragments: f32, or two or three bf16 terms
 template <typename A, typename C>
 constexpr int paged_query_bytes(int hd) {
@@ -84,7 +47,7 @@ constexpr int paged_query_bytes(int hd) {
 // of its norm: 0.0017; with one term of the weights 0.0022, of the queries too 0.0028, all in the same time (372, 370 us
 // of cold caches; 8 of 4000 rows, 32/8 heads, 34.3, 34.1; one of 128, 16 heads, 7.0, 6.9).
 // An f32 cache is multiplied in f32.
-template <typename A, typename C, int HD, bool PART>
+template <typename A, typename C, int HD, bool PART, bool WIN>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;
   constexpr int NT = F32 ? 1 : sizeof(A) == 2 ? 2 : 3;
@@ -133,7 +96,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
   const int r0 = split * a.split_rows, first = r0 + wave * KT;
   const int last_entry = max((int)p.table_stride - 1, 0);
   int page0 = -1, page1 = -1;
-  if (p.table_stride > 0) {
+  if (!WIN && p.table_stride > 0) {
     page0 = trow[min(first >> p.page_bits, last_entry)];
     page1 = trow[min((first + 16) >> p.page_bits, last_entry)];
   }
@@ -148,9 +111,11 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     return;
   }
   // one row past a whole number of ranges goes to the last range
-  const int nsplit = ranges_of(len, a.split_rows);
+  CachedRows<WIN> cr;
+  cr.init(a, len, rows);
+  const int nsplit = ranges_of(cr.walk, a.split_rows);
   if (split >= nsplit) return;
-  const int r1 = split == nsplit - 1 ? len : r0 + a.split_rows;
+  const int r1 = split == nsplit - 1 ? cr.walk : r0 + a.split_rows;
   const int kvd = p.n_kv * hd;
   bool lost = false;  // a page number out of range
 
@@ -161,7 +126,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     return ((int64_t)(ok ? page : 0) << p.page_bits) + (r & ((1 << p.page_bits) - 1));
   };
   auto base_of = [&](int r) -> int64_t {
-    r = r < r1 ? r : r0;
+    r = cr.row(r < r1 ? r : r0);
     return row_base(trow[r >> p.page_bits], r);
   };
   const C* kb = static_cast<const C*>(p.kpages) + hkv * hd;
@@ -193,8 +158,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
   };
   int64_t base[2] = {0, 0};
   if (first < r1) {
-    base[0] = row_base(page0, first);
-    base[1] = first + 16 < r1 ? row_base(page1, first + 16) : base[0];
+    if constexpr (WIN) {
+      base[0] = base_of(first);
+      base[1] = first + 16 < r1 ? base_of(first + 16) : base[0];
+    } else {
+      base[0] = row_base(page0, first);
+      base[1] = first + 16 < r1 ? row_base(page1, first + 16) : base[0];
+    }
     load_k(base);
     load_v(base);
   }
@@ -303,6 +273,16 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int i = 0; i < 4; i++) s[4 * t + i] = r + 16 * t + 4 * g + i < r1 ? d[t][i] : -INFINITY;
+    // a block that the window or the sinks end in
+    const bool cut[2] = {!cr.sees_block(cr.row(r)), !cr.sees_block(cr.row(r + 16))};
+    if constexpr (WIN) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        if (cut[t])
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (!cr.sees(cr.row(r + 16 * t) + 4 * g + i)) s[4 * t + i] = -INFINITY;
+    }
     if (more) load_k(base);
     float mx = s[0];
 #pragma unroll
@@ -319,10 +299,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
     }
 #pragma unroll
     for (int t = 0; t < E; t++) acc[t] *= alpha;
-    if (r + KT > r1) {  // rows past the end hold anything: 0 times it must stay 0
+    if (r + KT > r1 || cut[0] || cut[1]) {  // rows not seen hold anything: 0 times it must stay 0
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (r + 16 * (j >> 2) + 4 * g + (j & 3) >= r1)
+        if (r + 16 * (j >> 2) + 4 * g + (j & 3) >= r1 || !cr.sees(cr.row(r + 16 * (j >> 2)) + 4 * g + (j & 3)))
 #pragma unroll
           for (int q = 0; q < VP; q++)
 #pragma unroll
@@ -419,13 +399,15 @@ __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAtt
 
 // Joins the ranges' records of a (sequence, head), one workgroup each: head_dim / 4 lanes
 // a record, the lane groups' sums added in order.
-template <typename A>
+template <typename A, bool WIN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const PagesArgs& p = a.p;
   const int hq = blockIdx.x % p.n_q, b = blockIdx.x / p.n_q, hd = p.head_dim, len = a.lens[b];
-  const int64_t rows = (int64_t)len + (p.k != nullptr);
+  const int64_t rows = (int64_t)len + (p.k != nullptr || a.ahead);
   if (len < 0 || rows > a.max_len || rows > p.table_stride << p.page_bits) return;
-  const int n = ranges_of(len, a.split_rows);
+  CachedRows<WIN> cr;
+  cr.init(a, a.i8 && p.k != nullptr ? len & ~15 : len + a.ahead, rows);
+  const int n = ranges_of(cr.walk, a.split_rows);
   if (n <= 1) return;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float sums[256 * 4];
@@ -592,35 +574,37 @@ PagedPlan plan_paged_attention(int64_t batch, int64_t n_q, int64_t n_kv, int64_t
 
 namespace {
 
-template <typename A, typename C, int HD, bool PART>
+template <typename A, bool WIN>
+hipError_t run_merge(const PagedAttnArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_merge_kernel<A, WIN>), dim3((unsigned)(a.p.batch * a.p.n_q)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename A, typename C, int HD, bool PART, bool WIN>
 hipError_t run_paged(const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
   const int64_t htiles = (p.n_q / p.n_kv + 15) / 16;
   constexpr int kFixed = paged_query_bytes<A, C>(HD) + (2 * HD + kPagedWaves * 32 + 16) * 4;
   constexpr int kMaxLds = kFixed + kPagedWaves * 16 * HD * 4;
   const int lds = kFixed + kPagedWaves * std::min(p.n_q / p.n_kv, 16) * HD * 4;
-  const auto kernel = paged_attention_kernel<A, C, HD, PART>;
+  const auto kernel = paged_attention_kernel<A, C, HD, PART, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), kMaxLds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.nsplit * p.batch * p.n_kv * htiles)), dim3(kPagedThreads), lds, stream,
                      a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (a.nsplit > 1) {
-    hipLaunchKernelGGL(paged_merge_kernel<A>, dim3((unsigned)(p.batch * p.n_q)), dim3(256), 0, stream, a);
-    return hipGetLastError();
-  }
-  return hipSuccess;
+  return a.nsplit > 1 ? run_merge<A, WIN>(a, stream) : hipSuccess;
 }
 
-template <typename A, typename C>
+template <typename A, typename C, bool WIN>
 hipError_t run_paged_hd(const PagedAttnArgs& a, hipStream_t stream) {
   const int hd = a.p.head_dim;
-  if (hd == 64) return run_paged<A, C, 64, false>(a, stream);
-  if (hd == 128) return run_paged<A, C, 128, false>(a, stream);
-  if (hd == 256) return run_paged<A, C, 256, false>(a, stream);
-  if (hd < 64) return run_paged<A, C, 64, true>(a, stream);
-  if (hd < 128) return run_paged<A, C, 128, true>(a, stream);
-  return run_paged<A, C, 256, true>(a, stream);
+  if (hd == 64) return run_paged<A, C, 64, false, WIN>(a, stream);
+  if (hd == 128) return run_paged<A, C, 128, false, WIN>(a, stream);
+  if (hd == 256) return run_paged<A, C, 256, false, WIN>(a, stream);
+  if (hd < 64) return run_paged<A, C, 64, true, WIN>(a, stream);
+  if (hd < 128) return run_paged<A, C, 128, true, WIN>(a, stream);
+  return run_paged<A, C, 256, true, WIN>(a, stream);
 }
 
 template <typename A, typename C>
@@ -631,10 +615,21 @@ hipError_t run_append(const PagesAppendArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_paged_attention(int dtype, int cache_dtype, const PagedAttnArgs& a, hipStream_t stream) {
+template <bool WIN>
+static hipError_t launch_paged(int dtype, int cache_dtype, const PagedAttnArgs& a, hipStream_t stream) {
   if (dtype == RQ_F32)
-    return cache_dtype == RQ_F32 ? run_paged_hd<float, float>(a, stream) : run_paged_hd<float, __bf16>(a, stream);
-  return run_paged_hd<__bf16, __bf16>(a, stream);
+    return cache_dtype == RQ_F32 ? run_paged_hd<float, float, WIN>(a, stream)
+                                 : run_paged_hd<float, __bf16, WIN>(a, stream);
+  return run_paged_hd<__bf16, __bf16, WIN>(a, stream);
+}
+
+hipError_t launch_paged_attention(int dtype, int cache_dtype, const PagedAttnArgs& a, hipStream_t stream) {
+  return a.window > 0 ? launch_paged<true>(dtype, cache_dtype, a, stream)
+                      : launch_paged<false>(dtype, cache_dtype, a, stream);
+}
+
+hipError_t launch_paged_merge(int dtype, const PagedAttnArgs& a, hipStream_t stream) {
+  return dtype == RQ_F32 ? run_merge<float, true>(a, stream) : run_merge<__bf16, true>(a, stream);
 }
 
 hipError_t launch_pages_append(int dtype, int cache_dtype, const PagesAppendArgs& a, hipStream_t stream) {

@@ -1,0 +1,454 @@
+"""Int8 pages: append, one-token attention and stored rows, against the block's arithmetic in plain torch
+(q8_ref.py, bit for bit) and attention over the stored values in 64 bits (attn_ref.py states the tolerances)."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+THETA = 1e4
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+
+    if not t.cuda.is_available():
+        pytest.skip("no GPU")
+    return t
+
+
+@pytest.fixture(scope="module")
+def ctx(torch):
+    import raster_amd
+
+    c = raster_amd.Context(0)
+    yield c
+    c.close()
+
+
+def new_rows(torch, seed, act, rows, nq, nkv, hd):
+    ty = {"f32": torch.float32, "bf16": torch.bfloat16}[act]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    qkv = torch.randn((rows, (nq + 2 * nkv) * hd), generator=g, device="cuda").to(ty)
+    return qkv.split([nq * hd, nkv * hd, nkv * hd], 1)
+
+
+def near_codes(got, want, x, s):
+    """Rotations may differ in an angle's last bit: the codes agree, or x / s is by the border (127 steps of 2^-21)."""
+    off = got != want
+    return bool(((got.double() - x.double() / s.double()).abs()[off] <= 0.5 + 127 * 2.0 ** -21).all())
+
+
+def check_out(torch, ref, out, q, cache, lens, add, nq, nkv, hd, scale, window, sinks):
+    """out's rows against attention over the cache as it is stored; q: the rotated queries, f64 [batch, nq, hd]."""
+    half = ref.HALF[out.dtype]
+    hq = 2.0 ** -22 if out.dtype == torch.float32 else 2.0 ** -16  # three or two bf16 terms
+    for b, m in enumerate(lens):
+        if m < 0 or m + add == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        n = m + add
+        keys, values = cache.values("k", b, n), cache.values("v", b, n)
+        j = torch.arange(n, device="cuda")
+        see = (((n - 1 - j < window) | (j < sinks)) if window else j >= 0)[None]
+        for h in range(nq):
+            g = h // (nq // nkv)
+            want, _, bound = ref.attend(q[b, h:h + 1], keys[:, g], values[:, g], scale, see, half, hq)
+            got = out[b, h * hd:(h + 1) * hd].double()
+            assert bool(((got - want[0]).abs() <= bound[0]).all()), (b, h, float(((got - want[0]).abs() / bound).max()))
+
+
+# activations, heads, KV heads, head_dim, page, cached rows, window, sinks
+CASES = [
+    ("f32", 4, 4, 128, 16, [0], 0, 0),
+    ("f32", 16, 16, 128, 16, [128, 0, 31, 32, 33, 15, 16, 17], 0, 0),
+    ("f32", 8, 2, 64, 32, [7, 700, 255, 256, 257], 0, 0),
+    ("f32", 6, 2, 40, 16, [100, 3], 0, 0),
+    ("f32", 4, 1, 256, 16, [300, 40, 95], 0, 0),
+    ("f32", 2, 2, 136, 16, [77], 0, 0),
+    ("f32", 2, 1, 200, 32, [130, 4], 0, 0),
+    ("f32", 5, 1, 8, 16, [130, 4], 0, 0),
+    ("bf16", 32, 8, 128, 16, [2500, 77, 0, 1024, 4099], 0, 0),
+    ("bf16", 64, 2, 64, 128, [300, 5000], 0, 0),  # 32 heads a KV head: the row is appended in a launch before
+    ("bf16", 17, 1, 128, 16, [40, 0, 15, 16], 0, 0),
+    ("f32", 40, 2, 104, 16, [47, 200], 30, 5),
+    ("bf16", 3, 3, 80, 16, [90, 12], 0, 0),
+    ("bf16", 2, 1, 248, 16, [400, 33], 0, 0),
+    ("bf16", 8, 2, 128, 16, [1000, 0, 5, 16, 63, 64, 65, 300], 64, 4),
+    ("f32", 8, 2, 64, 16, [1000, 0, 5, 16, 1999], 1, 0),
+    ("f32", 4, 4, 128, 64, [1000, 100, 16, 40], 1, 1),
+    ("bf16", 4, 2, 256, 16, [500, 17, 16], 17, 33),
+    ("f32", 8, 8, 72, 32, [3000, 40], 1111, 16),
+]
+
+
+@pytest.mark.parametrize("act,nq,nkv,hd,page,lens,window,sinks", CASES)
+@pytest.mark.parametrize("mode", ["append", "read", "no_rope"])
+def test_attention(torch, ctx, act, nq, nkv, hd, page, lens, window, sinks, mode):
+    import attn_ref as ref
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 {act} {nq}/{nkv}x{hd} page={page} {lens} {window}+{sinks} {mode}", flush=True)
+    add = mode != "read"
+    lens = lens + [-1]
+    n = len(lens)
+    cache = q8_ref.Cache(hd + sum(lens), nkv, hd, [x + 1 for x in lens], page, lens, pad=3 if hd == 64 else 0)
+    q, k, v = new_rows(torch, sum(lens), act, n, nq, nkv, hd)
+    theta, scale = 0.0 if mode == "no_rope" else THETA, hd ** -0.5
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = cache.clone()
+    out = raster_amd.paged_attention(ctx, q, k if add else None, v if add else None, cache.k, cache.v, cache.table, lt,
+                                     nq, nkv, hd, theta, scale, max_len=max(lens) + 1, window=window, sinks=sinks,
+                                     **cache.scales())
+    pos = torch.tensor(lens, device="cuda")
+    k32 = q8_ref.rope32(k.float().view(n, nkv, hd), pos, theta)
+    if add:
+        for b, m in enumerate(lens):
+            if m >= 0:
+                want.append("k", b, m, k32[b:b + 1])
+                want.append("v", b, m, v[b:b + 1].float().view(1, nkv, hd))
+    if theta and add:  # (an angle's last bit)
+        for b, m in enumerate(lens):
+            if m < 0:
+                continue
+            at = (int(cache.table[b, m // page]), m % page)
+            s = cache.ks[at[0], at[1] // 16]
+            assert bool(((s - want.ks[at[0], at[1] // 16]).abs() <= 2.0 ** -22 * s).all())
+            codes = (c.k[at].view(nkv, hd) for c in (cache, want))
+            assert near_codes(*codes, k32[b], s[:, None])
+            want.k[at], want.ks[at[0], at[1] // 16] = cache.k[at], s
+    assert cache.same(want)
+    rq = ref.rope(q.double().view(n, nq, hd), pos, theta) if theta else q.double().view(n, nq, hd)
+    check_out(torch, ref, out, rq, cache, lens, add, nq, nkv, hd, scale, window, sinks)
+
+
+@pytest.mark.parametrize("act,nq,nkv,hd,page,lens,past", [
+    ("f32", 4, 2, 128, 16, [37, 0, 1, 16, 15, 2], [0, 5, 15, 1000, 1, 15]),
+    ("f32", 3, 1, 40, 32, [33, 2], [31, 5000]),
+    ("bf16", 32, 8, 128, 16, [300, 1, 77], [0, 128, 5]),
+    ("bf16", 2, 2, 8, 16, [5], [3]),
+    ("bf16", 2, 1, 256, 64, [70, 17, 18], [0, 15, 30]),
+    ("f32", 2, 1, 248, 16, [40], [9]),
+    ("bf16", 4, 4, 64, 128, [200, 16], [100, 0]),
+])
+@pytest.mark.parametrize("theta", [0.0, THETA])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append(torch, ctx, act, nq, nkv, hd, page, lens, past, theta, in_place):
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 append {act} {nq}/{nkv}x{hd} {lens} {past}", flush=True)
+    n, tail = sum(lens), 3
+    lens2, past2 = lens + [2], past + [-1]  # a sequence left out, and rows of none behind it
+    cache = q8_ref.Cache(n, nkv, hd, [a + b for a, b in zip(lens, past)] + [1], page, past + [0],
+                         pad=5 if in_place else 0)
+    want = cache.clone()
+    q, k, v = (x.contiguous() if not in_place else x for x in new_rows(torch, n, act, n + 2 + tail, nq, nkv, hd))
+    cu = torch.tensor([sum(lens2[:i]) for i in range(len(lens2) + 1)], dtype=torch.int32, device="cuda")
+    pt = torch.tensor(past2, dtype=torch.int32, device="cuda")
+    q0, k0, v0 = q.clone(), k.clone(), v.clone()
+    qo, ko = (q, k) if in_place else (torch.full_like(q, 7.0), torch.full_like(k, 7.0))
+    raster_amd.pages_append(ctx, q, k, v, cache.k, cache.v, cache.table, cu, pt, nq, nkv, hd, theta, q_out=qo, k_out=ko,
+                            **cache.scales())
+    at = 0
+    for b, (m, p0) in enumerate(zip(lens, past)):
+        if m == 0:
+            continue
+        pos = torch.arange(p0, p0 + m, device="cuda")
+        rows = slice(at, at + m)
+        q32, k32 = (q8_ref.rope32(x[rows].float().view(m, -1, hd), pos, theta) for x in (q0, k0))
+        for got, w in ((qo[rows], q32), (ko[rows], k32)):
+            w = w.reshape(m, -1)
+            tol = (2.0 ** -8 if act == "bf16" else 2.0 ** -22) * (w.abs() + 1)
+            assert bool(((got.float() - w).abs() <= tol).all()) if theta else torch.equal(got, w.to(got.dtype))
+        want.append("k", b, p0, k32)
+        want.append("v", b, p0, v0[rows].float().view(m, nkv, hd))
+        if theta:
+            pages, r = cache.table[b].long()[pos // page], pos % page
+            s = cache.ks[pages, r // 16]
+            assert bool(((s - want.ks[pages, r // 16]).abs() <= 2.0 ** -22 * s).all())
+            assert near_codes(cache.k[pages, r].view(m, nkv, hd), want.k[pages, r].view(m, nkv, hd), k32, s[..., None])
+            want.k[pages, r], want.ks[pages, r // 16] = cache.k[pages, r], s
+        at += m
+    assert cache.same(want)
+    assert torch.equal(qo[n:], q0[n:] if in_place else torch.full_like(qo[n:], 7.0))
+    assert torch.equal(ko[n:], k0[n:] if in_place else torch.full_like(ko[n:], 7.0))
+    assert torch.equal(v, v0)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (40, 2, 64)])
+def test_a_block_fills_row_by_row(torch, ctx, nq, nkv, hd):
+    """33 tokens one by one, of rising and falling size: codes rounded anew, scales that only rise in a block and
+    start anew with the next; the same bits when a step is repeated."""
+    import attn_ref as ref
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 row by row {nq}/{nkv}x{hd}", flush=True)
+    cache = q8_ref.Cache(1, nkv, hd, [40, 50], 16, [0, 13])
+    want = cache.clone()
+    for step in range(33):
+        lens = [step, 13 + step]
+        q, k, v = (x * (0.3 + (7 * step) % 11) for x in new_rows(torch, step, "f32", 2, nq, nkv, hd))
+        lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        for b in range(2):
+            for which, x in (("k", k), ("v", v)):
+                want.append(which, b, lens[b], x[b:b + 1].reshape(1, nkv, hd))
+        first = None
+        for _ in range(2):
+            out = raster_amd.paged_attention(ctx, q, k, v, cache.k, cache.v, cache.table, lt, nq, nkv, hd, 0.0, 0.05,
+                                             **cache.scales())
+            assert cache.same(want)
+            first = out if first is None else first
+            assert torch.equal(out, first)
+        check_out(torch, ref, out, q.double().view(2, nq, hd), cache, lens, 1, nq, nkv, hd, 0.05, 0, 0)
+
+
+def test_values_that_are_not_finite_and_zeros(torch, ctx):
+    """A NaN or inf makes its block NaN until the block starts anew, hidden or not, and no other head; zeros stay zeros."""
+    import q8_ref
+    import raster_amd
+
+    nq, nkv, hd = 4, 2, 64
+    print("[gpu] q8 not finite", flush=True)
+    cache = q8_ref.Cache(2, nkv, hd, [80, 80], 16, [20, 20])
+    q, k, v = (x.contiguous() for x in new_rows(torch, 1, "f32", 2, nq, nkv, hd))
+    k[0, 3], v[1, hd + 5] = float("nan"), float("inf")
+    args = (nq, nkv, hd, THETA, 0.1)
+
+    def step(lens, q, k, v, **kw):
+        lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        return raster_amd.paged_attention(ctx, q, k, v, cache.k, cache.v, cache.table, lt, *args, **cache.scales(), **kw)
+
+    out = step([20, 20], q, k, v)
+    bad = torch.isnan(out.view(2, nq, hd))
+    assert bool(bad[0, :2].all()) and not bool(bad[0, 2:].any())  # KV head 0 of sequence 0
+    assert bool(bad[1, 2:].all()) and not bool(bad[1, :2].any())
+    assert bool(torch.isnan(cache.ks[int(cache.table[0, 1]), 0, 0])) and bool(torch.isfinite(cache.vs[int(cache.table[0, 1]), 0]).all())
+    q, k, v = new_rows(torch, 2, "f32", 2, nq, nkv, hd)
+    assert bool(torch.isnan(step([21, 21], q, k, v)).any())  # still the same block
+    # rows 32 and on: a window that does not reach back to it
+    for r in range(32, 52):
+        out = step([r, r], *new_rows(torch, r, "f32", 2, nq, nkv, hd), window=1)
+        assert bool(torch.isfinite(out).all())
+    assert bool(torch.isfinite(step([52, 52], q, k, v, window=21)).all())
+    assert bool(torch.isfinite(step([53, 53], q, k, v, window=22, sinks=3)).all())
+    assert bool(torch.isnan(step([54, 54], q, k, v)).any())
+    # written from the block's first row on, it is as good as new
+    cu = torch.tensor([0, 16, 32], dtype=torch.int32, device="cuda")
+    x = new_rows(torch, 4, "f32", 32, nq, nkv, hd)
+    raster_amd.pages_append(ctx, *x, cache.k, cache.v, cache.table, cu,
+                            torch.tensor([16, 16], dtype=torch.int32, device="cuda"), nq, nkv, hd, THETA, **cache.scales())
+    assert bool(torch.isfinite(step([55, 55], q, k, v)).all())
+    # zeros
+    z = torch.zeros_like(k)
+    out = step([64, 64], q, z, z)
+    at = int(cache.table[0, 4])
+    assert bool((cache.ks[at, 0] == 0).all()) and bool((cache.k[at, 0] == 0).all()) and bool(torch.isfinite(out).all())
+    tiny = torch.full_like(k, 1e-44)  # max / 127 is 0 in f32
+    step([65, 65], q, tiny, tiny)
+    assert bool((cache.ks[at, 0] == 0).all()) and bool((cache.k[at, :2] == 0).all())
+    step([66, 66], q, k, v)
+    assert bool((cache.k[at, :2] == 0).all()) and bool((cache.k[at, 2] != 0).any())
+
+
+def test_bad_pages_and_lengths(torch, ctx):
+    import q8_ref
+    import raster_amd
+
+    print("[gpu] q8 bad pages", flush=True)
+    for nq, nkv in ((4, 2), (40, 2)):
+        hd, lens = 64, [40, 50, 60, 70]
+        start = q8_ref.Cache(5, nkv, hd, [n + 1 for n in lens], 16, lens)
+        q, k, v = new_rows(torch, 5, "f32", 4, nq, nkv, hd)
+        lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+        def call(c, table, lt, **kw):
+            return raster_amd.paged_attention(ctx, q, k, v, c.k, c.v, table, lt, nq, nkv, hd, THETA, hd ** -0.5,
+                                              **c.scales(), **kw)
+
+        whole = start.clone()
+        good = call(whole, start.table, lt)
+        bad, far = start.table.clone(), lt.clone()
+        bad[0, 1] = start.k.shape[0]  # read
+        bad[1, 3] = -1                # appended (row 50 is in page 3)
+        far[3] = 10 ** 6              # past the table
+        c = start.clone()
+        out = call(c, bad, far)
+        for b in (0, 1, 3):
+            assert bool(torch.isnan(out[b]).all())
+        assert torch.equal(out[2], good[2])
+        want = start.clone()  # sequences 0 and 2 wrote their blocks, nobody else anything
+        for b in (0, 2):
+            at = int(start.table[b, lens[b] // 16])
+            want.k[at], want.v[at], want.ks[at], want.vs[at] = whole.k[at], whole.v[at], whole.ks[at], whole.vs[at]
+        assert c.same(want)
+        c = start.clone()
+        out = call(c, start.table, lt, max_len=61)
+        assert torch.equal(out[:3], good[:3]) and bool(torch.isnan(out[3]).all())
+        at = int(start.table[3, 4])
+        assert torch.equal(c.k[at], start.k[at]) and torch.equal(c.ks[at].nan_to_num(), start.ks[at].nan_to_num())
+        # pages that the window has left are not looked up
+        gone = start.table.clone()
+        gone[2, 1:3] = -1
+        a, b = (call(start.clone(), t, lt, window=10, sinks=2) for t in (start.table, gone))
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+def test_append_without_a_page(torch, ctx):
+    import q8_ref
+    import raster_amd
+
+    print("[gpu] q8 append without a page", flush=True)
+    c = q8_ref.Cache(1, 2, 64, [40], 16, [0])
+    c.table[0, 1] = 10 ** 6
+    start = c.clone()
+    q, k, v = new_rows(torch, 1, "f32", 70, 2, 2, 64)
+    cu, past = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 70], [0]))
+    qo, ko = raster_amd.pages_append(ctx, q, k, v, c.k, c.v, c.table, cu, past, 2, 2, 64, THETA, **c.scales())
+    lost = torch.zeros(70, dtype=torch.bool, device="cuda")
+    lost[16:32] = lost[48:] = True
+    assert bool(torch.isnan(qo[lost]).all()) and bool(torch.isnan(ko[lost]).all()) and bool(torch.isfinite(qo[~lost]).all())
+    wrote = [int(c.table[0, i]) for i in (0, 2)]
+    keep = [i for i in range(c.k.shape[0]) if i not in wrote]
+    assert torch.equal(c.k[keep], start.k[keep]) and bool(torch.isnan(c.ks[keep]).all())
+    assert bool(torch.isfinite(c.ks[wrote]).all())
+
+
+@pytest.mark.parametrize("cache", ["i8", "f32", "bf16"])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("nkv,hd,page,lens", [(8, 128, 16, [37, 0, 200, 1]), (1, 8, 16, [5]), (3, 40, 32, [33, 100, 0]),
+                                              (2, 256, 64, [130, 64])])
+def test_rows(torch, ctx, cache, out, nkv, hd, page, lens):
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] rows {cache}->{out} {nkv}x{hd} {lens}", flush=True)
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16}
+    c = q8_ref.Cache(sum(lens), nkv, hd, lens, page, lens, pad=1)
+    kp, vp, sc = c.k, c.v, c.scales()
+    if cache != "i8":
+        g = torch.Generator(device="cuda").manual_seed(1)
+        kp, vp = (torch.randn(c.k.shape, generator=g, device="cuda").to(dt[cache]) for _ in range(2))
+        sc = {}
+    first, n = 2, sum(lens)
+    cu = torch.tensor([first + sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device="cuda")
+    rows = first + n + 3
+    wide = torch.full((rows, 2 * nkv * hd + 8), 7.0, dtype=dt[out], device="cuda")
+    k, v = wide[:, :nkv * hd], wide[:, nkv * hd:2 * nkv * hd]
+    table = c.table.clone()
+    if len(lens) > 2:
+        table[2, 1] = -1
+    raster_amd.pages_rows(ctx, kp, vp, table, cu, rows, nkv, hd, k_out=k, v_out=v, **sc)
+    at = first
+    for b, m in enumerate(lens):
+        if m == 0:
+            continue
+        mine = c.table[b, :-(-m // page)].long()
+        for got, pages, which in ((k, kp, "k"), (v, vp, "v")):
+            if cache == "i8":  # code * scale rounded to f32, then to the rows' type
+                s = (c.ks if which == "k" else c.vs)[mine].repeat_interleave(16, 1).view(-1, nkv, 1)[:m]
+                want = (pages[mine].view(-1, nkv, hd)[:m].float() * s).reshape(m, -1).to(dt[out])
+            else:
+                want = pages[mine].reshape(-1, nkv * hd)[:m].to(dt[out])
+            if b == 2:
+                want[page:2 * page] = float("nan")
+            assert torch.equal(got[at:at + m].nan_to_num(9.0), want.nan_to_num(9.0))
+        at += m
+    assert bool((wide[:first] == 7).all()) and bool((wide[at:] == 7).all()) and bool((wide[:, 2 * nkv * hd:] == 7).all())
+    k2, v2 = raster_amd.pages_rows(ctx, kp, vp, c.table, cu - first, n, nkv, hd, dt[out], **sc)
+    assert k2.shape == (n, nkv * hd) and k2.dtype == dt[out] and v2.dtype == dt[out]
+
+
+@pytest.mark.parametrize("batch", [65, 300, 5000])
+def test_many_sequences(torch, ctx, batch):
+    """Appended and read back, most sequences of a few rows or none."""
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 {batch} sequences", flush=True)
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 3, (batch,), generator=gen)
+    lens[batch // 3] = 40
+    n = int(lens.sum())
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).int().cuda()
+    table = torch.randperm(4 * batch, generator=gen).int().view(batch, 4).cuda()
+    kp, vp = (torch.zeros((4 * batch, 16, 64), dtype=torch.int8, device="cuda") for _ in range(2))
+    sc = dict(kscales=torch.zeros((4 * batch, 1, 1), device="cuda"), vscales=torch.zeros((4 * batch, 1, 1), device="cuda"))
+    q, k, v = new_rows(torch, batch, "f32", n, 1, 1, 64)
+    past = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    qo, ko = raster_amd.pages_append(ctx, q, k, v, kp, vp, table, cu, past, 1, 1, 64, 0.0, **sc)
+    assert torch.equal(qo, q) and torch.equal(ko, k)
+    k2, v2 = raster_amd.pages_rows(ctx, kp, vp, table, cu, n, 1, 64, **sc)
+    owner = torch.repeat_interleave(torch.arange(batch), lens)
+    block = torch.arange(n) - cu.cpu()[owner]
+    block = owner * 4 + block // 16
+    for x, y in ((k, k2), (v, v2)):
+        top = torch.zeros(4 * batch).scatter_reduce(0, block, x.abs().amax(1).cpu(), "amax")[block]
+        assert bool(((x - y).abs().amax(1).cpu() <= top / 127 * 0.5001).all())  # half a step, and f32's roundings
+
+
+def test_graphs(torch, ctx):
+    """Append, attention and rows captured, replayed on another stream between eager work."""
+    import q8_ref
+    import raster_amd
+
+    nq, nkv, hd, lens = 8, 2, 128, [300, 2000]
+    print("[gpu] q8 graphs", flush=True)
+    c = q8_ref.Cache(8, nkv, hd, [n + 1 for n in lens], 16, lens)
+    q, k, v = new_rows(torch, 1, "bf16", 2, nq, nkv, hd)
+    pq, pk, pv = new_rows(torch, 2, "bf16", 50, nq, nkv, hd)
+    lt = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu, past = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 20, 50], [280, 1970]))
+    rows = torch.tensor([0, 300, 2300], dtype=torch.int32, device="cuda")
+
+    def call():
+        got = raster_amd.pages_append(ctx, pq, pk, pv, c.k, c.v, c.table, cu, past, nq, nkv, hd, THETA, **c.scales())
+        out = raster_amd.paged_attention(ctx, q, k, v, c.k, c.v, c.table, lt, nq, nkv, hd, THETA, hd ** -0.5,
+                                         max_len=2001, **c.scales())
+        return [*got, out, *raster_amd.pages_rows(ctx, c.k, c.v, c.table, rows, 2300, nkv, hd, **c.scales())]
+
+    call()
+    want = [x.clone() for x in call()]
+    torch.cuda.synchronize()
+    held, gr, s = c.clone(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(gr, stream=s):
+        outs = call()
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(other):
+            gr.replay()
+        torch.cuda.synchronize()
+        again = call()
+        torch.cuda.synchronize()
+        for x, y, z in zip(outs, want, again):
+            assert torch.equal(x, y) and torch.equal(z, y)
+        assert c.same(held)
+
+
+def test_offsets_past_32_bits(torch, ctx):
+    """Pages of 4.6 GiB of codes a plane, the last ones used."""
+    import raster_amd
+
+    print("[gpu] q8 offsets past 2^32", flush=True)
+    nq, nkv, hd, total, used = 8, 8, 128, 300000, 64
+    data = torch.empty((2, total, 16, nkv * hd), dtype=torch.int8, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(2)
+    small = torch.randint(-127, 128, (2, used, 16, nkv * hd), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+    ssmall = torch.rand((2, used, 1, nkv), generator=g, device="cuda") + 0.01
+    scales = torch.empty((2, total, 1, nkv), device="cuda")
+    data[:, total - used:], scales[:, total - used:] = small, ssmall
+    table = torch.randperm(used, generator=torch.Generator().manual_seed(3)).int().view(2, -1).cuda()
+    lens = torch.tensor([300, 511], dtype=torch.int32, device="cuda")
+    q, k, v = new_rows(torch, 3, "bf16", 2, nq, nkv, hd)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    outs = []
+    for pages, sc, first in ((small, ssmall, 0), (data, scales, total - used)):
+        s = dict(kscales=sc[0], vscales=sc[1])
+        got = [raster_amd.paged_attention(ctx, q, k, v, pages[0], pages[1], table + first, lens, nq, nkv, hd, THETA,
+                                          hd ** -0.5, **s)]
+        raster_amd.pages_append(ctx, q, k, v, pages[0], pages[1], table + first, cu, lens - 100, nq, nkv, hd, THETA, **s)
+        got += raster_amd.pages_rows(ctx, pages[0], pages[1], table + first, cu * 200, 400, nkv, hd, **s)
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert torch.equal(data[:, total - used:], small) and torch.equal(scales[:, total - used:], ssmall)
