@@ -60,6 +60,22 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
+// The codes of a tile in registers, as of here: otherwise the compiler takes them apart where they are loaded, where that
+// waits for the loads and needs four registers for one.
+template <typename V, int N>
+__device__ __forceinline__ void keep_whole(V (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if constexpr (sizeof(V) == 4) {
+      uint32_t w = x[i][0];
+      asm volatile("" : "+v"(w));
+      x[i][0] = w;
+    } else {
+      asm volatile("" : "+v"(x[i]));
+    }
+  }
+}
+
 // the bf16 values of 8 codes
 __device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t lo, uint32_t hi) {
   float f[8];
@@ -93,7 +109,7 @@ constexpr int q8_fixed_bytes(int hd) {
 // (one wave the keys, one the values), writes it back, and one wave attends it from there. No other
 // workgroup reads it, so none can see it half written.
 template <typename A, int HD, bool PART>
-__global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAttnArgs a) {
   constexpr int NT = sizeof(A) == 2 ? 2 : 3;
   constexpr int KT = HD == 256 ? 32 : 64, NB = KT / kBlock, STEP = KT * kWaves;
   constexpr int KP = HD / 64, E = HD / 16, VW = E / 4;  // 16-byte pieces of a K row a lane; codes and words of a V row
@@ -141,6 +157,13 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
     }
   }
   const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  // Page numbers: lane t holds that of block t of a tile, so one load brings them all. Those of the wave's first
+  // tile are asked for with the length where no window moves it.
+  const int r0 = split * a.split_rows, first = r0 + wave * KT, lane_t = min(lane & 7, NB - 1);
+  const int last_entry = max((int)p.table_stride - 1, 0);
+  const bool moved = a.window != INT32_MAX;
+  int pages = -1;
+  if (!moved && p.table_stride > 0) pages = trow[min((first + kBlock * lane_t) >> p.page_bits, last_entry)];
   const int len = a.lens[b];
   A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + hq0 * hd;
   const int64_t rows = (int64_t)len + (add || a.ahead);
@@ -156,20 +179,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
   const int nsplit = ranges_of(cr.walk, a.split_rows);
   if (split >= nsplit) return;
   const bool last = split == nsplit - 1;
-  const int r0 = split * a.split_rows, r1 = last ? cr.walk : r0 + a.split_rows;
-  const int first = r0 + wave * KT;
+  const int r1 = last ? cr.walk : r0 + a.split_rows;
   const int kvd = p.n_kv * hd;
   bool lost = false;  // a page number out of range
 
-  // the row in the pages of row r (a multiple of 16) of the sequence
-  auto page_row = [&](int r) -> int64_t {
-    const int page = trow[r >> p.page_bits];
-    const bool ok = (uint32_t)page < (uint64_t)p.pages;
-    lost |= !ok;
-    return ((int64_t)(ok ? page : 0) << p.page_bits) + (r & ((1 << p.page_bits) - 1));
-  };
-  auto scale_at = [&](int64_t row) -> int64_t {
-    return (row >> p.page_bits) * a.scale_stride + ((row & ((1 << p.page_bits) - 1)) >> 4) * p.n_kv + hkv;
+  const int in_page = (1 << p.page_bits) - 1;
+  auto ask_pages = [&](int r) { pages = trow[min(cr.row(r + kBlock * lane_t) >> p.page_bits, last_entry)]; };
+  auto scale_at = [&](int64_t page, int row) -> int64_t {
+    return page * a.scale_stride + ((row & in_page) >> 4) * p.n_kv + hkv;
   };
   const int8_t* kb = static_cast<const int8_t*>(p.kpages) + hkv * hd;
   const int8_t* vb = static_cast<const int8_t*>(p.vpages) + hkv * hd;
@@ -177,30 +194,37 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
   u32x4 xk[NB][KP];
   VRow xv[NB * 4];
   float sc = 0.0f;  // lane t < NB: scale of the keys of block t, lane 8 + t: of its values
-  int64_t base[NB];
-  auto set_base = [&](int r) {  // blocks past the range's end: its first one
+  int64_t base[NB];  // rows in the pages, in scalar registers: an address is a scalar and one offset of the lane
+  auto set_base = [&](int r) {  // of the tile whose pages are there; blocks past the range's end: the first again
+    const int n = min((r1 - r + kBlock - 1) / kBlock, NB);  // blocks of the tile
+    lost |= lane_t < n && (uint32_t)pages >= (uint64_t)p.pages;
+    if ((uint32_t)pages >= (uint64_t)p.pages) pages = 0;
 #pragma unroll
-    for (int t = 0; t < NB; t++) base[t] = page_row(cr.row(r + kBlock * t < r1 ? r + kBlock * t : r0));
+    for (int t = 0; t < NB; t++) {
+      const int u = t < n ? t : 0;
+      base[t] = ((int64_t)__builtin_amdgcn_readlane(pages, u) << p.page_bits) + (cr.row(r + kBlock * u) & in_page);
+    }
   };
-  auto load_scales = [&]() {
-    int64_t at = base[0];
-#pragma unroll
-    for (int t = 1; t < NB; t++) at = (lane & 7) == t ? base[t] : at;
-    return (lane & 8 ? a.vscales : a.kscales)[scale_at(at)];
+  auto load_scales = [&](int r) {
+    const int n = min((r1 - r + kBlock - 1) / kBlock, NB);
+    const int row = cr.row(r + (lane_t < n ? kBlock * lane_t : 0));
+    const int first_page = __builtin_amdgcn_readlane(pages, 0);
+    return (lane & 8 ? a.vscales : a.kscales)[scale_at(lane_t < n ? pages : first_page, row)];
   };
+  const uint32_t k_off = col * kvd + (PART ? 0 : 16 * g), v_off = 4 * g * kvd;
   auto load_k = [&]() {
 #pragma unroll
     for (int t = 0; t < NB; t++) {
-      const int8_t* kp = kb + (base[t] + col) * kvd;
+      const int8_t* kp = kb + base[t] * kvd;
 #pragma unroll
       for (int u = 0; u < KP; u++) {
-        const int d = 64 * u + 16 * g;
         if constexpr (PART) {  // (a row's elements end at a multiple of 8; those past it meet zeros of the queries)
-          const u32x2 lo = *reinterpret_cast<const u32x2*>(kp + min(d, hd - 8));
-          const u32x2 hi = *reinterpret_cast<const u32x2*>(kp + min(d + 8, hd - 8));
+          const int d = 64 * u + 16 * g;
+          const u32x2 lo = *reinterpret_cast<const u32x2*>(kp + (k_off + min(d, hd - 8)));
+          const u32x2 hi = *reinterpret_cast<const u32x2*>(kp + (k_off + min(d + 8, hd - 8)));
           xk[t][u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
         } else {
-          xk[t][u] = *reinterpret_cast<const u32x4*>(kp + d);
+          xk[t][u] = *reinterpret_cast<const u32x4*>(kp + 64 * u + k_off);
         }
       }
     }
@@ -210,22 +234,37 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
     for (int t = 0; t < NB; t++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int8_t* vp = vb + (base[t] + 4 * g + j) * kvd;
+        const int8_t* vp = vb + (base[t] + j) * kvd;
         if constexpr (PART && E > 8) {
-          const u32x2 lo = *reinterpret_cast<const u32x2*>(vp + min(E * col, hd - 8));
-          const u32x2 hi = *reinterpret_cast<const u32x2*>(vp + min(E * col + 8, hd - 8));
+          const u32x2 lo = *reinterpret_cast<const u32x2*>(vp + (v_off + min(E * col, hd - 8)));
+          const u32x2 hi = *reinterpret_cast<const u32x2*>(vp + (v_off + min(E * col + 8, hd - 8)));
           xv[4 * t + j][0] = lo[0], xv[4 * t + j][1] = lo[1];
           xv[4 * t + j][VW - 2] = hi[0], xv[4 * t + j][VW - 1] = hi[1];
         } else {  // (elements past the head's end form rows that nobody stores)
-          xv[4 * t + j] = *reinterpret_cast<const VRow*>(vp + (PART ? min(E * col, hd - E) : E * col));
+          xv[4 * t + j] = *reinterpret_cast<const VRow*>(vp + (v_off + (PART ? min(E * col, hd - E) : E * col)));
         }
       }
   };
+  // the new row's block, from LDS, as block 0 of a tile
+  auto take_tail_k = [&]() {
+#pragma unroll
+    for (int u = 0; u < KP; u++)
+      xk[0][u] = *reinterpret_cast<const u32x4*>(tail_k + (col * HD + 64 * u + 16 * g) / 4);
+    sc = tail_s[lane & 8 ? 1 : 0];
+  };
+  auto take_tail_v = [&]() {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int w = 0; w < VW; w++) xv[j][w] = tail_v[((4 * g + j) * HD + E * col) / 4 + w];
+  };
   if (first < r1) {
+    if (moved) ask_pages(first);
     set_base(first);
     load_k();
-    sc = load_scales();
+    sc = load_scales(first);
     load_v();
+    ask_pages(first + STEP);
   }
 
   // the rotated queries as operands (zeros for heads and elements past the end)
@@ -252,10 +291,12 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
     }
   }
   if (add && last && wave < 2) {  // the new row's block
-    const bool store = (uint32_t)trow[tail_row >> p.page_bits] < (uint64_t)p.pages;
-    const int64_t at = page_row(tail_row);
+    const int page = trow[tail_row >> p.page_bits];
+    const bool store = (uint32_t)page < (uint64_t)p.pages;
+    lost |= !store;
+    const int64_t at = ((int64_t)(store ? page : 0) << p.page_bits) + (tail_row & in_page);
     int8_t* codes = static_cast<int8_t*>(wave == 0 ? p.kpages : p.vpages) + at * kvd + hkv * hd;
-    float* scale = (wave == 0 ? a.kscales : a.vscales) + scale_at(at);
+    float* scale = (wave == 0 ? a.kscales : a.vscales) + scale_at(store ? page : 0, tail_row);
     uint32_t* tail = wave == 0 ? tail_k : tail_v;
     const int words = hd / 4;
     uint32_t w[HD / 16];
@@ -312,9 +353,30 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
 #pragma unroll
   for (int t = 0; t < E; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
-  // The tile in xk and xv: of its rows those of block t count that are row `at[t]` of the sequence and on, before
-  // `end`, and seen. `after_k` is called when xk is free.
-  auto attend = [&](const int (&at)[NB], int end, const float (&ks)[NB], const float (&vs)[NB], auto after_k) {
+  // the wave's tiles, at the end the new row's block by the wave whose turn it is
+  int r = first;
+  const bool has_tail = add && last && wave == ((r1 - r0 + KT - 1) / KT) % kWaves;
+  bool tail = first >= r1;
+  if (tail && has_tail) {
+    take_tail_k();
+    take_tail_v();
+  }
+  for (bool go = !tail || has_tail; go;) {
+    const bool more = !tail && r + STEP < r1, then_tail = !tail && !more && has_tail;
+    // rows of block t count that are row at[t] of the sequence and on, before `end`, and seen
+    const int end = tail ? len + 1 : cr.row(r1 - 1) + 1;
+    int at[NB];
+    float ks[NB], vs[NB];
+#pragma unroll
+    for (int t = 0; t < NB; t++) {
+      at[t] = tail ? (t == 0 ? tail_row : INT32_MAX - kBlock)
+                   : r + kBlock * t < r1 ? cr.row(r + kBlock * t) : INT32_MAX - kBlock;
+      ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), t));
+      vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), 8 + t));
+    }
+    if (more) set_base(r + STEP);
+#pragma unroll
+    for (int t = 0; t < NB; t++) keep_whole(xk[t]);
     f32x4 d[NB] = {};
     int ql = lane;  // read anew for every tile: kept in registers they would cost a wave a SIMD
     asm volatile("" : "+v"(ql));
@@ -326,15 +388,23 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
         u32x4 qw[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) qw[n] = qp[(n * QS + 2 * u + h) * 64];
+        bf16x8 kf[NB];
 #pragma unroll
-        for (int t = 0; t < NB; t++) {
-          const bf16x8 kf = bf16_of_codes(xk[t][u][2 * h], xk[t][u][2 * h + 1]);
+        for (int t = 0; t < NB; t++) kf[t] = bf16_of_codes(xk[t][u][2 * h], xk[t][u][2 * h + 1]);
 #pragma unroll
-          for (int n = 0; n < NT; n++)
-            d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
-        }
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int t = 0; t < NB; t++)
+            d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);  // (left alone, the conversions of all steps come first and do not fit)
       }
-    after_k();
+    if (more) {
+      load_k();
+      sc = load_scales(r + STEP);
+      ask_pages(r + 2 * STEP);
+    } else if (then_tail) {
+      take_tail_k();
+    }
     float s[NB][4];
     uint32_t hidden[NB];  // bit i: row 4 g + i of the block
     bool cut = false;
@@ -375,6 +445,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
       }
 #pragma unroll
     for (int t = 0; t < E; t++) acc[t] *= alpha;
+    keep_whole(xv);
 #pragma unroll
     for (int t = 0; t < NB; t += 2) {  // 32 rows a product
       bf16x8 pb[NT];
@@ -389,57 +460,33 @@ __global__ __launch_bounds__(kThreads) void paged_attention_q8_kernel(PagedAttnA
         for (int n = 0; n < NT; n++) pb[n][j] = x[n];
       }
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        float f[8];
+      for (int e = 0; e < E; e += 4) {  // four elements, one word of the rows
+        bf16x8 vf[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = (float)(int8_t)(xv[4 * t + j][e >> 2] >> (8 * (e & 3)));
-        u32x4 y;
+        for (int i = 0; i < 4; i++) {
+          float f[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = high16_pair(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
+          for (int j = 0; j < 8; j++) f[j] = (float)(int8_t)(xv[4 * t + j][e >> 2] >> (8 * i));
+          u32x4 y;
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[j] = high16_pair(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
+          vf[i] = __builtin_bit_cast(bf16x8, y);
+        }
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, y), pb[n], acc[e], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            acc[e + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pb[n], acc[e + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-  };
-  const int end = cr.row(r1 - 1) + 1;  // (of a range without rows, not used)
-  for (int r = first; r < r1; r += STEP) {
-    const bool more = r + STEP < r1;
-    int at[NB];
-    float ks[NB], vs[NB];
-#pragma unroll
-    for (int t = 0; t < NB; t++) {
-      at[t] = r + kBlock * t < r1 ? cr.row(r + kBlock * t) : INT32_MAX - kBlock;
-      ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), t));
-      vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), 8 + t));
-    }
-    if (more) set_base(r + STEP);
-    attend(at, end, ks, vs, [&]() {
-      if (more) {
-        load_k();
-        sc = load_scales();
-      }
-    });
-    if (more) load_v();
-  }
-  // the new row's block, by the wave whose turn it is
-  if (add && last && wave == ((r1 - r0 + KT - 1) / KT) % kWaves) {
-    int at[NB];
-    float ks[NB], vs[NB];
-#pragma unroll
-    for (int t = 0; t < NB; t++) {
-      at[t] = t == 0 ? tail_row : INT32_MAX - kBlock;
-      ks[t] = t == 0 ? tail_s[0] : 0.0f;
-      vs[t] = t == 0 ? tail_s[1] : 0.0f;
-#pragma unroll
-      for (int u = 0; u < KP; u++)
-        xk[t][u] = t == 0 ? *reinterpret_cast<const u32x4*>(tail_k + (col * HD + 64 * u + 16 * g) / 4) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int w = 0; w < VW; w++) xv[4 * t + j][w] = t == 0 ? tail_v[((4 * g + j) * HD + E * col) / 4 + w] : 0;
-    }
-    attend(at, len + 1, ks, vs, []() {});
+    if (more)
+      load_v();
+    else if (then_tail)
+      take_tail_v();
+    go = more || then_tail;
+    tail = then_tail;
+    r += STEP;
   }
 
   // the waves' states
