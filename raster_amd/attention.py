@@ -173,13 +173,16 @@ def _scales(ctx, pg, kscales, vscales) -> tuple:
     if pg.dtype != RQ_I8:
         _need(kscales is None and vscales is None, "kscales and vscales are for int8 pages")
         return None, None, 0
-    shape, out = (pg.pages, pg.page_size // 16, pg.n_kv), []
+    pages, blocks, heads = shape = pg.pages, pg.page_size // 16, pg.n_kv
+    f32, dev, out = _t().float32, ctx.device, []
     for t in (kscales, vscales):
-        if (t is None or t.dtype != _t().float32 or t.get_device() != ctx.device or t.shape != shape
-                or not t[0].is_contiguous()):
-            raise ValueError(f"int8 pages need kscales and vscales, f32 CUDA tensors {list(shape)} of the context's "
-                             "device, a page's scales side by side")
-        out.append(t.stride(0) if shape[0] > 1 else max(t.stride(0), shape[1] * shape[2]))
+        if t is not None and t.dtype == f32 and t.get_device() == dev and t.shape == shape:
+            s0, s1, s2 = t.stride()  # (of a dimension of one, anything)
+            if (s2 == 1 or heads == 1) and (s1 == heads or blocks == 1):
+                out.append(s0 if pages > 1 else max(s0, blocks * heads))
+                continue
+        raise ValueError(f"int8 pages need kscales and vscales, f32 CUDA tensors {list(shape)} of the context's device, "
+                         "a page's scales side by side")
     _need(out[0] == out[1], "kscales and vscales must have one stride from page to page")
     return kscales.data_ptr(), vscales.data_ptr(), out[0]
 

@@ -25,6 +25,11 @@ struct PromptArgs {
   float* delta;  // [n_q][rows_q]: dout . out
   float* part;   // [nsplit][dv, dk][rows_k][n_kv * head_dim] when nsplit > 1
   int nsplit;
+  // With sink_tiles > 0 the gradients of every sequence's first sink_tiles tiles of 64 keys are summed by chunks of
+  // sink_chunk queries: sink_part [sink_slots][sink_tiles][n_kv][dv, dk][64][head_dim]
+  int sink_tiles, sink_chunk;
+  int64_t sink_slots;
+  float* sink_part;
 };
 
 // With a window (WIN) the query at position i of its sequence sees the keys j <= i with i - j < window or
@@ -77,9 +82,9 @@ __device__ __forceinline__ bool window_all(const PromptArgs& a, int pos, int key
 }
 
 struct PromptBwdPlan {
-  int nsplit;
-  int64_t groups;  // of the largest launch
-  size_t delta_bytes, work;
+  int nsplit, sink_tiles, sink_chunk;
+  int64_t groups, sink_slots;  // groups: of the largest launch
+  size_t delta_bytes, part_bytes, work;
 };
 PromptBwdPlan plan_prompt_bwd(const PromptArgs& a);  // of its sizes
 

@@ -286,3 +286,37 @@ def test_rows_of_no_sequence_and_graphs(torch, ctx):
             gr.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip((out, lse, *grads), want))
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,lens,window,sinks", [
+    ("bf16", 16, 8, 64, [2100, 3, 1300, 0, 777], 100, 4),
+    ("bf16", 8, 8, 128, [2500, 900], 256, 130),   # three tiles of sinks, the second sequence's window among them
+    ("bf16", 8, 8, 200, [2600, 640], 300, 1),
+    ("f32", 16, 8, 64, [2100, 30, 1500], 64, 64),
+    ("f32", 8, 8, 104, [3000, 200], 70, 500),
+    ("f32", 8, 8, 136, [3000, 100], 1, 2),
+])
+def test_gradient_of_sinks_by_chunks(torch, ctx, t, nq, nkv, hd, lens, window, sinks):
+    """Grids thick enough that the first keys' gradients are summed by chunks of queries (the call asks for room for
+    them); queries that are the end of longer sequences; the same bits on every run."""
+    import raster_amd
+
+    print(f"[gpu] window sinks by chunks {t} {nq}/{nkv}x{hd} {lens} {window}+{sinks}", flush=True)
+    for lk in (lens, [n + 37 if n else 50 for n in lens]):
+        def room(z):
+            p = _lib.Prompt({"f32": _lib.RQ_F32, "bf16": _lib.RQ_BF16}[t], len(lens), sum(lens), sum(lk), nq, nkv, hd,
+                            0x10000, 0x10000, 1, 0.125)
+            n = C.c_size_t()
+            _lib.call("rq_prompt_attention_window_bwd_work", C.byref(p), window, z, C.byref(n))
+            return n.value
+
+        assert room(sinks) > room(0)
+        q, k, v, do = data(torch, t, nq, nkv, hd, lens, lk, sum(lens))
+        cu, cu_k, scale = cu_of(torch, lens), None if lens == lk else cu_of(torch, lk), hd ** -0.5
+        lse = torch.empty((nq, sum(lens)), device="cuda")
+        see = dict(window=window, sinks=sinks, cu_k=cu_k)
+        out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse, **see)
+        grads = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, **see)
+        check_gradient(torch, q, k, v, do, grads, lens, lk, nq, nkv, hd, scale, window, sinks)
+        again = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, **see)
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
