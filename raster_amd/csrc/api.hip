@@ -1579,11 +1579,6 @@ struct CacheWindow {
   }
 };
 
-static PagedPlan paged_plan(int cache_dtype, int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim,
-                            int64_t max_len, const CacheWindow& w, int cu_count) {
-  return plan_paged_attention(batch, n_q, n_kv, head_dim, walked_rows(max_len, w.window, w.sinks), cu_count);
-}
-
 // Sequences, heads and rows of a paged attention call. What passes keeps max_len times the groups, and the
 // bytes of their records, within 64 bits.
 static int check_paged_size(int64_t batch, int64_t n_q, int64_t n_kv, int64_t max_len) {
@@ -1791,10 +1786,11 @@ int rq_paged_attention_window_work(rq_ctx h, int cache_dtype, int64_t batch, int
   if (int s = check_paged_size(batch, n_q, n_kv, max_len)) return s;
   if (!bytes) return fail(RQ_ERR_NULL, "bytes is NULL");
   if (int s = check_ctx(c)) return s;
-  *bytes = batch == 0 ? 0
-                      : paged_plan(cache_dtype, batch, n_q, n_kv, head_dim, max_len,
-                                   CacheWindow(max_len, window, sinks), c->cu_count)
-                            .work;
+  const CacheWindow seen(max_len, window, sinks);
+  const int64_t walked = walked_rows(max_len, seen.window, seen.sinks);
+  *bytes = batch == 0             ? 0
+           : cache_dtype == RQ_I8 ? plan_paged_attention_q8(batch, n_q, n_kv, head_dim, walked, c->cu_count).work
+                                  : plan_paged_attention(batch, n_q, n_kv, head_dim, walked, c->cu_count).work;
   return RQ_OK;
 }
 
@@ -1830,12 +1826,20 @@ int rq_paged_attention_window(rq_ctx h, const rq_pages* pg, float* kscales, floa
   if (int s = check_rows("out", out, out_stride, qw, dtype)) return s;
   if (int s = check_ctx(c)) return s;
   const CacheWindow seen(max_len, window, sinks);
-  const PagedPlan plan = paged_plan(pg->dtype, batch, n_q, pg->n_kv, pg->head_dim, max_len, seen, c->cu_count);
-  if (plan.work > 0 && !work) return fail(RQ_ERR_NULL, "work is NULL");
-  if (work_bytes < plan.work) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
+  const int64_t walked = walked_rows(max_len, seen.window, seen.sinks);
+  const bool i8 = pg->dtype == RQ_I8;
+  PagedPlan plan = {};
+  PagedQ8Plan plan8 = {};
+  if (i8)
+    plan8 = plan_paged_attention_q8(batch, n_q, pg->n_kv, pg->head_dim, walked, c->cu_count);
+  else
+    plan = plan_paged_attention(batch, n_q, pg->n_kv, pg->head_dim, walked, c->cu_count);
+  const size_t need = i8 ? plan8.work : plan.work;
+  if (need > 0 && !work) return fail(RQ_ERR_NULL, "work is NULL");
+  if (work_bytes < need) return fail(RQ_ERR_SHAPE, "work is smaller than rq_paged_attention_work says");
   if (((uintptr_t)work & 15) != 0) return fail(RQ_ERR_SHAPE, "work must be 16-byte aligned");
   const int64_t htiles = (n_q / pg->n_kv + 15) / 16;
-  if (plan.nsplit > kMaxGroups / (batch * pg->n_kv * htiles))
+  if (i8 ? plan8.groups > kMaxGroups : plan.nsplit > kMaxGroups / (batch * pg->n_kv * htiles))
     return fail(RQ_ERR_SHAPE, "batch times heads times rows too large for one launch");
   if (int s = set_device(c)) return s;
   PagedAttnArgs a = {};
@@ -1846,15 +1850,15 @@ int rq_paged_attention_window(rq_ctx h, const rq_pages* pg, float* kscales, floa
   a.max_len = max_len;
   a.window = seen.window;
   a.sinks = seen.sinks;
-  a.i8 = pg->dtype == RQ_I8;
   a.kscales = kscales, a.vscales = vscales, a.scale_stride = scale_stride;
   a.scale2 = (float)(scale * 1.4426950408889634);
   a.out = out;
   a.out_stride = out_stride;
-  a.split_rows = plan.split_rows;
+  a.split_rows = i8 ? plan8.split_rows : plan.split_rows;
   a.nsplit = plan.nsplit;
+  a.spare = plan8.spare, a.range_rows = plan8.range_rows, a.kv_heads = plan8.kv_heads;
   a.part = static_cast<float*>(work);
-  const hipError_t e = a.i8 ? launch_paged_attention_q8(dtype, a, (hipStream_t)stream)
+  const hipError_t e = i8 ? launch_paged_attention_q8(dtype, a, (hipStream_t)stream)
                             : launch_paged_attention(dtype, pg->dtype, a, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return RQ_OK;

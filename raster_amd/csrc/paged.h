@@ -31,8 +31,10 @@ struct PagedAttnArgs {
   int64_t out_stride;
   int split_rows, nsplit;  // cached rows of a workgroup, and ranges at max_len
   float* part;             // records of the ranges when nsplit > 1
-  // int8 pages: the scale of rows 16 i .. 16 i + 15 of a page and of a KV head is scales[page * scale_stride + i * n_kv + head]
-  int i8, ahead;  // ahead: the new row is in the pages already (and k is NULL)
+  // int8 pages: `spare` ranges more than there are sequences (0: a range a sequence), each of a multiple of split_rows rows,
+  // or, of a single sequence, of range_rows.
+  // The scale of rows 16 i .. 16 i + 15 of a page and of a KV head is scales[page * scale_stride + i * n_kv + head]
+  int spare, range_rows, kv_heads, ahead;  // kv_heads: of a workgroup; ahead: the new row is in the pages already (and k is NULL)
   float *kscales, *vscales;
   int64_t scale_stride;
 };
@@ -68,6 +70,14 @@ struct PagedPlan {
 // max_len: rows that are walked over (walked_rows)
 PagedPlan plan_paged_attention(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
                                int cu_count);
+// The same for int8 pages, whose rows a range the kernel takes from the real lengths.
+struct PagedQ8Plan {
+  int split_rows, spare, range_rows, kv_heads;
+  int64_t groups;  // workgroups of the largest launch
+  size_t work;
+};
+PagedQ8Plan plan_paged_attention_q8(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
+                                    int cu_count);
 // of max_len rows those that a query with a window walks over, whole blocks of 16 at both ends
 inline int64_t walked_rows(int64_t max_len, int64_t window, int64_t sinks) {
   return window > 0 ? std::min<int64_t>(max_len, (sinks + 15) / 16 * 16 + window + 16) : max_len;
@@ -77,7 +87,6 @@ hipError_t launch_paged_attention(int dtype, int cache_dtype, const PagedAttnArg
 hipError_t launch_pages_append(int dtype, int cache_dtype, const PagesAppendArgs& a, hipStream_t stream);
 // over int8 pages
 hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStream_t stream);
-hipError_t launch_paged_merge(int dtype, const PagedAttnArgs& a, hipStream_t stream);  // with a window
 hipError_t launch_pages_append_q8(int dtype, const PagesAppendArgs& a, hipStream_t stream);
 int64_t append_q8_slots(const PagesAppendArgs& a);  // of blocks: its workgroups, or a few times as many when they are few
 hipError_t launch_pages_rows(int dtype, int cache_dtype, const PagesRowsArgs& a, hipStream_t stream);

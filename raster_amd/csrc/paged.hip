@@ -403,10 +403,10 @@ template <typename A, bool WIN>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const PagesArgs& p = a.p;
   const int hq = blockIdx.x % p.n_q, b = blockIdx.x / p.n_q, hd = p.head_dim, len = a.lens[b];
-  const int64_t rows = (int64_t)len + (p.k != nullptr || a.ahead);
+  const int64_t rows = (int64_t)len + (p.k != nullptr);
   if (len < 0 || rows > a.max_len || rows > p.table_stride << p.page_bits) return;
   CachedRows<WIN> cr;
-  cr.init(a, a.i8 && p.k != nullptr ? len & ~15 : len + a.ahead, rows);
+  cr.init(a, len, rows);
   const int n = ranges_of(cr.walk, a.split_rows);
   if (n <= 1) return;
   __shared__ float red[4];
@@ -574,12 +574,6 @@ PagedPlan plan_paged_attention(int64_t batch, int64_t n_q, int64_t n_kv, int64_t
 
 namespace {
 
-template <typename A, bool WIN>
-hipError_t run_merge(const PagedAttnArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_merge_kernel<A, WIN>), dim3((unsigned)(a.p.batch * a.p.n_q)), dim3(256), 0, stream, a);
-  return hipGetLastError();
-}
-
 template <typename A, typename C, int HD, bool PART, bool WIN>
 hipError_t run_paged(const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
@@ -593,7 +587,11 @@ hipError_t run_paged(const PagedAttnArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)(a.nsplit * p.batch * p.n_kv * htiles)), dim3(kPagedThreads), lds, stream,
                      a);
   if (hipError_t e = hipGetLastError()) return e;
-  return a.nsplit > 1 ? run_merge<A, WIN>(a, stream) : hipSuccess;
+  if (a.nsplit > 1) {
+    hipLaunchKernelGGL((paged_merge_kernel<A, WIN>), dim3((unsigned)(p.batch * p.n_q)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
+  return hipSuccess;
 }
 
 template <typename A, typename C, bool WIN>
@@ -626,10 +624,6 @@ static hipError_t launch_paged(int dtype, int cache_dtype, const PagedAttnArgs& 
 hipError_t launch_paged_attention(int dtype, int cache_dtype, const PagedAttnArgs& a, hipStream_t stream) {
   return a.window > 0 ? launch_paged<true>(dtype, cache_dtype, a, stream)
                       : launch_paged<false>(dtype, cache_dtype, a, stream);
-}
-
-hipError_t launch_paged_merge(int dtype, const PagedAttnArgs& a, hipStream_t stream) {
-  return dtype == RQ_F32 ? run_merge<float, true>(a, stream) : run_merge<__bf16, true>(a, stream);
 }
 
 hipError_t launch_pages_append(int dtype, int cache_dtype, const PagesAppendArgs& a, hipStream_t stream) {

@@ -21,7 +21,7 @@ namespace rq {
 namespace {
 
 constexpr int kBlock = 16;
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256, kWaves = 4, kTileRows = 64;
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
 
@@ -60,8 +60,10 @@ __device__ __forceinline__ float wave_max(float x) {
   return x;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 // The codes of a tile in registers, as of here: otherwise the compiler takes them apart where they are loaded, where that
-// waits for the loads and needs four registers for one.
+// waits for the loads and needs several registers for one.
 template <typename V, int N>
 __device__ __forceinline__ void keep_whole(V (&x)[N]) {
 #pragma unroll
@@ -76,122 +78,242 @@ __device__ __forceinline__ void keep_whole(V (&x)[N]) {
   }
 }
 
-// the bf16 values of 8 codes
-__device__ __forceinline__ bf16x8 bf16_of_codes(uint32_t lo, uint32_t hi) {
-  float f[8];
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    f[j] = (float)(int8_t)(lo >> (8 * j));
-    f[4 + j] = (float)(int8_t)(hi >> (8 * j));
+// A number in NT signed digits of 8 bits, as an operand of the int8 products beside the codes: x = sum_n digit n * 256^n,
+// for |x| up to kDigitsMax<NT>. Queries are written so relative to a head's largest element, weights relative to their
+// tile's largest, so f32 calls lose 2^-24 of that (NT = 3), bf16 ones 2^-16 (NT = 2); sums over products are exact.
+template <int NT>
+constexpr int kDigitsMax = NT == 2 ? 0x7F7E : 0x7F7F7C;
+// the digits in the bytes of a word, from byte 0 on
+template <int NT>
+__device__ __forceinline__ uint32_t digits_of(int x) {
+  constexpr uint32_t kBias = NT == 2 ? 0x8080u : 0x808080u;
+  return ((uint32_t)x + kBias) ^ kBias;
+}
+// Digit n of four such words to word n
+template <int NT>
+__device__ __forceinline__ void pack_digits(const uint32_t (&x)[4], uint32_t (&d)[NT]) {
+  const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400);
+  d[0] = low16_pair(a, b);
+  d[1] = high16_pair(a, b);
+  if constexpr (NT == 3)
+    d[2] = low16_pair(__builtin_amdgcn_perm(x[1], x[0], 0x07030602), __builtin_amdgcn_perm(x[3], x[2], 0x07030602));
+}
+// Sum of digit products to their value
+__device__ __forceinline__ float value_of(int d0, int d1) { return (float)((d1 << 8) + d0); }
+__device__ __forceinline__ float value_of(int d0, int d1, int d2) {
+  return fmaf((float)((d2 << 8) + d1), 256.0f, (float)d0);
+}
+// The factor that takes numbers up to `most` to digits, not past f32's range. (By the hardware's reciprocal, to one
+// unit in the last place: an inverse of the same kind takes them back. The largest digit has room for it.)
+template <int NT>
+__device__ __forceinline__ float digit_factor(float most) {
+  return most > 0.0f ? fminf((float)kDigitsMax<NT> * __builtin_amdgcn_rcpf(most), 1e38f) : 0.0f;
+}
+
+// Ranges of rows, by the real lengths. Sequence b's walked rows are cut into ranges of R rows, one at least, and the
+// ranges of all sequences numbered in order: R so that there are no more than a sequence each and `spare` more. So the
+// grid needs no lengths, few of its workgroups find nothing to do, and those of a batch have about equally much. A single
+// sequence's R is the call's, so that nothing waits for its length.
+struct Range {
+  int b, at, count, first, rows;  // sequence, which of its ranges, how many (0: not known yet) and the number of the first; R
+};
+__device__ __forceinline__ int ranges_of_walk(int walk, int rows) {
+  return max(1, (int)((uint32_t)(walk + rows - 1) / (uint32_t)rows));
+}
+// walked rows of a sequence: those of the new row's block are not among them
+__device__ __forceinline__ int walked_of(const PagedAttnArgs& a, int len) {
+  const bool add = a.p.k != nullptr;
+  const int64_t rows = (int64_t)len + (add || a.ahead);
+  if (len < 0 || rows > a.max_len || rows > a.p.table_stride << a.p.page_bits) return 0;
+  CachedRows<true> cr;
+  cr.init(a, add ? len & ~(kBlock - 1) : (int)rows, rows);
+  return cr.walk;
+}
+// sums over the lanes up to each one
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t x) {
+#define RQ_SCAN_STEP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+  RQ_SCAN_STEP(0x111, 0xf);  // within 16 lanes: 1, 2, 4 and 8 before
+  RQ_SCAN_STEP(0x112, 0xf);
+  RQ_SCAN_STEP(0x114, 0xf);
+  RQ_SCAN_STEP(0x118, 0xf);
+  RQ_SCAN_STEP(0x142, 0xa);  // the last lane of the 16 before
+  RQ_SCAN_STEP(0x143, 0xc);  // and of the 32 before
+#undef RQ_SCAN_STEP
+  return x;
+}
+// By a whole wave: the range of number `number`, or the first of sequence -1 - number. b = -1: there is none.
+constexpr int kPlanned = 1024;  // sequences of a launch
+__device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int number) {
+  if (a.spare == 0) return {number < 0 ? -1 - number : number, 0, 1, number < 0 ? -1 - number : number, INT32_MAX};
+  if (a.range_rows > 0) return {0, max(number, 0), 0, 0, a.range_rows};
+  const int lane = threadIdx.x & 63, batch = a.p.batch, per = (batch + 63) / 64, b0 = lane * per;
+  const int b1 = min(b0 + per, batch);
+  // in units of a block (at most 2^26 a sequence, 2^30 for the first 16 of a lane), rounded up: 38 bits in all
+  int one = 0;  // of a lane's only sequence
+  uint32_t sum = 0;
+  for (int b = b0; b < b1; b++) {
+    one = walked_of(a, a.lens[b]);
+    sum += (uint32_t)(one + kBlock - 1) / kBlock;
   }
-  u32x4 y;
-#pragma unroll
-  for (int j = 0; j < 4; j++) y[j] = high16_pair(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
-  return __builtin_bit_cast(bf16x8, y);
+  const uint32_t high = scan_lanes(sum >> 16), low = scan_lanes(sum & 0xffff);  // 22 bits each and 6 more
+  const uint64_t blocks = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(high, 63) << 16) +
+                          (uint32_t)__builtin_amdgcn_readlane(low, 63);
+  // R spare >= all rows, up to a multiple of split_rows
+  const int shift = blocks >> 32 ? 8 : 0;
+  const uint64_t least = ((uint64_t)((uint32_t)(blocks >> shift) / (uint32_t)a.spare) + 1) << shift;
+  const uint32_t unit = a.split_rows / kBlock;
+  const int rows = (int)(((uint32_t)min(least, (uint64_t)1 << 26) + unit - 1) / unit * unit * kBlock);
+  auto walk_of = [&](int b) { return per == 1 ? one : walked_of(a, a.lens[b]); };
+  int mine = 0;
+  for (int b = b0; b < b1; b++) mine += ranges_of_walk(walk_of(b), rows);
+  Range r{-1, 0, 0, 0, rows};
+  int first = (int)scan_lanes(mine) - mine;
+  for (int b = b0; b < b1; b++) {
+    const int n = ranges_of_walk(walk_of(b), rows);
+    if (number < 0 ? b == -1 - number : number >= first && number < first + n) {
+      r.b = b;
+      r.at = number < 0 ? 0 : number - first;
+      r.count = n;
+      r.first = first;
+    }
+    first += n;
+  }
+  const uint64_t found = __builtin_amdgcn_ballot_w64(r.b >= 0);
+  if (found == 0) return r;
+  const int src = __builtin_ctzll(found);
+  r.b = __builtin_amdgcn_readlane(r.b, src);
+  r.at = __builtin_amdgcn_readlane(r.at, src);
+  r.count = __builtin_amdgcn_readlane(r.count, src);
+  r.first = __builtin_amdgcn_readlane(r.first, src);
+  return r;
 }
 
-// LDS: queries as fragments of NT bf16 terms, the block that the new row goes into (keys, values), its scales
-template <typename A>
-constexpr int q8_fixed_bytes(int hd) {
-  return 16 * hd * 2 * (sizeof(A) == 2 ? 2 : 3) + 2 * kBlock * hd + (kWaves * 32 + 4) * 4;
+// LDS: the digits of HW KV heads' queries, the blocks that the new row goes into (keys, values), the waves' maxima and
+// sums, the queries' maxima and factors, the blocks' scales
+template <typename A, int HD, int HW>
+constexpr int q8_fixed_bytes() {
+  return HW * (16 * HD * (sizeof(A) == 2 ? 2 : 3) + 2 * kBlock * HD + 2 * 16 * 4) + (kWaves * 32 + 8) * 4;
 }
 
-// One workgroup: up to 16 query heads of a KV head, one range of a sequence's cached rows; its waves take tiles
-// of KT rows in turn. As in the kernel over f32 and bf16 pages: S^T = K Q^T with keys in the rows of a 16x16 MFMA and heads in its
-// columns, the weights the B operand of O^T += V^T P^T as they lie. Codes are exact in bf16 and are made bf16 in
-// registers; a block's scale is one factor of its 16 scores and of its 16 weights, so the queries (NT
-// bf16 terms) and the weights (NT terms) carry all the rounding that there is.
-// Of K a lane reads 16 codes of its row, which are the operands of two MFMAs: slots 8 g .. 8 g + 7 of step
-// 2 u + p hold the elements 64 u + 16 g + 8 p and on, in the queries too. Of V it reads E = HD / 16 neighbouring
-// codes of the rows of its group.
+// One workgroup: up to 16 query heads of each of HW KV heads, one range of a sequence's cached rows. kWaves / HW
+// waves share a KV head and take tiles of 64 of its rows in turn (32 past 128 elements, for the registers). S^T = K Q^T with keys in the rows of a 16x16x64 int8 MFMA
+// and heads in its columns: the 16 codes that a lane reads of its row are an operand as they lie, the queries' digits
+// the other. A lane's 16 scores of a column, 4 g + i of block t, are its weights, whose digits in slot 4 t + i are an
+// operand of O^T += V^T P^T as they lie; of V a lane reads E = HD / 16 neighbouring codes of the rows 4 g + i and
+// turns 4 rows x 4 codes in registers (8 byte permutations). A block's scale is one factor of its scores and of its weights.
+// Row i of result tile e is element E i + e. Each tile's weighted values are whole numbers, added to the f32 sums with the
+// factor of their weights. (Codes made bf16 for bf16 products: twice the instructions, 32 sequences of 0 to 8191 rows 56 us, now @@B@@.)
 //
-// The block that the new row goes into is not walked over: the workgroup of the last range forms it anew in LDS
-// (one wave the keys, one the values), writes it back, and one wave attends it from there. No other
+// With many rows, HW = 4: the workgroup reads whole pieces of 512 bytes and more of a row at a time, where with HW = 1
+// each KV head's 128 bytes are read by other compute units at other times: 8 sequences of 33 to 65 Ki rows 4.1 against 5.3 TB/s
+// with the loads alone. With few, HW = 1: more waves at a sequence, each with less to walk.
+//
+// The block that the new row goes into is not walked over: the workgroup of the last range forms it anew in LDS,
+// writes it back, and one wave attends it from there. No other
 // workgroup reads it, so none can see it half written.
-template <typename A, int HD, bool PART>
+template <typename A, int HD, bool PART, int HW>
 __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAttnArgs a) {
   constexpr int NT = sizeof(A) == 2 ? 2 : 3;
-  constexpr int KT = HD == 256 ? 32 : 64, NB = KT / kBlock, STEP = KT * kWaves;
+  constexpr int NB = HD == 256 ? 2 : 4, KT = NB * kBlock, RW = kWaves / HW, STEP = KT * RW;
   constexpr int KP = HD / 64, E = HD / 16, VW = E / 4;  // 16-byte pieces of a K row a lane; codes and words of a V row
-  constexpr int QS = HD / 32;                           // steps of 32 elements
+  constexpr int kQuery = 16 * HD * NT;                  // bytes of a KV head's queries
   extern __shared__ __attribute__((aligned(16))) float sm[];
   const PagesArgs& p = a.p;
   const int hd = p.head_dim, half = hd / 2, group = p.n_q / p.n_kv, htiles = (group + 15) / 16, nh = min(group, 16);
-  uint32_t* tail_k = reinterpret_cast<uint32_t*>(sm + 16 * HD * 2 * NT / 4);  // [16][HD] codes
-  uint32_t* tail_v = tail_k + kBlock * HD / 4;
-  float* wm = reinterpret_cast<float*>(tail_v + kBlock * HD / 4);  // [waves][16]
+  uint32_t* tails = reinterpret_cast<uint32_t*>(sm + HW * kQuery / 4);  // [HW][keys, values][16][HD] codes
+  float* wm = reinterpret_cast<float*>(tails + HW * 2 * kBlock * HD / 4);  // [waves][16]
   float* wl = wm + kWaves * 16;
-  float* tail_s = wl + kWaves * 16;  // its scales
-  float* wacc = tail_s + 4;          // [waves][heads][HD]; before that cos and sin [2][HD / 2]
+  uint32_t* qmax = reinterpret_cast<uint32_t*>(wl + kWaves * 16);  // [HW][16] bits of the queries' largest |x|
+  float* qinv = reinterpret_cast<float*>(qmax + HW * 16);          // [HW][16] what a digits' unit stands for
+  float* tail_s = qinv + HW * 16;                                   // [HW][2] the blocks' scales
+  float* wacc = tail_s + 8;  // [waves][heads][HD]; before that cos and sin [2][HD / 2]
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), hw = wave / RW, rw = wave % RW;
   int id = blockIdx.x;
   const int ht = id % htiles;
   id /= htiles;
-  const int hkv = id % p.n_kv;
-  id /= p.n_kv;
-  const int b = id % p.batch, split = id / p.batch;
-  const int hq0 = hkv * group + ht * 16, heads = min(group - ht * 16, 16);
+  const int hkv0 = id % (p.n_kv / HW) * HW, hkv = hkv0 + hw;
+  id /= p.n_kv / HW;
+  const Range range = range_of(a, id);
+  if (range.b < 0) return;
+  const int b = range.b, split = range.at;
+  const int heads = min(group - ht * 16, 16);
+  const int per_head = heads * half;  // pairs of query elements of a KV head
   // the query rows, asked for with the length
-  constexpr int NE = HD / 32;
-  const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + hq0 * hd;
+  constexpr int NE = HW * HD / 32;
+  const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + (hkv0 * group + ht * 16) * hd;
   A q0[NE], q1[NE];
 #pragma unroll
   for (int n = 0; n < NE; n++) {
-    const int i = min(tid + n * kThreads, heads * half - 1), hh = i / half, e = i - hh * half;
-    q0[n] = qrow[hh * hd + e];
-    q1[n] = qrow[hh * hd + e + half];
+    const int i = min(tid + n * kThreads, HW * per_head - 1), k = HW > 1 ? i / per_head : 0, j = i - k * per_head;
+    const int hh = j / half, e = j - hh * half;
+    q0[n] = qrow[(k * group + hh) * hd + e];
+    q1[n] = qrow[(k * group + hh) * hd + e + half];
   }
-  // the new row: its keys by wave 0, its values by wave 1
+  // the new row: task t is the keys (t even) or the values of KV head t / 2, by wave t % kWaves
   const bool add = p.k != nullptr;
-  constexpr int NP = HD > 128 ? 2 : 1;  // pairs a lane
-  A n0[NP], n1[NP];
-  if (add && wave < 2) {
-    const A* row = wave == 0 ? static_cast<const A*>(p.k) + (int64_t)b * p.k_stride
-                             : static_cast<const A*>(p.v) + (int64_t)b * p.v_stride;
+  constexpr int NP = HD > 128 ? 2 : 1, TASKS = (2 * HW + kWaves - 1) / kWaves;  // pairs a lane, tasks a wave
+  A n0[TASKS][NP], n1[TASKS][NP];
+  if (add)
 #pragma unroll
-    for (int n = 0; n < NP; n++) {
-      const int e = hkv * hd + min(lane + 64 * n, half - 1);
-      n0[n] = row[e];
-      n1[n] = row[e + half];
+    for (int k = 0; k < TASKS; k++) {
+      const int task = min(wave + k * kWaves, 2 * HW - 1);
+      const A* row = task & 1 ? static_cast<const A*>(p.v) + (int64_t)b * p.v_stride
+                              : static_cast<const A*>(p.k) + (int64_t)b * p.k_stride;
+#pragma unroll
+      for (int n = 0; n < NP; n++) {
+        const int e = (hkv0 + task / 2) * hd + min(lane + 64 * n, half - 1);
+        n0[k][n] = row[e];
+        n1[k][n] = row[e + half];
+      }
     }
-  }
   const int32_t* trow = p.table + (int64_t)b * p.table_stride;
   // Page numbers: lane t holds that of block t of a tile, so one load brings them all. Those of the wave's first
   // tile are asked for with the length where no window moves it.
-  const int r0 = split * a.split_rows, first = r0 + wave * KT, lane_t = min(lane & 7, NB - 1);
+  const int r0 = split == 0 ? 0 : split * range.rows, first = r0 + rw * KT, lane_t = min(lane & 7, NB - 1);
   const int last_entry = max((int)p.table_stride - 1, 0);
   const bool moved = a.window != INT32_MAX;
   int pages = -1;
   if (!moved && p.table_stride > 0) pages = trow[min((first + kBlock * lane_t) >> p.page_bits, last_entry)];
   const int len = a.lens[b];
-  A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + hq0 * hd;
+  A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + (hkv0 * group + ht * 16) * hd;
+  // element i of the workgroup's results: KV head k, query head hh, element d
+  auto place = [&](int i, int* k, int* hh, int* d) {
+    *k = HW > 1 ? i / (heads * hd) : 0;
+    const int j = i - *k * heads * hd;
+    *hh = j / hd;
+    *d = j - *hh * hd;
+  };
   const int64_t rows = (int64_t)len + (add || a.ahead);
   const bool bad = rows > a.max_len || rows > p.table_stride << p.page_bits;
   if (len < 0 || bad || rows == 0) {  // idle slot or nothing to see: zeros; more rows than the call allows: NaN
     if (split == 0)
-      for (int i = tid; i < heads * hd; i += kThreads) orow[i] = (A)(bad && len >= 0 ? NAN : 0.0f);
+      for (int i = tid; i < HW * heads * hd; i += kThreads) {
+        int k, hh, d;
+        place(i, &k, &hh, &d);
+        orow[(k * group + hh) * hd + d] = (A)(bad && len >= 0 ? NAN : 0.0f);
+      }
     return;
   }
   const int tail_row = len & ~(kBlock - 1), before = len & (kBlock - 1);  // of the block that the new row goes into
   CachedRows<true> cr;
   cr.init(a, add ? tail_row : (int)rows, rows);
-  const int nsplit = ranges_of(cr.walk, a.split_rows);
+  const int nsplit = range.count ? range.count : ranges_of_walk(cr.walk, range.rows);
   if (split >= nsplit) return;
   const bool last = split == nsplit - 1;
-  const int r1 = last ? cr.walk : r0 + a.split_rows;
+  const int r1 = last ? cr.walk : r0 + range.rows;
   const int kvd = p.n_kv * hd;
   bool lost = false;  // a page number out of range
 
   const int in_page = (1 << p.page_bits) - 1;
   auto ask_pages = [&](int r) { pages = trow[min(cr.row(r + kBlock * lane_t) >> p.page_bits, last_entry)]; };
-  auto scale_at = [&](int64_t page, int row) -> int64_t {
-    return page * a.scale_stride + ((row & in_page) >> 4) * p.n_kv + hkv;
+  auto scale_at = [&](int64_t page, int row, int head) -> int64_t {
+    return page * a.scale_stride + ((row & in_page) >> 4) * p.n_kv + head;
   };
   const int8_t* kb = static_cast<const int8_t*>(p.kpages) + hkv * hd;
   const int8_t* vb = static_cast<const int8_t*>(p.vpages) + hkv * hd;
   typedef uint32_t VRow __attribute__((ext_vector_type(VW)));
-  u32x4 xk[NB][KP];
+  i32x4 xk[NB][KP];
   VRow xv[NB * 4];
   float sc = 0.0f;  // lane t < NB: scale of the keys of block t, lane 8 + t: of its values
   int64_t base[NB];  // rows in the pages, in scalar registers: an address is a scalar and one offset of the lane
@@ -209,7 +331,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     const int n = min((r1 - r + kBlock - 1) / kBlock, NB);
     const int row = cr.row(r + (lane_t < n ? kBlock * lane_t : 0));
     const int first_page = __builtin_amdgcn_readlane(pages, 0);
-    return (lane & 8 ? a.vscales : a.kscales)[scale_at(lane_t < n ? pages : first_page, row)];
+    return (lane & 8 ? a.vscales : a.kscales)[scale_at(lane_t < n ? pages : first_page, row, hkv)];
   };
   const uint32_t k_off = col * kvd + (PART ? 0 : 16 * g), v_off = 4 * g * kvd;
   auto load_k = [&]() {
@@ -222,9 +344,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
           const int d = 64 * u + 16 * g;
           const u32x2 lo = *reinterpret_cast<const u32x2*>(kp + (k_off + min(d, hd - 8)));
           const u32x2 hi = *reinterpret_cast<const u32x2*>(kp + (k_off + min(d + 8, hd - 8)));
-          xk[t][u] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+          xk[t][u] = __builtin_bit_cast(i32x4, u32x4{lo[0], lo[1], hi[0], hi[1]});
         } else {
-          xk[t][u] = *reinterpret_cast<const u32x4*>(kp + 64 * u + k_off);
+          xk[t][u] = *reinterpret_cast<const i32x4*>(kp + 64 * u + k_off);
         }
       }
     }
@@ -246,11 +368,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
       }
   };
   // the new row's block, from LDS, as block 0 of a tile
+  const uint32_t* tail_k = tails + hw * (2 * kBlock * HD / 4);
+  const uint32_t* tail_v = tail_k + kBlock * HD / 4;
   auto take_tail_k = [&]() {
 #pragma unroll
     for (int u = 0; u < KP; u++)
-      xk[0][u] = *reinterpret_cast<const u32x4*>(tail_k + (col * HD + 64 * u + 16 * g) / 4);
-    sc = tail_s[lane & 8 ? 1 : 0];
+      xk[0][u] = *reinterpret_cast<const i32x4*>(tail_k + (col * HD + 64 * u + 16 * g) / 4);
+    sc = tail_s[2 * hw + (lane & 8 ? 1 : 0)];
   };
   auto take_tail_v = [&]() {
 #pragma unroll
@@ -267,95 +391,114 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     ask_pages(first + STEP);
   }
 
-  // the rotated queries as operands (zeros for heads and elements past the end)
+  // the rotated queries' digits as operands (zeros for heads and elements past the end)
   float* cs = wacc;
   if (p.rope && tid < half) rope_angle(len, tid, hd, p.log2_theta, cs + tid, cs + HD / 2 + tid);
-  for (int i = tid; i < 16 * HD * 2 * NT / 16; i += kThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
+  for (int i = tid; i < HW * kQuery / 16; i += kThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
+  if (tid < HW * 16) qmax[tid] = 0;
   __syncthreads();
-  auto put_query = [&](int hh, int e, float x) {
-    __bf16 t[NT];
-    split_terms<NT>(x, t);
-    __bf16* at = reinterpret_cast<__bf16*>(sm) +
-                 ((2 * (e >> 6) + ((e >> 3) & 1)) * 64 + ((e >> 4) & 3) * 16 + hh) * 8 + (e & 7);
-#pragma unroll
-    for (int n = 0; n < NT; n++) at[n * 16 * HD] = t[n];
-  };
+  float y0[NE], y1[NE];
 #pragma unroll
   for (int n = 0; n < NE; n++) {
-    const int i = tid + n * kThreads, hh = i / half, e = i - hh * half;
-    if (i < heads * half) {
-      float y0 = (float)q0[n], y1 = (float)q1[n];
-      if (p.rope) rotate(y0, y1, cs[e], cs[HD / 2 + e], &y0, &y1);
-      put_query(hh, e, y0);
-      put_query(hh, e + half, y1);
+    const int i = tid + n * kThreads, k = HW > 1 ? i / per_head : 0, j = i - k * per_head, hh = j / half, e = j - hh * half;
+    if (i < HW * per_head) {
+      y0[n] = (float)q0[n], y1[n] = (float)q1[n];
+      if (p.rope) rotate(y0[n], y1[n], cs[e], cs[HD / 2 + e], &y0[n], &y1[n]);
+      // (bits of absolute values are in their order, NaN last)
+      atomicMax(&qmax[k * 16 + hh], max(__float_as_uint(fabsf(y0[n])), __float_as_uint(fabsf(y1[n]))));
     }
   }
-  if (add && last && wave < 2) {  // the new row's block
-    const int page = trow[tail_row >> p.page_bits];
-    const bool store = (uint32_t)page < (uint64_t)p.pages;
-    lost |= !store;
-    const int64_t at = ((int64_t)(store ? page : 0) << p.page_bits) + (tail_row & in_page);
-    int8_t* codes = static_cast<int8_t*>(wave == 0 ? p.kpages : p.vpages) + at * kvd + hkv * hd;
-    float* scale = (wave == 0 ? a.kscales : a.vscales) + scale_at(store ? page : 0, tail_row);
-    uint32_t* tail = wave == 0 ? tail_k : tail_v;
-    const int words = hd / 4;
-    uint32_t w[HD / 16];
+  if (add && last) {  // the new row's block
 #pragma unroll
-    for (int n = 0; n < HD / 16; n++) {
-      const int i = lane + 64 * n, r = i / words, c = i - r * words;
-      w[n] = r < before ? *reinterpret_cast<const uint32_t*>(codes + (int64_t)r * kvd + 4 * c) : 0;
-    }
-    const float s0 = before > 0 ? *scale : 0.0f;
-    float y0[NP], y1[NP], amax = 0.0f;
-    bool good = true;
+    for (int k = 0; k < TASKS; k++) {
+      const int task = wave + k * kWaves, head = hkv0 + task / 2;
+      if (task >= 2 * HW) break;
+      const bool is_v = task & 1;
+      const int page = trow[tail_row >> p.page_bits];
+      const bool store = (uint32_t)page < (uint64_t)p.pages;
+      lost |= !store;
+      const int64_t at = ((int64_t)(store ? page : 0) << p.page_bits) + (tail_row & in_page);
+      int8_t* codes = static_cast<int8_t*>(is_v ? p.vpages : p.kpages) + at * kvd + head * hd;
+      float* scale = (is_v ? a.vscales : a.kscales) + scale_at(store ? page : 0, tail_row, head);
+      uint32_t* tail = tails + task * (kBlock * HD / 4);
+      const int words = hd / 4;
+      uint32_t w[HD / 16];
 #pragma unroll
-    for (int n = 0; n < NP; n++) {
-      const int e = min(lane + 64 * n, half - 1);
-      y0[n] = (float)n0[n], y1[n] = (float)n1[n];
-      if (wave == 0 && p.rope) rotate(y0[n], y1[n], cs[e], cs[HD / 2 + e], &y0[n], &y1[n]);
-      amax = fmaxf(amax, fmaxf(fabsf(y0[n]), fabsf(y1[n])));
-      good = good && finite(y0[n]) && finite(y1[n]);
-    }
-    const float s = raised(wave_max(amax), __all(good), s0);
-    const bool anew = s > s0;
-    const float ratio = anew ? __fdiv_rn(s0, s) : 1.0f;
-#pragma unroll
-    for (int n = 0; n < HD / 16; n++) {
-      const int i = lane + 64 * n, r = i / words, c = i - r * words;
-      if (r < before) {
-        const uint32_t y = anew ? recoded(w[n], ratio) : w[n];
-        tail[(r * HD >> 2) + c] = y;
-        if (anew && store) *reinterpret_cast<uint32_t*>(codes + (int64_t)r * kvd + 4 * c) = y;
+      for (int n = 0; n < HD / 16; n++) {
+        const int i = lane + 64 * n, r = i / words, c = i - r * words;
+        w[n] = r < before ? *reinterpret_cast<const uint32_t*>(codes + (int64_t)r * kvd + 4 * c) : 0;
       }
-    }
+      const float s0 = before > 0 ? *scale : 0.0f;
+      float z0[NP], z1[NP], amax = 0.0f;
+      bool good = true;
 #pragma unroll
-    for (int n = 0; n < NP; n++) {
-      const int e = lane + 64 * n;
-      if (e < half) {
-        const int8_t c0 = (int8_t)code_of(y0[n], s), c1 = (int8_t)code_of(y1[n], s);
-        int8_t* t = reinterpret_cast<int8_t*>(tail) + before * HD + e;
-        t[0] = c0;
-        t[half] = c1;
-        if (store) {
-          codes[(int64_t)before * kvd + e] = c0;
-          codes[(int64_t)before * kvd + e + half] = c1;
+      for (int n = 0; n < NP; n++) {
+        const int e = min(lane + 64 * n, half - 1);
+        z0[n] = (float)n0[k][n], z1[n] = (float)n1[k][n];
+        if (!is_v && p.rope) rotate(z0[n], z1[n], cs[e], cs[HD / 2 + e], &z0[n], &z1[n]);
+        amax = fmaxf(amax, fmaxf(fabsf(z0[n]), fabsf(z1[n])));
+        good = good && finite(z0[n]) && finite(z1[n]);
+      }
+      const float s = raised(wave_max(amax), __all(good), s0);
+      const bool anew = s > s0;
+      const float ratio = anew ? __fdiv_rn(s0, s) : 1.0f;
+#pragma unroll
+      for (int n = 0; n < HD / 16; n++) {
+        const int i = lane + 64 * n, r = i / words, c = i - r * words;
+        if (r < before) {
+          const uint32_t y = anew ? recoded(w[n], ratio) : w[n];
+          tail[(r * HD >> 2) + c] = y;
+          if (anew && store) *reinterpret_cast<uint32_t*>(codes + (int64_t)r * kvd + 4 * c) = y;
         }
       }
-    }
-    if (lane == 0) {
-      tail_s[wave] = s;
-      if (store) *scale = s;
+#pragma unroll
+      for (int n = 0; n < NP; n++) {
+        const int e = lane + 64 * n;
+        if (e < half) {
+          const int8_t c0 = (int8_t)code_of(z0[n], s), c1 = (int8_t)code_of(z1[n], s);
+          int8_t* t = reinterpret_cast<int8_t*>(tail) + before * HD + e;
+          t[0] = c0;
+          t[half] = c1;
+          if (store) {
+            codes[(int64_t)before * kvd + e] = c0;
+            codes[(int64_t)before * kvd + e + half] = c1;
+          }
+        }
+      }
+      if (lane == 0) {
+        tail_s[task] = s;
+        if (store) *scale = s;
+      }
     }
   }
   __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NE; n++) {
+    const int i = tid + n * kThreads, k = HW > 1 ? i / per_head : 0, j = i - k * per_head, hh = j / half, e = j - hh * half;
+    if (i < HW * per_head) {
+      const float f = digit_factor<NT>(__uint_as_float(qmax[k * 16 + hh]));
+      if (e == 0) qinv[k * 16 + hh] = f > 0.0f ? __builtin_amdgcn_rcpf(f) : __uint_as_float(qmax[k * 16 + hh]);  // (0, or NaN for NaN)
+      char* at = reinterpret_cast<char*>(sm) + k * kQuery;
+#pragma unroll
+      for (int z = 0; z < 2; z++) {
+        const int d = e + z * half;
+        const uint32_t x = digits_of<NT>((int)rintf((z ? y1[n] : y0[n]) * f));
+#pragma unroll
+        for (int m = 0; m < NT; m++)
+          at[((m * KP + (d >> 6)) * 64 + 16 * ((d >> 4) & 3) + hh) * 16 + (d & 15)] = (char)(x >> (8 * m));
+      }
+    }
+  }
+  __syncthreads();
+  const float qs = col < heads ? qinv[hw * 16 + col] * a.scale2 : 0.0f;
 
   f32x4 acc[E];
 #pragma unroll
   for (int t = 0; t < E; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, l = 0.0f;
-  // the wave's tiles, at the end the new row's block by the wave whose turn it is
+  // the wave's tiles, at the end the new row's block by the wave of its head whose turn it is
   int r = first;
-  const bool has_tail = add && last && wave == ((r1 - r0 + KT - 1) / KT) % kWaves;
+  const bool has_tail = add && last && rw == ((r1 - r0 + KT - 1) / KT) % RW;
   bool tail = first >= r1;
   if (tail && has_tail) {
     take_tail_k();
@@ -369,35 +512,43 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     float ks[NB], vs[NB];
 #pragma unroll
     for (int t = 0; t < NB; t++) {
-      at[t] = tail ? (t == 0 ? tail_row : INT32_MAX - kBlock)
-                   : r + kBlock * t < r1 ? cr.row(r + kBlock * t) : INT32_MAX - kBlock;
+      const bool there = tail ? t == 0 : r + kBlock * t < r1;
+      at[t] = !there ? INT32_MAX - kBlock : tail ? tail_row : cr.row(r + kBlock * t);
       ks[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), t));
-      vs[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), 8 + t));
+      vs[t] = there ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc), 8 + t)) : 0.0f;
     }
     if (more) set_base(r + STEP);
-#pragma unroll
-    for (int t = 0; t < NB; t++) keep_whole(xk[t]);
-    f32x4 d[NB] = {};
     int ql = lane;  // read anew for every tile: kept in registers they would cost a wave a SIMD
     asm volatile("" : "+v"(ql));
-    const u32x4* qp = reinterpret_cast<const u32x4*>(sm) + ql;
+    const i32x4* qp = reinterpret_cast<const i32x4*>(reinterpret_cast<const char*>(sm) + hw * kQuery) + ql;
+    float s[NB][4];
 #pragma unroll
-    for (int u = 0; u < KP; u++)
+    for (int t0 = 0; t0 < NB; t0 += 2) {  // two blocks at a time, for the registers
+      i32x4 d[NT][2] = {};
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        u32x4 qw[NT];
+      for (int u = 0; u < KP; u++) {
+        i32x4 qw[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n++) qw[n] = qp[(n * QS + 2 * u + h) * 64];
-        bf16x8 kf[NB];
-#pragma unroll
-        for (int t = 0; t < NB; t++) kf[t] = bf16_of_codes(xk[t][u][2 * h], xk[t][u][2 * h + 1]);
+        for (int n = 0; n < NT; n++) qw[n] = qp[(n * KP + u) * 64];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int t = 0; t < NB; t++)
-            d[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], __builtin_bit_cast(bf16x8, qw[n]), d[t], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);  // (left alone, the conversions of all steps come first and do not fit)
+          for (int t = 0; t < 2; t++)
+            d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xk[t0 + t][u], qw[n], d[n][t], 0, 0, 0);
       }
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const float f = ks[t0 + t] * qs;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (NT == 2)
+            s[t0 + t][i] = value_of(d[0][t][i], d[1][t][i]) * f;
+          else
+            s[t0 + t][i] = value_of(d[0][t][i], d[1][t][i], d[2][t][i]) * f;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if (more) {
       load_k();
       sc = load_scales(r + STEP);
@@ -405,25 +556,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     } else if (then_tail) {
       take_tail_k();
     }
-    float s[NB][4];
-    uint32_t hidden[NB];  // bit i: row 4 g + i of the block
-    bool cut = false;
 #pragma unroll
     for (int t = 0; t < NB; t++) {
-      const float f = ks[t] * a.scale2;
-      const bool c = at[t] + kBlock > end || !cr.sees_block(at[t]);
-      cut = cut || c;
-#pragma unroll
-      for (int i = 0; i < 4; i++) s[t][i] = d[t][i] * f;
-      hidden[t] = 0;
-      if (c)
+      if (at[t] + kBlock > end || !cr.sees_block(at[t]))
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int row = at[t] + 4 * g + i;
-          if (row >= end || !cr.sees(row)) {
-            s[t][i] = -INFINITY;
-            hidden[t] |= 1u << i;
-          }
+          if (row >= end || !cr.sees(row)) s[t][i] = -INFINITY;
         }
     }
     float mx = s[0][0];
@@ -433,53 +572,77 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
       for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mn;
-    l *= alpha;
+    // Weights (with the scale of their block) are digits relative to the tile's largest: the tile's own maximum
+    // first, so that none of a tile is lost beside another tile's
+    const float top = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f, vsum = 0.0f, wmax = 0.0f;
 #pragma unroll
-    for (int t = 0; t < NB; t++)
+    for (int t = 0; t < NB; t++) {
+      vsum += vs[t];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
-        l += s[t][i];
+        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - top);
+        sum += s[t][i];
+        s[t][i] *= vs[t];
+        wmax = fmaxf(wmax, s[t][i]);
       }
+    }
+    wmax = fmaxf(wmax, __shfl_xor(wmax, 16, 64));
+    wmax = fmaxf(wmax, __shfl_xor(wmax, 32, 64));
+    const float to_digits = digit_factor<NT>(wmax);
+    i32x4 pd[NT] = {};
 #pragma unroll
-    for (int t = 0; t < E; t++) acc[t] *= alpha;
+    for (int t = 0; t < NB; t++) {
+      uint32_t x[4], y[NT];
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = (uint32_t)(int)fmaf(s[t][i], to_digits, 0.5f) + (NT == 2 ? 0x8080u : 0x808080u);
+      pack_digits<NT>(x, y);
+#pragma unroll
+      for (int n = 0; n < NT; n++) pd[n][t] = (int)(y[n] ^ 0x80808080u);
+    }
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref), beta = __builtin_amdgcn_exp2f(mx - ref);
+    m = mn;
+    l = fmaf(l, alpha, sum * beta);
+    // (a scale that is not finite makes the factor NaN)
+    const float from_digits = (to_digits > 0.0f ? __builtin_amdgcn_rcpf(to_digits) : 0.0f) + 0.0f * vsum;
+    const float wf = from_digits * beta;
     keep_whole(xv);
 #pragma unroll
-    for (int t = 0; t < NB; t += 2) {  // 32 rows a product
-      bf16x8 pb[NT];
+    for (int w = 0; w < VW; w++)  // four elements, one word of the rows
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int u = t + (j >> 2);
-        float w = s[u][j & 3] * vs[u];
-        if (cut && (hidden[u] >> (j & 3) & 1)) w = 0.0f;  // what is not seen may have any scale
-        __bf16 x[NT];
-        split_terms<NT>(w, x);
+      for (int e = 0; e < 4; e += 2) {
+        i32x4 vf[2] = {};
 #pragma unroll
-        for (int n = 0; n < NT; n++) pb[n][j] = x[n];
-      }
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {  // four elements, one word of the rows
-        bf16x8 vf[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float f[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) f[j] = (float)(int8_t)(xv[4 * t + j][e >> 2] >> (8 * i));
-          u32x4 y;
-#pragma unroll
-          for (int j = 0; j < 4; j++) y[j] = high16_pair(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
-          vf[i] = __builtin_bit_cast(bf16x8, y);
+        for (int t = 0; t < NB; t++) {
+          const uint32_t pick = e == 0 ? 0x05010400 : 0x07030602;
+          const uint32_t x = __builtin_amdgcn_perm(xv[4 * t + 1][w], xv[4 * t][w], pick);
+          const uint32_t y = __builtin_amdgcn_perm(xv[4 * t + 3][w], xv[4 * t + 2][w], pick);
+          vf[0][t] = (int)low16_pair(x, y);
+          vf[1][t] = (int)high16_pair(x, y);
         }
+        i32x4 o[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            acc[e + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pb[n], acc[e + i], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < 2; i++)
+            o[n][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[i], pd[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          f32x4& sum_e = acc[4 * w + e + i];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float x;
+            if constexpr (NT == 2)
+              x = value_of(o[0][i][j], o[1][i][j]);
+            else
+              x = value_of(o[0][i][j], o[1][i][j], o[2][i][j]);
+            sum_e[j] = fmaf(x, wf, sum_e[j] * alpha);
+          }
+          asm volatile("" : "+v"(sum_e));  // (else the sums sink past the next loads)
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (left alone, all products come first and do not fit)
       }
-    }
     if (more)
       load_v();
     else if (then_tail)
@@ -502,30 +665,78 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     wl[wave * 16 + col] = l;
   }
   const bool any_lost = __syncthreads_or(lost);
-  for (int i = tid; i < heads * hd; i += kThreads) {
-    const int hh = i / hd, d = i - hh * hd;
-    float mx = wm[hh];
+  for (int i = tid; i < HW * heads * hd; i += kThreads) {
+    int k, hh, d;
+    place(i, &k, &hh, &d);
+    const int w0 = k * RW;
+    float mx = wm[w0 * 16 + hh];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, wm[w * 16 + hh]);
+    for (int w = 1; w < RW; w++) mx = fmaxf(mx, wm[(w0 + w) * 16 + hh]);
     const float ref = mx == -INFINITY ? 0.0f : mx;
     float o = 0.0f, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-      const float f = __builtin_amdgcn_exp2f(wm[w * 16 + hh] - ref);
-      sum += f * wl[w * 16 + hh];
-      o += f * wacc[(w * nh + hh) * HD + d];
+    for (int w = 0; w < RW; w++) {
+      const float f = __builtin_amdgcn_exp2f(wm[(w0 + w) * 16 + hh] - ref);
+      sum += f * wl[(w0 + w) * 16 + hh];
+      o += f * wacc[((w0 + w) * nh + hh) * HD + d];
     }
     if (any_lost) sum = NAN;
     if (nsplit == 1) {
-      orow[i] = (A)(sum == 0.0f ? 0.0f : o / sum);
+      orow[(k * group + hh) * hd + d] = (A)(sum == 0.0f ? 0.0f : o / sum);
     } else {
-      float* rec = a.part + (((int64_t)b * p.n_q + hq0 + hh) * a.nsplit + split) * (kRec + hd);
+      const int hq = (hkv0 + k) * group + ht * 16 + hh;
+      float* rec = a.part + ((int64_t)id * p.n_q + hq) * (kRec + hd);
       rec[kRec + d] = o;
       if (d == 0) {
         rec[0] = mx;
         rec[1] = sum;
       }
     }
+  }
+}
+
+// Joins the ranges' records of a (sequence, head), one workgroup each: head_dim / 4 lanes
+// a record, the lane groups' sums added in order.
+template <typename A>
+__global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
+  const PagesArgs& p = a.p;
+  const int hq = blockIdx.x % p.n_q, b = blockIdx.x / p.n_q, hd = p.head_dim;
+  const Range range = range_of(a, -1 - b);
+  const int n = range.count ? range.count : ranges_of_walk(walked_of(a, a.lens[b]), range.rows);
+  if (n <= 1) return;
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) float sums[256 * 4];
+  __shared__ float lsum[128];
+  const int tid = threadIdx.x, dl = hd / 4, groups = 256 / dl, grp = tid / dl, d = tid % dl;
+  const int64_t rs = (int64_t)p.n_q * (kRec + hd);
+  const float* rec = a.part + ((int64_t)range.first * p.n_q + hq) * (kRec + hd);
+  float mx = -INFINITY;
+  for (int r = tid; r < n; r += 256) mx = fmaxf(mx, rec[r * rs]);
+  mx = wave_max(mx);
+  if ((tid & 63) == 0) red[tid >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = mx == -INFINITY ? 0.0f : mx;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float sum = 0.0f;
+  if (grp < groups) {
+    for (int r = grp; r < n; r += groups) {
+      const float f = __builtin_amdgcn_exp2f(rec[r * rs] - ref);
+      sum += f * rec[r * rs + 1];
+      o += f * *reinterpret_cast<const f32x4*>(rec + r * rs + kRec + 4 * d);
+    }
+    *reinterpret_cast<f32x4*>(&sums[4 * tid]) = o;
+    if (d == 0) lsum[grp] = sum;
+  }
+  __syncthreads();
+  if (tid < dl) {
+    for (int k = 1; k < groups; k++) {
+      o += *reinterpret_cast<const f32x4*>(&sums[4 * (k * dl + tid)]);
+      sum += lsum[k];
+    }
+    A* out = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + hq * hd + 4 * tid;
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = (A)(sum == 0.0f ? 0.0f : o[e] / sum);
   }
 }
 
@@ -645,28 +856,36 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
 
 namespace {
 
-template <typename A, int HD, bool PART>
+template <typename A, int HD, bool PART, int HW>
 hipError_t run_paged_q8(const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
   const int64_t htiles = (p.n_q / p.n_kv + 15) / 16;
-  constexpr int kMaxLds = q8_fixed_bytes<A>(HD) + kWaves * 16 * HD * 4;
-  const int lds = q8_fixed_bytes<A>(HD) + kWaves * std::min(p.n_q / p.n_kv, 16) * HD * 4;
-  const auto kernel = paged_attention_q8_kernel<A, HD, PART>;
+  constexpr int kFixed = q8_fixed_bytes<A, HD, HW>(), kMaxLds = kFixed + kWaves * 16 * HD * 4;
+  const int lds = kFixed + kWaves * std::min(p.n_q / p.n_kv, 16) * HD * 4;
+  const auto kernel = paged_attention_q8_kernel<A, HD, PART, HW>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), kMaxLds, &allowed)) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.nsplit * p.batch * p.n_kv * htiles)), dim3(kThreads), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((p.batch + a.spare) * (p.n_kv / HW) * htiles)), dim3(kThreads), lds,
+                     stream, a);
   return hipGetLastError();
+}
+
+template <typename A, int HD, bool PART>
+hipError_t run_paged_q8_heads(const PagedAttnArgs& a, hipStream_t stream) {
+  if constexpr (HD <= 128)
+    if (a.kv_heads == 4) return run_paged_q8<A, HD, PART, 4>(a, stream);
+  return run_paged_q8<A, HD, PART, 1>(a, stream);
 }
 
 template <typename A>
 hipError_t run_paged_q8_hd(const PagedAttnArgs& a, hipStream_t stream) {
   const int hd = a.p.head_dim;
-  if (hd == 64) return run_paged_q8<A, 64, false>(a, stream);
-  if (hd == 128) return run_paged_q8<A, 128, false>(a, stream);
-  if (hd == 256) return run_paged_q8<A, 256, false>(a, stream);
-  if (hd < 64) return run_paged_q8<A, 64, true>(a, stream);
-  if (hd < 128) return run_paged_q8<A, 128, true>(a, stream);
-  return run_paged_q8<A, 256, true>(a, stream);
+  if (hd == 64) return run_paged_q8_heads<A, 64, false>(a, stream);
+  if (hd == 128) return run_paged_q8_heads<A, 128, false>(a, stream);
+  if (hd == 256) return run_paged_q8_heads<A, 256, false>(a, stream);
+  if (hd < 64) return run_paged_q8_heads<A, 64, true>(a, stream);
+  if (hd < 128) return run_paged_q8_heads<A, 128, true>(a, stream);
+  return run_paged_q8_heads<A, 256, true>(a, stream);
 }
 
 template <typename A, int HD>
@@ -759,6 +978,32 @@ int64_t append_q8_slots(const PagesAppendArgs& a) {
   return a.cu ? a.rows / kBlock + 2 * (int64_t)a.p.batch : a.p.batch;
 }
 
+PagedQ8Plan plan_paged_attention_q8(int64_t batch, int64_t n_q, int64_t n_kv, int64_t head_dim, int64_t max_len,
+                                    int cu_count) {
+  batch = std::min<int64_t>(batch, kPlanned);
+  const int64_t htiles = (n_q / n_kv + 15) / 16;
+  PagedQ8Plan p;
+  // Four KV heads a workgroup where a CU can have many rows times KV heads; us, one head / four, and rows at max_len (caches cold,
+  // 32/8 heads x 128 unless said): 32 of 2000 44 / 47, 2000   64 of 1000 44 / 50, 2000   8 of 4000 27 / 33, 1000   4 of 16000, 16/16
+  // heads 68 / 62, 4000   64 of 1 to 4000 91 / 79, 8000   32 of 1 to 8191 (f32) 94 / 81, 8191   32 of 8000 131 / 112, 8000   16 of
+  // 16000, 64/8 x 64 96 / 71, 8000   16 of 1 to 32000 141 / 117, 16000   8 of 33 to 65 Ki, 64/8 heads 210 / 178, 16384
+  const bool wide = n_kv % 4 == 0 && head_dim <= 128 && htiles == 1;
+  p.kv_heads = wide && max_len * batch * n_kv > 3500 * (int64_t)cu_count ? 4 : 1;
+  const int64_t heads = n_kv / p.kv_heads * htiles;
+  p.split_rows = kTileRows * kWaves / p.kv_heads;
+  // As many ranges more than sequences as give every CU two workgroups; where there are many sequences, whose short ends add up, no
+  // more than that in all (64 of 1 to 4000 96 -> 83, but 8 of 33 to 65 Ki 178 -> 190), and half as many at least. A sequence of one or two
+  // rounds of tiles stays whole: the join would cost more.
+  const int64_t most = max_len <= 2 * p.split_rows ? 0 : batch * (max_len / p.split_rows), two = 2 * cu_count / heads;
+  p.spare = (int)std::min<int64_t>(std::max<int64_t>({4 * batch >= two ? two - batch : two, two / 2, 1}), most);
+  p.range_rows = 0;
+  if (batch == 1 && p.spare > 0)
+    p.range_rows = (int)((max_len / (p.spare + 1) + p.split_rows) / p.split_rows * p.split_rows);
+  p.groups = (batch + p.spare) * heads;
+  p.work = p.spare > 0 ? (size_t)((batch + p.spare) * n_q * (kRec + head_dim)) * sizeof(float) : 0;
+  return p;
+}
+
 hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
   PagedAttnArgs r = a;
@@ -775,8 +1020,28 @@ hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStrea
     r.ahead = 1;
   }
   if (r.window == 0) r.window = INT32_MAX;
-  if (hipError_t e = dtype == RQ_F32 ? run_paged_q8_hd<float>(r, stream) : run_paged_q8_hd<__bf16>(r, stream)) return e;
-  return r.nsplit > 1 ? launch_paged_merge(dtype, r, stream) : hipSuccess;
+  const int64_t e = dtype == RQ_F32 ? 4 : 2;
+  for (int64_t b = 0; b < p.batch; b += kPlanned) {  // (records of the last launch are joined before the next one's are written)
+    PagedAttnArgs n = r;
+    n.p.batch = (int)std::min<int64_t>(kPlanned, p.batch - b);
+    n.p.table += b * p.table_stride;
+    n.lens += b;
+    auto from = [&](const void* x, int64_t stride) { return x ? static_cast<const char*>(x) + b * stride * e : nullptr; };
+    n.p.q = from(r.p.q, p.q_stride);
+    n.p.k = from(r.p.k, p.k_stride);
+    n.p.v = from(r.p.v, p.v_stride);
+    n.out = static_cast<char*>(r.out) + b * r.out_stride * e;
+    if (hipError_t s = dtype == RQ_F32 ? run_paged_q8_hd<float>(n, stream) : run_paged_q8_hd<__bf16>(n, stream)) return s;
+    if (n.spare > 0) {
+      const dim3 grid((unsigned)(n.p.batch * p.n_q));
+      if (dtype == RQ_F32)
+        hipLaunchKernelGGL(paged_q8_merge_kernel<float>, grid, dim3(256), 0, stream, n);
+      else
+        hipLaunchKernelGGL(paged_q8_merge_kernel<__bf16>, grid, dim3(256), 0, stream, n);
+      if (hipError_t s = hipGetLastError()) return s;
+    }
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_pages_append_q8(int dtype, const PagesAppendArgs& a, hipStream_t stream) {

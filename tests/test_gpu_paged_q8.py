@@ -39,22 +39,35 @@ def near_codes(got, want, x, s):
 
 
 def check_out(torch, ref, out, q, cache, lens, add, nq, nkv, hd, scale, window, sinks):
-    """out's rows against attention over the cache as it is stored; q: the rotated queries, f64 [batch, nq, hd]."""
+    """out's rows against attention over the cache as it is stored; q: the rotated queries, f64 [batch, nq, hd].
+
+    Beside attn_ref's roundings two of the kernel's own: queries and weights are whole numbers of `step` = 1 / (2 M) of the
+    largest of their head, or tile, M = 0x7F7F7C for f32 results and 0x7F7E for bf16 ones (the factors by a reciprocal of one unit in
+    the last place: 2^-22 more). A query's element is off by at most step * max |q|, a score by that times the sum of |k|, a
+    weight, relatively, by twice as much (its own score and the sum); a weight with its block's scale, w, by at most step * max w,
+    and so element d of the result by that times the sum of the rows' |code| there."""
     half = ref.HALF[out.dtype]
-    hq = 2.0 ** -22 if out.dtype == torch.float32 else 2.0 ** -16  # three or two bf16 terms
+    step = 0.5 / (0x7F7F7C if out.dtype == torch.float32 else 0x7F7E) * (1 + 2.0 ** -20)
     for b, m in enumerate(lens):
         if m < 0 or m + add == 0:
             assert bool((out[b] == 0).all())
             continue
         n = m + add
         keys, values = cache.values("k", b, n), cache.values("v", b, n)
+        scales = cache.vs[cache._mine(b, n)].reshape(-1, nkv).double().repeat_interleave(16, 0)[:n]
         j = torch.arange(n, device="cuda")
         see = (((n - 1 - j < window) | (j < sinks)) if window else j >= 0)[None]
         for h in range(nq):
             g = h // (nq // nkv)
-            want, _, bound = ref.attend(q[b, h:h + 1], keys[:, g], values[:, g], scale, see, half, hq)
+            qh, kh, vh = q[b, h:h + 1], keys[:, g], values[:, g]
+            want, lse, bound = ref.attend(qh, kh, vh, scale, see, half, 2.0 ** -22)
+            p = torch.where(see, torch.exp(qh @ kh.T * scale - lse[:, None]), 0.0)[0]
+            off = step * qh.abs().max() * (kh.abs().sum(1) * see[0]).max() * scale
+            codes = torch.where(scales[:, g:g + 1] > 0, vh / scales[:, g:g + 1], 0.0).abs() * see[0][:, None]
+            extra = 2 * off * (p @ vh.abs()) + step * (p * scales[:, g]).max() * codes.sum(0)
             got = out[b, h * hd:(h + 1) * hd].double()
-            assert bool(((got - want[0]).abs() <= bound[0]).all()), (b, h, float(((got - want[0]).abs() / bound).max()))
+            assert bool(((got - want[0]).abs() <= bound[0] + extra).all()), (
+                b, h, float(((got - want[0]).abs() / (bound[0] + extra)).max()))
 
 
 # activations, heads, KV heads, head_dim, page, cached rows, window, sinks
