@@ -31,7 +31,8 @@ A whole step can be captured in one HIP graph (no call allocates).
 Batches of sequences run over a PagedCache (paged.py): prefill takes the packed
 prompts through a layer (pages_append, prompt_attention), step_paged one new
 token of each sequence (paged_attention), with the fused linears up to 16
-sequences and the unfused glue beyond.
+sequences and the unfused glue beyond. The cache may be f32, bf16 or int8, and a layer
+may see a sliding window with sinks only.
 """
 from __future__ import annotations
 
@@ -99,11 +100,15 @@ class DecoderLayer:
     layout for q, k, v, o, gate, up, down."""
 
     def __init__(self, ctx: Context, weights, gain1, gain2, d: int, n_q: int, n_kv: int, head_dim: int, ffn: int,
-                 eps: float = 1e-5, theta: float = 1e4, fused: bool = True):
+                 eps: float = 1e-5, theta: float = 1e4, fused: bool = True, window: int | None = None, sinks: int = 0):
+        """window: prefill and step_paged attend the last `window` tokens up to each one and the
+        sequence's first `sinks`; None or 0: all."""
         import torch
 
         if n_q % n_kv:
             raise ValueError("n_q must be a multiple of n_kv")
+        _need((window or 0) >= 0 and sinks >= 0, "window and sinks must not be negative")
+        self.seen = dict(window=window, sinks=sinks)
         self.ctx, self.fused = ctx, fused
         self.d, self.n_q, self.n_kv, self.hd, self.ffn = d, n_q, n_kv, head_dim, ffn
         self.eps, self.theta = eps, theta
@@ -127,7 +132,8 @@ class DecoderLayer:
     def step(self, x, kcache, vcache, pos: int):
         """x: f32 [d] on the device; kcache / vcache: f32 [>= pos+1, n_kv*head_dim].
         Appends this token's k / v at `pos`, attends positions 0..pos and
-        returns the layer output [d]."""
+        returns the layer output [d]. For a layer without a window."""
+        _need(not self.seen["window"], "a layer with a window goes on over a PagedCache (step_paged)")
         if self.fused:
             return self._step_fused(x, kcache, vcache, pos)
         torch = _t()
@@ -198,9 +204,10 @@ class DecoderLayer:
         (int32 [batch + 1] on the device; ranges of lens[b] rows) the next tokens of cache sequence
         seqs[b], for which cache.reserve has made room. Their keys and values go
         into the cache's pages of `layer`; each token attends its sequence up to
-        itself, rows stored before included, keys and values as the pages hold them (a
-        bf16 cache rounds them), however a prompt is cut. Returns [rows, d]. After the last
-        layer, cache.advance(seqs, lens)."""
+        itself, or the layer's window, rows stored before included, keys and values as the pages hold them (a
+        bf16 cache rounds them), however a prompt is cut (int8: a block of 16 tokens has one scale, so
+        its last tokens' size and where a prompt is cut show in its values' rounding). Returns [rows, d].
+        After the last layer, cache.advance(seqs, lens)."""
         torch = _t()
         _need(len(seqs) == len(lens) == cu.numel() - 1 and sum(lens) == x.shape[0],
               "cu, seqs and lens must be of one batch, and x of its rows")
@@ -208,16 +215,18 @@ class DecoderLayer:
         view = cache.view(seqs)
         q, k, v = self._split_qkv(self.w_qkv.matmul(rms_norm(torch, x, self.g1, self.eps)))
         pages_append(self.ctx, q, k, v, cache.kpages(layer), cache.vpages(layer), view.table, cu, view.lens, self.n_q,
-                     self.n_kv, self.hd, self.theta, q_out=q, k_out=k)
+                     self.n_kv, self.hd, self.theta, q_out=q, k_out=k, **cache.layer_scales(layer))
         cu_k = None
         past = [cache.length(s) for s in seqs]
-        if any(past):  # rows stored before: the keys are the cache's, the new rows among them
-            k, v = (t.to(x.dtype) for t in cache.rows(layer, seqs, lens))
-            ends = np.cumsum([0] + [n0 + n for n0, n in zip(past, lens)])
-            cu_k = torch.tensor(ends, dtype=torch.int32, device=x.device)
+        if any(past) or cache.scales is not None:  # rows stored before: the keys are the cache's, the new rows among them
+            k, v = cache.rows(layer, seqs, lens, x.dtype)
+            if any(past):
+                ends = np.cumsum([0] + [n0 + n for n0, n in zip(past, lens)])
+                cu_k = torch.tensor(ends, dtype=torch.int32, device=x.device)
         else:  # as they are stored, like those of a prompt that goes on and of step_paged
             k, v = (t.to(cache.data.dtype).to(x.dtype) for t in (k, v))
-        at = prompt_attention(self.ctx, q, k, v, cu, self.n_q, self.n_kv, self.hd, 1.0 / math.sqrt(self.hd), cu_k=cu_k)
+        at = prompt_attention(self.ctx, q, k, v, cu, self.n_q, self.n_kv, self.hd, 1.0 / math.sqrt(self.hd), cu_k=cu_k,
+                              **self.seen)
         return self._mlp(residual_add(x, self.w_o.matmul(at)))
 
     def step_paged(self, x, cache, layer: int, view):
@@ -231,7 +240,7 @@ class DecoderLayer:
         qkv = self.w_qkv.matmul_fused(x, norm_gain=self.g1, norm_eps=self.eps) if fused else self.w_qkv.matmul(xn)
         at = paged_attention(self.ctx, *self._split_qkv(qkv), cache.kpages(layer), cache.vpages(layer), view.table,
                              view.lens, self.n_q, self.n_kv, self.hd, self.theta, 1.0 / math.sqrt(self.hd),
-                             max_len=view.max_len)
+                             max_len=view.max_len, **self.seen, **cache.layer_scales(layer))
         if not fused:
             return self._mlp(residual_add(x, self.w_o.matmul(at)))
         x1 = self.w_o.matmul_fused(at, residual=x)

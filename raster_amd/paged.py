@@ -12,6 +12,10 @@ holds until its rows are used up, forks or not. The sequences' page table and le
 when they have changed, on the current stream; a graph captured over the device
 arrays goes on reading them, so its replays follow later changes. One cache is used
 by one thread and on one stream at a time.
+
+With dtype int8 the rows are codes, and `scales` holds one f32 scale for each 16 rows and KV head, in
+every plane beside the pages; they are copied and moved together. A row of 128 elements a head takes
+0.52 of a bf16 one's bytes.
 """
 from __future__ import annotations
 
@@ -20,7 +24,7 @@ from typing import NamedTuple
 
 import numpy as np
 
-from .attention import pages_copy
+from .attention import pages_copy, pages_rows
 from .quant import Context, _need, _t
 
 __all__ = ["PagedCache", "PagedView"]
@@ -47,9 +51,12 @@ class _Pages(list):
 
 
 class PagedCache:
+    scales = None  # int8: f32 [2 * layers, pages, 1, scales of a page]
+
     def __init__(self, ctx: Context, layers: int, pages: int, n_kv: int, head_dim: int, page_size: int = 16,
                  max_seqs: int = 16, seq_pages: int | None = None, dtype=None):
-        """max_seqs sequences of at most seq_pages pages each (default: all of them)."""
+        """max_seqs sequences of at most seq_pages pages each (default: all of them). dtype:
+        f32 (default), bf16 or int8."""
         torch = _t()
         _need(layers > 0 and pages > 0 and max_seqs > 0, "layers, pages and max_seqs must be positive")
         _need(page_size >= 16 and page_size & (page_size - 1) == 0, "page_size must be a power of two from 16 on")
@@ -57,6 +64,8 @@ class PagedCache:
         dev = torch.device("cuda", ctx.device)
         self.data = torch.zeros((2 * layers, pages, page_size, n_kv * head_dim), dtype=dtype or torch.float32,
                                 device=dev)
+        if self.data.dtype == torch.int8:  # (a page's scales end at a multiple of 16 bytes, for the copies)
+            self.scales = torch.zeros((2 * layers, pages, 1, (page_size // 16 * n_kv + 3) // 4 * 4), device=dev)
         self._refs = [0] * pages
         self._free = list(range(pages))  # a heap: the lowest page first
         self._pages: dict[int, list[int]] = {}
@@ -74,6 +83,19 @@ class PagedCache:
 
     def vpages(self, layer: int):
         return self.data[2 * layer + 1]
+
+    def layer_scales(self, layer: int) -> dict:
+        """The operators' kscales and vscales for a layer's pages; {} but for int8."""
+        if self.scales is None:
+            return {}
+        shape = (self.data.shape[1], self.page_size // 16, self.n_kv)
+        return {name: plane[:, 0, :shape[1] * shape[2]].unflatten(1, shape[1:])
+                for name, plane in (("kscales", self.scales[2 * layer]), ("vscales", self.scales[2 * layer + 1]))}
+
+    def _copy(self, src, dst) -> None:
+        pages_copy(self.ctx, self.data, src, dst)
+        if self.scales is not None:
+            pages_copy(self.ctx, self.scales, src, dst)
 
     def view(self, seqs=None, max_len: int | None = None) -> PagedView:
         """The device arrays of `seqs`, as of now; None: of all slots, those without a
@@ -145,7 +167,7 @@ class PagedCache:
             self._refs[p] += 1
         if own:
             held[-1] = self._take()
-            pages_copy(self.ctx, self.data, [pages[len(held) - 1]], [held[-1]])
+            self._copy([pages[len(held) - 1]], [held[-1]])
         held.room = n
         self._pages[new], self._len[new] = held, n
         self._host_table[new, :len(held)] = held
@@ -191,7 +213,7 @@ class PagedCache:
         for s, n in zip(seqs, rows):
             self._pages[s].room = max(self._pages[s].room, self._len[s] + n)
         if src:
-            pages_copy(self.ctx, self.data, src, dst)
+            self._copy(src, dst)
 
     def need_own(self, seqs, rows=1) -> None:
         """ValueError when the next rows (a number, or one a sequence) of one of `seqs` would go to a page
@@ -232,7 +254,7 @@ class PagedCache:
         src = [p for p in used if p >= len(used)]
         dst = [p for p in range(len(used)) if not self._refs[p]]
         if src:
-            pages_copy(self.ctx, self.data, src, dst)
+            self._copy(src, dst)
             to = dict(zip(src, dst))
             for old, new in to.items():
                 self._refs[new], self._refs[old] = self._refs[old], 0
@@ -243,21 +265,25 @@ class PagedCache:
             self._dirty = True
         return len(used)
 
-    def rows(self, layer: int, seqs, more=0):
+    def rows(self, layer: int, seqs, more=0, dtype=None):
         """The stored rows of `seqs`, one after another, and `more` (a number, or one a
         sequence) behind each that are appended but not advanced over yet: (keys, values)
-        [rows, n_kv * head_dim], copies."""
+        [rows, n_kv * head_dim], copies, of `dtype` (f32 or bf16; default the cache's, f32 for int8)."""
         torch = _t()
-        seqs, at = list(seqs), [np.zeros(0, np.int64)]
+        seqs = list(seqs)
         more = [more] * len(seqs) if isinstance(more, int) else list(more)
-        for s, n in zip(seqs, more):
-            n += self._len[self._known(s)]
-            pages = np.array(self._pages[s], np.int64)
-            _need(0 <= n <= len(pages) * self.page_size, f"sequence {s} has no {n} rows")
-            at.append((pages[:, None] * self.page_size + np.arange(self.page_size)).ravel()[:n])
-        at = torch.from_numpy(np.concatenate(at)).to(self.data.device)
-        width = self.data.shape[3]
-        return tuple(x.view(-1, width)[at] for x in (self.kpages(layer), self.vpages(layer)))
+        _need(len(more) == len(seqs), "one number of rows for each sequence")
+        lens = [self._len[self._known(s)] + n for s, n in zip(seqs, more)]
+        for s, n in zip(seqs, lens):
+            _need(0 <= n <= len(self._pages[s]) * self.page_size, f"sequence {s} has no {n} rows")
+        self.sync()
+        dev = self.data.device
+        table = self._table[torch.tensor(seqs, dtype=torch.long, device=dev)]
+        cu = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device=dev)
+        if dtype is None:
+            dtype = torch.float32 if self.scales is not None else self.data.dtype
+        return pages_rows(self.ctx, self.kpages(layer), self.vpages(layer), table, cu, sum(lens), self.n_kv,
+                          self.head_dim, dtype, **self.layer_scales(layer))
 
     def _take(self) -> int:
         p = heapq.heappop(self._free)
