@@ -164,7 +164,8 @@ def _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch):
     if len(ts) != 2 or ts[0] != batch:
         raise ValueError("table must be [batch, pages of a sequence]")
     n = ts[1]
-    return Pages(RQ_I8 if kpages.dtype == _t().int8 else _code(kpages), kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
+    code = RQ_I8 if kpages.dtype == _t().int8 else _code(kpages)
+    return Pages(code, kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
                  _i32(table, ctx, batch * n, "table"), n)
 
 
@@ -173,18 +174,21 @@ def _scales(ctx, pg, kscales, vscales) -> tuple:
     if pg.dtype != RQ_I8:
         _need(kscales is None and vscales is None, "kscales and vscales are for int8 pages")
         return None, None, 0
-    pages, blocks, heads = shape = pg.pages, pg.page_size // 16, pg.n_kv
-    f32, dev, out = _t().float32, ctx.device, []
-    for t in (kscales, vscales):
-        if t is not None and t.dtype == f32 and t.get_device() == dev and t.shape == shape:
-            s0, s1, s2 = t.stride()  # (of a dimension of one, anything)
-            if (s2 == 1 or heads == 1) and (s1 == heads or blocks == 1):
-                out.append(s0 if pages > 1 else max(s0, blocks * heads))
-                continue
-        raise ValueError(f"int8 pages need kscales and vscales, f32 CUDA tensors {list(shape)} of the context's device, "
-                         "a page's scales side by side")
-    _need(out[0] == out[1], "kscales and vscales must have one stride from page to page")
-    return kscales.data_ptr(), vscales.data_ptr(), out[0]
+    shape = pages, blocks, heads = pg.pages, pg.page_size // 16, pg.n_kv
+    if (kscales is None or vscales is None or kscales.shape != shape or vscales.shape != shape
+            or kscales.dtype != _t().float32 or vscales.dtype != kscales.dtype
+            or kscales.get_device() != ctx.device or vscales.get_device() != ctx.device):
+        _bad_scales(shape)
+    stride = s0, s1, s2 = kscales.stride()
+    # (of a dimension of one, a stride may be anything)
+    if vscales.stride() != stride or (s2 != 1 and heads != 1) or (s1 != heads and blocks != 1):
+        _bad_scales(shape)
+    return kscales.data_ptr(), vscales.data_ptr(), s0 if pages > 1 else max(s0, blocks * heads)
+
+
+def _bad_scales(shape):
+    raise ValueError(f"int8 pages need kscales and vscales, f32 CUDA tensors {list(shape)} of the context's device with "
+                     "the same strides, a page's scales side by side")
 
 
 _work_sizes: dict = {}  # rq_paged_attention_window_work by its arguments
@@ -280,9 +284,17 @@ def pages_rows(ctx: Context, kpages, vpages, table, cu, rows: int, n_kv: int, he
     pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
     sc = _scales(ctx, pg, kscales, vscales)
     raw, scope = _on(stream, kpages)
-    dtype = (_t().float32 if k_out is None else k_out.dtype) if dtype is None else dtype
-    k_out, v_out = (_empty(scope, (rows, kw), kpages, dtype) if t is None else t for t in (k_out, v_out))
-    ks, vs = _rows(k_out, ctx, rows, kw, dtype, "k_out"), _rows(v_out, ctx, rows, kw, dtype, "v_out")
+    if dtype is None:
+        dtype = _t().float32 if k_out is None else k_out.dtype
+    ks = vs = kw
+    if k_out is None:
+        k_out = _empty(scope, (rows, kw), kpages, dtype)
+    else:
+        ks = _rows(k_out, ctx, rows, kw, dtype, "k_out")
+    if v_out is None:
+        v_out = _empty(scope, (rows, kw), kpages, dtype)
+    else:
+        vs = _rows(v_out, ctx, rows, kw, dtype, "v_out")
     call("rq_pages_rows", ctx.handle, C.byref(pg), *sc, _code(k_out), _i32(cu, ctx, batch + 1, "cu"), batch, rows,
          k_out.data_ptr(), ks, v_out.data_ptr(), vs, raw)
     return k_out, v_out

@@ -54,6 +54,35 @@ __device__ __forceinline__ void rotate(float x0, float x1, float c, float s, flo
   *y1 = a1 + b1;
 }
 
+// The angle of pair i in turns for one position; cos and sin of `turns`. Whole turns are taken off in 64 bits, then quarters, and
+// |x| <= pi / 4 is left for Taylor's series to x^15 and x^16 (2^-54): a fifth of the instructions of a general sincospi.
+__device__ __forceinline__ double turns_of(int i, int head_dim, double log2_theta) {
+  return exp2(-2.0 * (double)i / (double)head_dim * log2_theta) * 0.15915494309189535;
+}
+__device__ __forceinline__ void cos_sin_turns(double turns, float* c, float* s) {
+  turns -= rint(turns);
+  const double quarter = rint(4.0 * turns), x = (turns - 0.25 * quarter) * 6.283185307179586, z = x * x;
+  double sn = -1.0 / 1307674368000.0, cn = 1.0 / 20922789888000.0;
+  sn = fma(sn, z, 1.0 / 6227020800.0);
+  cn = fma(cn, z, -1.0 / 87178291200.0);
+  sn = fma(sn, z, -1.0 / 39916800.0);
+  cn = fma(cn, z, 1.0 / 479001600.0);
+  sn = fma(sn, z, 1.0 / 362880.0);
+  cn = fma(cn, z, -1.0 / 3628800.0);
+  sn = fma(sn, z, -1.0 / 5040.0);
+  cn = fma(cn, z, 1.0 / 40320.0);
+  sn = fma(sn, z, 1.0 / 120.0);
+  cn = fma(cn, z, -1.0 / 720.0);
+  sn = fma(sn, z, -1.0 / 6.0);
+  cn = fma(cn, z, 1.0 / 24.0);
+  sn = fma(sn * z, x, x);
+  cn = fma(fma(cn, z, -0.5), z, 1.0);
+  const int q = (int)quarter;
+  const double sv = q & 1 ? cn : sn, cv = q & 1 ? sn : cn;
+  *s = (float)(q & 2 ? -sv : sv);
+  *c = (float)((q + 1) & 2 ? -cv : cv);
+}
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
@@ -393,7 +422,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
 
   // the rotated queries' digits as operands (zeros for heads and elements past the end)
   float* cs = wacc;
-  if (p.rope && tid < half) rope_angle(len, tid, hd, p.log2_theta, cs + tid, cs + HD / 2 + tid);
+  if (p.rope && tid < half) cos_sin_turns(len * turns_of(tid, hd, p.log2_theta), cs + tid, cs + HD / 2 + tid);
   for (int i = tid; i < HW * kQuery / 16; i += kThreads) reinterpret_cast<u32x4*>(sm)[i] = u32x4{0, 0, 0, 0};
   if (tid < HW * 16) qmax[tid] = 0;
   __syncthreads();
@@ -743,10 +772,11 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 // RoPE and append of packed rows, a workgroup the rows of one block and some of the heads, a wave a head at a time:
 // its rows stay in registers between their maximum and their codes.
 // Without cu row b is the one row of sequence b, at position past[b].
-template <typename A, int HD>
+template <typename A, int HD, int V>
 __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendArgs a, int chunks) {
   const PagesArgs& p = a.p;
-  __shared__ float cs[2][kBlock][HD / 2];
+  __shared__ __attribute__((aligned(16))) float cs[2][kBlock][HD / 2];
+  __shared__ double turns[HD / 2];
   const int tid = threadIdx.x, lane = tid & 63, hd = p.head_dim, half = hd / 2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = blockIdx.x % chunks;
@@ -773,15 +803,17 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
   const int in_page = (int)(block * kBlock & ((1 << p.page_bits) - 1));
   const int64_t at = ok ? ((int64_t)page << p.page_bits) + in_page : 0;  // of the block's first row
   if (p.rope) {
+    if (tid < half) turns[tid] = turns_of(tid, hd, p.log2_theta);
+    __syncthreads();
     for (int i = tid; i < rows * half; i += kThreads) {
       const int r = i / half, e = i - r * half;
-      rope_angle(pos0 + r, e, hd, p.log2_theta, &cs[0][r][e], &cs[1][r][e]);
+      cos_sin_turns((double)(pos0 + r) * turns[e], &cs[0][r][e], &cs[1][r][e]);
     }
     __syncthreads();
   }
-  typedef A A4 __attribute__((ext_vector_type(4)));
-  constexpr int N = kBlock * HD / 8 / 64;  // groups of 4 pairs a lane
-  const int hp = half / 4, kvd = p.n_kv * hd, tasks = p.n_q + 2 * p.n_kv;
+  typedef A AV __attribute__((ext_vector_type(V)));
+  constexpr int N = (kBlock * HD / 2 / V + 63) / 64;  // groups of V pairs a lane
+  const int hp = half / V, kvd = p.n_kv * hd, tasks = p.n_q + 2 * p.n_kv;
   for (int task = chunk * kWaves + wave; task < tasks; task += chunks * kWaves) {
     const int what = task < p.n_q ? 0 : task < p.n_q + p.n_kv ? 1 : 2;  // q, k, v
     const int head = what == 0 ? task : what == 1 ? task - p.n_q : task - p.n_q - p.n_kv;
@@ -790,24 +822,24 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
     const int64_t xs = what == 0 ? p.q_stride : what == 1 ? p.k_stride : p.v_stride;
     A* out = what == 2 ? nullptr : static_cast<A*>(what == 0 ? a.q_out : a.k_out);
     const int64_t os = what == 0 ? a.q_out_stride : a.k_out_stride;
-    A4 x0[N], x1[N];
+    AV x0[N], x1[N];
 #pragma unroll
     for (int k = 0; k < N; k++) {
-      const int i = lane + 64 * k, r = i / hp, e = 4 * (i - r * hp);
+      const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
       if (r < rows) {
-        x0[k] = *reinterpret_cast<const A4*>(x + (row0 + r) * xs + e);
-        x1[k] = *reinterpret_cast<const A4*>(x + (row0 + r) * xs + e + half);
+        x0[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e);
+        x1[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e + half);
       }
     }
-    float y0[N][4], y1[N][4], amax = 0.0f;
+    float y0[N][V], y1[N][V], amax = 0.0f;
     bool good = true;
 #pragma unroll
     for (int k = 0; k < N; k++) {
-      const int i = lane + 64 * k, r = i / hp, e = 4 * (i - r * hp);
+      const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
       if (r >= rows) continue;
-      A4 z0, z1;
+      AV z0, z1;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < V; j++) {
         y0[k][j] = (float)x0[k][j], y1[k][j] = (float)x1[k][j];
         if (what < 2 && p.rope) rotate(y0[k][j], y1[k][j], cs[0][r][e + j], cs[1][r][e + j], &y0[k][j], &y1[k][j]);
         amax = fmaxf(amax, fmaxf(fabsf(y0[k][j]), fabsf(y1[k][j])));
@@ -817,8 +849,8 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
       }
       if (out != nullptr) {
         A* o = out + (row0 + r) * os + head * hd + e;
-        *reinterpret_cast<A4*>(o) = z0;
-        *reinterpret_cast<A4*>(o + half) = z1;
+        *reinterpret_cast<AV*>(o) = z0;
+        *reinterpret_cast<AV*>(o + half) = z1;
       }
     }
     if (what == 0 || !ok) continue;
@@ -834,19 +866,26 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
         *w = recoded(*w, ratio);
       }
     }
+    typedef uint32_t CV __attribute__((ext_vector_type(V / 4)));
 #pragma unroll
     for (int k = 0; k < N; k++) {
-      const int i = lane + 64 * k, r = i / hp, e = 4 * (i - r * hp);
+      const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
       if (r >= rows) continue;
-      int d0[4], d1[4];
+      CV w0, w1;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        d0[j] = code_of(y0[k][j], s);
-        d1[j] = code_of(y1[k][j], s);
+      for (int n = 0; n < V / 4; n++) {
+        int d0[4], d1[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          d0[j] = code_of(y0[k][4 * n + j], s);
+          d1[j] = code_of(y1[k][4 * n + j], s);
+        }
+        w0[n] = pack4(d0);
+        w1[n] = pack4(d1);
       }
       int8_t* o = codes + (int64_t)(before + r) * kvd + e;
-      *reinterpret_cast<uint32_t*>(o) = pack4(d0);
-      *reinterpret_cast<uint32_t*>(o + half) = pack4(d1);
+      *reinterpret_cast<CV*>(o) = w0;
+      *reinterpret_cast<CV*>(o + half) = w1;
     }
     if (lane == 0) *scale = s;
   }
@@ -888,21 +927,21 @@ hipError_t run_paged_q8_hd(const PagedAttnArgs& a, hipStream_t stream) {
   return run_paged_q8_heads<A, 256, true>(a, stream);
 }
 
-template <typename A, int HD>
+template <typename A, int HD, int V>
 hipError_t run_append_q8(const PagesAppendArgs& a, hipStream_t stream) {
   // A wave takes one head of a small call, more of a large one, so that the angles are formed less often
   const int64_t slots = append_q8_slots(a), tasks = a.p.n_q + 2 * a.p.n_kv;
   const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((tasks + kWaves - 1) / kWaves, (2048 + slots - 1) / slots));
-  hipLaunchKernelGGL((pages_append_q8_kernel<A, HD>), dim3((unsigned)(slots * chunks)), dim3(kThreads), 0, stream, a,
+  hipLaunchKernelGGL((pages_append_q8_kernel<A, HD, V>), dim3((unsigned)(slots * chunks)), dim3(kThreads), 0, stream, a,
                      (int)chunks);
   return hipGetLastError();
 }
 
-template <typename A>
+template <typename A, int V>
 hipError_t run_append_q8_hd(const PagesAppendArgs& a, hipStream_t stream) {
-  if (a.p.head_dim <= 64) return run_append_q8<A, 64>(a, stream);
-  if (a.p.head_dim <= 128) return run_append_q8<A, 128>(a, stream);
-  return run_append_q8<A, 256>(a, stream);
+  if (a.p.head_dim <= 64) return run_append_q8<A, 64, V>(a, stream);
+  if (a.p.head_dim <= 128) return run_append_q8<A, 128, V>(a, stream);
+  return run_append_q8<A, 256, V>(a, stream);
 }
 
 // The stored rows of sequences, packed: a workgroup ROWS of them, whose places in the pages are looked up first.
@@ -1045,7 +1084,9 @@ hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStrea
 }
 
 hipError_t launch_pages_append_q8(int dtype, const PagesAppendArgs& a, hipStream_t stream) {
-  return dtype == RQ_F32 ? run_append_q8_hd<float>(a, stream) : run_append_q8_hd<__bf16>(a, stream);
+  // 16 bytes a load where a half of a head is whole ones of them
+  if (dtype == RQ_F32) return run_append_q8_hd<float, 4>(a, stream);
+  return a.p.head_dim % 16 == 0 ? run_append_q8_hd<__bf16, 8>(a, stream) : run_append_q8_hd<__bf16, 4>(a, stream);
 }
 
 hipError_t launch_pages_rows(int dtype, int cache_dtype, const PagesRowsArgs& a, hipStream_t stream) {
