@@ -483,8 +483,21 @@ static int fwd_split_groups(int dtype, const PromptArgs& a) {
   if (a.rows_k < 64 * (int64_t)a.batch) return f32 ? 2 : 0;  // hardly a tile of keys to split
   const bool few_queries = a.rows_k >= 4 * a.rows_q;  // every tile sees most keys
   if (f32 && few_queries) return f32_few_queries_groups(a, narrow);
-  const int one = broad ? 0 : narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
-  const int two = broad && !few_queries ? 320 : narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
+  int one = broad ? 0 : narrow ? (f32 ? 320 : 256) : few_queries ? 256 : f32 ? 152 : 128;
+  int two = broad && !few_queries ? 320 : narrow ? (f32 ? 640 : 576) : f32 ? 352 : 448;
+  // With a window a workgroup walks it and its own queries' keys: fewer queries a workgroup cost more of them, the
+  // sooner the shorter the window. us, windows of 32 / 128 / 400, 128, 64 and 32 queries:
+  //   f32   x 128: 512 (80) 38, 26, 32 / 53, 31, 33 / 85, 51, 39   1024 (144) 39, 27, 53 / 54, 33, 61 / 95, 58, 81
+  //         1024 (32/8, 288) 41, 50, 99 / 56, 61, 110 / 97, 107, 144   2048 (272), 64 / 256 / 1024: 47, 53, 103 / 75, 84, 147 / 185, 194, 240
+  //         16/2 x 64: 1024 (144) 25, 17, 22 / 34, 20, 23 / 56, 33, 33   4096 (528) 39, 42, 69 / 51, 52, 78 / 89, 95, 121
+  //   bf16  x 128: 512 (80) 17, 12, 14 / 20, 14, 14 / 22, 18, 15   1024 (144) 17, 13, 23 / 20, 14, 25 / 28, 20, 29
+  //         16/2 x 64: 1024 (144) 15, 11, 12 / 18, 11, 12 / 24, 16, 15
+  if (a.window > 0 && !few_queries) {
+    if (f32)
+      one = 96, two = narrow ? 400 : 256;
+    else if (a.window <= 256)
+      one = 0;
+  }
   const int64_t groups = tile_slots(a.rows_q, a.batch, 128) * a.n_q * 256;
   return groups <= (int64_t)one * a.cu_count ? 1 : groups <= (int64_t)two * a.cu_count ? 2 : 0;
 }
@@ -504,7 +517,10 @@ int prompt_fwd_tile(int dtype, const PromptArgs& a) {
   // us, this / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 52 / 43, 4 x 1024 68 / 58, 4 x 3000
   // 314 / 312, 4 x 4096 548 / 548, 4096 139 / 142, 8192 502 / 520, 16384 1919 / 2021; 16/16 heads: 4096
   // 106 / 103, 4 x 4096 279 / 281, 8192 256 / 267.
-  const bool pair = dtype == RQ_BF16 && a.head_dim > 64 && a.head_dim <= 128 && a.rows_q / a.batch > 4096;
+  // With a window the wider tile has more at both of its edges: 16384 tokens, 32/8 heads, windows of 256, 1024 and 4096 301 / 196,
+  // 457 / 367, 1010 / 970; 32768, 16/4 heads, 8192 1816 / 1847, 16384 2957 / 3065.
+  const bool pair = dtype == RQ_BF16 && a.head_dim > 64 && a.head_dim <= 128 && a.rows_q / a.batch > 4096 &&
+                    (a.window == 0 || a.window >= 8192);
   return pair ? 256 : 128;
 }
 

@@ -104,11 +104,14 @@ CASES = [
     ("f32", 3, 3, 40, [77], [77]),
     ("f32", 2, 1, 256, [170, 9], [170, 9]),
     ("f32", 2, 2, 128, [5, 64, 100], [300, 64, 40]),
+    ("bf16", 4, 2, 128, [700], [700]),
+    ("bf16", 4, 2, 48, [700, 33], [700, 33]),
     ("f32", 128, 8, 40, [300, 129, 90], [300, 129, 90]),
+    ("f32", 32, 8, 64, [300, 129, 90], [300, 129, 90]),
     ("f32", 64, 8, 128, [300, 129, 90], [300, 129, 90]),
     ("f32", 128, 8, 104, [300, 0, 90], [310, 129, 90]),
 ]
-WINDOWS = [(1, 0), (7, 3), (32, 0), (33, 1), (64, 4), (100, 70), (250, 4)]
+WINDOWS = [(1, 0), (7, 3), (32, 0), (33, 1), (64, 4), (100, 70), (250, 4), (300, 4)]
 
 
 def data(torch, t, nq, nkv, hd, lq, lk, seed):
@@ -150,6 +153,8 @@ LONG = [
     (4, 4, 128, [4200], [9000], 4096, 4),
     (4, 4, 128, [4999], [0], 16, 1),
     (4, 2, 128, [6000], [6000], 1, 0),
+    (6, 2, 128, [12500], [12500], 8192, 3),         # the kernel of 256 queries
+    (6, 6, 72, [6100, 5000], [15000, 5000], 8200, 70),
 ]
 
 
@@ -158,6 +163,8 @@ def test_long_sequences(torch, ctx, nq, nkv, hd, lq, lk, window, sinks):
     import raster_amd
 
     print(f"[gpu] window long {nq}/{nkv}x{hd} {lq} {lk} {window}+{sinks}", flush=True)
+    if window >= 8192:
+        assert tile(ctx, "bf16", nq, nkv, hd, lq, lk, window, sinks) == 256
     q, k, v, do = data(torch, "bf16", nq, nkv, hd, lq, lk, sum(lq))
     cu, cu_k, scale = cu_of(torch, lq), None if lq == lk else cu_of(torch, lk), hd ** -0.5
     lse = torch.empty((nq, sum(lq)), device="cuda")
@@ -320,3 +327,14 @@ def test_gradient_of_sinks_by_chunks(torch, ctx, t, nq, nkv, hd, lens, window, s
         check_gradient(torch, q, k, v, do, grads, lens, lk, nq, nkv, hd, scale, window, sinks)
         again = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, **see)
         assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+def test_every_kernel_has_a_case(ctx):
+    """The tiles that the cases here reach, by type and padded head size."""
+    seen = {(t, 64 if hd <= 64 else 128 if hd <= 128 else 256, tile(ctx, t, nq, nkv, hd, lq, lk, w, z))
+            for t, nq, nkv, hd, lq, lk in CASES for w, z in WINDOWS}
+    seen |= {("bf16", 64 if hd <= 64 else 128, tile(ctx, "bf16", nq, nkv, hd, lq, lk, w, z))
+             for nq, nkv, hd, lq, lk, w, z in LONG}
+    want = {(t, w, n) for t in ("f32", "bf16") for w in (64, 128) for n in (32, 64, 128)}
+    want |= {("bf16", 256, 64), ("bf16", 256, 128), ("f32", 256, 128), ("bf16", 128, 256)}
+    assert want <= seen, want - seen
