@@ -26,7 +26,7 @@ struct PromptArgs {
   float* part;   // [nsplit][dv, dk][rows_k][n_kv * head_dim] when nsplit > 1
   int nsplit;
   // With sink_tiles > 0 the gradients of every sequence's first sink_tiles tiles of 64 keys are summed by chunks of
-  // sink_chunk queries: sink_part [sink_slots][sink_tiles][n_kv][dv, dk][64][head_dim]
+  // sink_chunk queries: sink_part [sink_slots][nsplit][sink_tiles][n_kv][dv, dk][64][head_dim]
   int sink_tiles, sink_chunk;
   int64_t sink_slots;
   float* sink_part;

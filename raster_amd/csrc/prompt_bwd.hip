@@ -226,8 +226,10 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
   constexpr int kBuf = 2 * kTile + 2 * BQ * 4;  // Q, dO, then L and D of the rows
   constexpr int kShare = Handover<T>::N * 16 * 64, kPair = NT * kShare;  // weights of 32 keys and 32 or all queries
   const int group = a.n_q / a.n_kv;
-  const int hkv = block % a.n_kv, rest = block / a.n_kv, parts = WIN && sink ? a.sink_tiles : a.nsplit, split = rest % parts;
-  const int64_t slot = rest / parts;  // a sequence's first keys, which most queries see, first
+  const int hkv = block % a.n_kv, rest = block / a.n_kv, split = rest % a.nsplit;
+  const int sink_tile = WIN && sink ? rest / a.nsplit % a.sink_tiles : 0;
+  // a sequence's first keys, which most queries see, first
+  const int64_t slot = WIN && sink ? rest / a.nsplit / a.sink_tiles : rest / a.nsplit;
   TileSpan tk;
   int chunk = 0;  // first query of the chunk
   if (WIN && sink) {
@@ -237,7 +239,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
     const int64_t k0 = clamp_cu(a.cu_k, tk.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tk.seq + 1, a.rows_k);
     tk.begin = k0;
     tk.len = (int)(k1 > k0 ? k1 - k0 : 0);
-    tk.row0 = split * kDkvKeys;
+    tk.row0 = sink_tile * kDkvKeys;
     if (tk.row0 >= tk.len) return;
   } else {
     tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, kDkvKeys, slot);
@@ -270,9 +272,7 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
                         : WIN && tk.row0 >= a.sinks ? min(lq, tk.row0 + kDkvKeys - 1 - off + a.window) : lq;
   const int per_head = qend > qstart ? (qend - qstart + BQ - 1) / BQ : 0;
   const int64_t steps = (int64_t)per_head * group;
-  const bool whole_chunk = WIN && sink;
-  const int s0 = whole_chunk ? 0 : (int)(steps * split / a.nsplit);
-  const int s1 = whole_chunk ? (int)steps : (int)(steps * (split + 1) / a.nsplit);
+  const int s0 = (int)(steps * split / a.nsplit), s1 = (int)(steps * (split + 1) / a.nsplit);
   Stage<T, HD, BQ, THREADS> qs, os;
   float rowv = 0.0f;  // L (the first BQ threads) or D (as many more) of the next tile's rows
   auto load = [&](int hq, int r) {
@@ -376,7 +376,8 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
   const float factor = is_k ? a.scale : 1.0f;
   const int64_t at = tk.begin + kj;
   if (WIN && sink) {
-    float* part = a.sink_part + (((slot * a.sink_tiles + split) * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * a.head_dim);
+    float* part = a.sink_part + ((((slot * a.nsplit + split) * a.sink_tiles + sink_tile) * a.n_kv + hkv) * 2 + is_k) *
+                                   (kDkvKeys * a.head_dim);
     store_rows<float, HD>(part + (kj - tk.row0) * a.head_dim, acc, factor, h, a.head_dim);
   } else if (a.nsplit > 1) {
     float* part = a.part + ((int64_t)(2 * split + is_k) * a.rows_k + at) * (a.n_kv * a.head_dim) + hkv * a.head_dim;
@@ -421,14 +422,14 @@ __global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a) {
   const int64_t k0 = clamp_cu(a.cu_k, b, a.rows_k), k1 = clamp_cu(a.cu_k, b + 1, a.rows_k);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), keys = (int)min(k1 - k0 - tile * kDkvKeys, (int64_t)kDkvKeys);
   const int64_t slot = q0 / a.sink_chunk + b;
-  const int chunks = (lq + a.sink_chunk - 1) / a.sink_chunk, hd = a.head_dim;
+  const int parts = (lq + a.sink_chunk - 1) / a.sink_chunk * a.nsplit, hd = a.head_dim;
   const int64_t step = (int64_t)a.sink_tiles * a.n_kv * 2 * kDkvKeys * hd;
   typedef T T4 __attribute__((ext_vector_type(4)));
   for (int i = part_of * 256 + threadIdx.x; i < 2 * keys * (hd / 4); i += kSinkParts * 256) {
     const int is_k = i >= keys * (hd / 4), j = is_k ? i - keys * (hd / 4) : i, row = j / (hd / 4), e = 4 * (j % (hd / 4));
-    const float* part = a.sink_part + slot * step + ((tile * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * hd) + row * hd + e;
+    const float* part = a.sink_part + slot * a.nsplit * step + ((tile * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * hd) + row * hd + e;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = 0; c < chunks; c++) x += *reinterpret_cast<const f32x4*>(part + c * step);
+    for (int c = 0; c < parts; c++) x += *reinterpret_cast<const f32x4*>(part + c * step);
     T4 y;
 #pragma unroll
     for (int n = 0; n < 4; n++) y[n] = (T)x[n];
@@ -643,7 +644,7 @@ template <typename T, int HD, int BK, int QG, bool WIN>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prompt_grad_kernel(PromptArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int block = blockIdx.x;
-  const int sinks = WIN ? (int)(a.sink_slots * a.sink_tiles * a.n_kv) : 0;
+  const int sinks = WIN ? (int)(a.sink_slots * a.sink_tiles * a.n_kv * a.nsplit) : 0;
   const int dkv = sinks + (int)(a.k_slots * a.n_kv * a.nsplit);
   if (block < dkv)
     dkv_body<T, HD, WIN>(a, block < sinks ? block : block - sinks, block < sinks, lds);
@@ -677,18 +678,18 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   const auto kernel = prompt_grad_kernel<T, HD, BK, QG, WIN>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
-  const int64_t sinks = a.sink_slots * a.sink_tiles * a.n_kv;
+  const int64_t sinks = a.sink_slots * a.sink_tiles * a.n_kv * a.nsplit;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(sinks + a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256),
                      lds, stream, a);
   if (hipError_t e = hipGetLastError()) return e;
-  if (WIN && a.sink_tiles > 0) {
-    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * kSinkParts)), dim3(256), 0,
-                       stream, a);
-    return hipGetLastError();
-  }
   if (a.nsplit > 1 && a.rows_k > 0) {
     const int64_t n = a.rows_k * (a.n_kv * a.head_dim / 4);
     hipLaunchKernelGGL(prompt_dkv_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (WIN && a.sink_tiles > 0) {  // (after the parts' sums, which know nothing of these keys and write what was there)
+    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * kSinkParts)), dim3(256), 0,
+                       stream, a);
     return hipGetLastError();
   }
   return hipSuccess;
@@ -697,30 +698,31 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
 }  // namespace
 
 // Parts of the (head, query tile) steps of the keys' gradients: enough that the grid is
-// kDkvGroups workgroups, while a part keeps 4 query tiles of the longest sequence that the rows allow.
-// (With a window a key's queries are those of the window.)
+// 768 workgroups, while a part keeps 4 query tiles of the longest sequence that the rows allow.
+// With a window, whose keys all have about as many queries, fewer and longer parts: us of forward and gradient, 768 and 4 /
+// 512 and 5: 129, 300, 64, 511 (f32, 16/2 x 64, window 100) 72 / 68   2048 (f32, 16/2 x 64, 64) 131 / 117   2048 (f32, 32/8 x 128, 64) 408 / 386
+// 2048 (bf16, 32/8 x 128, 256) 151 / 141
 PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
-  constexpr int64_t kDkvGroups = 768;
   const int64_t batch = a.batch, rows_q = a.rows_q, rows_k = a.rows_k, n_q = a.n_q, n_kv = a.n_kv, head_dim = a.head_dim;
   const int64_t groups = std::max<int64_t>(1, (rows_k + kDkvKeys - 1) / kDkvKeys * n_kv);
+  const int64_t most = a.window > 0 ? 512 : 768, least_steps = a.window > 0 ? 5 : 4;
   int64_t longest = rows_q / std::max<int64_t>(batch, 1);
   if (a.window > 0) longest = std::min<int64_t>(longest, a.window + kDkvKeys);
   const int64_t steps = longest / 32 * (n_q / n_kv);
   PromptBwdPlan p;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kDkvGroups / groups, steps / 4, 16}));
-  // Chunks of the first keys' queries, of about as many steps as the other keys have: where the grid is thick enough
-  // (a thin one splits all steps anyway) and a sequence can be longer than the window and a chunk; with many
-  // sinks their tiles are workgroups enough.
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({most / groups, steps / least_steps, 16}));
+  // Chunks of the first keys' queries, of about as many steps as the other keys have and in as many parts, where a sequence can be longer
+  // than the window and a chunk; with many sinks their tiles are workgroups enough.
   p.sink_tiles = p.sink_chunk = 0;
   p.sink_slots = 0;
   const int tiles = (a.sinks + kDkvKeys - 1) / kDkvKeys;
   const int chunk = std::min(std::max((a.window + 63) / 64 * 64, 256), 2048);
-  if (a.window > 0 && p.nsplit == 1 && tiles > 0 && tiles <= 8 && rows_q > a.window + chunk) {
+  if (a.window > 0 && tiles > 0 && tiles <= 8 && rows_q > a.window + chunk) {
     p.sink_tiles = tiles;
     p.sink_chunk = chunk;
     p.sink_slots = tile_slots(rows_q, batch, chunk);
   }
-  const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv;
+  const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv * p.nsplit;
   p.groups = std::max(sinks + tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
                       std::max<int64_t>((rows_q * n_q * kDeltaLanes + 255) / 256, std::max<int64_t>(batch * n_q * kExactTiles, batch * n_kv * p.sink_tiles * kSinkParts)));
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
