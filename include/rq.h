@@ -569,8 +569,9 @@ int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, in
 /* rq_prompt_attention and its gradient with a sliding window and sinks: the query at position i = its row +
  * keys - queries of its sequence sees the keys j <= i with i - j < window, or with j < sinks (the first tokens, which
  * stay visible). window 0: all keys up to i, as without; else causal must be 1. A query sees itself at least, so only one
- * before the first key (more queries than keys) sees nothing. Otherwise as above; the reach of a NaN or an inf in
- * keys or values that a query does not see is the same on both sides of the window. */
+ * before the first key (more queries than keys) sees nothing. Otherwise as above; a NaN or an inf in
+ * keys or values that a query does not see reaches as far before its window as behind it, one in the rows behind the sinks, of
+ * the same 64, queries whose window begins less than 320 after it. */
 int rq_prompt_attention_window(rq_ctx ctx, const rq_prompt* p, int64_t window, int64_t sinks, const void* q,
                                int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                                void* out, int64_t out_stride, float* lse, void* stream);

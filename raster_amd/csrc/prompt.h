@@ -58,17 +58,25 @@ template <bool WIN>
 struct Walk {  // the keys of a workgroup's steps
   __device__ __forceinline__ int leave_out(const PromptArgs&, int, int) { return 0; }
   __device__ __forceinline__ int key(int at) const { return at; }
+  __device__ __forceinline__ int rows_from(int key, int lk) const { return lk - key; }  // that are read from `key` on
 };
 template <>
 struct Walk<true> {
-  int sink_end, skip;
+  int sink_end, sink_rows, skip;
   // pos: position of the first query, bk: keys of a step. Returns how many keys are left out.
   __device__ __forceinline__ int leave_out(const PromptArgs& a, int pos, int bk) {
     sink_end = (a.sinks + bk - 1) / bk * bk;
-    skip = max(max(pos - a.window + 1, 0) / bk * bk - sink_end, 0);
+    const int begin = max(pos - a.window + 1, 0);
+    skip = max(begin / bk * bk - sink_end, 0);
+    // behind the sinks, where no query's window reaches, rows are taken as zeros: a NaN in their values must not
+    // reach every later query
+    sink_rows = begin >= sink_end ? a.sinks : sink_end;
     return skip;
   }
   __device__ __forceinline__ int key(int at) const { return at < sink_end ? at : at + skip; }
+  __device__ __forceinline__ int rows_from(int key, int lk) const {
+    return (key < sink_end ? min(lk, sink_rows) : lk) - key;
+  }
 };
 
 // whether the query at `pos` sees by its window or the sinks any, or all, of the n keys from `key` on

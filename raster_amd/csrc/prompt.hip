@@ -213,8 +213,8 @@ __global__ __launch_bounds__(256) void prompt_fwd_kernel(PromptArgs a) {
   if (!w.init(a, wave, lane)) return;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int key) {
-    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
-    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.rows_from(key, w.lk), a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.rows_from(key, w.lk), a.head_dim, tid);
   };
   if (w.nk > 0) load(w.key(0));
   Queries<T, HD, BK> x;
@@ -272,8 +272,8 @@ __global__ __launch_bounds__(512, 2) void prompt_fwd_pair_kernel(PromptArgs a) {
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int t) {
     const int key = w.key(t * BK);
-    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
-    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.rows_from(key, w.lk), a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.rows_from(key, w.lk), a.head_dim, tid);
   };
   auto k_tile = [&](int t) { return lds + (t & 1) * kTile; };
   auto v_tile = [&](int t) { return lds + (2 + t % 3) * kTile; };
@@ -342,8 +342,8 @@ __global__ __launch_bounds__(256) void prompt_fwd_split_kernel(PromptArgs a) {
   if (!w.init(a, wave / KG, lane)) return;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int key) {
-    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.lk - key, a.head_dim, tid);
-    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.lk - key, a.head_dim, tid);
+    ks.load(w.k + (int64_t)key * a.k_stride, a.k_stride, w.rows_from(key, w.lk), a.head_dim, tid);
+    vs.load(w.v + (int64_t)key * a.v_stride, a.v_stride, w.rows_from(key, w.lk), a.head_dim, tid);
   };
   if (w.nk > 0) load(w.key(0));
   Queries<T, HD, 32> x;

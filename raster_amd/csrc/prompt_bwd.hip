@@ -296,81 +296,96 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
     load(hq, r);
     store(lds);
   }
-  for (int step = s0, buf = 0; step < s1; step++, buf ^= 1) {
-    const char* qt = lds + buf * kBuf;
-    const char* ot = qt + kTile;
-    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile) + (is_k ? BQ : 0) + 4 * h;
-    int next_hq = hq + 1, next_r = r;
-    if (next_hq == (hkv + 1) * group) next_hq = hkv * group, next_r -= BQ;
-    if (step + 1 < s1) load(next_hq, next_r);
-    __syncthreads();
-    const bool seen = (!a.causal || r + BQ - 1 + off >= w_key) && window_any<WIN>(a, r + off, w_key, 32);
-    const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off) &&
-                       window_all<WIN>(a, r + BQ - 1 + off, w_key, 32);
-    // value i of product t: query r + 32 t + 8 (i / 4) + 4 h + i % 4, the lane's key
-    auto see = [&](int t, int i) {
-      const int qi = r + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-      return qi < lq && live && (!a.causal || kj <= qi + off) && window_any<WIN>(a, qi + off, kj, 1);
-    };
-    float x[NT][16];
-    Frag pf[NT][2];  // bf16: weights and their gradients rounded to nearest for the products
-    if (seen) {
-      const char* t1 = is_k ? ot : qt;
-      f32x16 s[NT] = {};
+  // From the last queries down. Of a tile with sinks first those that see nothing else of the wave's keys: what they gave to
+  // keys that are no sinks is 0 times their rows, and a NaN in one must not stay there.
+  int behind = s0;
+  if (WIN && tk.row0 < a.sinks) {
+    const int near = (w_key + 31 + a.window - off - qstart + BQ - 1) / BQ;  // query tiles before those
+    behind = min(max((per_head - min(max(near, 0), per_head)) * group, s0), s1);
+  }
+  int step = s0, buf = 0;
+#pragma unroll 1
+  for (int part = WIN ? 0 : 1; part < 2; part++) {
+    const int stop = part == 0 ? behind : s1;
+    for (; step < stop; step++, buf ^= 1) {
+      const char* qt = lds + buf * kBuf;
+      const char* ot = qt + kTile;
+      const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile) + (is_k ? BQ : 0) + 4 * h;
+      int next_hq = hq + 1, next_r = r;
+      if (next_hq == (hkv + 1) * group) next_hq = hkv * group, next_r -= BQ;
+      if (step + 1 < s1) load(next_hq, next_r);
+      __syncthreads();
+      const bool seen = (!a.causal || r + BQ - 1 + off >= w_key) && window_any<WIN>(a, r + off, w_key, 32);
+      const bool whole = r + BQ <= lq && w_key + 32 <= tk.len && (!a.causal || w_key + 31 <= r + off) &&
+                         window_all<WIN>(a, r + BQ - 1 + off, w_key, 32);
+      // value i of product t: query r + 32 t + 8 (i / 4) + 4 h + i % 4, the lane's key
+      auto see = [&](int t, int i) {
+        const int qi = r + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
+        return qi < lq && live && (!a.causal || kj <= qi + off) && window_any<WIN>(a, qi + off, kj, 1);
+      };
+      float x[NT][16];
+      Frag pf[NT][2];  // bf16: weights and their gradients rounded to nearest for the products
+      if (seen) {
+        const char* t1 = is_k ? ot : qt;
+        f32x16 s[NT] = {};
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++) s[t] = tile_mma(TL::frag(t1, 32 * t + (lane & 31), d, h), f[d], s[t]);
-      if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 1>();
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 32 * t + 8 * g);
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            x[t][4 * g + j] = is_k ? s[t][4 * g + j] - c[j] : fmaf(s[t][4 * g + j], a.scale2, -c[j]);
-        }
-        if (!is_k) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) x[t][i] = __builtin_amdgcn_exp2f(x[t][i]);
-          if (!whole)
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
-#pragma unroll
-          for (int u = 0; u < 2; u++) tile_pack(x[t] + 8 * u, pf[t][u]);
-          Handover<T>::put(pair + t * kShare, x[t]);
-        }
-      }
-    }
-    __syncthreads();
-    if (seen) {
-      if (is_k) {
+          for (int d = 0; d < HD / 16; d++) s[t] = tile_mma(TL::frag(t1, 32 * t + (lane & 31), d, h), f[d], s[t]);
+        if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 1>();
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-          float p[16];
-          Handover<T>::take(pair + t * kShare, p);
 #pragma unroll
-          for (int i = 0; i < 16; i++) x[t][i] *= p[i];
-          if (!whole)  // what is masked has weight 0, and its other factor may be anything
+          for (int g = 0; g < 4; g++) {
+            const f32x4 c = *reinterpret_cast<const f32x4*>(rows + 32 * t + 8 * g);
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
-          tile_pack(x[t], pf[t][0]);
-          tile_pack(x[t] + 8, pf[t][1]);
+            for (int j = 0; j < 4; j++)
+              x[t][4 * g + j] = is_k ? s[t][4 * g + j] - c[j] : fmaf(s[t][4 * g + j], a.scale2, -c[j]);
+          }
+          if (!is_k) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[t][i] = __builtin_amdgcn_exp2f(x[t][i]);
+            if (!whole)
+#pragma unroll
+              for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; u++) tile_pack(x[t] + 8 * u, pf[t][u]);
+            Handover<T>::put(pair + t * kShare, x[t]);
+          }
         }
       }
-      const char* t2 = is_k ? qt : ot;
+      __syncthreads();
+      if (seen) {
+        if (is_k) {
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+          for (int t = 0; t < NT; t++) {
+            float p[16];
+            Handover<T>::take(pair + t * kShare, p);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+            for (int i = 0; i < 16; i++) x[t][i] *= p[i];
+            if (!whole)  // what is masked has weight 0, and its other factor may be anything
 #pragma unroll
-          for (int d = 0; d < HD / 32; d++)
-            acc[d] = tile_mma(TL::frag_t(t2, 32 * t + 16 * u, d, lane), pf[t][u], acc[d]);
-      if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 2>();
+              for (int i = 0; i < 16; i++) x[t][i] = see(t, i) ? x[t][i] : 0.0f;
+            tile_pack(x[t], pf[t][0]);
+            tile_pack(x[t] + 8, pf[t][1]);
+          }
+        }
+        const char* t2 = is_k ? qt : ot;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++)
+              acc[d] = tile_mma(TL::frag_t(t2, 32 * t + 16 * u, d, lane), pf[t][u], acc[d]);
+        if constexpr (sizeof(T) == 2) order_products<NT * HD / 16, 2>();
+      }
+      if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
+      hq = next_hq, r = next_r;
     }
-    if (step + 1 < s1) store(lds + (buf ^ 1) * kBuf);
-    hq = next_hq, r = next_r;
+    if (WIN && part == 0 && tk.row0 < a.sinks && kj >= a.sinks)
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++) acc[d] = f32x16{};
   }
   if (!live) return;
   const float factor = is_k ? a.scale : 1.0f;
@@ -497,10 +512,10 @@ __device__ __forceinline__ void dq_body(const PromptArgs& a, int block, char* ld
   const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load_k = [&](int key) {
-    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, lk - key, a.head_dim, tid);
+    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, walk.rows_from(key, lk), a.head_dim, tid);
   };
   auto load_v = [&](int key) {
-    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, lk - key, a.head_dim, tid);
+    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, walk.rows_from(key, lk), a.head_dim, tid);
   };
   if (nk > 0) {
     load_k(walk.key(0));
@@ -582,8 +597,8 @@ __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, ch
   const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
   Stage<T, HD, BK, THREADS> ks, vs;
   auto load = [&](int key) {
-    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, lk - key, a.head_dim, tid);
-    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, lk - key, a.head_dim, tid);
+    ks.load(kbase + (int64_t)key * a.k_stride, a.k_stride, walk.rows_from(key, lk), a.head_dim, tid);
+    vs.load(vbase + (int64_t)key * a.v_stride, a.v_stride, walk.rows_from(key, lk), a.head_dim, tid);
   };
   if (nk > 0) load(walk.key(0));
   const T* qrow = live ? static_cast<const T*>(a.q) + (tq.begin + qi) * a.q_stride + hq * a.head_dim : nullptr;

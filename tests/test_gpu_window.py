@@ -338,3 +338,40 @@ def test_every_kernel_has_a_case(ctx):
     want = {(t, w, n) for t in ("f32", "bf16") for w in (64, 128) for n in (32, 64, 128)}
     want |= {("bf16", 256, 64), ("bf16", 256, 128), ("f32", 256, 128), ("bf16", 128, 256)}
     assert want <= seen, want - seen
+
+
+@pytest.mark.parametrize("t,nq,n,window,sinks", [(t, *c) for t in ("bf16", "f32") for c in (
+    (2, 1500, 64, 4), (16, 1500, 64, 4), (2, 5000, 200, 1), (16, 5000, 200, 70))] + [("bf16", 6, 12500, 8192, 2)])
+def test_nan_behind_the_sinks(torch, ctx, t, nq, n, window, sinks):
+    """Keys and values of NaN in the sinks' own tile, but no sinks, reach no query whose window begins 320 rows after them;
+    a query and a gradient of NaN reach the sinks and their window's keys, and no other 95 rows from those."""
+    import raster_amd
+
+    nkv, hd, at = nq // 2, 128, sinks + 7
+    print(f"[gpu] window NaN behind the sinks {t} {nq} heads {n}", flush=True)
+    q, k, v, do = (x.clone() for x in data(torch, t, nq, nkv, hd, [n], [n], 8))
+    cu, scale = cu_of(torch, [n]), hd ** -0.5
+
+    def both():
+        lse = torch.empty((nq, n), device="cuda")
+        out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse, window=window, sinks=sinks)
+        return [out, *raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, window=window,
+                                                      sinks=sinks)]
+
+    clean, kept = both(), (k[at].clone(), v[at].clone())
+    k[at], v[at] = float("nan"), float("inf")
+    dirty = both()
+    far = at + window + 320
+    assert bool(torch.isnan(dirty[0][at:at + window]).all())
+    for a, b in zip(clean[:2], dirty[:2]):
+        assert torch.equal(a[:at - 94], b[:at - 94]) if at > 94 else True
+        assert torch.equal(a[far:], b[far:])
+    k[at], v[at] = kept
+    last = n - 10
+    q[last], do[last] = float("nan"), float("inf")
+    dirty = both()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[:sinks] = False
+    keep[max(0, last - window + 1 - 94):] = False
+    for a, b in zip(clean[2:], dirty[2:]):
+        assert bool(torch.isnan(b[:sinks]).all()) and torch.equal(a[keep], b[keep])
