@@ -465,3 +465,89 @@ def test_offsets_past_32_bits(torch, ctx):
         outs.append(got)
     assert all(torch.equal(a, b) for a, b in zip(*outs))
     assert torch.equal(data[:, total - used:], small) and torch.equal(scales[:, total - used:], ssmall)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,batch", [(4, 2, 64, 1500), (8, 4, 64, 2100), (20, 1, 40, 1030)])
+def test_attention_of_many_sequences(torch, ctx, nq, nkv, hd, batch):
+    """More sequences than one launch plans for, a few long ones among short and idle ones, q, k, v and out as columns of
+    wider arrays: as in batches of 100, up to the ranges that long ones are cut into, and the same bits in the cache."""
+    import raster_amd
+
+    print(f"[gpu] q8 attention of {batch} sequences {nq}/{nkv}x{hd}", flush=True)
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(-1, 40, (batch,), generator=gen)
+    lens[[3, batch // 2, batch - 2]] = torch.tensor([1900, 700, 2000])
+    need = (lens + 16) // 16
+    first = torch.cat([torch.zeros(1, dtype=torch.long), need.cumsum(0)])
+    table = torch.full((batch, 127), -1, dtype=torch.int32)
+    order = torch.randperm(int(first[-1]), generator=gen).int()
+    for b in range(batch):
+        table[b, :need[b]] = order[first[b]:first[b + 1]]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = [torch.randint(-127, 128, (int(first[-1]), 16, nkv * hd), generator=g, device="cuda", dtype=torch.int32)
+             .to(torch.int8) for _ in range(2)]
+    scales = [torch.rand((int(first[-1]), 1, nkv), generator=g, device="cuda") * 0.02 + 0.01 for _ in range(2)]
+    wide = torch.randn((batch, (nq + 2 * nkv) * hd + 16), generator=g, device="cuda")
+    q, k, v, _ = wide.split([nq * hd, nkv * hd, nkv * hd, 16], 1)
+    table, lt = table.cuda(), lens.int().cuda()
+
+    def call(at):
+        p, s = [x.clone() for x in pages], [x.clone() for x in scales]
+        out = torch.full((batch, nq * hd + 8), 7.0, device="cuda")
+        for i in range(0, batch, at):
+            j = slice(i, i + at)
+            raster_amd.paged_attention(ctx, q[j], k[j], v[j], p[0], p[1], table[j], lt[j], nq, nkv, hd, THETA, hd ** -0.5,
+                                       max_len=2001, out=out[j, 4:-4] if nq * hd % 4 else out[j, 4:4 + nq * hd],
+                                       kscales=s[0], vscales=s[1])
+        return out, p + s
+
+    a, b = call(batch), call(100)
+    assert all(torch.equal(x, y) for x, y in zip(a[1], b[1]))
+    assert bool((a[0][:, :4] == 7).all()) and bool((a[0][:, 4 + nq * hd:] == 7).all())
+    x, y = a[0][:, 4:4 + nq * hd], b[0][:, 4:4 + nq * hd]
+    assert bool((x[lens < 0] == 0).all())
+    # weights are 23-bit shares of a tile's largest, sums in f32: a few 2^-23 of the row's largest value
+    assert bool(((x - y).abs() <= 2.0 ** -19 * y.abs().amax(1, keepdim=True)).all())
+
+
+def test_streams_and_threads(torch, ctx):
+    """Calls on streams of their own from four threads over caches of their own: the bits of the same calls in turn."""
+    import threading
+
+    import q8_ref
+    import raster_amd
+
+    nq, nkv, hd, lens = 8, 2, 128, [300, 2000, 15]
+    print("[gpu] q8 threads", flush=True)
+    sets = []
+    for i in range(4):
+        c = q8_ref.Cache(i, nkv, hd, [n + 8 for n in lens], 16, lens)
+        sets.append((c, c.clone(), [new_rows(torch, 10 * i + s, "f32", 3, nq, nkv, hd) for s in range(5)]))
+
+    def steps(c, rows, stream):
+        outs = []
+        for s, (q, k, v) in enumerate(rows):
+            lt = torch.tensor([n + s for n in lens], dtype=torch.int32).to("cuda", non_blocking=False)
+            if stream is not None:
+                stream.wait_stream(torch.cuda.default_stream())
+            outs.append(raster_amd.paged_attention(ctx, q, k, v, c.k, c.v, c.table, lt, nq, nkv, hd, THETA, hd ** -0.5,
+                                                   stream=stream, window=600 if s % 2 else 0, sinks=2, **c.scales()))
+            if stream is not None:
+                stream.synchronize()
+        return outs
+
+    want = [steps(c, rows, None) for c, _, rows in sets]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def run(i):
+        got[i] = steps(sets[i][1], sets[i][2], torch.cuda.Stream())
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for (c, d, _), x, y in zip(sets, want, got):
+        assert d.same(c) and all(torch.equal(p, r) for p, r in zip(x, y))
