@@ -25,7 +25,7 @@ import ctypes as C
 from array import array
 
 from ._lib import RQ_I8, Pages, Prompt, call
-from .quant import Context, _current_stream, _dtype_code, _need, _stream_ptr, _t
+from .quant import Context, _current_stream, _dtype_code, _dtypes, _need, _stream_ptr, _t
 
 __all__ = ["prompt_attention", "prompt_attention_bwd", "paged_attention", "pages_append", "pages_rows", "pages_copy"]
 
@@ -93,7 +93,9 @@ def _prompt(ctx, q, k, v, cu, cu_k, n_q, n_kv, head_dim, scale, causal):
 
 
 def _window(window, sinks) -> tuple:
-    """(window, sinks) as the C entries take them."""
+    """(window, sinks) as the C entries take them; () for neither."""
+    if not window and not sinks:
+        return ()
     window = 0 if window is None else window
     _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
     return min(window, _FAR), min(sinks, _FAR)
@@ -124,8 +126,9 @@ def prompt_attention(ctx: Context, q, k, v, cu, n_q: int, n_kv: int, head_dim: i
         os = _rows(out, ctx, q.shape[0], width, q.dtype, "out")
     if lse is not None:
         _check_lse(lse, ctx, n_q * q.shape[0])
-    call("rq_prompt_attention_window", ctx.handle, C.byref(p), *_window(window, sinks), q.data_ptr(), qs, k.data_ptr(),
-         ks, v.data_ptr(), vs, out.data_ptr(), os, None if lse is None else lse.data_ptr(), raw)
+    seen = _window(window, sinks)
+    call("rq_prompt_attention_window" if seen else "rq_prompt_attention", ctx.handle, C.byref(p), *seen, q.data_ptr(), qs,
+         k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os, None if lse is None else lse.data_ptr(), raw)
     return out
 
 
@@ -141,14 +144,15 @@ def prompt_attention_bwd(ctx: Context, dout, q, k, v, out, lse, cu, n_q: int, n_
     os = _rows(out, ctx, rows, qw, dtype, "out")
     _check_lse(lse, ctx, n_q * rows)
     need, seen = C.c_size_t(), _window(window, sinks)
-    call("rq_prompt_attention_window_bwd_work", C.byref(p), *seen, C.byref(need))
+    name = "rq_prompt_attention_window_bwd" if seen else "rq_prompt_attention_bwd"
+    call(name + "_work", C.byref(p), *seen, C.byref(need))
     raw, scope = _on(stream, q)
     work = _empty(scope, need.value // 4, q, _t().float32)
     dq = _empty(scope, (rows, qw), q) if dq is None else dq
     dk, dv = (_empty(scope, (rows_k, kw), q) if t is None else t for t in (dk, dv))
     dqs = _rows(dq, ctx, rows, qw, dtype, "dq")
     dks, dvs = _rows(dk, ctx, rows_k, kw, dtype, "dk"), _rows(dv, ctx, rows_k, kw, dtype, "dv")
-    call("rq_prompt_attention_window_bwd", ctx.handle, C.byref(p), *seen, dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
+    call(name, ctx.handle, C.byref(p), *seen, dout.data_ptr(), dos, q.data_ptr(), qs, k.data_ptr(), ks,
          v.data_ptr(), vs, out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(),
          dvs, work.data_ptr(), need.value, raw)
     return dq, dk, dv
@@ -164,7 +168,9 @@ def _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch):
     if len(ts) != 2 or ts[0] != batch:
         raise ValueError("table must be [batch, pages of a sequence]")
     n = ts[1]
-    code = RQ_I8 if kpages.dtype == _t().int8 else _code(kpages)
+    code = _dtypes.get(kpages.dtype)
+    if code is None:
+        code = RQ_I8 if kpages.dtype == _t().int8 else _code(kpages)
     return Pages(code, kpages.data_ptr(), vpages.data_ptr(), shape[0], shape[1], n_kv, head_dim,
                  _i32(table, ctx, batch * n, "table"), n)
 
@@ -191,15 +197,16 @@ def _bad_scales(shape):
                      "the same strides, a page's scales side by side")
 
 
-_work_sizes: dict = {}  # rq_paged_attention_window_work by its arguments
+_work_sizes: dict = {}  # rq_paged_attention_work and rq_paged_attention_window_work by their arguments
 
 
-def _paged_work(ctx, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks) -> int:
-    key = (ctx.device, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks)
+def _paged_work(ctx, *args) -> int:
+    """args: those of rq_paged_attention_work (batch, n_q, n_kv, head_dim, max_len), or of the other."""
+    key = (ctx.device, *args)
     n = _work_sizes.get(key)
     if n is None:
         need = C.c_size_t()
-        call("rq_paged_attention_window_work", ctx.handle, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks,
+        call("rq_paged_attention_work" if len(args) == 5 else "rq_paged_attention_window_work", ctx.handle, *args,
              C.byref(need))
         if len(_work_sizes) >= 4096:
             _work_sizes.clear()
@@ -210,13 +217,14 @@ def _paged_work(ctx, cache, batch, n_q, n_kv, head_dim, max_len, window, sinks) 
 def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int, n_kv: int, head_dim: int,
                     theta: float, scale: float, max_len: int | None = None, out=None, stream=None,
                     window: int | None = None, sinks: int = 0, kscales=None, vscales=None):
-    """rq_paged_attention (with a window or int8 pages rq_paged_attention_window): one new token of each sequence b (rows of q [batch,
-    n_q*head_dim], k and v [batch, n_kv*head_dim]) at position lens[b] of its
-    pages (kpages, vpages [pages, page_size, n_kv*head_dim], table int32 [batch,
-    pages of a sequence]): RoPE, append, attention over rows 0 .. lens[b] -> out
-    [batch, n_q*head_dim]. k and v None: nothing appended, rows 0 .. lens[b] - 1. max_len:
-    no sequence is longer, the new row included (default: what the table holds). window: the
-    last `window` rows and the first `sinks` are attended; None or 0: all."""
+    """rq_paged_attention (with a window or int8 pages rq_paged_attention_window): one new
+    token of each sequence b (rows of q [batch, n_q*head_dim], k and v [batch,
+    n_kv*head_dim]) at position lens[b] of its pages (kpages, vpages [pages, page_size,
+    n_kv*head_dim], table int32 [batch, pages of a sequence]): RoPE, append, attention over
+    rows 0 .. lens[b] -> out [batch, n_q*head_dim]. k and v None: nothing appended, rows
+    0 .. lens[b] - 1. max_len: no sequence is longer, the new row included (default: what the
+    table holds). window: the last `window` rows and the first `sinks` are attended; None or
+    0: all."""
     code, dtype, qw, kw = _code(q), q.dtype, n_q * head_dim, n_kv * head_dim
     qs = _rows(q, ctx, None, qw, dtype, "q")
     batch = q.shape[0]
@@ -229,15 +237,21 @@ def paged_attention(ctx: Context, q, k, v, kpages, vpages, table, lens, n_q: int
     pg = _pages(ctx, kpages, vpages, table, n_kv, head_dim, batch)
     if max_len is None:
         max_len = table.shape[1] * kpages.shape[1]
-    sc, seen = _scales(ctx, pg, kscales, vscales), _window(window, sinks)
-    need = _paged_work(ctx, pg.dtype, batch, n_q, n_kv, head_dim, max_len, *seen)
+    more = _window(window, sinks)
+    if more or kscales is not None or vscales is not None or pg.dtype == RQ_I8:
+        name, more = "rq_paged_attention_window", more or (0, 0)
+        need = _paged_work(ctx, pg.dtype, batch, n_q, n_kv, head_dim, max_len, *more)
+        more = _scales(ctx, pg, kscales, vscales) + more
+    else:
+        name = "rq_paged_attention"
+        need = _paged_work(ctx, batch, n_q, n_kv, head_dim, max_len)
     raw, scope = _on(stream, q)
     work = _empty(scope, need // 4, q, _t().float32) if need else None
     if out is None:
         out, os = _empty(scope, (batch, qw), q), qw
     else:
         os = _rows(out, ctx, batch, qw, dtype, "out")
-    call("rq_paged_attention_window", ctx.handle, C.byref(pg), *sc, *seen, code, q.data_ptr(), qs, kd, ks, vd, vs,
+    call(name, ctx.handle, C.byref(pg), *more, code, q.data_ptr(), qs, kd, ks, vd, vs,
          _i32(lens, ctx, batch, "lens"), batch, n_q, max_len, theta, scale, out.data_ptr(), os,
          work.data_ptr() if need else None, need, raw)
     return out
@@ -266,8 +280,9 @@ def pages_append(ctx: Context, q, k, v, kpages, vpages, table, cu, past, n_q: in
         k_out = _empty(scope, (rows, kw), q)
     else:
         kos = _rows(k_out, ctx, rows, kw, dtype, "k_out")
-    sc = _scales(ctx, pg, kscales, vscales)
-    name, sc = ("rq_pages_append_q8", sc) if pg.dtype == RQ_I8 else ("rq_pages_append", ())
+    name, sc = "rq_pages_append", ()
+    if pg.dtype == RQ_I8 or kscales is not None or vscales is not None:
+        name, sc = "rq_pages_append_q8", _scales(ctx, pg, kscales, vscales)
     call(name, ctx.handle, C.byref(pg), *sc, code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
          _i32(cu, ctx, batch + 1, "cu"), _i32(past, ctx, batch, "past"), batch, rows, n_q, theta,
          q_out.data_ptr(), qos, k_out.data_ptr(), kos, raw)

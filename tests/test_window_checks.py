@@ -73,6 +73,7 @@ def test_python_arguments():
         with pytest.raises(ValueError):
             attention._window(kw.get("window"), kw.get("sinks", 0))
     assert attention._window(None, 3) == (0, 3) and attention._window(7, 0) == (7, 0)
+    assert attention._window(None, 0) == attention._window(0, 0) == ()
     assert attention._window(2 ** 80, 2 ** 90) == (1 << 40, 1 << 40)
     with pytest.raises(ValueError):  # (a CPU tensor is refused before anything is called)
         x = torch.zeros(4, 64)
