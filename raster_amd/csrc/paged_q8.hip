@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "attn_tile.h"
 #include "paged_tile.h"
@@ -110,6 +111,8 @@ __device__ __forceinline__ void keep_whole(V (&x)[N]) {
 // A number in NT signed digits of 8 bits, as an operand of the int8 products beside the codes: x = sum_n digit n * 256^n,
 // for |x| up to kDigitsMax<NT>. Queries are written so relative to a head's largest element, weights relative to their
 // tile's largest, so f32 calls lose 2^-24 of that (NT = 3), bf16 ones 2^-16 (NT = 2); sums over products are exact.
+template <typename A>
+constexpr int kDigits = sizeof(A) == 2 ? 2 : 3;
 template <int NT>
 constexpr int kDigitsMax = NT == 2 ? 0x7F7E : 0x7F7F7C;
 // the digits in the bytes of a word, from byte 0 on
@@ -126,6 +129,23 @@ __device__ __forceinline__ void pack_digits(const uint32_t (&x)[4], uint32_t (&d
   d[1] = high16_pair(a, b);
   if constexpr (NT == 3)
     d[2] = low16_pair(__builtin_amdgcn_perm(x[1], x[0], 0x07030602), __builtin_amdgcn_perm(x[3], x[2], 0x07030602));
+}
+// Byte n of four such words as a word, n the lane's: pick = n | (n + 4) << 8
+__device__ __forceinline__ uint32_t pack_digit(const uint32_t (&x)[4], uint32_t pick) {
+  return low16_pair(__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick));
+}
+// Sums over the columns that hold the digits of one number (8 or 4 apart), in each of them, the same bits in all: column c
+// takes column c + 8 first, and of the two sums that there are then each column adds one to the other. (They have
+// to be the same: a weight's digits are taken in different columns, each from its own copy.)
+template <int APART>
+__device__ __forceinline__ float sum_digits(float x) {
+#pragma clang fp contract(off)  // (x is a product; fused into the sum it would differ from column to column)
+  auto turned = [](float y, auto by) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x120 + decltype(by)::value, 0xf, 0xf, true));
+  };
+  x += turned(x, std::integral_constant<int, 8>{});
+  if constexpr (APART == 4) x += turned(x, std::integral_constant<int, 4>{});
+  return x;
 }
 // Sum of digit products to their value
 __device__ __forceinline__ float value_of(int d0, int d1) { return (float)((d1 << 8) + d0); }
@@ -170,82 +190,125 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t x) {
 #undef RQ_SCAN_STEP
   return x;
 }
-// By a whole wave: the range of number `number`, or the first of sequence -1 - number. b = -1: there is none.
-constexpr int kPlanned = 1024;  // sequences of a launch
-__device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int number) {
-  if (a.spare == 0) return {number < 0 ? -1 - number : number, 0, 1, number < 0 ? -1 - number : number, INT32_MAX};
-  if (a.range_rows > 0) return {0, max(number, 0), 0, 0, a.range_rows};
-  const int lane = threadIdx.x & 63, batch = a.p.batch, per = (batch + 63) / 64, b0 = lane * per;
-  const int b1 = min(b0 + per, batch);
-  // in units of a block (at most 2^26 a sequence, 2^30 for the first 16 of a lane), rounded up: 38 bits in all
-  int one = 0;  // of a lane's only sequence
-  uint32_t sum = 0;
-  for (int b = b0; b < b1; b++) {
-    one = walked_of(a, a.lens[b]);
-    sum += (uint32_t)(one + kBlock - 1) / kBlock;
-  }
-  const uint32_t high = scan_lanes(sum >> 16), low = scan_lanes(sum & 0xffff);  // 22 bits each and 6 more
-  const uint64_t blocks = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(high, 63) << 16) +
-                          (uint32_t)__builtin_amdgcn_readlane(low, 63);
-  // R spare >= all rows, up to a multiple of split_rows
+// R of a call with `blocks` blocks of walked rows (at most 2^26 a sequence): R spare >= all rows, a multiple of split_rows
+__device__ __forceinline__ int rows_a_range(const PagedAttnArgs& a, uint64_t blocks) {
   const int shift = blocks >> 32 ? 8 : 0;
   const uint64_t least = ((uint64_t)((uint32_t)(blocks >> shift) / (uint32_t)a.spare) + 1) << shift;
   const uint32_t unit = a.split_rows / kBlock;
-  const int rows = (int)(((uint32_t)min(least, (uint64_t)1 << 26) + unit - 1) / unit * unit * kBlock);
-  auto walk_of = [&](int b) { return per == 1 ? one : walked_of(a, a.lens[b]); };
-  int mine = 0;
-  for (int b = b0; b < b1; b++) mine += ranges_of_walk(walk_of(b), rows);
-  Range r{-1, 0, 0, 0, rows};
-  int first = (int)scan_lanes(mine) - mine;
-  for (int b = b0; b < b1; b++) {
-    const int n = ranges_of_walk(walk_of(b), rows);
-    if (number < 0 ? b == -1 - number : number >= first && number < first + n) {
-      r.b = b;
-      r.at = number < 0 ? 0 : number - first;
-      r.count = n;
-      r.first = first;
-    }
-    first += n;
-  }
-  const uint64_t found = __builtin_amdgcn_ballot_w64(r.b >= 0);
-  if (found == 0) return r;
-  const int src = __builtin_ctzll(found);
-  r.b = __builtin_amdgcn_readlane(r.b, src);
-  r.at = __builtin_amdgcn_readlane(r.at, src);
-  r.count = __builtin_amdgcn_readlane(r.count, src);
-  r.first = __builtin_amdgcn_readlane(r.first, src);
-  return r;
+  // (a scalar: the compiler divides in vector registers, and everything that follows from it would stay there)
+  return __builtin_amdgcn_readfirstlane((int)(((uint32_t)min(least, (uint64_t)1 << 26) + unit - 1) / unit * unit * kBlock));
 }
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+
+// By a whole workgroup: the range of number `number`, or the first of sequence -1 - number. b = -1: there is none. Up to 64
+// sequences each wave looks by itself, a lane a sequence; more are planned by all threads (300 sequences of 1 to 1000 rows in
+// ranges by waves alone 150 us, so 125).
+constexpr int kEach = 4, kPlanned = kThreads * kEach;  // sequences of a thread, of a launch
+__device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int number) {
+  if (a.spare == 0) return {number < 0 ? -1 - number : number, 0, 1, number < 0 ? -1 - number : number, INT32_MAX};
+  if (a.range_rows > 0) return {0, max(number, 0), 0, 0, a.range_rows};
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, batch = a.p.batch;
+  if (batch <= 64) {
+    const int walk = lane < batch ? walked_of(a, a.lens[lane]) : 0;
+    const uint32_t sum = (uint32_t)(walk + kBlock - 1) / kBlock;
+    const uint64_t blocks = ((uint64_t)last_lane(scan_lanes(sum >> 16)) << 16) + last_lane(scan_lanes(sum & 0xffff));
+    const int rows = rows_a_range(a, blocks), n = lane < batch ? ranges_of_walk(walk, rows) : 0;
+    const int first = (int)scan_lanes(n) - n;
+    const bool mine = number < 0 ? lane == -1 - number : number >= first && number < first + n;
+    const uint64_t found = __builtin_amdgcn_ballot_w64(mine);
+    if (found == 0) return {-1, 0, 0, 0, rows};
+    const int b = __builtin_ctzll(found), f = __builtin_amdgcn_readlane(first, b);
+    return {b, number < 0 ? 0 : number - f, __builtin_amdgcn_readlane(n, b), f, rows};
+  }
+  __shared__ uint32_t high[kWaves], low[kWaves], count[kWaves];
+  __shared__ int found[3];
+  int walk[kEach], n[kEach], mine = 0;
+  uint32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; i++) walk[i] = a.lens[min(tid * kEach + i, batch - 1)];
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    walk[i] = tid * kEach + i < batch ? walked_of(a, walk[i]) : 0;
+    sum += (uint32_t)(walk[i] + kBlock - 1) / kBlock;
+  }
+  const uint32_t h = scan_lanes(sum >> 16), l = scan_lanes(sum & 0xffff);
+  if (lane == 63) high[wave] = h, low[wave] = l;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  uint64_t blocks = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) blocks += ((uint64_t)high[w] << 16) + low[w];
+  const int rows = rows_a_range(a, blocks);
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    n[i] = tid * kEach + i < batch ? ranges_of_walk(walk[i], rows) : 0;
+    mine += n[i];
+  }
+  const uint32_t upto = scan_lanes(mine);
+  if (lane == 63) count[wave] = upto;
+  __syncthreads();
+  int first = (int)upto - mine;
+  for (int w = 0; w < wave; w++) first += count[w];
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    const int b = tid * kEach + i;
+    if (b < batch && (number < 0 ? b == -1 - number : number >= first && number < first + n[i]))
+      found[0] = b, found[1] = first, found[2] = n[i];
+    first += n[i];
+  }
+  __syncthreads();
+  const int b = __builtin_amdgcn_readfirstlane(found[0]);
+  if (b < 0) return {-1, 0, 0, 0, rows};
+  const int f = __builtin_amdgcn_readfirstlane(found[1]);
+  return {b, number < 0 ? 0 : number - f, __builtin_amdgcn_readfirstlane(found[2]), f, rows};
+}
+
+// columns from one digit of a head to the next, where all digits of a group's heads fit into 16 of them
+template <typename A>
+constexpr int kApart = kDigits<A> == 2 ? 8 : 4;
 
 // LDS: the digits of HW KV heads' queries, the blocks that the new row goes into (keys, values), the waves' maxima and
 // sums, the queries' maxima and factors, the blocks' scales
-template <typename A, int HD, int HW>
+template <typename A, int HD, int HW, bool SPREAD>
 constexpr int q8_fixed_bytes() {
-  return HW * (16 * HD * (sizeof(A) == 2 ? 2 : 3) + 2 * kBlock * HD + 2 * 16 * 4) + (kWaves * 32 + 8) * 4;
+  return HW * (16 * HD * (SPREAD ? 1 : kDigits<A>) + 2 * kBlock * HD + 2 * 16 * 4) + (kWaves * 32 + 8) * 4;
 }
 
-// One workgroup: up to 16 query heads of each of HW KV heads, one range of a sequence's cached rows. kWaves / HW
-// waves share a KV head and take tiles of 64 of its rows in turn (32 past 128 elements, for the registers). S^T = K Q^T with keys in the rows of a 16x16x64 int8 MFMA
-// and heads in its columns: the 16 codes that a lane reads of its row are an operand as they lie, the queries' digits
-// the other. A lane's 16 scores of a column, 4 g + i of block t, are its weights, whose digits in slot 4 t + i are an
-// operand of O^T += V^T P^T as they lie; of V a lane reads E = HD / 16 neighbouring codes of the rows 4 g + i and
-// turns 4 rows x 4 codes in registers (8 byte permutations). A block's scale is one factor of its scores and of its weights.
-// Row i of result tile e is element E i + e. Each tile's weighted values are whole numbers, added to the f32 sums with the
-// factor of their weights. (Codes made bf16 for bf16 products: twice the instructions, 32 sequences of 0 to 8191 rows 56 us, now @@B@@.)
+// One workgroup: up to 16 query heads of each of HW KV heads, one range of a sequence's cached rows. kWaves / HW waves
+// share a KV head and take tiles of 64 of its rows in turn (32 past 128 elements, for the registers).
+//
+// S^T = K Q^T with keys in the rows of a 16x16x64 int8 MFMA and heads in its columns: the 16 codes that a lane reads of
+// its row are an operand as they lie, the queries' digits the other. A lane's 16 scores of a column, 4 g + i of block t,
+// are its weights, whose digits in slot 4 t + i are an operand of O^T += V^T P^T as they lie; of V a lane reads
+// E = HD / 16 neighbouring codes of the rows 4 g + i and turns 4 rows x 4 codes in registers (8 byte permutations). A
+// block's scale is one factor of its scores and of its weights. Row i of result tile e is element E i + e. Each tile's
+// weighted values are whole numbers, added to the f32 sums with the factor of their weights. (Codes made bf16 for
+// bf16 products: twice the instructions, 32 sequences of 0 to 8191 rows, 117 MB, 56 us, this way 45.)
+//
+// SPREAD: the digits of a group's heads fit into the 16 columns together (up to 8 heads in bf16, 4 in f32): column
+// c + kApart n holds digit n of head c, one product does for all digits, and no column is idle. A score is the sum over
+// its columns; weights are the same in each and give their own digit; the results' columns are summed at the end.
+// The 117 MB 44.4 -> 39.5 us (f32, 3 digits), of it 2 us by keeping the rows' places in scalar registers.
 //
 // With many rows, HW = 4: the workgroup reads whole pieces of 512 bytes and more of a row at a time, where with HW = 1
-// each KV head's 128 bytes are read by other compute units at other times: 8 sequences of 33 to 65 Ki rows 4.1 against 5.3 TB/s
-// with the loads alone. With few, HW = 1: more waves at a sequence, each with less to walk.
+// each KV head's 128 bytes are read by other compute units at other times: 8 sequences of 33 to 65 Ki rows 4.1 against
+// 5.3 TB/s with the loads alone. With few, HW = 1: more waves at a sequence, each with less to walk.
+//
+// Bound: those 8 sequences, 888 MB, 165 to 175 us with 6 us for the join, 5.1 to 5.4 TB/s in the kernel, where loads alone
+// reach 5.3: by the memory. The 117 MB, about 230 rows a workgroup, 34 us: 11 of them until the first rows are
+// there (lengths, plan, table, rows one after the other), then four tiles a wave of 630 vector instructions each,
+// half of the time that is left. One sequence of 128 rows 9 us: those loads one after the other. A third workgroup a CU
+// (the registers of SPREAD allow it) 42.6, and 888 MB 211: the ranges are shorter and the join is longer.
 //
 // The block that the new row goes into is not walked over: the workgroup of the last range forms it anew in LDS,
-// writes it back, and one wave attends it from there. No other
-// workgroup reads it, so none can see it half written.
-template <typename A, int HD, bool PART, int HW>
+// writes it back, and one wave attends it from there. No other workgroup reads it, so none can see it half written.
+template <typename A, int HD, bool PART, int HW, bool SPREAD>
 __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAttnArgs a) {
-  constexpr int NT = sizeof(A) == 2 ? 2 : 3;
+  constexpr int NT = kDigits<A>, APART = kApart<A>;
+  constexpr int NM = SPREAD ? 1 : NT;  // operands for the digits
   constexpr int NB = HD == 256 ? 2 : 4, KT = NB * kBlock, RW = kWaves / HW, STEP = KT * RW;
   constexpr int KP = HD / 64, E = HD / 16, VW = E / 4;  // 16-byte pieces of a K row a lane; codes and words of a V row
-  constexpr int kQuery = 16 * HD * NT;                  // bytes of a KV head's queries
+  constexpr int kQuery = 16 * HD * NM;                  // bytes of a KV head's queries
   extern __shared__ __attribute__((aligned(16))) float sm[];
   const PagesArgs& p = a.p;
   const int hd = p.head_dim, half = hd / 2, group = p.n_q / p.n_kv, htiles = (group + 15) / 16, nh = min(group, 16);
@@ -269,7 +332,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
   const int heads = min(group - ht * 16, 16);
   const int per_head = heads * half;  // pairs of query elements of a KV head
   // the query rows, asked for with the length
-  constexpr int NE = HW * HD / 32;
+  constexpr int kPairs = HW * (SPREAD ? APART : 16) * HD / 2, NE = (kPairs + kThreads - 1) / kThreads;
   const A* qrow = static_cast<const A*>(p.q) + (int64_t)b * p.q_stride + (hkv0 * group + ht * 16) * hd;
   A q0[NE], q1[NE];
 #pragma unroll
@@ -304,7 +367,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
   const bool moved = a.window != INT32_MAX;
   int pages = -1;
   if (!moved && p.table_stride > 0) pages = trow[min((first + kBlock * lane_t) >> p.page_bits, last_entry)];
-  const int len = a.lens[b];
+  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);  // (as loaded it stays in vector registers, with all that follows)
   A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + (hkv0 * group + ht * 16) * hd;
   // element i of the workgroup's results: KV head k, query head hh, element d
   auto place = [&](int i, int* k, int* hh, int* d) {
@@ -514,12 +577,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
         const uint32_t x = digits_of<NT>((int)rintf((z ? y1[n] : y0[n]) * f));
 #pragma unroll
         for (int m = 0; m < NT; m++)
-          at[((m * KP + (d >> 6)) * 64 + 16 * ((d >> 4) & 3) + hh) * 16 + (d & 15)] = (char)(x >> (8 * m));
+          at[(((SPREAD ? 0 : m * KP) + (d >> 6)) * 64 + 16 * ((d >> 4) & 3) + (SPREAD ? m * APART : 0) + hh) * 16 +
+             (d & 15)] = (char)(x >> (8 * m));
       }
     }
   }
   __syncthreads();
-  const float qs = col < heads ? qinv[hw * 16 + col] * a.scale2 : 0.0f;
+  // the column's head, its digit and that one's weight
+  const int hcol = SPREAD ? col & (APART - 1) : col, digit = SPREAD ? col / APART : 0;
+  const float unit = digit == 0 ? 1.0f : digit == 1 ? 256.0f : digit == 2 ? 65536.0f : 0.0f;
+  const uint32_t pick = digit | (digit + 4) << 8;
+  const float qs = hcol < heads ? qinv[hw * 16 + hcol] * a.scale2 * unit : 0.0f;
 
   f32x4 acc[E];
 #pragma unroll
@@ -553,14 +621,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     float s[NB][4];
 #pragma unroll
     for (int t0 = 0; t0 < NB; t0 += 2) {  // two blocks at a time, for the registers
-      i32x4 d[NT][2] = {};
+      i32x4 d[NM][2] = {};
 #pragma unroll
       for (int u = 0; u < KP; u++) {
-        i32x4 qw[NT];
+        i32x4 qw[NM];
 #pragma unroll
-        for (int n = 0; n < NT; n++) qw[n] = qp[(n * KP + u) * 64];
+        for (int n = 0; n < NM; n++) qw[n] = qp[(n * KP + u) * 64];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NM; n++)
 #pragma unroll
           for (int t = 0; t < 2; t++)
             d[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xk[t0 + t][u], qw[n], d[n][t], 0, 0, 0);
@@ -570,7 +638,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
         const float f = ks[t0 + t] * qs;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          if constexpr (NT == 2)
+          if constexpr (SPREAD)
+            s[t0 + t][i] = sum_digits<APART>((float)d[0][t][i] * f);
+          else if constexpr (NT == 2)
             s[t0 + t][i] = value_of(d[0][t][i], d[1][t][i]) * f;
           else
             s[t0 + t][i] = value_of(d[0][t][i], d[1][t][i], d[2][t][i]) * f;
@@ -619,15 +689,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     wmax = fmaxf(wmax, __shfl_xor(wmax, 16, 64));
     wmax = fmaxf(wmax, __shfl_xor(wmax, 32, 64));
     const float to_digits = digit_factor<NT>(wmax);
-    i32x4 pd[NT] = {};
+    i32x4 pd[NM] = {};
 #pragma unroll
     for (int t = 0; t < NB; t++) {
-      uint32_t x[4], y[NT];
+      uint32_t x[4], y[NM];
 #pragma unroll
       for (int i = 0; i < 4; i++) x[i] = (uint32_t)(int)fmaf(s[t][i], to_digits, 0.5f) + (NT == 2 ? 0x8080u : 0x808080u);
-      pack_digits<NT>(x, y);
+      if constexpr (SPREAD)
+        y[0] = pack_digit(x, pick);
+      else
+        pack_digits<NT>(x, y);
 #pragma unroll
-      for (int n = 0; n < NT; n++) pd[n][t] = (int)(y[n] ^ 0x80808080u);
+      for (int n = 0; n < NM; n++) pd[n][t] = (int)(y[n] ^ 0x80808080u);
     }
     const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn;
     const float alpha = __builtin_amdgcn_exp2f(m - ref), beta = __builtin_amdgcn_exp2f(mx - ref);
@@ -635,7 +708,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     l = fmaf(l, alpha, sum * beta);
     // (a scale that is not finite makes the factor NaN)
     const float from_digits = (to_digits > 0.0f ? __builtin_amdgcn_rcpf(to_digits) : 0.0f) + 0.0f * vsum;
-    const float wf = from_digits * beta;
+    const float wf = SPREAD ? from_digits * beta * unit : from_digits * beta;
     keep_whole(xv);
 #pragma unroll
     for (int w = 0; w < VW; w++)  // four elements, one word of the rows
@@ -650,9 +723,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
           vf[0][t] = (int)low16_pair(x, y);
           vf[1][t] = (int)high16_pair(x, y);
         }
-        i32x4 o[NT][2];
+        i32x4 o[NM][2];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NM; n++)
 #pragma unroll
           for (int i = 0; i < 2; i++)
             o[n][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[i], pd[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
@@ -662,7 +735,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             float x;
-            if constexpr (NT == 2)
+            if constexpr (SPREAD)
+              x = (float)o[0][i][j];
+            else if constexpr (NT == 2)
               x = value_of(o[0][i][j], o[1][i][j]);
             else
               x = value_of(o[0][i][j], o[1][i][j], o[2][i][j]);
@@ -684,6 +759,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
   // the waves' states
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  if constexpr (SPREAD)
+#pragma unroll
+    for (int t = 0; t < E; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[t][i] = sum_digits<APART>(acc[t][i]);
   if (col < nh)
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -725,7 +805,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
 }
 
 // Joins the ranges' records of a (sequence, head), one workgroup each: head_dim / 4 lanes
-// a record, the lane groups' sums added in order.
+// a record, the lane groups' sums added in order. 6 us of which 4 are the launch and the plan, done again here: with all records asked for
+// at once 0.3 less.
 template <typename A>
 __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
   const PagesArgs& p = a.p;
@@ -770,8 +851,9 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 }
 
 // RoPE and append of packed rows, a workgroup the rows of one block and some of the heads, a wave a head at a time:
-// its rows stay in registers between their maximum and their codes.
-// Without cu row b is the one row of sequence b, at position past[b].
+// its rows stay in registers between their maximum and their codes: each value is read once and each code written once.
+// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45.6 us, 4.4 TB/s (a copy reaches 4.9); 56 with 8 bytes a
+// load, 72 with an angle's sine and cosine by the general functions. Without cu row b is the one row of sequence b, at position past[b].
 template <typename A, int HD, int V>
 __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendArgs a, int chunks) {
   const PagesArgs& p = a.p;
@@ -895,13 +977,13 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
 
 namespace {
 
-template <typename A, int HD, bool PART, int HW>
+template <typename A, int HD, bool PART, int HW, bool SPREAD>
 hipError_t run_paged_q8(const PagedAttnArgs& a, hipStream_t stream) {
   const PagesArgs& p = a.p;
   const int64_t htiles = (p.n_q / p.n_kv + 15) / 16;
-  constexpr int kFixed = q8_fixed_bytes<A, HD, HW>(), kMaxLds = kFixed + kWaves * 16 * HD * 4;
+  constexpr int kFixed = q8_fixed_bytes<A, HD, HW, SPREAD>(), kMaxLds = kFixed + kWaves * 16 * HD * 4;
   const int lds = kFixed + kWaves * std::min(p.n_q / p.n_kv, 16) * HD * 4;
-  const auto kernel = paged_attention_q8_kernel<A, HD, PART, HW>;
+  const auto kernel = paged_attention_q8_kernel<A, HD, PART, HW, SPREAD>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), kMaxLds, &allowed)) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((p.batch + a.spare) * (p.n_kv / HW) * htiles)), dim3(kThreads), lds,
@@ -911,9 +993,11 @@ hipError_t run_paged_q8(const PagedAttnArgs& a, hipStream_t stream) {
 
 template <typename A, int HD, bool PART>
 hipError_t run_paged_q8_heads(const PagedAttnArgs& a, hipStream_t stream) {
+  const bool spread = a.p.n_q / a.p.n_kv <= kApart<A>;
   if constexpr (HD <= 128)
-    if (a.kv_heads == 4) return run_paged_q8<A, HD, PART, 4>(a, stream);
-  return run_paged_q8<A, HD, PART, 1>(a, stream);
+    if (a.kv_heads == 4)
+      return spread ? run_paged_q8<A, HD, PART, 4, true>(a, stream) : run_paged_q8<A, HD, PART, 4, false>(a, stream);
+  return spread ? run_paged_q8<A, HD, PART, 1, true>(a, stream) : run_paged_q8<A, HD, PART, 1, false>(a, stream);
 }
 
 template <typename A>
@@ -946,6 +1030,7 @@ hipError_t run_append_q8_hd(const PagesAppendArgs& a, hipStream_t stream) {
 
 // The stored rows of sequences, packed: a workgroup ROWS of them, whose places in the pages are looked up first.
 // C: the pages' type (int8: codes times the block's scale), T: the rows'.
+// Bound by the memory, 16 or 32 bytes a store: 63 MB 14 us, 4.5 TB/s. Four rows a workgroup, so that a few hundred rows fill the card.
 template <typename C, typename T, int ROWS>
 __global__ __launch_bounds__(256) void pages_rows_kernel(PagesRowsArgs a) {
   const PagesArgs& p = a.p;
@@ -1023,17 +1108,24 @@ PagedQ8Plan plan_paged_attention_q8(int64_t batch, int64_t n_q, int64_t n_kv, in
   const int64_t htiles = (n_q / n_kv + 15) / 16;
   PagedQ8Plan p;
   // Four KV heads a workgroup where a CU can have many rows times KV heads; us, one head / four, and rows at max_len (caches cold,
-  // 32/8 heads x 128 unless said): 32 of 2000 44 / 47, 2000   64 of 1000 44 / 50, 2000   8 of 4000 27 / 33, 1000   4 of 16000, 16/16
-  // heads 68 / 62, 4000   64 of 1 to 4000 91 / 79, 8000   32 of 1 to 8191 (f32) 94 / 81, 8191   32 of 8000 131 / 112, 8000   16 of
-  // 16000, 64/8 x 64 96 / 71, 8000   16 of 1 to 32000 141 / 117, 16000   8 of 33 to 65 Ki, 64/8 heads 210 / 178, 16384
+  // bf16, 32/8 heads x 128 unless said): 64 of 1000 45 / 48, 2000   32 of 2000 44 / 45, 2000   8 of 4000 27 / 31, 1000   4 of 16000,
+  // 16/16 heads 71 / 65, 4000   64 of 1 to 4000 93 / 81, 8000   32 of 8000 133 / 123, 8000   32 of 1 to 8191 (f32) 120 / 80, 8191
+  // 16 of 16000, 64/8 x 64 103 / 74, 8000   16 of 1 to 32000 157 / 120, 16000   8 of 33 to 65 Ki, 64/8 heads 270 / 189, 16384
   const bool wide = n_kv % 4 == 0 && head_dim <= 128 && htiles == 1;
   p.kv_heads = wide && max_len * batch * n_kv > 3500 * (int64_t)cu_count ? 4 : 1;
+  // Many short sequences fill the card unbroken, and no lengths have to be looked at nor results joined: one head / four in
+  // ranges, one / four unbroken: 300 of 1 to 1000 116 / 125, 94 / 104   128 of 1 to 2000 91 / 99, 81 / 113   128 of 2000 135 / 139,
+  // 126 / 132   1000 of 1 to 500, 16/8 x 64 107 / 117, 106 / 84. Not where one long one may have to wait for a workgroup (3 of 4000
+  // and 97 of 1 to 200 33, unbroken 56).
+  const int64_t most_groups = batch * n_kv * htiles, enough = 3 * (int64_t)cu_count;
+  const bool whole = max_len <= 2048 && most_groups >= enough;
+  if (whole) p.kv_heads = wide && most_groups / 4 >= enough ? 4 : 1;
   const int64_t heads = n_kv / p.kv_heads * htiles;
   p.split_rows = kTileRows * kWaves / p.kv_heads;
   // As many ranges more than sequences as give every CU two workgroups; where there are many sequences, whose short ends add up, no
   // more than that in all (64 of 1 to 4000 96 -> 83, but 8 of 33 to 65 Ki 178 -> 190), and half as many at least. A sequence of one or two
   // rounds of tiles stays whole: the join would cost more.
-  const int64_t most = max_len <= 2 * p.split_rows ? 0 : batch * (max_len / p.split_rows), two = 2 * cu_count / heads;
+  const int64_t most = whole || max_len <= 2 * p.split_rows ? 0 : batch * (max_len / p.split_rows), two = 2 * cu_count / heads;
   p.spare = (int)std::min<int64_t>(std::max<int64_t>({4 * batch >= two ? two - batch : two, two / 2, 1}), most);
   p.range_rows = 0;
   if (batch == 1 && p.spare > 0)

@@ -91,6 +91,14 @@ CASES = [
     ("f32", 4, 4, 128, 64, [1000, 100, 16, 40], 1, 1),
     ("bf16", 4, 2, 256, 16, [500, 17, 16], 17, 33),
     ("f32", 8, 8, 72, 32, [3000, 40], 1111, 16),
+    # groups of 4, 5, 8 and 9 heads, where the digits stop fitting beside each other; few and many rows
+    ("f32", 32, 8, 64, 16, [2500, 77, 0, 1024, 4099], 0, 0),
+    ("f32", 40, 8, 64, 16, [2500, 77, 0, 1024, 4099], 0, 0),
+    ("bf16", 64, 8, 128, 16, [2500, 77, 0, 1024, 4099], 0, 0),
+    ("bf16", 36, 4, 128, 16, [2500, 77, 0, 1024], 0, 0),
+    ("f32", 20, 4, 128, 32, [28000, 3, 64, 500, 27001, 0, 17, 900], 0, 0),
+    ("bf16", 32, 4, 128, 32, [28000, 3, 64, 500, 27001, 0, 17, 900], 0, 0),
+    ("bf16", 36, 4, 64, 32, [28000, 3, 64, 500, 27001, 0, 17, 900], 0, 0),
 ]
 
 
@@ -468,18 +476,19 @@ def test_offsets_past_32_bits(torch, ctx):
 
 
 @pytest.mark.parametrize("nq,nkv,hd,batch", [(4, 2, 64, 1500), (8, 4, 64, 2100), (20, 1, 40, 1030)])
-def test_attention_of_many_sequences(torch, ctx, nq, nkv, hd, batch):
+@pytest.mark.parametrize("max_len", [2001, 4001])  # (sequences of up to 2048 rows stay whole where there are many)
+def test_attention_of_many_sequences(torch, ctx, nq, nkv, hd, batch, max_len):
     """More sequences than one launch plans for, a few long ones among short and idle ones, q, k, v and out as columns of
     wider arrays: as in batches of 100, up to the ranges that long ones are cut into, and the same bits in the cache."""
     import raster_amd
 
-    print(f"[gpu] q8 attention of {batch} sequences {nq}/{nkv}x{hd}", flush=True)
+    print(f"[gpu] q8 attention of {batch} sequences {nq}/{nkv}x{hd} {max_len}", flush=True)
     gen = torch.Generator().manual_seed(batch)
     lens = torch.randint(-1, 40, (batch,), generator=gen)
     lens[[3, batch // 2, batch - 2]] = torch.tensor([1900, 700, 2000])
     need = (lens + 16) // 16
     first = torch.cat([torch.zeros(1, dtype=torch.long), need.cumsum(0)])
-    table = torch.full((batch, 127), -1, dtype=torch.int32)
+    table = torch.full((batch, 251), -1, dtype=torch.int32)
     order = torch.randperm(int(first[-1]), generator=gen).int()
     for b in range(batch):
         table[b, :need[b]] = order[first[b]:first[b + 1]]
@@ -497,7 +506,7 @@ def test_attention_of_many_sequences(torch, ctx, nq, nkv, hd, batch):
         for i in range(0, batch, at):
             j = slice(i, i + at)
             raster_amd.paged_attention(ctx, q[j], k[j], v[j], p[0], p[1], table[j], lt[j], nq, nkv, hd, THETA, hd ** -0.5,
-                                       max_len=2001, out=out[j, 4:-4] if nq * hd % 4 else out[j, 4:4 + nq * hd],
+                                       max_len=max_len, out=out[j, 4:-4] if nq * hd % 4 else out[j, 4:4 + nq * hd],
                                        kscales=s[0], vscales=s[1])
         return out, p + s
 
