@@ -568,10 +568,10 @@ int rq_prompt_attention_bwd(rq_ctx ctx, const rq_prompt* p, const void* dout, in
 
 /* rq_prompt_attention and its gradient with a sliding window and sinks: the query at position i = its row +
  * keys - queries of its sequence sees the keys j <= i with i - j < window, or with j < sinks (the first tokens, which
- * stay visible). window 0: all keys up to i, as without; else causal must be 1. A query sees itself at least, so only one
- * before the first key (more queries than keys) sees nothing. Otherwise as above; a NaN or an inf in
- * keys or values that a query does not see reaches as far before its window as behind it, one in the rows behind the sinks, of
- * the same 64, queries whose window begins less than 320 after it. */
+ * stay visible). window 0: all keys up to i, as without; else causal must be 1. A query sees itself at least, so
+ * only one before the first key (more queries than keys) sees nothing. Otherwise as above; a NaN or an inf in keys
+ * or values that a query does not see reaches as far before its window as behind it, one in the rows behind the
+ * sinks, of the same 64, queries whose window begins less than 320 after it. */
 int rq_prompt_attention_window(rq_ctx ctx, const rq_prompt* p, int64_t window, int64_t sinks, const void* q,
                                int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                                void* out, int64_t out_stride, float* lse, void* stream);
@@ -624,10 +624,10 @@ int rq_paged_attention(rq_ctx ctx, const rq_pages* pg, int dtype, const void* q,
                        int64_t n_q, int64_t max_len, double theta, double scale, void* out, int64_t out_stride,
                        void* work, size_t work_bytes, void* stream);
 
-/* rq_paged_attention with a sliding window, over pages of any type. The new token, at position lens[b] (without k and v
- * the last stored row), sees the last `window` rows up to its own and the first `sinks`; window 0: all. Pages
- * without a row that is seen, nor in its block of 16 rows, are not looked up. kscales and vscales: NULL but for int8 pages (below).
- * rq_paged_attention_window_work: as rq_paged_attention_work, by the type of the pages. */
+/* rq_paged_attention with a sliding window, over pages of any type. The new token, at position lens[b] (without k
+ * and v the last stored row), sees the last `window` rows up to its own and the first `sinks`; window 0: all. Pages
+ * without a row that is seen, nor in its block of 16 rows, are not looked up. kscales and vscales: NULL but for
+ * int8 pages (below). rq_paged_attention_window_work: as rq_paged_attention_work, by the type of the pages. */
 int rq_paged_attention_window_work(rq_ctx ctx, int cache_dtype, int64_t batch, int64_t n_q, int64_t n_kv,
                                    int64_t head_dim, int64_t max_len, int64_t window, int64_t sinks, size_t* bytes);
 int rq_paged_attention_window(rq_ctx ctx, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride,
@@ -637,18 +637,18 @@ int rq_paged_attention_window(rq_ctx ctx, const rq_pages* pg, float* kscales, fl
                               void* work, size_t work_bytes, void* stream);
 
 /* Pages in 8 bits (rq_pages with dtype RQ_I8). A block is 16 rows from a multiple of 16 on, of one KV head, keys and
- * values apart: int8 codes of -127 .. 127 and an f32 scale, the values code * scale. The scale of rows 16 i .. 16 i + 15 of page
- * pg and head h is kscales[pg * scale_stride + i * n_kv + h] (scale_stride at least page_size / 16 * n_kv), vscales alike.
- * Appending rows x to a block whose scale is s0 (0 when its first row is among them) sets s = max(s0, max|x| * (1/127)),
- * stores round(x / s), ties to even, and rounds the codes of the rows before them to round(code * (s0 / s)) when s > s0; what
- * lies behind them in the block stays. All of it in f32, every operation rounded by itself (the rotation of k too), so codes and scales
- * do not depend on how a call is spread; they do on how rows are cut into calls, by the codes rounded anew. An x or s0 that is not finite makes s
- * NaN: what attends or reads the block gets NaN until its first row is written again. A block whose x are all 0, or so small that
- * s is 0, holds zeros.
- * rq_paged_attention_window appends the new row so and attends it, and the rows of its block, as they are
- * stored; the block it goes into must be of its sequence alone (rows of other blocks may be shared). Queries
- * and weights enter as for bf16 pages, codes exactly. With more than 16 query heads a KV head the row is appended in a launch before.
- * Types: dtype RQ_F32 or RQ_BF16. */
+ * values apart: int8 codes of -127 .. 127 and an f32 scale, the values code * scale. The scale of rows 16 i .. 16 i
+ * + 15 of page pg and head h is kscales[pg * scale_stride + i * n_kv + h] (scale_stride at least page_size / 16 *
+ * n_kv), vscales alike. Appending rows x to a block whose scale is s0 (0 when its first row is among them) sets s =
+ * max(s0, max|x| * (1/127)), stores round(x / s), ties to even, and rounds the codes of the rows before them to
+ * round(code * (s0 / s)) when s > s0; what lies behind them in the block stays. All of it in f32, every operation
+ * rounded by itself (the rotation of k too), so codes and scales do not depend on how a call is spread; they do on
+ * how rows are cut into calls, by the codes rounded anew. An x or s0 that is not finite makes s NaN: what attends
+ * or reads the block gets NaN until its first row is written again. A block whose x are all 0, or so small that s
+ * is 0, holds zeros. rq_paged_attention_window appends the new row so and attends it, and the rows of its block, as
+ * they are stored; the block it goes into must be of its sequence alone (rows of other blocks may be shared).
+ * Queries and weights enter as for bf16 pages, codes exactly. With more than 16 query heads a KV head the row is
+ * appended in a launch before. Types: dtype RQ_F32 or RQ_BF16. */
 
 /* rq_pages_append into int8 pages. */
 int rq_pages_append_q8(rq_ctx ctx, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride, int dtype,
@@ -657,9 +657,10 @@ int rq_pages_append_q8(rq_ctx ctx, const rq_pages* pg, float* kscales, float* vs
                        int64_t n_q, double theta, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
                        void* stream);
 
-/* Stored rows as values of `dtype` (RQ_F32 or RQ_BF16, rounded to nearest), from pages of any type: rows 0, 1, ... of sequence b to the rows
- * cu[b] .. cu[b+1] - 1 (as in rq_prompt, `rows` in all) of k_out and v_out [rows][n_kv * head_dim]. A row whose page
- * is missing gets NaN; rows of no sequence are not written. kscales and vscales: NULL but for int8 pages. */
+/* Stored rows as values of `dtype` (RQ_F32 or RQ_BF16, rounded to nearest), from pages of any type: rows 0, 1, ...
+ * of sequence b to the rows cu[b] .. cu[b+1] - 1 (as in rq_prompt, `rows` in all) of k_out and v_out [rows][n_kv *
+ * head_dim]. A row whose page is missing gets NaN; rows of no sequence are not written. kscales and vscales: NULL
+ * but for int8 pages. */
 int rq_pages_rows(rq_ctx ctx, const rq_pages* pg, const float* kscales, const float* vscales, int64_t scale_stride,
                   int dtype, const int32_t* cu, int64_t batch, int64_t rows, void* k_out, int64_t k_out_stride,
                   void* v_out, int64_t v_out_stride, void* stream);

@@ -31,10 +31,11 @@ struct PagedAttnArgs {
   int64_t out_stride;
   int split_rows, nsplit;  // cached rows of a workgroup, and ranges at max_len
   float* part;             // records of the ranges when nsplit > 1
-  // int8 pages: `spare` ranges more than there are sequences (0: a range a sequence), each of a multiple of split_rows rows,
-  // or, of a single sequence, of range_rows.
-  // The scale of rows 16 i .. 16 i + 15 of a page and of a KV head is scales[page * scale_stride + i * n_kv + head]
-  int spare, range_rows, kv_heads, ahead;  // kv_heads: of a workgroup; ahead: the new row is in the pages already (and k is NULL)
+  // int8 pages: `spare` ranges more than there are sequences (0: a range a sequence), each of a multiple of
+  // split_rows rows, or, of a single sequence, of range_rows. The scale of rows 16 i .. 16 i + 15 of a page and of a
+  // KV head is scales[page * scale_stride + i * n_kv + head]
+  // kv_heads: of a workgroup; ahead: the new row is in the pages already (and k is NULL)
+  int spare, range_rows, kv_heads, ahead;
   float *kscales, *vscales;
   int64_t scale_stride;
 };
@@ -88,7 +89,8 @@ hipError_t launch_pages_append(int dtype, int cache_dtype, const PagesAppendArgs
 // over int8 pages
 hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStream_t stream);
 hipError_t launch_pages_append_q8(int dtype, const PagesAppendArgs& a, hipStream_t stream);
-int64_t append_q8_slots(const PagesAppendArgs& a);  // of blocks: its workgroups, or a few times as many when they are few
+// of blocks: its workgroups, or a few times as many when they are few
+int64_t append_q8_slots(const PagesAppendArgs& a);
 hipError_t launch_pages_rows(int dtype, int cache_dtype, const PagesRowsArgs& a, hipStream_t stream);
 // workgroups of one page and plane
 int64_t pages_copy_groups(int64_t page_bytes);

@@ -42,11 +42,15 @@ constexpr int paged_query_bytes(int hd) {
 // busy 0.79); 32 of 0 to 8191 rows, 32/8 heads, f32 over bf16: 45 + 5 us for 233 MB, 5.1 TB/s. One sequence of
 // 128 rows (f32, 16 heads): 9.7 us, the chain length - page number - row - scores - values of one workgroup a head.
 //
+// With a window (WIN) the ranges are of the rows that are walked, the sinks' blocks and from the window's first block
+// on (paged_tile.h): 16 sequences of 1 to 65535 rows, window 4096 and 4 sinks, 32/8 heads, bf16, 197 MB: 35 + 4.5 us,
+// 5.0 TB/s; without the window the same sequences have 1.25 GB.
+//
 // Over a bf16 cache the rotated queries and the weights P go in as NT bf16 terms: 3 for f32 activations (to
-// 2^-24), 2 for bf16 ones (to 2^-17): the result's own rounding is what is left. Error of 8 sequences of 33 to 65 Ki rows,
-// of its norm: 0.0017; with one term of the weights 0.0022, of the queries too 0.0028, all in the same time (372, 370 us
-// of cold caches; 8 of 4000 rows, 32/8 heads, 34.3, 34.1; one of 128, 16 heads, 7.0, 6.9).
-// An f32 cache is multiplied in f32.
+// 2^-24), 2 for bf16 ones (to 2^-17): the result's own rounding is what is left. Error of 8 sequences of 33 to 65 Ki
+// rows, of its norm: 0.0017; with one term of the weights 0.0022, of the queries too 0.0028, all in the same time
+// (372, 370 us of cold caches; 8 of 4000 rows, 32/8 heads, 34.3, 34.1; one of 128, 16 heads, 7.0, 6.9). An f32 cache
+// is multiplied in f32.
 template <typename A, typename C, int HD, bool PART, bool WIN>
 __global__ __launch_bounds__(kPagedThreads) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr bool F32 = sizeof(C) == 4;

@@ -55,8 +55,9 @@ __device__ __forceinline__ void rotate(float x0, float x1, float c, float s, flo
   *y1 = a1 + b1;
 }
 
-// The angle of pair i in turns for one position; cos and sin of `turns`. Whole turns are taken off in 64 bits, then quarters, and
-// |x| <= pi / 4 is left for Taylor's series to x^15 and x^16 (2^-54): a fifth of the instructions of a general sincospi.
+// The angle of pair i in turns for one position; cos and sin of `turns`. Whole turns are taken off in 64 bits, then
+// quarters, and |x| <= pi / 4 is left for Taylor's series to x^15 and x^16 (2^-54): a fifth of the instructions of a
+// general sincospi.
 __device__ __forceinline__ double turns_of(int i, int head_dim, double log2_theta) {
   return exp2(-2.0 * (double)i / (double)head_dim * log2_theta) * 0.15915494309189535;
 }
@@ -92,8 +93,8 @@ __device__ __forceinline__ float wave_max(float x) {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// The codes of a tile in registers, as of here: otherwise the compiler takes them apart where they are loaded, where that
-// waits for the loads and needs several registers for one.
+// The codes of a tile in registers, as of here: otherwise the compiler takes them apart where they are loaded, where
+// that waits for the loads and needs several registers for one.
 template <typename V, int N>
 __device__ __forceinline__ void keep_whole(V (&x)[N]) {
 #pragma unroll
@@ -108,9 +109,10 @@ __device__ __forceinline__ void keep_whole(V (&x)[N]) {
   }
 }
 
-// A number in NT signed digits of 8 bits, as an operand of the int8 products beside the codes: x = sum_n digit n * 256^n,
-// for |x| up to kDigitsMax<NT>. Queries are written so relative to a head's largest element, weights relative to their
-// tile's largest, so f32 calls lose 2^-24 of that (NT = 3), bf16 ones 2^-16 (NT = 2); sums over products are exact.
+// A number in NT signed digits of 8 bits, as an operand of the int8 products beside the codes: x = sum_n digit n *
+// 256^n, for |x| up to kDigitsMax<NT>. Queries are written so relative to a head's largest element, weights relative
+// to their tile's largest, so f32 calls lose 2^-24 of that (NT = 3), bf16 ones 2^-16 (NT = 2); sums over products are
+// exact.
 template <typename A>
 constexpr int kDigits = sizeof(A) == 2 ? 2 : 3;
 template <int NT>
@@ -134,9 +136,9 @@ __device__ __forceinline__ void pack_digits(const uint32_t (&x)[4], uint32_t (&d
 __device__ __forceinline__ uint32_t pack_digit(const uint32_t (&x)[4], uint32_t pick) {
   return low16_pair(__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick));
 }
-// Sums over the columns that hold the digits of one number (8 or 4 apart), in each of them, the same bits in all: column c
-// takes column c + 8 first, and of the two sums that there are then each column adds one to the other. (They have
-// to be the same: a weight's digits are taken in different columns, each from its own copy.)
+// Sums over the columns that hold the digits of one number (8 or 4 apart), in each of them, the same bits in all:
+// column c takes column c + 8 first, and of the two sums that there are then each column adds one to the other. (They
+// have to be the same: a weight's digits are taken in different columns, each from its own copy.)
 template <int APART>
 __device__ __forceinline__ float sum_digits(float x) {
 #pragma clang fp contract(off)  // (x is a product; fused into the sum it would differ from column to column)
@@ -161,10 +163,11 @@ __device__ __forceinline__ float digit_factor(float most) {
 
 // Ranges of rows, by the real lengths. Sequence b's walked rows are cut into ranges of R rows, one at least, and the
 // ranges of all sequences numbered in order: R so that there are no more than a sequence each and `spare` more. So the
-// grid needs no lengths, few of its workgroups find nothing to do, and those of a batch have about equally much. A single
-// sequence's R is the call's, so that nothing waits for its length.
+// grid needs no lengths, few of its workgroups find nothing to do, and those of a batch have about equally much. A
+// single sequence's R is the call's, so that nothing waits for its length.
 struct Range {
-  int b, at, count, first, rows;  // sequence, which of its ranges, how many (0: not known yet) and the number of the first; R
+  // sequence, which of its ranges, how many (0: not known yet) and the number of the first; R
+  int b, at, count, first, rows;
 };
 __device__ __forceinline__ int ranges_of_walk(int walk, int rows) {
   return max(1, (int)((uint32_t)(walk + rows - 1) / (uint32_t)rows));
@@ -190,7 +193,8 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t x) {
 #undef RQ_SCAN_STEP
   return x;
 }
-// R of a call with `blocks` blocks of walked rows (at most 2^26 a sequence): R spare >= all rows, a multiple of split_rows
+// R of a call with `blocks` blocks of walked rows (at most 2^26 a sequence): R spare >= all rows, a multiple of
+// split_rows
 __device__ __forceinline__ int rows_a_range(const PagedAttnArgs& a, uint64_t blocks) {
   const int shift = blocks >> 32 ? 8 : 0;
   const uint64_t least = ((uint64_t)((uint32_t)(blocks >> shift) / (uint32_t)a.spare) + 1) << shift;
@@ -200,9 +204,9 @@ __device__ __forceinline__ int rows_a_range(const PagedAttnArgs& a, uint64_t blo
 }
 __device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
 
-// By a whole workgroup: the range of number `number`, or the first of sequence -1 - number. b = -1: there is none. Up to 64
-// sequences each wave looks by itself, a lane a sequence; more are planned by all threads (300 sequences of 1 to 1000 rows in
-// ranges by waves alone 150 us, so 125).
+// By a whole workgroup: the range of number `number`, or the first of sequence -1 - number. b = -1: there is none. Up
+// to 64 sequences each wave looks by itself, a lane a sequence; more are planned by all threads (300 sequences of 1
+// to 1000 rows in ranges by waves alone 150 us, so 125).
 constexpr int kEach = 4, kPlanned = kThreads * kEach;  // sequences of a thread, of a launch
 __device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int number) {
   if (a.spare == 0) return {number < 0 ? -1 - number : number, 0, 1, number < 0 ? -1 - number : number, INT32_MAX};
@@ -278,12 +282,12 @@ constexpr int q8_fixed_bytes() {
 // share a KV head and take tiles of 64 of its rows in turn (32 past 128 elements, for the registers).
 //
 // S^T = K Q^T with keys in the rows of a 16x16x64 int8 MFMA and heads in its columns: the 16 codes that a lane reads of
-// its row are an operand as they lie, the queries' digits the other. A lane's 16 scores of a column, 4 g + i of block t,
-// are its weights, whose digits in slot 4 t + i are an operand of O^T += V^T P^T as they lie; of V a lane reads
-// E = HD / 16 neighbouring codes of the rows 4 g + i and turns 4 rows x 4 codes in registers (8 byte permutations). A
-// block's scale is one factor of its scores and of its weights. Row i of result tile e is element E i + e. Each tile's
-// weighted values are whole numbers, added to the f32 sums with the factor of their weights. (Codes made bf16 for
-// bf16 products: twice the instructions, 32 sequences of 0 to 8191 rows, 117 MB, 56 us, this way 45.)
+// its row are an operand as they lie, the queries' digits the other. A lane's 16 scores of a column, 4 g + i of block
+// t, are its weights, whose digits in slot 4 t + i are an operand of O^T += V^T P^T as they lie; of V a lane reads E
+// = HD / 16 neighbouring codes of the rows 4 g + i and turns 4 rows x 4 codes in registers (8 byte permutations). A
+// block's scale is one factor of its scores and of its weights. Row i of result tile e is element E i + e. Each
+// tile's weighted values are whole numbers, added to the f32 sums with the factor of their weights. (Codes made bf16
+// for bf16 products: twice the instructions, 32 sequences of 0 to 8191 rows, 117 MB, 56 us, this way 45.)
 //
 // SPREAD: the digits of a group's heads fit into the 16 columns together (up to 8 heads in bf16, 4 in f32): column
 // c + kApart n holds digit n of head c, one product does for all digits, and no column is idle. A score is the sum over
@@ -294,11 +298,11 @@ constexpr int q8_fixed_bytes() {
 // each KV head's 128 bytes are read by other compute units at other times: 8 sequences of 33 to 65 Ki rows 4.1 against
 // 5.3 TB/s with the loads alone. With few, HW = 1: more waves at a sequence, each with less to walk.
 //
-// Bound: those 8 sequences, 888 MB, 165 to 175 us with 6 us for the join, 5.1 to 5.4 TB/s in the kernel, where loads alone
-// reach 5.3: by the memory. The 117 MB, about 230 rows a workgroup, 34 us: 11 of them until the first rows are
+// Bound: those 8 sequences, 888 MB, 165 to 175 us with 6 us for the join, 5.1 to 5.4 TB/s in the kernel, where loads
+// alone reach 5.3: by the memory. The 117 MB, about 230 rows a workgroup, 34 us: 11 of them until the first rows are
 // there (lengths, plan, table, rows one after the other), then four tiles a wave of 630 vector instructions each,
-// half of the time that is left. One sequence of 128 rows 9 us: those loads one after the other. A third workgroup a CU
-// (the registers of SPREAD allow it) 42.6, and 888 MB 211: the ranges are shorter and the join is longer.
+// half of the time that is left. One sequence of 128 rows 9 us: those loads one after the other. A third workgroup a
+// CU (the registers of SPREAD allow it) 42.6, and 888 MB 211: the ranges are shorter and the join is longer.
 //
 // The block that the new row goes into is not walked over: the workgroup of the last range forms it anew in LDS,
 // writes it back, and one wave attends it from there. No other workgroup reads it, so none can see it half written.
@@ -367,7 +371,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
   const bool moved = a.window != INT32_MAX;
   int pages = -1;
   if (!moved && p.table_stride > 0) pages = trow[min((first + kBlock * lane_t) >> p.page_bits, last_entry)];
-  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);  // (as loaded it stays in vector registers, with all that follows)
+  // (as loaded it would stay in vector registers, with all that follows)
+  const int len = __builtin_amdgcn_readfirstlane(a.lens[b]);
   A* orow = static_cast<A*>(a.out) + (int64_t)b * a.out_stride + (hkv0 * group + ht * 16) * hd;
   // element i of the workgroup's results: KV head k, query head hh, element d
   auto place = [&](int i, int* k, int* hh, int* d) {
@@ -569,7 +574,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
     const int i = tid + n * kThreads, k = HW > 1 ? i / per_head : 0, j = i - k * per_head, hh = j / half, e = j - hh * half;
     if (i < HW * per_head) {
       const float f = digit_factor<NT>(__uint_as_float(qmax[k * 16 + hh]));
-      if (e == 0) qinv[k * 16 + hh] = f > 0.0f ? __builtin_amdgcn_rcpf(f) : __uint_as_float(qmax[k * 16 + hh]);  // (0, or NaN for NaN)
+      // (a head of zeros: 0, of NaN: NaN)
+      if (e == 0) qinv[k * 16 + hh] = f > 0.0f ? __builtin_amdgcn_rcpf(f) : __uint_as_float(qmax[k * 16 + hh]);
       char* at = reinterpret_cast<char*>(sm) + k * kQuery;
 #pragma unroll
       for (int z = 0; z < 2; z++) {
@@ -805,8 +811,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_q8_kernel(PagedAt
 }
 
 // Joins the ranges' records of a (sequence, head), one workgroup each: head_dim / 4 lanes
-// a record, the lane groups' sums added in order. 6 us of which 4 are the launch and the plan, done again here: with all records asked for
-// at once 0.3 less.
+// a record, the lane groups' sums added in order. 6 us of which 4 are the launch and the plan, done again here: with
+// all records asked for at once 0.3 less.
 template <typename A>
 __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
   const PagesArgs& p = a.p;
@@ -852,8 +858,9 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 
 // RoPE and append of packed rows, a workgroup the rows of one block and some of the heads, a wave a head at a time:
 // its rows stay in registers between their maximum and their codes: each value is read once and each code written once.
-// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45.6 us, 4.4 TB/s (a copy reaches 4.9); 56 with 8 bytes a
-// load, 72 with an angle's sine and cosine by the general functions. Without cu row b is the one row of sequence b, at position past[b].
+// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45.6 us, 4.4 TB/s (a copy reaches 4.9); 56 with
+// 8 bytes a load, 72 with an angle's sine and cosine by the general functions. Without cu row b is the one row of
+// sequence b, at position past[b].
 template <typename A, int HD, int V>
 __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendArgs a, int chunks) {
   const PagesArgs& p = a.p;
@@ -1030,7 +1037,8 @@ hipError_t run_append_q8_hd(const PagesAppendArgs& a, hipStream_t stream) {
 
 // The stored rows of sequences, packed: a workgroup ROWS of them, whose places in the pages are looked up first.
 // C: the pages' type (int8: codes times the block's scale), T: the rows'.
-// Bound by the memory, 16 or 32 bytes a store: 63 MB 14 us, 4.5 TB/s. Four rows a workgroup, so that a few hundred rows fill the card.
+// Bound by the memory, 16 or 32 bytes a store: 63 MB 14 us, 4.5 TB/s. Four rows a workgroup, so that a few hundred
+// rows fill the card.
 template <typename C, typename T, int ROWS>
 __global__ __launch_bounds__(256) void pages_rows_kernel(PagesRowsArgs a) {
   const PagesArgs& p = a.p;
@@ -1107,24 +1115,25 @@ PagedQ8Plan plan_paged_attention_q8(int64_t batch, int64_t n_q, int64_t n_kv, in
   batch = std::min<int64_t>(batch, kPlanned);
   const int64_t htiles = (n_q / n_kv + 15) / 16;
   PagedQ8Plan p;
-  // Four KV heads a workgroup where a CU can have many rows times KV heads; us, one head / four, and rows at max_len (caches cold,
-  // bf16, 32/8 heads x 128 unless said): 64 of 1000 45 / 48, 2000   32 of 2000 44 / 45, 2000   8 of 4000 27 / 31, 1000   4 of 16000,
-  // 16/16 heads 71 / 65, 4000   64 of 1 to 4000 93 / 81, 8000   32 of 8000 133 / 123, 8000   32 of 1 to 8191 (f32) 120 / 80, 8191
-  // 16 of 16000, 64/8 x 64 103 / 74, 8000   16 of 1 to 32000 157 / 120, 16000   8 of 33 to 65 Ki, 64/8 heads 270 / 189, 16384
+  // Four KV heads a workgroup where a CU can have many rows times KV heads; us, one head / four, and rows at max_len
+  // (caches cold, bf16, 32/8 heads x 128 unless said): 64 of 1000 45 / 48, 2000 | 32 of 2000 44 / 45, 2000 | 8 of
+  // 4000 27 / 31, 1000 | 4 of 16000, 16/16 heads 71 / 65, 4000 | 64 of 1 to 4000 93 / 81, 8000 | 32 of 8000 133 /
+  // 123, 8000 | 32 of 1 to 8191 (f32) 120 / 80, 8191 | 16 of 16000, 64/8 x 64 103 / 74, 8000 | 16 of 1 to 32000 157 /
+  // 120, 16000 | 8 of 33 to 65 Ki, 64/8 heads 270 / 189, 16384
   const bool wide = n_kv % 4 == 0 && head_dim <= 128 && htiles == 1;
   p.kv_heads = wide && max_len * batch * n_kv > 3500 * (int64_t)cu_count ? 4 : 1;
-  // Many short sequences fill the card unbroken, and no lengths have to be looked at nor results joined: one head / four in
-  // ranges, one / four unbroken: 300 of 1 to 1000 116 / 125, 94 / 104   128 of 1 to 2000 91 / 99, 81 / 113   128 of 2000 135 / 139,
-  // 126 / 132   1000 of 1 to 500, 16/8 x 64 107 / 117, 106 / 84. Not where one long one may have to wait for a workgroup (3 of 4000
-  // and 97 of 1 to 200 33, unbroken 56).
+  // Many short sequences fill the card unbroken, and no lengths have to be looked at nor results joined: one head /
+  // four in ranges, one / four unbroken: 300 of 1 to 1000 116 / 125, 94 / 104 | 128 of 1 to 2000 91 / 99, 81 / 113 |
+  // 128 of 2000 135 / 139, 126 / 132 | 1000 of 1 to 500, 16/8 x 64 107 / 117, 106 / 84. Not where one long one may
+  // have to wait for a workgroup (3 of 4000 and 97 of 1 to 200 33, unbroken 56).
   const int64_t most_groups = batch * n_kv * htiles, enough = 3 * (int64_t)cu_count;
   const bool whole = max_len <= 2048 && most_groups >= enough;
   if (whole) p.kv_heads = wide && most_groups / 4 >= enough ? 4 : 1;
   const int64_t heads = n_kv / p.kv_heads * htiles;
   p.split_rows = kTileRows * kWaves / p.kv_heads;
-  // As many ranges more than sequences as give every CU two workgroups; where there are many sequences, whose short ends add up, no
-  // more than that in all (64 of 1 to 4000 96 -> 83, but 8 of 33 to 65 Ki 178 -> 190), and half as many at least. A sequence of one or two
-  // rounds of tiles stays whole: the join would cost more.
+  // As many ranges more than sequences as give every CU two workgroups; where there are many sequences, whose short
+  // ends add up, no more than that in all (64 of 1 to 4000 96 -> 83, but 8 of 33 to 65 Ki 178 -> 190), and half as
+  // many at least. A sequence of one or two rounds of tiles stays whole: the join would cost more.
   const int64_t most = whole || max_len <= 2 * p.split_rows ? 0 : batch * (max_len / p.split_rows), two = 2 * cu_count / heads;
   p.spare = (int)std::min<int64_t>(std::max<int64_t>({4 * batch >= two ? two - batch : two, two / 2, 1}), most);
   p.range_rows = 0;
@@ -1152,7 +1161,8 @@ hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStrea
   }
   if (r.window == 0) r.window = INT32_MAX;
   const int64_t e = dtype == RQ_F32 ? 4 : 2;
-  for (int64_t b = 0; b < p.batch; b += kPlanned) {  // (records of the last launch are joined before the next one's are written)
+  // (a launch's records are joined before the next one's are written)
+  for (int64_t b = 0; b < p.batch; b += kPlanned) {
     PagedAttnArgs n = r;
     n.p.batch = (int)std::min<int64_t>(kPlanned, p.batch - b);
     n.p.table += b * p.table_stride;

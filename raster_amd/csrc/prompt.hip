@@ -17,10 +17,17 @@
 //
 // Bound by the matrix instructions: 4 head_dim operations for every (query, key) pair that sees the other
 // against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 502 to 511 us, 1.08 PFLOP/s, 558 us on a
-// card warm from other work (a library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens 124 us, 0.74; 37
-// tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16 heads x 128,
-// 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the masked
-// halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.
+// card warm from other work (a library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens
+// 124 us, 0.74; 37 tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16
+// heads x 128, 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the
+// masked halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.
+//
+// With a window (WIN) j > i - window too, or j < sinks. A workgroup walks the sinks' tiles and those from its first
+// query's window on, so the work is queries times window, and a tile is masked where an edge runs through it. 16384
+// tokens, 32/8 heads x 128, bf16, window 4096 and 4 sinks: 970 to 1030 us by card, 0.94 to 0.99 PFLOP/s of the pairs
+// that count; a tile more at each edge than that is computed, one part in 32. The f32 prompts above with windows of
+// 256: 77 to 81 us, 44 TFLOP/s: shorter walks, so a larger part of each is cut tiles, the first loads and the join of
+// the waves.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -488,7 +495,8 @@ static int fwd_split_groups(int dtype, const PromptArgs& a) {
   // With a window a workgroup walks it and its own queries' keys: fewer queries a workgroup cost more of them, the
   // sooner the shorter the window. us, windows of 32 / 128 / 400, 128, 64 and 32 queries:
   //   f32   x 128: 512 (80) 38, 26, 32 / 53, 31, 33 / 85, 51, 39   1024 (144) 39, 27, 53 / 54, 33, 61 / 95, 58, 81
-  //         1024 (32/8, 288) 41, 50, 99 / 56, 61, 110 / 97, 107, 144   2048 (272), 64 / 256 / 1024: 47, 53, 103 / 75, 84, 147 / 185, 194, 240
+  //         1024 (32/8, 288) 41, 50, 99 / 56, 61, 110 / 97, 107, 144
+  //         2048 (272), 64 / 256 / 1024: 47, 53, 103 / 75, 84, 147 / 185, 194, 240
   //         16/2 x 64: 1024 (144) 25, 17, 22 / 34, 20, 23 / 56, 33, 33   4096 (528) 39, 42, 69 / 51, 52, 78 / 89, 95, 121
   //   bf16  x 128: 512 (80) 17, 12, 14 / 20, 14, 14 / 22, 18, 15   1024 (144) 17, 13, 23 / 20, 14, 25 / 28, 20, 29
   //         16/2 x 64: 1024 (144) 15, 11, 12 / 18, 11, 12 / 24, 16, 15
@@ -517,8 +525,8 @@ int prompt_fwd_tile(int dtype, const PromptArgs& a) {
   // us, this / the other, bf16, causal: 32/8 heads x 128: 8 x 512 tokens 52 / 43, 4 x 1024 68 / 58, 4 x 3000
   // 314 / 312, 4 x 4096 548 / 548, 4096 139 / 142, 8192 502 / 520, 16384 1919 / 2021; 16/16 heads: 4096
   // 106 / 103, 4 x 4096 279 / 281, 8192 256 / 267.
-  // With a window the wider tile has more at both of its edges: 16384 tokens, 32/8 heads, windows of 256, 1024 and 4096 301 / 196,
-  // 457 / 367, 1010 / 970; 32768, 16/4 heads, 8192 1816 / 1847, 16384 2957 / 3065.
+  // With a window the wider tile has more at both of its edges: 16384 tokens, 32/8 heads, windows of 256, 1024 and
+  // 4096 301 / 196, 457 / 367, 1010 / 970; 32768, 16/4 heads, 8192 1816 / 1847, 16384 2957 / 3065.
   const bool pair = dtype == RQ_BF16 && a.head_dim > 64 && a.head_dim <= 128 && a.rows_q / a.batch > 4096 &&
                     (a.window == 0 || a.window >= 8192);
   return pair ? 256 : 128;

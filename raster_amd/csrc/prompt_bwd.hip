@@ -18,6 +18,11 @@
 // (dQ alone 195, dK and dV alone 350), 0.73 PFLOP/s of the 7 products, matrix pipe busy 0.34. f32, 129, 300, 64
 // and 511 tokens, 16/2 heads x 64: 4.8 + 53 + 6.8 us (the parts' sum).
 //
+// With a window (WIN) each walk is of the tiles that the window or the sinks reach: 4096, 777, 1500, 331, 1999 and 64
+// tokens, bf16, 32/8 heads x 128, window 1024 and 4 sinks: 25 + 6 us for D, 600 for the rest, 5 for the sinks' sum
+// (160 the forward), 0.5 PFLOP/s of the pairs that count: shorter walks, in
+// which the first loads and the masked tiles at both edges weigh more.
+//
 // Rounded to bf16 in the bf16 kernels: P for dV, dS for dK and dQ (operands of their products), and the results.
 #include <algorithm>
 #include <atomic>
@@ -213,10 +218,10 @@ constexpr int dkv_lds() {  // twice Q, dO, L and D of a step, and two pairs' wei
 }
 
 //
-// With `sink` (WIN) one of the first keys' tiles, which all later queries see, and one chunk of the queries; the sums go to
-// a.sink_part and prompt_sink_sum_kernel adds them in order. As one workgroup's steps those tiles would be the last to
-// end, long after the others, which see the queries of the window only: forward and gradient of 4096, 777, 1500, 331,
-// 1999 and 64 tokens, bf16, 32/8 heads x 128, window 1024 and 4 sinks: 1181 us, by chunks 773.
+// With `sink` (WIN) one of the first keys' tiles, which all later queries see, and one chunk of the queries; the sums
+// go to a.sink_part and prompt_sink_sum_kernel adds them in order. As one workgroup's steps those tiles would be the
+// last to end, long after the others, which see the queries of the window only: forward and gradient of 4096, 777,
+// 1500, 331, 1999 and 64 tokens, bf16, 32/8 heads x 128, window 1024 and 4 sinks: 1181 us, by chunks 740 to 780.
 template <typename T, int HD, bool WIN>
 __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool sink, char* lds) {
   using TL = Tile<T, HD>;
@@ -296,8 +301,8 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
     load(hq, r);
     store(lds);
   }
-  // From the last queries down. Of a tile with sinks first those that see nothing else of the wave's keys: what they gave to
-  // keys that are no sinks is 0 times their rows, and a NaN in one must not stay there.
+  // From the last queries down. Of a tile with sinks first those that see nothing else of the wave's keys: what they
+  // gave to keys that are no sinks is 0 times their rows, and a NaN in one must not stay there.
   int behind = s0;
   if (WIN && tk.row0 < a.sinks) {
     const int near = (w_key + 31 + a.window - off - qstart + BQ - 1) / BQ;  // query tiles before those
@@ -442,7 +447,8 @@ __global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   for (int i = part_of * 256 + threadIdx.x; i < 2 * keys * (hd / 4); i += kSinkParts * 256) {
     const int is_k = i >= keys * (hd / 4), j = is_k ? i - keys * (hd / 4) : i, row = j / (hd / 4), e = 4 * (j % (hd / 4));
-    const float* part = a.sink_part + slot * a.nsplit * step + ((tile * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * hd) + row * hd + e;
+    const float* part =
+        a.sink_part + slot * a.nsplit * step + ((tile * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * hd) + row * hd + e;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c = 0; c < parts; c++) x += *reinterpret_cast<const f32x4*>(part + c * step);
     T4 y;
@@ -703,8 +709,8 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     if (hipError_t e = hipGetLastError()) return e;
   }
   if (WIN && a.sink_tiles > 0) {  // (after the parts' sums, which know nothing of these keys and write what was there)
-    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * kSinkParts)), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * kSinkParts)),
+                       dim3(256), 0, stream, a);
     return hipGetLastError();
   }
   return hipSuccess;
@@ -714,9 +720,9 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
 
 // Parts of the (head, query tile) steps of the keys' gradients: enough that the grid is
 // 768 workgroups, while a part keeps 4 query tiles of the longest sequence that the rows allow.
-// With a window, whose keys all have about as many queries, fewer and longer parts: us of forward and gradient, 768 and 4 /
-// 512 and 5: 129, 300, 64, 511 (f32, 16/2 x 64, window 100) 72 / 68   2048 (f32, 16/2 x 64, 64) 131 / 117   2048 (f32, 32/8 x 128, 64) 408 / 386
-// 2048 (bf16, 32/8 x 128, 256) 151 / 141
+// With a window, whose keys all have about as many queries, fewer and longer parts: us of forward and gradient, 768
+// and 4 / 512 and 5: 129, 300, 64, 511 (f32, 16/2 x 64, window 100) 72 / 68 | 2048 (f32, 16/2 x 64, 64) 131 / 117 |
+// 2048 (f32, 32/8 x 128, 64) 408 / 386 | 2048 (bf16, 32/8 x 128, 256) 151 / 141
 PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   const int64_t batch = a.batch, rows_q = a.rows_q, rows_k = a.rows_k, n_q = a.n_q, n_kv = a.n_kv, head_dim = a.head_dim;
   const int64_t groups = std::max<int64_t>(1, (rows_k + kDkvKeys - 1) / kDkvKeys * n_kv);
@@ -726,8 +732,8 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   const int64_t steps = longest / 32 * (n_q / n_kv);
   PromptBwdPlan p;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({most / groups, steps / least_steps, 16}));
-  // Chunks of the first keys' queries, of about as many steps as the other keys have and in as many parts, where a sequence can be longer
-  // than the window and a chunk; with many sinks their tiles are workgroups enough.
+  // Chunks of the first keys' queries, of about as many steps as the other keys have and in as many parts, where a
+  // sequence can be longer than the window and a chunk; with many sinks their tiles are workgroups enough.
   p.sink_tiles = p.sink_chunk = 0;
   p.sink_slots = 0;
   const int tiles = (a.sinks + kDkvKeys - 1) / kDkvKeys;
@@ -739,7 +745,8 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   }
   const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv * p.nsplit;
   p.groups = std::max(sinks + tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
-                      std::max<int64_t>((rows_q * n_q * kDeltaLanes + 255) / 256, std::max<int64_t>(batch * n_q * kExactTiles, batch * n_kv * p.sink_tiles * kSinkParts)));
+                      std::max<int64_t>({(rows_q * n_q * kDeltaLanes + 255) / 256, batch * n_q * kExactTiles,
+                                                batch * n_kv * p.sink_tiles * kSinkParts}));
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
   p.part_bytes = p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0;
   p.work = p.delta_bytes + p.part_bytes + (size_t)(sinks * 2 * kDkvKeys * head_dim) * sizeof(float);
@@ -748,8 +755,8 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
 
 // dQ of 64 queries a workgroup (two waves over the same 32) or of 128. f32 products are long enough
 // that the finer grid is all that counts; in bf16 128 queries read keys and values half as often,
-// which is the better from about two workgroups a CU on (one and a quarter past 128 elements). us of the whole gradient, 128 / 64 queries,
-// causal, 16/16 heads x 128 unless said (workgroups of 128 queries):
+// which is the better from about two workgroups a CU on (one and a quarter past 128 elements). us of the whole
+// gradient, 128 / 64 queries, causal, 16/16 heads x 128 unless said (workgroups of 128 queries):
 //   bf16  512 tokens (80) 47 / 42   2048 (272) 102 / 87   2048 (32/8 heads, 544) 188 / 183   8 x 512 (640) 78 / 79
 //         8 x 512 (32/8, 1280) 123 / 127   16/2 x 64: 2048 (272) 75 / 67
 //   bf16  x 256: 512 (80) 90 / 78   2048 (272) 276 / 245   64/8 heads, 512 (320) 136 / 132   8 x 256 (384) 86 / 90
