@@ -34,6 +34,27 @@ __device__ __forceinline__ float raised(float amax, bool all_finite, float s0) {
 __device__ __forceinline__ int code_of(float x, float s) {
   return s > 0.0f ? (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.0f), 127.0f) : 0;
 }
+__device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
+  return (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)(c[3] & 255) << 24;
+}
+// four of them; inv: 1 / s. x inv is off by at most 2.3e-5 from the rounded x / s (127 times 3 roundings), so where it is further from
+// a half than that it rounds alike: a third of the instructions of the divisions. (Not for tiny s, whose inverse
+// and quotients have fewer bits.)
+__device__ __forceinline__ uint32_t codes_of(const float* x, float s, float inv) {
+  int c[4];
+  float q[4], far = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    q[j] = x[j] * inv;
+    const float r = rintf(q[j]);
+    far = fmaxf(far, fabsf(q[j] - r));
+    c[j] = (int)r;
+  }
+  if (!(s >= 1e-30f && far <= 0.49997f))
+#pragma unroll
+    for (int j = 0; j < 4; j++) c[j] = code_of(x[j], s);
+  return pack4(c);
+}
 // four codes of a block whose scale rises from s0 to s
 __device__ __forceinline__ uint32_t recoded(uint32_t w, float ratio) {
   uint32_t y = 0;
@@ -43,9 +64,6 @@ __device__ __forceinline__ uint32_t recoded(uint32_t w, float ratio) {
     y |= (uint32_t)(c & 255) << (8 * j);
   }
   return y;
-}
-__device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
-  return (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)(c[3] & 255) << 24;
 }
 // x0, x1 rotated: every operation rounded by itself
 __device__ __forceinline__ void rotate(float x0, float x1, float c, float s, float* y0, float* y1) {
@@ -891,6 +909,28 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
   const bool ok = (uint32_t)page < (uint64_t)p.pages;
   const int in_page = (int)(block * kBlock & ((1 << p.page_bits) - 1));
   const int64_t at = ok ? ((int64_t)page << p.page_bits) + in_page : 0;  // of the block's first row
+  typedef A AV __attribute__((ext_vector_type(V)));
+  constexpr int N = (kBlock * HD / 2 / V + 63) / 64;  // groups of V pairs a lane
+  const int hp = half / V, kvd = p.n_kv * hd, tasks = p.n_q + 2 * p.n_kv;
+  const int task0 = (a.q_out == nullptr ? p.n_q : 0) + chunk * kWaves + wave;
+  // a task's rows, asked for before the angles are formed, or before the rows of the one before are rounded
+  AV x0[N], x1[N];
+  auto ask = [&](int task) {
+    if (task >= tasks) return;
+    const int what = task < p.n_q ? 0 : task < p.n_q + p.n_kv ? 1 : 2;  // q, k, v
+    const int head = what == 0 ? task : what == 1 ? task - p.n_q : task - p.n_q - p.n_kv;
+    const A* x = static_cast<const A*>(what == 0 ? p.q : what == 1 ? p.k : p.v) + head * hd;
+    const int64_t xs = what == 0 ? p.q_stride : what == 1 ? p.k_stride : p.v_stride;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
+      if (r < rows) {
+        x0[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e);
+        x1[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e + half);
+      }
+    }
+  };
+  ask(task0);
   if (p.rope) {
     if (tid < half) turns[tid] = turns_of(tid, hd, p.log2_theta);
     __syncthreads();
@@ -900,53 +940,46 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
     }
     __syncthreads();
   }
-  typedef A AV __attribute__((ext_vector_type(V)));
-  constexpr int N = (kBlock * HD / 2 / V + 63) / 64;  // groups of V pairs a lane
-  const int hp = half / V, kvd = p.n_kv * hd, tasks = p.n_q + 2 * p.n_kv;
-  for (int task = chunk * kWaves + wave; task < tasks; task += chunks * kWaves) {
-    const int what = task < p.n_q ? 0 : task < p.n_q + p.n_kv ? 1 : 2;  // q, k, v
+  for (int task = task0; task < tasks; task += chunks * kWaves) {
+    const int what = task < p.n_q ? 0 : task < p.n_q + p.n_kv ? 1 : 2;
     const int head = what == 0 ? task : what == 1 ? task - p.n_q : task - p.n_q - p.n_kv;
-    if (what == 0 && a.q_out == nullptr) continue;
-    const A* x = static_cast<const A*>(what == 0 ? p.q : what == 1 ? p.k : p.v) + head * hd;
-    const int64_t xs = what == 0 ? p.q_stride : what == 1 ? p.k_stride : p.v_stride;
     A* out = what == 2 ? nullptr : static_cast<A*>(what == 0 ? a.q_out : a.k_out);
     const int64_t os = what == 0 ? a.q_out_stride : a.k_out_stride;
-    AV x0[N], x1[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
-      if (r < rows) {
-        x0[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e);
-        x1[k] = *reinterpret_cast<const AV*>(x + (row0 + r) * xs + e + half);
-      }
-    }
-    float y0[N][V], y1[N][V], amax = 0.0f;
-    bool good = true;
+    float y0[N][V], y1[N][V];
+    uint32_t most = 0;  // bits of the largest |y|: they are in the order of the numbers, infinities and NaN last
 #pragma unroll
     for (int k = 0; k < N; k++) {
       const int i = lane + 64 * k, r = i / hp, e = V * (i - r * hp);
       if (r >= rows) continue;
-      AV z0, z1;
 #pragma unroll
       for (int j = 0; j < V; j++) {
         y0[k][j] = (float)x0[k][j], y1[k][j] = (float)x1[k][j];
         if (what < 2 && p.rope) rotate(y0[k][j], y1[k][j], cs[0][r][e + j], cs[1][r][e + j], &y0[k][j], &y1[k][j]);
-        amax = fmaxf(amax, fmaxf(fabsf(y0[k][j]), fabsf(y1[k][j])));
-        good = good && finite(y0[k][j]) && finite(y1[k][j]);
-        z0[j] = (A)(ok ? y0[k][j] : NAN);  // no page for the row: its outputs say so
-        z1[j] = (A)(ok ? y1[k][j] : NAN);
       }
       if (out != nullptr) {
+        AV z0, z1;
+#pragma unroll
+        for (int j = 0; j < V; j++) z0[j] = (A)y0[k][j], z1[j] = (A)y1[k][j];
+        if (!ok)  // no page for the row: its outputs say so
+#pragma unroll
+          for (int j = 0; j < V; j++) z0[j] = z1[j] = (A)NAN;
         A* o = out + (row0 + r) * os + head * hd + e;
         *reinterpret_cast<AV*>(o) = z0;
         *reinterpret_cast<AV*>(o + half) = z1;
       }
+      if (what > 0)
+#pragma unroll
+        for (int j = 0; j < V; j++)
+          most = max(most, max(__float_as_uint(y0[k][j]) & 0x7fffffff, __float_as_uint(y1[k][j]) & 0x7fffffff));
     }
+    ask(task + chunks * kWaves);
     if (what == 0 || !ok) continue;
     int8_t* codes = static_cast<int8_t*>(what == 1 ? p.kpages : p.vpages) + at * kvd + head * hd;
     float* scale = (what == 1 ? a.kscales : a.vscales) + page * a.scale_stride + (in_page >> 4) * p.n_kv + head;
     const float s0 = before > 0 ? *scale : 0.0f;
-    const float s = raised(wave_max(amax), __all(good), s0);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, off, 64));
+    const float s = raised(__uint_as_float(most), most < 0x7f800000, s0), inv = __fdiv_rn(1.0f, s);
     if (s > s0 && before > 0) {
       const float ratio = __fdiv_rn(s0, s);
       for (int i = lane; i < before * (hd / 4); i += 64) {
@@ -963,14 +996,8 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
       CV w0, w1;
 #pragma unroll
       for (int n = 0; n < V / 4; n++) {
-        int d0[4], d1[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          d0[j] = code_of(y0[k][4 * n + j], s);
-          d1[j] = code_of(y1[k][4 * n + j], s);
-        }
-        w0[n] = pack4(d0);
-        w1[n] = pack4(d1);
+        w0[n] = codes_of(&y0[k][4 * n], s, inv);
+        w1[n] = codes_of(&y1[k][4 * n], s, inv);
       }
       int8_t* o = codes + (int64_t)(before + r) * kvd + e;
       *reinterpret_cast<CV*>(o) = w0;
