@@ -89,7 +89,7 @@ hipError_t launch_pages_append(int dtype, int cache_dtype, const PagesAppendArgs
 // over int8 pages
 hipError_t launch_paged_attention_q8(int dtype, const PagedAttnArgs& a, hipStream_t stream);
 hipError_t launch_pages_append_q8(int dtype, const PagesAppendArgs& a, hipStream_t stream);
-// of blocks: its workgroups, or a few times as many when they are few
+// of blocks: the workgroups that its rows take at least
 int64_t append_q8_slots(const PagesAppendArgs& a);
 hipError_t launch_pages_rows(int dtype, int cache_dtype, const PagesRowsArgs& a, hipStream_t stream);
 // workgroups of one page and plane

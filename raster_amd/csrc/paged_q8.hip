@@ -37,9 +37,9 @@ __device__ __forceinline__ int code_of(float x, float s) {
 __device__ __forceinline__ uint32_t pack4(const int (&c)[4]) {
   return (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)(c[3] & 255) << 24;
 }
-// four of them; inv: 1 / s. x inv is off by at most 2.3e-5 from the rounded x / s (127 times 3 roundings), so where it is further from
-// a half than that it rounds alike: a third of the instructions of the divisions. (Not for tiny s, whose inverse
-// and quotients have fewer bits.)
+// four of them; inv: 1 / s. x inv is off by at most 2.3e-5 from the rounded x / s (127 times 3 roundings), so where
+// it is further from a half than that it rounds alike: a third of the instructions of the divisions. (Not for tiny s,
+// whose inverse and quotients have fewer bits.)
 __device__ __forceinline__ uint32_t codes_of(const float* x, float s, float inv) {
   int c[4];
   float q[4], far = 0.0f;
@@ -876,9 +876,9 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 
 // RoPE and append of packed rows, a workgroup the rows of one block and some of the heads, a wave a head at a time:
 // its rows stay in registers between their maximum and their codes: each value is read once and each code written once.
-// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45.6 us, 4.4 TB/s (a copy reaches 4.9); 56 with
-// 8 bytes a load, 72 with an angle's sine and cosine by the general functions. Without cu row b is the one row of
-// sequence b, at position past[b].
+// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45 us, 4.5 TB/s (a copy reaches 4.9). 72 with
+// an angle's sine and cosine by the general functions, 56 with 8 bytes a load, 50 with divisions and no load ahead of
+// the angles. Without cu row b is the one row of sequence b, at position past[b].
 template <typename A, int HD, int V>
 __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendArgs a, int chunks) {
   const PagesArgs& p = a.p;
@@ -1047,9 +1047,11 @@ hipError_t run_paged_q8_hd(const PagedAttnArgs& a, hipStream_t stream) {
 
 template <typename A, int HD, int V>
 hipError_t run_append_q8(const PagesAppendArgs& a, hipStream_t stream) {
-  // A wave takes one head of a small call, more of a large one, so that the angles are formed less often
+  // A wave takes one head, though every workgroup forms its rows' angles; more only where the grid has no room. us, by
+  // about 2048 workgroups / so: 8192 rows (32/8 x 128, bf16) 45.8 / 46.0, in f32 94 / 78, 16000 (64/8) 150 / 129
   const int64_t slots = append_q8_slots(a), tasks = a.p.n_q + 2 * a.p.n_kv;
-  const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((tasks + kWaves - 1) / kWaves, (2048 + slots - 1) / slots));
+  const int64_t chunks =
+      std::max<int64_t>(1, std::min((tasks + kWaves - 1) / kWaves, kMaxGroups / std::max<int64_t>(slots, 1)));
   hipLaunchKernelGGL((pages_append_q8_kernel<A, HD, V>), dim3((unsigned)(slots * chunks)), dim3(kThreads), 0, stream, a,
                      (int)chunks);
   return hipGetLastError();
