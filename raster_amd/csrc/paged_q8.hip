@@ -882,7 +882,8 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 template <typename A, int HD, int V>
 __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendArgs a, int chunks) {
   const PagesArgs& p = a.p;
-  __shared__ __attribute__((aligned(16))) float cs[2][kBlock][HD / 2];
+  // (rows 16 bytes apart more than they are long: 8 lanes read 16 of every 32 bytes of a row, the next 8 of the next row)
+  __shared__ __attribute__((aligned(16))) float cs[2][kBlock][HD / 2 + 4];
   __shared__ double turns[HD / 2];
   const int tid = threadIdx.x, lane = tid & 63, hd = p.head_dim, half = hd / 2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
