@@ -647,8 +647,10 @@ int rq_paged_attention_window(rq_ctx ctx, const rq_pages* pg, float* kscales, fl
  * or reads the block gets NaN until its first row is written again. A block whose x are all 0, or so small that s
  * is 0, holds zeros. rq_paged_attention_window appends the new row so and attends it, and the rows of its block, as
  * they are stored; the block it goes into must be of its sequence alone (rows of other blocks may be shared).
- * Queries and weights enter as for bf16 pages, codes exactly. With more than 16 query heads a KV head the row is
- * appended in a launch before. Types: dtype RQ_F32 or RQ_BF16. */
+ * Queries enter with 23 bits (bf16: 15) of a head's largest element, weights with as many of the largest product of
+ * a weight and its block's scale among 64 rows, codes exactly; queries and values that are all below 1e-31 with
+ * fewer. With more than 16 query heads a KV head the row is appended in a launch before. Types: dtype RQ_F32 or
+ * RQ_BF16. */
 
 /* rq_pages_append into int8 pages. */
 int rq_pages_append_q8(rq_ctx ctx, const rq_pages* pg, float* kscales, float* vscales, int64_t scale_stride, int dtype,

@@ -172,11 +172,12 @@ __device__ __forceinline__ float value_of(int d0, int d1) { return (float)((d1 <
 __device__ __forceinline__ float value_of(int d0, int d1, int d2) {
   return fmaf((float)((d2 << 8) + d1), 256.0f, (float)d0);
 }
-// The factor that takes numbers up to `most` to digits, not past f32's range. (By the hardware's reciprocal, to one
-// unit in the last place: an inverse of the same kind takes them back. The largest digit has room for it.)
+// The factor that takes numbers up to `most` to digits. (By the hardware's reciprocal, to one unit in the last place: an
+// inverse of the same kind takes them back. The largest digit has room for it.) Up to 2^126, whose inverse is the
+// smallest that the hardware forms: numbers below 1e-31 get fewer digits.
 template <int NT>
 __device__ __forceinline__ float digit_factor(float most) {
-  return most > 0.0f ? fminf((float)kDigitsMax<NT> * __builtin_amdgcn_rcpf(most), 1e38f) : 0.0f;
+  return most > 0.0f ? fminf((float)kDigitsMax<NT> * __builtin_amdgcn_rcpf(most), 0x1p126f) : 0.0f;
 }
 
 // Ranges of rows, by the real lengths. Sequence b's walked rows are cut into ranges of R rows, one at least, and the

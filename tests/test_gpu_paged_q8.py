@@ -197,6 +197,75 @@ def test_append(torch, ctx, act, nq, nkv, hd, page, lens, past, theta, in_place)
     assert torch.equal(v, v0)
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("most", [127.0, 1.0, 3.7e5, 3e38, 1.28e-28, 1.26e-28, 1e-36, 3e-38, 2e-43])
+def test_codes_where_two_are_as_near(torch, ctx, act, most):
+    """Values halfway between two codes and the floats beside those, with scales up to the largest and down to
+    denormal ones: the codes of the definition, bit for bit, from prompts and from single tokens."""
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 ties {act} {most}", flush=True)
+    dt = torch.float32 if act == "f32" else torch.bfloat16
+    top = torch.tensor(most).to(dt).float()
+    s = top * torch.tensor(1 / 127)
+    x = (torch.arange(-127, 127) + 0.5) * s
+    inf = torch.tensor(float("inf"))
+    x = torch.stack([x, torch.nextafter(x, inf), torch.nextafter(x, -inf)]).flatten().to(dt).float()
+    x = x[x.abs() <= top]
+    x = torch.cat([top[None], x, torch.zeros(16 * 128)])[:16 * 128].view(16, 1, 128)
+    codes, scales = torch.zeros((1, 16, 1, 128), dtype=torch.int8), torch.zeros((1, 1))
+    q8_ref.put(codes, scales, 0, x)
+    one = codes.clone()
+    for single in (False, True):
+        cache = q8_ref.Cache(1, 1, 128, [16], 16, [0])
+        k = x.view(16, 128).to("cuda", dt)
+        if single:
+            for i in range(16):
+                raster_amd.paged_attention(ctx, k[i:i + 1], k[i:i + 1], k[i:i + 1], cache.k, cache.v, cache.table,
+                                           torch.tensor([i], dtype=torch.int32, device="cuda"), 1, 1, 128, 0.0, 0.1,
+                                           max_len=16, **cache.scales())
+        else:
+            raster_amd.pages_append(ctx, k, k, k, cache.k, cache.v, cache.table,
+                                    torch.tensor([0, 16], dtype=torch.int32, device="cuda"),
+                                    torch.zeros(1, dtype=torch.int32, device="cuda"), 1, 1, 128, 0.0, **cache.scales())
+        page = int(cache.table[0, 0])
+        for pages, sc in ((cache.k, cache.ks), (cache.v, cache.vs)):
+            assert float(sc[page, 0, 0]) == float(scales[0, 0])
+            assert torch.equal(pages[page].cpu().view(16, 1, 128), one[0])
+
+
+@pytest.mark.parametrize("act,nq", [("f32", 4), ("f32", 8), ("bf16", 8), ("bf16", 16)])
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_small_and_large_values(torch, ctx, act, nq, size):
+    """Values far from 1. Weights times scales are whole numbers, 2^126 at most for 1: the largest of a tile has p = 1 and
+    a scale of more than 1e-30 / 127 = 8e-33 (a block's largest of 1024 normal values is above 1), so 6.7e5 units at least, or
+    0x7F7E for bf16 results. Each is off by half of one, which the row's code multiplies; 2^-7 of the sum of p |v|
+    is more than all other roundings (bf16's 2^-8, the scores')."""
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 size {size} {act} {nq}", flush=True)
+    n, nkv, hd = 200, 2, 64
+    cache = q8_ref.Cache(5, nkv, hd, [n], 16, [n])
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache.append("v", 0, 0, torch.randn((n, nkv, hd), generator=g, device="cuda") * size)
+    dt = torch.float32 if act == "f32" else torch.bfloat16
+    q = torch.randn((1, nq * hd), generator=g, device="cuda").to(dt)
+    out = raster_amd.paged_attention(ctx, q, None, None, cache.k, cache.v, cache.table,
+                                     torch.tensor([n], dtype=torch.int32, device="cuda"), nq, nkv, hd, 0.0, hd ** -0.5,
+                                     max_len=n, **cache.scales())
+    keys, values = cache.values("k", 0, n), cache.values("v", 0, n)
+    for h in range(nq):
+        kv = h // (nq // nkv)
+        p = torch.softmax(keys[:, kv] @ q[0, h * hd:(h + 1) * hd].double() * hd ** -0.5, 0)
+        want, most = p @ values[:, kv], p @ values[:, kv].abs()
+        scales = cache.vs[cache._mine(0, n)].reshape(-1, nkv)[:, kv].double().repeat_interleave(16)[:n]
+        off = 0.5 / (6.7e5 if act == "f32" else 0x7F7E) * (p * scales).max()
+        bound = 2.0 ** -7 * most + off * (values[:, kv] / scales[:, None]).abs().sum(0)
+        assert bool(((out[0, h * hd:(h + 1) * hd].double() - want).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (40, 2, 64)])
 def test_a_block_fills_row_by_row(torch, ctx, nq, nkv, hd):
     """33 tokens one by one, of rising and falling size: codes rounded anew, scales that only rise in a block and
