@@ -877,7 +877,7 @@ __global__ __launch_bounds__(256) void paged_q8_merge_kernel(PagedAttnArgs a) {
 
 // RoPE and append of packed rows, a workgroup the rows of one block and some of the heads, a wave a head at a time:
 // its rows stay in registers between their maximum and their codes: each value is read once and each code written once.
-// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 45 us, 4.5 TB/s (a copy reaches 4.9). 72 with
+// Bound by the memory: 8192 rows of 32/8 heads x 128 in bf16, 201 MB, 44 us, 4.6 TB/s (a copy reaches 4.9). 72 with
 // an angle's sine and cosine by the general functions, 56 with 8 bytes a load, 50 with divisions and no load ahead of
 // the angles. Without cu row b is the one row of sequence b, at position past[b].
 template <typename A, int HD, int V>

@@ -516,6 +516,42 @@ def test_graphs(torch, ctx):
         assert c.same(held)
 
 
+@pytest.mark.parametrize("batch,max_len", [(1, 2500), (30, 2500), (90, 2500), (130, 2500), (400, 1500)])
+def test_a_graph_follows_the_lengths(torch, ctx, batch, max_len):
+    """One captured call replayed over new lengths, ranges planned by waves, by workgroups or not at all: the
+    eager call's bits."""
+    import raster_amd
+
+    print(f"[gpu] q8 graph over lengths {batch} {max_len}", flush=True)
+    nq, nkv, hd, pages = 8, 2, 64, 400
+    gen = torch.Generator(device="cuda").manual_seed(batch)
+    kp, vp = (torch.randint(-127, 128, (pages, 16, nkv * hd), generator=gen, device="cuda", dtype=torch.int32)
+              .to(torch.int8) for _ in range(2))
+    ks, vs = (torch.rand((pages, 1, nkv), generator=gen, device="cuda") * 0.02 + 0.01 for _ in range(2))
+    table = torch.randint(0, pages, (batch, (max_len + 15) // 16), generator=gen, device="cuda", dtype=torch.int32)
+    q = torch.randn((batch, nq * hd), generator=gen, device="cuda")
+    lens = torch.full((batch,), 40, dtype=torch.int32, device="cuda")
+
+    def call():
+        return raster_amd.paged_attention(ctx, q, None, None, kp, vp, table, lens, nq, nkv, hd, THETA, hd ** -0.5,
+                                          max_len=max_len, kscales=ks, vscales=vs)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = call()
+    for top in (max_len, 300, 0, max_len):
+        lens.copy_(torch.randint(-1, top + 1, (batch,), generator=gen, device="cuda", dtype=torch.int32))
+        lens[batch // 2] = top
+        graph.replay()
+        got = out.clone()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and not bool(torch.isnan(want).any())
+        assert bool((want[lens <= 0] == 0).all()) and (top == 0 or bool((want[batch // 2] != 0).any()))
+
+
 def test_offsets_past_32_bits(torch, ctx):
     """Pages of 4.6 GiB of codes a plane, the last ones used."""
     import raster_amd
