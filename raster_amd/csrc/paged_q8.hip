@@ -174,10 +174,11 @@ __device__ __forceinline__ float value_of(int d0, int d1, int d2) {
 }
 // The factor that takes numbers up to `most` to digits. (By the hardware's reciprocal, to one unit in the last place: an
 // inverse of the same kind takes them back. The largest digit has room for it.) Up to 2^126, whose inverse is the
-// smallest that the hardware forms: numbers below 1e-31 get fewer digits.
+// smallest that the hardware forms: numbers below 1e-31 get fewer digits. Of numbers past 2^126 it forms none, so of a
+// sixteenth of them; those powers of two change no other bit.
 template <int NT>
 __device__ __forceinline__ float digit_factor(float most) {
-  return most > 0.0f ? fminf((float)kDigitsMax<NT> * __builtin_amdgcn_rcpf(most), 0x1p126f) : 0.0f;
+  return most > 0.0f ? fminf((float)kDigitsMax<NT> * 0.0625f * __builtin_amdgcn_rcpf(most * 0.0625f), 0x1p126f) : 0.0f;
 }
 
 // Ranges of rows, by the real lengths. Sequence b's walked rows are cut into ranges of R rows, one at least, and the

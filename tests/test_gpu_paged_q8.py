@@ -665,3 +665,47 @@ def test_streams_and_threads(torch, ctx):
     torch.cuda.synchronize()
     for (c, d, _), x, y in zip(sets, want, got):
         assert d.same(c) and all(torch.equal(p, r) for p, r in zip(x, y))
+
+
+@pytest.mark.parametrize("act,nq", [("f32", 4), ("f32", 8), ("bf16", 8), ("bf16", 16), ("bf16", 40)])
+@pytest.mark.parametrize("most", [8e37, 1e38, 3.3e38])
+def test_queries_up_to_the_largest(torch, ctx, act, nq, most):
+    """Queries whose largest element is past 2^126 over normal keys: scores so far apart that one key has all the weight.
+
+    A score is off by step * max |q| times the sum of |k| (check_out) and by (hd + 4) 2^-24 of the products' magnitudes, or
+    2^-22 of them. Where the best is ahead of the second by more than twice that and 1000, every other weight is below
+    2^-1000, 0 in f32. The best one is 1 (f32: exp2 of its own difference, 0), with its block's scale a whole number of
+    steps of the tile's largest scale; the sum of weights is 1, its join with other ranges exact: the row's values, off by
+    step * the largest scale * |code|, a few 2^-24 and the result's rounding."""
+    import attn_ref as ref
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 queries {most} {act} {nq}", flush=True)
+    nkv, hd, lens, scale = 2, 64, [200, 2500], 0.01
+    cache = q8_ref.Cache(6, nkv, hd, lens, 16, lens)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn((2, nq, hd), generator=g, device="cuda")
+    q = (q / q.abs().amax(2, keepdim=True) * most).to(torch.float32 if act == "f32" else torch.bfloat16)
+    out = raster_amd.paged_attention(ctx, q.view(2, -1), None, None, cache.k, cache.v, cache.table,
+                                     torch.tensor(lens, dtype=torch.int32, device="cuda"), nq, nkv, hd, 0.0, scale,
+                                     max_len=2500, **cache.scales())
+    half = ref.HALF[out.dtype]
+    step = 0.5 / (0x7F7F7C if act == "f32" else 0x7F7E) * (1 + 2.0 ** -20)
+    sure = 0
+    for b, n in enumerate(lens):
+        keys, values = cache.values("k", b, n), cache.values("v", b, n)
+        scales = cache.vs[cache._mine(b, n)].reshape(-1, nkv).double()
+        for h in range(nq):
+            qh, kh, vh = q[b, h].double(), keys[:, h // (nq // nkv)], values[:, h // (nq // nkv)]
+            top, at = (kh @ qh * scale).topk(2)
+            off = step * qh.abs().max() * kh.abs().sum(1).max() * scale + 2.0 ** -22 * (kh.abs() @ qh.abs()).max() * scale
+            got = out[b, h * hd:(h + 1) * hd].double()
+            assert bool(torch.isfinite(got).all())
+            if top[0] - top[1] <= 2 * off + 1000:
+                continue
+            sure += 1
+            s = scales[:, h // (nq // nkv)]
+            want, code = vh[at[0]], vh[at[0]].abs() / s[at[0] // 16]
+            assert bool(((got - want).abs() <= (half + 2.0 ** -21) * want.abs() + step * s.max() * code).all()), (b, h)
+    assert sure >= nq
