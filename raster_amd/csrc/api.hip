@@ -1639,6 +1639,7 @@ static int pages_append(rq_ctx h, const rq_pages* pg, float* kscales, float* vsc
   a.rows = rows;
   a.q_out = q_out, a.k_out = k_out;
   a.q_out_stride = q_out_stride, a.k_out_stride = k_out_stride;
+  a.max_len = INT64_MAX;
   a.kscales = kscales, a.vscales = vscales, a.scale_stride = scale_stride;
   if (pg->dtype == RQ_I8 && append_q8_slots(a) > kMaxGroups)
     return fail(RQ_ERR_SHAPE, "too many rows and sequences for one launch");

@@ -47,7 +47,7 @@ struct PagesAppendArgs {
   void *q_out, *k_out;  // k_out may be NULL
   int64_t q_out_stride, k_out_stride;
   // int8 pages only; cu NULL: row b is the one row of sequence b, and q_out may be NULL
-  int64_t max_len;  // 0: any, else rows past it are not stored
+  int64_t max_len;  // rows past it are not stored
   float *kscales, *vscales;
   int64_t scale_stride;
 };

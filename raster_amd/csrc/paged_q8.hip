@@ -907,7 +907,7 @@ __global__ __launch_bounds__(kThreads) void pages_append_q8_kernel(PagesAppendAr
   if (pos0 >= pos1) return;
   const int rows = (int)(pos1 - pos0), before = (int)(pos0 - block * kBlock);
   const int64_t row0 = c0 + pos0 - past;  // packed row of the first
-  const bool inside = pos0 < p.table_stride << p.page_bits && (a.max_len == 0 || pos1 <= a.max_len);
+  const bool inside = pos0 < p.table_stride << p.page_bits && pos1 <= a.max_len;
   const int page = inside ? p.table[(int64_t)b * p.table_stride + (pos0 >> p.page_bits)] : -1;
   const bool ok = (uint32_t)page < (uint64_t)p.pages;
   const int in_page = (int)(block * kBlock & ((1 << p.page_bits) - 1));

@@ -709,3 +709,21 @@ def test_queries_up_to_the_largest(torch, ctx, act, nq, most):
             want, code = vh[at[0]], vh[at[0]].abs() / s[at[0] // 16]
             assert bool(((got - want).abs() <= (half + 2.0 ** -21) * want.abs() + step * s.max() * code).all()), (b, h)
     assert sure >= nq
+
+
+def test_no_rows_allowed(torch, ctx):
+    """max_len 0 allows no row: nothing is stored, whatever the heads a KV head; results are NaN, an idle slot's zeros."""
+    import q8_ref
+    import raster_amd
+
+    for nq, nkv in ((4, 2), (40, 2)):
+        print(f"[gpu] q8 max_len 0 {nq}/{nkv}", flush=True)
+        lens = [40, 0, -1, 47]
+        cache = q8_ref.Cache(5, nkv, 64, [n + 1 for n in lens], 16, lens)
+        start = cache.clone()
+        q, k, v = (9 * x for x in new_rows(torch, 5, "f32", 4, nq, nkv, 64))  # (larger than what is there: a scale would rise)
+        out = raster_amd.paged_attention(ctx, q, k, v, cache.k, cache.v, cache.table,
+                                         torch.tensor(lens, dtype=torch.int32, device="cuda"), nq, nkv, 64, THETA, 0.1,
+                                         max_len=0, **cache.scales())
+        assert cache.same(start)
+        assert bool(torch.isnan(out[[0, 1, 3]]).all()) and bool((out[2] == 0).all())
