@@ -727,3 +727,41 @@ def test_no_rows_allowed(torch, ctx):
                                          max_len=0, **cache.scales())
         assert cache.same(start)
         assert bool(torch.isnan(out[[0, 1, 3]]).all()) and bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("nq", [4, 8])
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_small_and_large_values_in_f32(torch, ctx, nq, size):
+    """f32 results over values far from 1, by the roundings of f32 arithmetic. At 1e30 check_out's bounds scale with the
+    values. At 1e-30 weights have 6.7e5 units only (test_small_and_large_values); beside those attend's bound."""
+    import attn_ref as ref
+    import q8_ref
+    import raster_amd
+
+    print(f"[gpu] q8 size in f32 {size} {nq}", flush=True)
+    n, nkv, hd = 200, 2, 64
+    cache = q8_ref.Cache(5, nkv, hd, [n], 16, [n])
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache.append("v", 0, 0, torch.randn((n, nkv, hd), generator=g, device="cuda") * size)
+    q = torch.randn((1, nq * hd), generator=g, device="cuda")
+    out = raster_amd.paged_attention(ctx, q, None, None, cache.k, cache.v, cache.table,
+                                     torch.tensor([n], dtype=torch.int32, device="cuda"), nq, nkv, hd, 0.0, hd ** -0.5,
+                                     max_len=n, **cache.scales())
+    qd = q.double().view(1, nq, hd)
+    if size > 1:
+        check_out(torch, ref, out, qd, cache, [n], 0, nq, nkv, hd, hd ** -0.5, 0, 0)
+        return
+    keys, values = cache.values("k", 0, n), cache.values("v", 0, n)
+    step = 0.5 / 0x7F7F7C * (1 + 2.0 ** -20)
+    see = torch.ones((1, n), dtype=torch.bool, device="cuda")
+    for h in range(nq):
+        kv = h // (nq // nkv)
+        qh, kh, vh = qd[0, h:h + 1], keys[:, kv], values[:, kv]
+        scales = cache.vs[cache._mine(0, n)].reshape(-1, nkv)[:, kv].double().repeat_interleave(16)[:n]
+        # (in units of the values, so that attend's 1e-30 for results of 0 counts for nothing)
+        want, lse, bound = ref.attend(qh, kh, vh / size, hd ** -0.5, see, ref.HALF[torch.float32], 2.0 ** -22)
+        p = torch.softmax(qh @ kh.T * hd ** -0.5, 1)[0]
+        off = step * qh.abs().max() * kh.abs().sum(1).max() * hd ** -0.5
+        units = 0.5 / 6.7e5 * (p * scales).max() / size * (vh / scales[:, None]).abs().sum(0)
+        got = out[0, h * hd:(h + 1) * hd].double() / size
+        assert bool(((got - want[0]).abs() <= bound[0] + 2 * off * (p @ vh.abs()) / size + units).all())
