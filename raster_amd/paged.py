@@ -276,14 +276,61 @@ class PagedCache:
         lens = [self._len[self._known(s)] + n for s, n in zip(seqs, more)]
         for s, n in zip(seqs, lens):
             _need(0 <= n <= len(self._pages[s]) * self.page_size, f"sequence {s} has no {n} rows")
-        self.sync()
-        dev = self.data.device
-        table = self._table[torch.tensor(seqs, dtype=torch.long, device=dev)]
-        cu = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device=dev)
         if dtype is None:
             dtype = torch.float32 if self.scales is not None else self.data.dtype
+        if not self._for_operators():
+            at = [np.arange(n) % self.page_size + np.repeat(np.array(self._pages[s], np.int64), self.page_size)[:n] * self.page_size
+                  for s, n in zip(seqs, lens)]
+            at = torch.from_numpy(np.concatenate([np.zeros(0, np.int64), *at])).to(self.data.device)
+            return tuple(x.view(-1, x.shape[-1])[at].to(dtype) for x in (self.kpages(layer), self.vpages(layer)))
+        self.sync()
+        calls = self._cut(seqs, lens)
+        if len(calls) == 1:
+            return self._rows(layer, *calls[0], dtype)
+        k, v = (torch.empty((sum(lens), self.n_kv * self.head_dim), dtype=dtype, device=self.data.device) for _ in range(2))
+        done = 0
+        for call in calls:
+            part = slice(done, done + sum(call[2]))
+            self._rows(layer, *call, dtype, k_out=k[part], v_out=v[part])
+            done = part.stop
+        return k, v
+
+    def _rows(self, layer: int, seqs, page: int, lens, dtype, **out):
+        """lens[i] rows of seqs[i] from page number `page` of it on (not 0: of one sequence)."""
+        torch, dev = _t(), self.data.device
+        if page:
+            table = self._table[seqs[0], page:][None]
+        else:
+            table = self._table[torch.tensor(seqs, dtype=torch.long, device=dev)]
+        cu = torch.tensor(np.cumsum([0] + lens), dtype=torch.int32, device=dev)
         return pages_rows(self.ctx, self.kpages(layer), self.vpages(layer), table, cu, sum(lens), self.n_kv,
-                          self.head_dim, dtype, **self.layer_scales(layer))
+                          self.head_dim, dtype, **out, **self.layer_scales(layer))
+
+    def _cut(self, seqs, lens) -> list:
+        """The rows of seqs in turn as (sequences, first page, rows of each), a pages_rows each, which takes fewer than
+        2^24 rows: many sequences from their first page on, or pages of a longer one."""
+        most = (1 << 24) - 1
+        whole = most // self.page_size * self.page_size
+        calls, room = [], -1
+        for s, n in zip(seqs, lens):
+            if n > whole:
+                calls += [([s], r // self.page_size, [min(whole, n - r)]) for r in range(0, n, whole)]
+                room = -1
+            elif n <= room:
+                calls[-1][0].append(s)
+                calls[-1][2].append(n)
+                room -= n
+            else:
+                calls.append(([s], 0, [n]))
+                room = most - n
+        return calls or [([], 0, [])]
+
+    def _for_operators(self) -> bool:
+        """Whether the operators take the cache's pages: others are a place for rows only."""
+        torch = _t()
+        return (self.data.dtype in (torch.float32, torch.bfloat16, torch.int8) and self.head_dim % 8 == 0
+                and self.head_dim <= 256 and self.page_size <= 65536 and self.n_kv <= 65535
+                and self.n_kv * self.head_dim <= 1 << 22)
 
     def _take(self) -> int:
         p = heapq.heappop(self._free)
