@@ -70,6 +70,8 @@ __global__ __launch_bounds__(256) void prompt_delta_kernel(PromptArgs a) {
 // the first queries of a sequence as much as all other roundings together (error of dQ of 37, 5 and 12
 // tokens, in roundings of the result: 1.60; of 777, 1500, 331 and 64: 1.50). Here D is formed from the
 // weights, sum_j p_ij dO_i . V_j (1.42 and 1.43; with 256 keys 1.43).
+// This kernel takes a sequence's first queries, those with at most kExactKeys keys up to themselves; with a window and
+// sinks of no more than that in all, every query is one of few keys, and prompt_delta_few_kernel's.
 // One workgroup a sequence and head (without a causal mask several, for its many queries): a wave
 // 32 queries and 32 keys. 5.5 us beside the other kernel's 19 at 6719 tokens in six sequences, 32/8 heads x 128
 // (from registers, each lane its row, 15: 64 cache lines a load).
@@ -127,6 +129,72 @@ __global__ __launch_bounds__(256) void prompt_delta_exact_kernel(PromptArgs a) {
       a.delta[(int64_t)hq * a.rows_q + first + tid] = part[tid >> 5][tid & 31] + part[2 + (tid >> 5)][tid & 31];
     __syncthreads();
   }
+}
+
+// D of all queries from their weights where window + sinks <= kExactKeys: 64 queries a workgroup, its sinks' tile and
+// those that its window reaches, a wave 32 queries and 32 keys of each. It takes the place of both others. Error of dQ
+// of its norm, D from the rounded O and this way, queries from 64 on: window 2 0.0037 / 0.0023, 8 and 4 sinks 0.0026 /
+// 0.0023, 32 0.0025 / 0.0024, 60 and 4 sinks 0.0025 / 0.0024 (100 and 4 sinks, O: 0.0024). us of the whole gradient, so:
+// 4096, 777, 1500, 331, 1999 and 64 tokens, 32/8 heads x 128, window 2 213 / 230, 60 and 4 sinks 275 / 302; 1000 and
+// 500, 16/4 x 256, 2 57 / 61; 512, 16/2 x 64, 2 41 / 39; 37, 5 and 12, 32/8 x 128, 33 / 30.
+static bool few_keys(const PromptArgs& a) { return a.window > 0 && a.window + a.sinks <= kExactKeys; }
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void prompt_delta_few_kernel(PromptArgs a) {
+  using TL = Tile<T, HD>;
+  constexpr int kTile = TL::bytes(64);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float part[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, i = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qb = 32 * (wave & 1), kb = 32 * (wave >> 1);
+  const int group = a.n_q / a.n_kv, hkv = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv, hq = hkv * group + rest % group;
+  const TileSpan tq = tile_of_slot(a.cu_q, a.batch, a.rows_q, 64, rest / group);
+  if (tq.len == 0) return;
+  const int64_t k0 = clamp_cu(a.cu_k, tq.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tq.seq + 1, a.rows_k);
+  const int lk = (int)(k1 > k0 ? k1 - k0 : 0), n = min(tq.len - tq.row0, 64), pos = tq.row0 + lk - tq.len;
+  const int64_t first = tq.begin + tq.row0;
+  Walk<true> walk;
+  const int nk = min(max(pos + n, 0), lk) - walk.leave_out(a, pos, 64);
+  const T* kbase = static_cast<const T*>(a.k) + k0 * a.k_stride + hkv * a.head_dim;
+  const T* vbase = static_cast<const T*>(a.v) + k0 * a.v_stride + hkv * a.head_dim;
+  Stage<T, HD, 64, 256> x, y;
+  auto load = [&](int key) {
+    x.load(kbase + (int64_t)key * a.k_stride, a.k_stride, walk.rows_from(key, lk), a.head_dim, tid);
+    y.load(vbase + (int64_t)key * a.v_stride, a.v_stride, walk.rows_from(key, lk), a.head_dim, tid);
+  };
+  x.load(static_cast<const T*>(a.q) + first * a.q_stride + hq * a.head_dim, a.q_stride, n, a.head_dim, tid);
+  y.load(static_cast<const T*>(a.dout) + first * a.dout_stride + hq * a.head_dim, a.dout_stride, n, a.head_dim, tid);
+  x.store(lds + 2 * kTile, tid);
+  y.store(lds + 3 * kTile, tid);
+  if (nk > 0) load(walk.key(0));
+  const int r = qb + i;
+  Seen<true> see;
+  see.init(a, tq.row0 + r, lk - tq.len, lk);
+  const float lse = base2_lse(a.lse[(int64_t)hq * a.rows_q + first + min(r, n - 1)]);
+  float sum = 0.0f;
+  for (int at = 0; at < nk; at += 64) {
+    x.store(lds, tid);
+    y.store(lds + kTile, tid);
+    if (at + 64 < nk) load(walk.key(at + 64));
+    __syncthreads();
+    const int key = walk.key(at) + kb;
+    if (key <= pos + qb + 31 && window_any<true>(a, pos + qb, key, 32)) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) {
+        s = tile_mma(TL::frag(lds, kb + i, d, h), TL::frag(lds + 2 * kTile, r, d, h), s);
+        dp = tile_mma(TL::frag(lds + kTile, kb + i, d, h), TL::frag(lds + 3 * kTile, r, d, h), dp);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (see.sees(key + 8 * (j >> 2) + 4 * h + (j & 3)))
+          sum += __builtin_amdgcn_exp2f(fmaf(s[j], a.scale2, -lse)) * dp[j];
+    }
+    __syncthreads();
+  }
+  sum += __shfl_xor(sum, 32, 64);
+  if (h == 0) part[wave][i] = sum;
+  __syncthreads();
+  if (tid < n) a.delta[(int64_t)hq * a.rows_q + first + tid] = part[tid >> 5][tid & 31] + part[2 + (tid >> 5)][tid & 31];
 }
 
 template <typename T, int HD>
@@ -678,19 +746,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prom
 template <typename T, int HD, int BK, int QG, bool WIN>
 hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   using TL = Tile<T, HD>;
-  if (a.rows_q > 0) {
+  const bool few = WIN && sizeof(T) == 2 && few_keys(a);
+  if (a.rows_q > 0 && !few) {
     const int64_t n = a.rows_q * a.n_q * kDeltaLanes;
     hipLaunchKernelGGL(prompt_delta_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
     if (hipError_t e = hipGetLastError()) return e;
-    if (sizeof(T) == 2) {
-      constexpr int lds = 4 * Tile<__bf16, HD>::bytes(64);
-      const auto kernel = prompt_delta_exact_kernel<__bf16, HD>;
-      static std::atomic<uint64_t> allowed{0};
-      if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
-      const int64_t groups = (int64_t)a.batch * a.n_q * (a.causal ? 1 : kExactTiles);
-      hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, stream, a);
-      if (hipError_t e = hipGetLastError()) return e;
-    }
+  }
+  if (a.rows_q > 0 && sizeof(T) == 2) {
+    constexpr int lds = 4 * Tile<__bf16, HD>::bytes(64);
+    const auto kernel = few ? prompt_delta_few_kernel<__bf16, HD> : prompt_delta_exact_kernel<__bf16, HD>;
+    static std::atomic<uint64_t> allowed[2];
+    if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed[few])) return e;
+    const int64_t groups = few ? tile_slots(a.rows_q, a.batch, 64) * a.n_q
+                               : (int64_t)a.batch * a.n_q * (a.causal ? 1 : kExactTiles);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, stream, a);
+    if (hipError_t e = hipGetLastError()) return e;
   }
   constexpr int dq_lds = QG == 4 ? 4 * TL::bytes(BK) : std::max(2 * TL::bytes(128 / QG), 4 * 32 * (HD + 4) * 4);
   constexpr int lds = std::max(dkv_lds<T, HD>(), dq_lds);

@@ -375,3 +375,61 @@ def test_nan_behind_the_sinks(torch, ctx, t, nq, n, window, sinks):
     keep[max(0, last - window + 1 - 94):] = False
     for a, b in zip(clean[2:], dirty[2:]):
         assert bool(torch.isnan(b[:sinks]).all()) and torch.equal(a[keep], b[keep])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 200])
+@pytest.mark.parametrize("window,sinks,lq,lk", [
+    (2, 0, [700, 90], [700, 90]),
+    (4, 1, [300, 65, 1000], [300, 65, 1000]),
+    (8, 0, [600, 0, 5], [600, 30, 5]),
+    (16, 16, [500], [500]),
+    (60, 4, [333, 200], [333, 200]),
+    (1, 63, [400], [400]),
+    (20, 5, [100, 300, 40], [700, 200, 0]),  # the end of a sequence; more queries than keys; no keys
+])
+def test_gradient_of_few_keys(torch, ctx, hd, window, sinks, lq, lk):
+    """bf16, no query sees more than 64 keys: dout . out is formed from the weights, not from the rounded out.
+
+    Elementwise, with U = 2^-24 and H = 2^-8: a weight p is off by d p (attn_ref.py: scores and log-sum-exp), dout . V_j by
+    hd U of its magnitudes (e), D = sum p_j (dout . V_j) by sum p_j (d |dout . V_j| + e) and 64 + 4 roundings of its terms.
+    dS = p (dout . V_j - D) by d |dS|, p times the errors of both and of their difference, and as an operand by H and 2^-16
+    (weights are handed over in 24 bits)."""
+    import attn_ref as ref
+    import raster_amd
+
+    nq, nkv, scale = 4, 2, hd ** -0.5
+    print(f"[gpu] window gradient of few keys x{hd} {lq} {lk} {window}+{sinks}", flush=True)
+    q, k, v, do = data(torch, "bf16", nq, nkv, hd, lq, lk, hd + sum(lq) + window)
+    cu, cu_k = cu_of(torch, lq), None if lq == lk else cu_of(torch, lk)
+    lse = torch.empty((nq, sum(lq)), device="cuda")
+    see = dict(window=window, sinks=sinks, cu_k=cu_k)
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse, **see)
+    dq, dk, _ = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, **see)
+    U, H = 2.0 ** -24, 2.0 ** -8
+    a0 = b0 = 0
+    for a, b in zip(lq, lk):
+        see = seen(torch, a, b, window, sinks)
+        for j in range(nkv):
+            kj, vj = heads(k[b0:b0 + b], j, hd), heads(v[b0:b0 + b], j, hd)
+            wk, bk = (torch.zeros((b, hd), dtype=torch.float64, device="cuda") for _ in range(2))
+            for h in range(j * (nq // nkv), (j + 1) * (nq // nkv)):
+                qh, dh = heads(q[a0:a0 + a], h, hd), heads(do[a0:a0 + a], h, hd)
+                x = (qh @ kj.T * scale).masked_fill(~see, -torch.inf)
+                p = torch.where(see, torch.exp(x - torch.logsumexp(x, 1)[:, None].clamp(min=-1e300)), 0.0)
+                dp, e = dh @ vj.T, hd * U * (dh.abs() @ vj.abs().T)
+                delta = (p * dp).sum(1, keepdim=True)
+                ds = p * (dp - delta)
+                mag = (qh.abs() @ kj.abs().T * scale).masked_fill(~see, 0.0)
+                d = 2 * (hd + 4) * U * ref._largest(mag) + 8 * U
+                edelta = (p * ((d + 68 * U) * dp.abs() + e)).sum(1, keepdim=True)
+                eds = (H + 2.0 ** -15 + d + U) * ds.abs() + p * (edelta + e)
+                adds = (max(a, b) + 4) * U
+                bq = H * (ds @ kj * scale).abs() + (eds + adds * ds.abs()) @ kj.abs() * scale + 1e-30
+                off = (heads(dq[a0:a0 + a], h, hd) - ds @ kj * scale).abs()
+                assert bool((off <= bq).all()), (a, b, h, "dq", float((off / bq).max()))
+                wk += ds.T @ qh * scale
+                bk += (eds + adds * ds.abs()).T @ qh.abs() * scale
+            bk += H * wk.abs() + 1e-30
+            off = (heads(dk[b0:b0 + b], j, hd) - wk).abs()
+            assert bool((off <= bk).all()), (a, b, j, "dk", float((off / bk).max()))
+        a0, b0 = a0 + a, b0 + b
