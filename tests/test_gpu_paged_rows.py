@@ -79,3 +79,22 @@ def test_rows_past_one_launch(torch, ctx, dtype, page, lens):
         if scales is not None:
             want = want.float() * scales.reshape(-1, 1)[at // 16]
         assert torch.equal(x, want)
+
+
+def test_rows_leaves_the_views_alone(torch, ctx):
+    """A captured graph's view follows the cache from the next view() or sync() on, not from a look at its rows."""
+    print("[gpu] rows and views", flush=True)
+    cache, seqs = of(torch, ctx, torch.float32, 2, 64, 16, [100, 7])
+    view = cache.view()
+    table, lens = view.table.clone(), view.lens.clone()
+    cache.free(seqs[1])
+    s = cache.add()
+    cache.reserve([s], 30)
+    cache.advance([s], 30)
+    lens2 = [30, 100]
+    at = by_index(torch, cache, [s, seqs[0]], lens2)
+    for got, pages in zip(cache.rows(1, [s, seqs[0]]), (cache.kpages(1), cache.vpages(1))):
+        assert torch.equal(got, pages.view(-1, 128)[at])
+    assert torch.equal(view.table, table) and torch.equal(view.lens, lens)
+    cache.sync()
+    assert not torch.equal(view.table, table) and int(view.lens[s]) == 30
