@@ -318,8 +318,8 @@ constexpr int q8_fixed_bytes() {
 // each KV head's 128 bytes are read by other compute units at other times: 8 sequences of 33 to 65 Ki rows 4.1 against
 // 5.3 TB/s with the loads alone. With few, HW = 1: more waves at a sequence, each with less to walk.
 //
-// Bound: those 8 sequences, 888 MB, 165 to 175 us with 6 us for the join, 5.1 to 5.4 TB/s in the kernel, where loads
-// alone reach 5.3: by the memory. The 117 MB, about 230 rows a workgroup, 34 us: 11 of them until the first rows are
+// Bound: those 8 sequences, 888 MB, 165 to 175 us by card with 6 us for the join, 5.1 to 5.4 TB/s over both: by the
+// memory (a plain read of a large array 6.1; these loads alone, on a card where the call took 175, 5.3). The 117 MB, about 230 rows a workgroup, 34 us: 11 of them until the first rows are
 // there (lengths, plan, table, rows one after the other), then four tiles a wave of 630 vector instructions each,
 // half of the time that is left. One sequence of 128 rows 9 us: those loads one after the other. A third workgroup a
 // CU (the registers of SPREAD allow it) 42.6, and 888 MB 211: the ranges are shorter and the join is longer.

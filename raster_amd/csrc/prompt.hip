@@ -17,7 +17,7 @@
 //
 // Bound by the matrix instructions: 4 head_dim operations for every (query, key) pair that sees the other
 // against a few bytes. Measured, causal: bf16, 8192 tokens, 32/8 heads x 128, 502 to 511 us, 1.08 PFLOP/s, 558 us on a
-// card warm from other work (a library's 8192^3 product reaches 1.03 here); 2048, 777, 1500, 331, 1999 and 64 tokens
+// card warm from other work (a library's 8192^3 product reaches 1.3); 2048, 777, 1500, 331, 1999 and 64 tokens
 // 124 us, 0.74; 37 tokens 6.0 us, a launch and one tile's latencies. f32, 613, 1, 1024, 250 and 89 queries, 16/16
 // heads x 128, 117 us, 59 TFLOP/s (product 153): the matrix pipe is busy 0.40 of the time, a third of that on the
 // masked halves of cut tiles, the rest is one wave a SIMD waiting for its tiles.

@@ -206,7 +206,9 @@ class DecoderLayer:
         into the cache's pages of `layer`; each token attends its sequence up to
         itself, or the layer's window, rows stored before included, keys and values as the pages hold them (a
         bf16 cache rounds them), however a prompt is cut (int8: a block of 16 tokens has one scale, so
-        its last tokens' size and where a prompt is cut show in its values' rounding). Returns [rows, d].
+        its last tokens' size and where a prompt is cut show in its values' rounding). Of a prompt that goes on, all
+        stored rows are copied out of the pages, with a window too: 16 bytes a KV head's element in f32 (read, written, keys
+        and values). Returns [rows, d].
         After the last layer, cache.advance(seqs, lens)."""
         torch = _t()
         _need(len(seqs) == len(lens) == cu.numel() - 1 and sum(lens) == x.shape[0],

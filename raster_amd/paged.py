@@ -14,8 +14,8 @@ arrays goes on reading them, so its replays follow later changes. One cache is u
 by one thread and on one stream at a time.
 
 With dtype int8 the rows are codes, and `scales` holds one f32 scale for each 16 rows and KV head, in
-every plane beside the pages; they are copied and moved together. A row of 128 elements a head takes
-0.52 of a bf16 one's bytes.
+every plane beside the pages; they are copied and moved together. Rows of 128 elements a head take
+0.501 of bf16 ones' bytes (0.504 at most, with the scales of a page filled up to 16 bytes).
 """
 from __future__ import annotations
 
