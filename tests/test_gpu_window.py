@@ -433,3 +433,12 @@ def test_gradient_of_few_keys(torch, ctx, hd, window, sinks, lq, lk):
             off = (heads(dk[b0:b0 + b], j, hd) - wk).abs()
             assert bool((off <= bk).all()), (a, b, j, "dk", float((off / bk).max()))
         a0, b0 = a0 + a, b0 + b
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+@pytest.mark.parametrize("window,sinks", [(3, 0), (40, 2), (1, 63)])
+def test_nan_around_few_keys(torch, ctx, t, window, sinks):
+    """As above where no query sees more than 64 keys."""
+    test_nan_far_outside_the_window(torch, ctx, t, 700, window, sinks)
+    if sinks:
+        test_nan_behind_the_sinks(torch, ctx, t, 2, 1500, window, sinks)
