@@ -259,6 +259,14 @@ struct Handover {
   }
 };
 
+// The slot of a sequence's first chunk, the others behind it. Sequences of up to sink_whole queries are not cut: where
+// that is a chunk, two chunks and more have room in slots of half a chunk before the next sequence's; where all
+// sequences are (-1), they take a slot each and one for each chunk of rows, as tile_of_slot does.
+__device__ __forceinline__ int64_t sink_slot0(const PromptArgs& a, int b) {
+  const bool cut_all = a.sink_whole < 0;
+  return (uint32_t)clamp_cu(a.cu_q, b, a.rows_q) / (uint32_t)(cut_all ? a.sink_chunk : a.sink_chunk / 2) + (cut_all ? b : 0);
+}
+
 // dK and dV of 64 keys: query tiles of 32 or 64 rows through LDS, two waves for each 32
 // keys. One holds K and dV: it forms S = Q K^T and P, and adds dO^T P to dV; the
 // other holds V and dK: it forms dO V^T meanwhile, takes P over through LDS and adds
@@ -306,9 +314,8 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
   TileSpan tk;
   int chunk = 0;  // first query of the chunk
   if (WIN && sink) {
-    tk = tile_of_slot(a.cu_q, a.batch, a.rows_q, a.sink_chunk, slot);
-    if (tk.len == 0) return;
-    chunk = tk.row0;
+    tk.seq = count_first(a.batch, [&](int b) { return sink_slot0(a, b) <= slot; }) - 1;
+    if (tk.seq < 0) return;
     const int64_t k0 = clamp_cu(a.cu_k, tk.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tk.seq + 1, a.rows_k);
     tk.begin = k0;
     tk.len = (int)(k1 > k0 ? k1 - k0 : 0);
@@ -316,10 +323,17 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
     if (tk.row0 >= tk.len) return;
   } else {
     tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, kDkvKeys, slot);
-    if (tk.len == 0 || (WIN && tk.row0 < a.sink_tiles * kDkvKeys)) return;
+    if (tk.len == 0) return;
   }
   const int64_t q0 = clamp_cu(a.cu_q, tk.seq, a.rows_q), q1 = clamp_cu(a.cu_q, tk.seq + 1, a.rows_q);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), off = tk.len - lq;
+  if (WIN && sink) {
+    const int64_t c = slot - sink_slot0(a, tk.seq);
+    if (lq <= a.sink_whole || c < 0 || c * a.sink_chunk >= lq) return;
+    chunk = (int)c * a.sink_chunk;
+  } else if (WIN && tk.row0 < a.sink_tiles * kDkvKeys && lq > a.sink_whole) {
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool is_k = wave & 1;  // this wave forms dK
@@ -509,7 +523,8 @@ __global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a) {
   const int64_t q0 = clamp_cu(a.cu_q, b, a.rows_q), q1 = clamp_cu(a.cu_q, b + 1, a.rows_q);
   const int64_t k0 = clamp_cu(a.cu_k, b, a.rows_k), k1 = clamp_cu(a.cu_k, b + 1, a.rows_k);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), keys = (int)min(k1 - k0 - tile * kDkvKeys, (int64_t)kDkvKeys);
-  const int64_t slot = q0 / a.sink_chunk + b;
+  if (lq <= a.sink_whole) return;
+  const int64_t slot = sink_slot0(a, b);
   const int parts = (lq + a.sink_chunk - 1) / a.sink_chunk * a.nsplit, hd = a.head_dim;
   const int64_t step = (int64_t)a.sink_tiles * a.n_kv * 2 * kDkvKeys * hd;
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -804,14 +819,20 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({most / groups, steps / least_steps, 16}));
   // Chunks of the first keys' queries, of about as many steps as the other keys have and in as many parts, where a
   // sequence can be longer than the window and a chunk; with many sinks their tiles are workgroups enough.
-  p.sink_tiles = p.sink_chunk = 0;
+  p.sink_tiles = p.sink_chunk = p.sink_whole = 0;
   p.sink_slots = 0;
   const int tiles = (a.sinks + kDkvKeys - 1) / kDkvKeys;
   const int chunk = std::min(std::max((a.window + 63) / 64 * 64, 256), 2048);
   if (a.window > 0 && tiles > 0 && tiles <= 8 && rows_q > a.window + chunk) {
     p.sink_tiles = tiles;
     p.sink_chunk = chunk;
-    p.sink_slots = tile_slots(rows_q, batch, chunk);
+    // Where most sequences are shorter than a chunk, a slot for each would be most of the workspace (64 KV heads x 256, 10000
+    // sequences, 500 sinks: 671 GB), so those of one chunk stay whole, which is faster there too. us, a slot a
+    // sequence at least / so, bf16, 4 sinks: 500 of 100 (8/4 x 128, window 40) 479 / 433, 100 of 60 and one of 3000 (32/8,
+    // 256) 315 / 296; but 16 of 500 (32/8, 256) 280 / 307, 4 of 2047 (32/8, 1024) 571 / 580.
+    const bool many = batch > rows_q / chunk;
+    p.sink_whole = many ? chunk : -1;
+    p.sink_slots = many ? rows_q / (chunk / 2) + 1 : tile_slots(rows_q, batch, chunk);
   }
   const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv * p.nsplit;
   p.groups = std::max(sinks + tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,

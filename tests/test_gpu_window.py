@@ -442,3 +442,24 @@ def test_nan_around_few_keys(torch, ctx, t, window, sinks):
     test_nan_far_outside_the_window(torch, ctx, t, 700, window, sinks)
     if sinks:
         test_nan_behind_the_sinks(torch, ctx, t, 2, 1500, window, sinks)
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,window,sinks", [("bf16", 4, 4, 128, 100, 4), ("bf16", 8, 4, 64, 40, 70),
+                                                      ("f32", 4, 4, 64, 300, 130), ("f32", 2, 2, 128, 7, 9)])
+@pytest.mark.parametrize("more", [0, 37])
+def test_gradient_of_sinks_of_many_sequences(torch, ctx, t, nq, nkv, hd, window, sinks, more):
+    """Long sequences among many short ones and ones of about a chunk of queries (256; of 300 keys 320)."""
+    import raster_amd
+
+    print(f"[gpu] window sinks of many {t} {nq}/{nkv}x{hd} {window}+{sinks}", flush=True)
+    lens = [1, 0, 257, 3, 900, 255, 256, 1, 0, 0, 321, 319, 320, 2, 512, 513, 5, 640, 641, 1, 130, 2, 2, 700, 0]
+    lk = [n + more for n in lens]
+    q, k, v, do = data(torch, t, nq, nkv, hd, lens, lk, window)
+    cu, cu_k, scale = cu_of(torch, lens), None if lens == lk else cu_of(torch, lk), hd ** -0.5
+    lse = torch.empty((nq, sum(lens)), device="cuda")
+    see = dict(window=window, sinks=sinks, cu_k=cu_k)
+    out = raster_amd.prompt_attention(ctx, q, k, v, cu, nq, nkv, hd, scale, lse=lse, **see)
+    nan = [torch.full_like(x, float("nan")) for x in (q, k, v)]
+    grads = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, dq=nan[0], dk=nan[1],
+                                            dv=nan[2], **see)
+    check_gradient(torch, q, k, v, do, grads, lens, lk, nq, nkv, hd, scale, window, sinks)

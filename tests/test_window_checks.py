@@ -79,3 +79,14 @@ def test_python_arguments():
         x = torch.zeros(4, 64)
         attention.prompt_attention(type("C", (), {"device": 0, "handle": None})(), x, x, x,
                                    torch.zeros(2, dtype=torch.int32), 1, 1, 64, 0.1, window=3)
+
+
+@pytest.mark.parametrize("window,sinks", [(64, 4), (1000, 500)])
+def test_work_does_not_grow_with_the_sequences(window, sinks):
+    """The sinks' partial sums are of chunks of 256 queries or more, and of at most two for each of so many, whatever the
+    sequences: 64 keys' dK and dV in f32, for each 64 sinks and KV head."""
+    rows = 400000
+    for batch in (1, 7, 1000, 1563, 5000, 100000, 10 ** 7):
+        p = prompt(batch=batch, rows_q=rows, rows_k=rows, n_q=16, n_kv=16, head_dim=128)
+        more = work(p, window, sinks)[1] - work(p, window, 0)[1]
+        assert more <= (rows // 128 + 1) * -(-sinks // 64) * 16 * 2 * 64 * 128 * 4, batch
