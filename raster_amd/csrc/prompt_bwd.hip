@@ -514,12 +514,15 @@ __global__ __launch_bounds__(256) void prompt_dkv_sum_kernel(PromptArgs a) {
   *reinterpret_cast<T4*>(static_cast<T*>(a.dk) + row * a.dk_stride + e) = yk;
 }
 
-// dK and dV of the first keys from their chunks: kSinkParts workgroups the 64 keys of a sequence and KV head.
-constexpr int kSinkParts = 16;
+// dK and dV of the first keys from their chunks: `wgs` workgroups the 64 keys of a sequence and KV head, one where there
+// are too many sequences for more (the limit on D's workgroups keeps those within one launch's).
+int64_t sink_sum_parts(int64_t batch, int64_t n_kv, int64_t tiles) {
+  return batch * n_kv * tiles * 16 <= kMaxGroups ? 16 : 1;
+}
 template <typename T>
-__global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a) {
-  const int part_of = blockIdx.x % kSinkParts, hkv = blockIdx.x / kSinkParts % a.n_kv;
-  const int rest = blockIdx.x / kSinkParts / a.n_kv, tile = rest % a.sink_tiles, b = rest / a.sink_tiles;
+__global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a, int wgs) {
+  const int part_of = blockIdx.x % wgs, hkv = blockIdx.x / wgs % a.n_kv;
+  const int rest = blockIdx.x / wgs / a.n_kv, tile = rest % a.sink_tiles, b = rest / a.sink_tiles;
   const int64_t q0 = clamp_cu(a.cu_q, b, a.rows_q), q1 = clamp_cu(a.cu_q, b + 1, a.rows_q);
   const int64_t k0 = clamp_cu(a.cu_k, b, a.rows_k), k1 = clamp_cu(a.cu_k, b + 1, a.rows_k);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), keys = (int)min(k1 - k0 - tile * kDkvKeys, (int64_t)kDkvKeys);
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a) {
   const int parts = (lq + a.sink_chunk - 1) / a.sink_chunk * a.nsplit, hd = a.head_dim;
   const int64_t step = (int64_t)a.sink_tiles * a.n_kv * 2 * kDkvKeys * hd;
   typedef T T4 __attribute__((ext_vector_type(4)));
-  for (int i = part_of * 256 + threadIdx.x; i < 2 * keys * (hd / 4); i += kSinkParts * 256) {
+  for (int i = part_of * 256 + threadIdx.x; i < 2 * keys * (hd / 4); i += wgs * 256) {
     const int is_k = i >= keys * (hd / 4), j = is_k ? i - keys * (hd / 4) : i, row = j / (hd / 4), e = 4 * (j % (hd / 4));
     const float* part =
         a.sink_part + slot * a.nsplit * step + ((tile * a.n_kv + hkv) * 2 + is_k) * (kDkvKeys * hd) + row * hd + e;
@@ -794,8 +797,9 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
     if (hipError_t e = hipGetLastError()) return e;
   }
   if (WIN && a.sink_tiles > 0) {  // (after the parts' sums, which know nothing of these keys and write what was there)
-    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * kSinkParts)),
-                       dim3(256), 0, stream, a);
+    const int64_t wgs = sink_sum_parts(a.batch, a.n_kv, a.sink_tiles);
+    hipLaunchKernelGGL(prompt_sink_sum_kernel<T>, dim3((unsigned)(a.batch * a.sink_tiles * a.n_kv * wgs)), dim3(256), 0,
+                       stream, a, (int)wgs);
     return hipGetLastError();
   }
   return hipSuccess;
@@ -837,7 +841,7 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv * p.nsplit;
   p.groups = std::max(sinks + tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
                       std::max<int64_t>({(rows_q * n_q * kDeltaLanes + 255) / 256, batch * n_q * kExactTiles,
-                                                batch * n_kv * p.sink_tiles * kSinkParts}));
+                                         batch * n_kv * p.sink_tiles * sink_sum_parts(batch, n_kv, p.sink_tiles)}));
   p.delta_bytes = ((size_t)(n_q * rows_q) * sizeof(float) + 255) & ~(size_t)255;
   p.part_bytes = p.nsplit > 1 ? (size_t)(2 * p.nsplit * rows_k * n_kv * head_dim) * sizeof(float) : 0;
   p.work = p.delta_bytes + p.part_bytes + (size_t)(sinks * 2 * kDkvKeys * head_dim) * sizeof(float);

@@ -463,3 +463,30 @@ def test_gradient_of_sinks_of_many_sequences(torch, ctx, t, nq, nkv, hd, window,
     grads = raster_amd.prompt_attention_bwd(ctx, do, q, k, v, out, lse, cu, nq, nkv, hd, scale, dq=nan[0], dk=nan[1],
                                             dv=nan[2], **see)
     check_gradient(torch, q, k, v, do, grads, lens, lk, nq, nkv, hd, scale, window, sinks)
+
+
+def test_gradient_of_sinks_of_very_many_sequences(torch, ctx):
+    """9000 sequences x 16 KV heads x 8 tiles of sinks, one workgroup for each where there are 16 for each otherwise: the
+    long ones in the middle as by themselves, up to the order of sums; the rest, of one token each, have dq = dk = 0."""
+    import raster_amd
+
+    nq = nkv = 16
+    hd, batch, see, scale = 8, 9000, dict(window=30, sinks=500), 0.3
+    print("[gpu] window sinks of very many", flush=True)
+    lens = [1] * batch
+    lens[batch // 2], lens[batch // 2 + 1] = 1200, 600
+    n, at = sum(lens), batch // 2
+    q, k, v, do = data(torch, "f32", nq, nkv, hd, lens, lens, 4)
+
+    def both(s, cu):
+        x = [t[s] for t in (q, k, v, do)]
+        lse = torch.empty((nq, x[0].shape[0]), device="cuda")
+        out = raster_amd.prompt_attention(ctx, *x[:3], cu, nq, nkv, hd, scale, lse=lse, **see)
+        return raster_amd.prompt_attention_bwd(ctx, x[3], *x[:3], out, lse, cu, nq, nkv, hd, scale, **see)
+
+    many, alone = both(slice(0, n), cu_of(torch, lens)), both(slice(at, at + 1800), cu_of(torch, [1200, 600]))
+    for a, b in zip(many, alone):
+        assert bool(((a[at:at + 1800] - b).abs() <= 2.0 ** -16 * b.abs().max()).all())
+    for a in many[:2]:
+        assert float(a[:at].abs().max()) <= 1e-5 and float(a[at + 1800:].abs().max()) <= 1e-5
+    assert torch.allclose(many[2][:at], do[:at], rtol=1e-6, atol=0)

@@ -90,3 +90,11 @@ def test_work_does_not_grow_with_the_sequences(window, sinks):
         p = prompt(batch=batch, rows_q=rows, rows_k=rows, n_q=16, n_kv=16, head_dim=128)
         more = work(p, window, sinks)[1] - work(p, window, 0)[1]
         assert more <= (rows // 128 + 1) * -(-sinks // 64) * 16 * 2 * 64 * 128 * 4, batch
+
+
+@pytest.mark.parametrize("sinks", [0, 4, 500])
+def test_many_sequences_with_sinks_are_taken(sinks):
+    """Launches of fewer than 2^24 workgroups for 100000 sequences, with sinks as without."""
+    for batch in (1, 1000, 100000):
+        p = prompt(batch=batch, rows_q=400000, rows_k=400000, n_q=16, n_kv=16, head_dim=128)
+        assert bwd(p, 64, sinks, **{s: 2048 for s in ("dos", "qs", "ks", "vs", "os", "dqs", "dks", "dvs")}) == RQ_ERR_HANDLE
