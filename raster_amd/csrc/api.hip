@@ -1766,7 +1766,7 @@ int rq_prompt_attention_window_bwd(rq_ctx h, const rq_prompt* p, int64_t window,
   a.nsplit = plan.nsplit;
   a.part = reinterpret_cast<float*>(static_cast<char*>(work) + plan.delta_bytes);
   a.sink_tiles = plan.sink_tiles, a.sink_chunk = plan.sink_chunk, a.sink_slots = plan.sink_slots;
-  a.sink_whole = plan.sink_whole;
+  a.few_cut = plan.few_cut;
   a.sink_part = reinterpret_cast<float*>(static_cast<char*>(work) + plan.delta_bytes + plan.part_bytes);
   const hipError_t e = launch_prompt_bwd(p->dtype, a, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "prompt attention gradient launch");

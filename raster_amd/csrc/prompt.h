@@ -25,9 +25,9 @@ struct PromptArgs {
   float* delta;  // [n_q][rows_q]: dout . out
   float* part;   // [nsplit][dv, dk][rows_k][n_kv * head_dim] when nsplit > 1
   int nsplit;
-  // With sink_tiles > 0 the gradients of the first sink_tiles tiles of 64 keys of every sequence of more than sink_whole
-  // queries are summed by chunks of sink_chunk queries: sink_part [sink_slots][nsplit][sink_tiles][n_kv][dv, dk][64][head_dim]
-  int sink_tiles, sink_chunk, sink_whole;
+  // With sink_tiles > 0 the gradients of the first sink_tiles tiles of 64 keys of every sequence (few_cut: of more than
+  // sink_chunk queries) are summed by chunks of sink_chunk queries: sink_part [sink_slots][nsplit][sink_tiles][n_kv][dv, dk][64][head_dim]
+  int sink_tiles, sink_chunk, few_cut;
   int64_t sink_slots;
   float* sink_part;
 };
@@ -90,7 +90,7 @@ __device__ __forceinline__ bool window_all(const PromptArgs& a, int pos, int key
 }
 
 struct PromptBwdPlan {
-  int nsplit, sink_tiles, sink_chunk, sink_whole;
+  int nsplit, sink_tiles, sink_chunk, few_cut;
   int64_t groups, sink_slots;  // groups: of the largest launch
   size_t delta_bytes, part_bytes, work;
 };

@@ -259,12 +259,13 @@ struct Handover {
   }
 };
 
-// The slot of a sequence's first chunk, the others behind it. Sequences of up to sink_whole queries are not cut: where
-// that is a chunk, two chunks and more have room in slots of half a chunk before the next sequence's; where all
-// sequences are (-1), they take a slot each and one for each chunk of rows, as tile_of_slot does.
+// The slot of a sequence's first chunk, the others behind it. All sequences cut: as in tile_of_slot, one each and one for
+// each chunk of rows. Only those of more than a chunk (few_cut): two chunks and more have room in slots of half a
+// chunk before the next sequence's. (Which, by an argument and not the template: 8767 tokens in six sequences 595 -> 601 us.)
+template <bool FEW_CUT>
 __device__ __forceinline__ int64_t sink_slot0(const PromptArgs& a, int b) {
-  const bool cut_all = a.sink_whole < 0;
-  return (uint32_t)clamp_cu(a.cu_q, b, a.rows_q) / (uint32_t)(cut_all ? a.sink_chunk : a.sink_chunk / 2) + (cut_all ? b : 0);
+  const int64_t q0 = clamp_cu(a.cu_q, b, a.rows_q);
+  return FEW_CUT ? q0 / (a.sink_chunk / 2) : q0 / a.sink_chunk + b;
 }
 
 // dK and dV of 64 keys: query tiles of 32 or 64 rows through LDS, two waves for each 32
@@ -298,7 +299,7 @@ constexpr int dkv_lds() {  // twice Q, dO, L and D of a step, and two pairs' wei
 // go to a.sink_part and prompt_sink_sum_kernel adds them in order. As one workgroup's steps those tiles would be the
 // last to end, long after the others, which see the queries of the window only: forward and gradient of 4096, 777,
 // 1500, 331, 1999 and 64 tokens, bf16, 32/8 heads x 128, window 1024 and 4 sinks: 1181 us, by chunks 740 to 780.
-template <typename T, int HD, bool WIN>
+template <typename T, int HD, bool WIN, bool FEW_CUT>
 __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool sink, char* lds) {
   using TL = Tile<T, HD>;
   using Frag = typename TL::Frag;
@@ -314,8 +315,14 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
   TileSpan tk;
   int chunk = 0;  // first query of the chunk
   if (WIN && sink) {
-    tk.seq = count_first(a.batch, [&](int b) { return sink_slot0(a, b) <= slot; }) - 1;
-    if (tk.seq < 0) return;
+    if constexpr (FEW_CUT) {
+      tk.seq = count_first(a.batch, [&](int b) { return sink_slot0<true>(a, b) <= slot; }) - 1;
+      if (tk.seq < 0) return;
+    } else {
+      tk = tile_of_slot(a.cu_q, a.batch, a.rows_q, a.sink_chunk, slot);
+      if (tk.len == 0) return;
+      chunk = tk.row0;
+    }
     const int64_t k0 = clamp_cu(a.cu_k, tk.seq, a.rows_k), k1 = clamp_cu(a.cu_k, tk.seq + 1, a.rows_k);
     tk.begin = k0;
     tk.len = (int)(k1 > k0 ? k1 - k0 : 0);
@@ -323,16 +330,15 @@ __device__ __forceinline__ void dkv_body(const PromptArgs& a, int block, bool si
     if (tk.row0 >= tk.len) return;
   } else {
     tk = tile_of_slot(a.cu_k, a.batch, a.rows_k, kDkvKeys, slot);
-    if (tk.len == 0) return;
+    if (tk.len == 0 || (WIN && !FEW_CUT && tk.row0 < a.sink_tiles * kDkvKeys)) return;
   }
   const int64_t q0 = clamp_cu(a.cu_q, tk.seq, a.rows_q), q1 = clamp_cu(a.cu_q, tk.seq + 1, a.rows_q);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), off = tk.len - lq;
-  if (WIN && sink) {
-    const int64_t c = slot - sink_slot0(a, tk.seq);
-    if (lq <= a.sink_whole || c < 0 || c * a.sink_chunk >= lq) return;
-    chunk = (int)c * a.sink_chunk;
-  } else if (WIN && tk.row0 < a.sink_tiles * kDkvKeys && lq > a.sink_whole) {
-    return;
+  if constexpr (FEW_CUT) {
+    const int64_t c = slot - sink_slot0<true>(a, tk.seq);
+    if (sink && (lq <= a.sink_chunk || c < 0 || c * a.sink_chunk >= lq)) return;
+    if (!sink && tk.row0 < a.sink_tiles * kDkvKeys && lq > a.sink_chunk) return;
+    if (sink) chunk = (int)c * a.sink_chunk;
   }
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -526,8 +532,8 @@ __global__ __launch_bounds__(256) void prompt_sink_sum_kernel(PromptArgs a, int 
   const int64_t q0 = clamp_cu(a.cu_q, b, a.rows_q), q1 = clamp_cu(a.cu_q, b + 1, a.rows_q);
   const int64_t k0 = clamp_cu(a.cu_k, b, a.rows_k), k1 = clamp_cu(a.cu_k, b + 1, a.rows_k);
   const int lq = (int)(q1 > q0 ? q1 - q0 : 0), keys = (int)min(k1 - k0 - tile * kDkvKeys, (int64_t)kDkvKeys);
-  if (lq <= a.sink_whole) return;
-  const int64_t slot = sink_slot0(a, b);
+  if (a.few_cut && lq <= a.sink_chunk) return;
+  const int64_t slot = a.few_cut ? sink_slot0<true>(a, b) : sink_slot0<false>(a, b);
   const int parts = (lq + a.sink_chunk - 1) / a.sink_chunk * a.nsplit, hd = a.head_dim;
   const int64_t step = (int64_t)a.sink_tiles * a.n_kv * 2 * kDkvKeys * hd;
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -747,14 +753,14 @@ __device__ __forceinline__ void dq_split_body(const PromptArgs& a, int block, ch
 
 // Both in one launch, so that the short workgroups of one fill the compute units that the
 // last long ones of the other leave idle.
-template <typename T, int HD, int BK, int QG, bool WIN>
+template <typename T, int HD, int BK, int QG, bool WIN, bool FEW_CUT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && HD <= 128 ? 2 : 1) void prompt_grad_kernel(PromptArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int block = blockIdx.x;
   const int sinks = WIN ? (int)(a.sink_slots * a.sink_tiles * a.n_kv * a.nsplit) : 0;
   const int dkv = sinks + (int)(a.k_slots * a.n_kv * a.nsplit);
   if (block < dkv)
-    dkv_body<T, HD, WIN>(a, block < sinks ? block : block - sinks, block < sinks, lds);
+    dkv_body<T, HD, WIN, FEW_CUT>(a, block < sinks ? block : block - sinks, block < sinks, lds);
   else if constexpr (QG == 4)
     dq_body<T, HD, BK, WIN>(a, block - dkv, lds);
   else
@@ -784,9 +790,10 @@ hipError_t run_bwd(PromptArgs a, hipStream_t stream) {
   constexpr int lds = std::max(dkv_lds<T, HD>(), dq_lds);
   a.k_slots = a.rows_k > 0 ? tile_slots(a.rows_k, a.batch, kDkvKeys) : 0;
   a.q_slots = a.rows_q > 0 ? tile_slots(a.rows_q, a.batch, 32 * QG) : 0;
-  const auto kernel = prompt_grad_kernel<T, HD, BK, QG, WIN>;
-  static std::atomic<uint64_t> allowed{0};
-  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed)) return e;
+  const bool few_cut = WIN && a.few_cut;
+  const auto kernel = few_cut ? prompt_grad_kernel<T, HD, BK, QG, WIN, WIN> : prompt_grad_kernel<T, HD, BK, QG, WIN, false>;
+  static std::atomic<uint64_t> allowed[2];
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds, &allowed[few_cut])) return e;
   const int64_t sinks = a.sink_slots * a.sink_tiles * a.n_kv * a.nsplit;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(sinks + a.k_slots * a.n_kv * a.nsplit + a.q_slots * a.n_q)), dim3(256),
                      lds, stream, a);
@@ -823,7 +830,7 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({most / groups, steps / least_steps, 16}));
   // Chunks of the first keys' queries, of about as many steps as the other keys have and in as many parts, where a
   // sequence can be longer than the window and a chunk; with many sinks their tiles are workgroups enough.
-  p.sink_tiles = p.sink_chunk = p.sink_whole = 0;
+  p.sink_tiles = p.sink_chunk = p.few_cut = 0;
   p.sink_slots = 0;
   const int tiles = (a.sinks + kDkvKeys - 1) / kDkvKeys;
   const int chunk = std::min(std::max((a.window + 63) / 64 * 64, 256), 2048);
@@ -834,9 +841,8 @@ PromptBwdPlan plan_prompt_bwd(const PromptArgs& a) {
     // sequences, 500 sinks: 671 GB), so those of one chunk stay whole, which is faster there too. us, a slot a
     // sequence at least / so, bf16, 4 sinks: 500 of 100 (8/4 x 128, window 40) 479 / 433, 100 of 60 and one of 3000 (32/8,
     // 256) 315 / 296; but 16 of 500 (32/8, 256) 280 / 307, 4 of 2047 (32/8, 1024) 571 / 580.
-    const bool many = batch > rows_q / chunk;
-    p.sink_whole = many ? chunk : -1;
-    p.sink_slots = many ? rows_q / (chunk / 2) + 1 : tile_slots(rows_q, batch, chunk);
+    p.few_cut = batch > rows_q / chunk;
+    p.sink_slots = p.few_cut ? rows_q / (chunk / 2) + 1 : tile_slots(rows_q, batch, chunk);
   }
   const int64_t sinks = p.sink_slots * p.sink_tiles * n_kv * p.nsplit;
   p.groups = std::max(sinks + tile_slots(rows_k, batch, kDkvKeys) * n_kv * p.nsplit + tile_slots(rows_q, batch, 64) * n_q,
